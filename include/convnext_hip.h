@@ -330,6 +330,58 @@ int cnx_attention_bwd_supported(int32_t N, int32_t head_dim);
 int cnx_attention_bwd(const void* qkv, const void* out, const void* dout, const float* lse, void* dqkv, float* dvec,
                       int64_t B, int32_t N, int32_t H, int32_t head_dim, float scale, void* stream);
 
+/* Softmax attention over any number of tokens and its backward pass (csrc/mha_kernels.hip); cnx_attention_fwd / _bwd above are the
+ * packed self-attention of up to 416 tokens.
+ *     out = softmax(scale * q k^T) v        q, out [B, Nq, H, d], k, v [B, Nk, Hkv, d]; query head h reads key head h / (H / Hkv)
+ * bf16 or fp16 (dtype), d = 64 or 128 (cnx_mha_supported), products on the matrix cores, statistics and sums in fp32.  Any strides with
+ * the last dimension contiguous and every head 16-byte aligned; `strides` (host): elements between samples, tokens and heads of each
+ * tensor in the order given at the function.  q_lens / kv_lens [B] (nullable, clamped to [0, Nq] / [0, Nk]): queries and keys at or beyond
+ * them are padding: never used, padded queries give zeros (lse -inf), padded rows of every gradient are zeros.  causal: query i sees keys
+ * j <= i + kv_len - q_len (the last query sees the last key).  A query that sees no key gives zeros and no gradient.  A masked key's own
+ * values have no influence, except that causal order needs finite v: the tile that holds a row's last key may hold later ones.
+ * lse [B, H, Nq] (nullable in the forward) = log sum exp of the scaled scores.  ws: cnx_mha_ws_floats(...) floats (0 = none: NULL is
+ * fine), for calls with few rows, whose keys are split over workgroups; dvec: B * H * Nq floats.  scale > 0.  Deterministic. */
+int cnx_mha_supported(int32_t head_dim);
+int64_t cnx_mha_ws_floats(int64_t B, int32_t Nq, int32_t Nk, int32_t H, int32_t Hkv, int32_t head_dim);
+/* strides: q, k, v, out x (sample, token, head) = 12 values */
+int cnx_mha_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const int32_t* q_lens, const int32_t* kv_lens, float* ws,
+                const int64_t* strides, int dtype, int64_t B, int32_t Nq, int32_t Nk, int32_t H, int32_t Hkv, int32_t head_dim,
+                int32_t causal, float scale, void* stream);
+/* strides: q, k, v, out, dout, dq, dk, dv x (sample, token, head) = 24 values */
+int cnx_mha_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse, void* dq, void* dk,
+                void* dv, float* dvec, const int32_t* q_lens, const int32_t* kv_lens, float* ws, const int64_t* strides, int dtype,
+                int64_t B, int32_t Nq, int32_t Nk, int32_t H, int32_t Hkv, int32_t head_dim, int32_t causal, float scale, void* stream);
+
+/* Per-head RMS norm of queries and keys and their rotation by positions in one pass (csrc/rope_kernels.hip), the operator in front of an
+ * attention with normalised heads and / or rotary positions:
+ *     z = x * (mean(x^2) + eps)^-1/2 * w   (norm != 0; w: wq / wk [d], NULL = 1; otherwise z = x)
+ *     y = z with pair i of every head turned by  angle = positions[.., n, axis(i)] * inv_freq[i]      (positions == NULL: y = z)
+ * q [B, N, Hq, d], k [B, N, Hk, d] (Hq, Hk may differ, one of them may be 0), any strides with the last dimension contiguous and every
+ * head 16-byte aligned.  `strides` (host): elements between samples, tokens and heads of each tensor, in the order of the comment at the
+ * function.  Pairs: (i, i + d / 2), or (2 i, 2 i + 1) with interleaved != 0.  axes (1 .. 4) and sections[axes] (host, number of pairs of
+ * each axis, sum d / 2): time, height, width, ... in the order of the last dimension of positions [(B,) N, axes] (contiguous,
+ * CNX_POS_F32 / _I32 / _I64; pos_batch_stride = N * axes, or 0 for positions that the samples share).  inv_freq [d / 2] fp32.
+ * Angles are formed in 64 bits; statistics and sums in fp32.  dtype: APGD_F32, APGD_BF16, APGD_F16; weights fp32 or of that type
+ * (w_dtype).  d: a multiple of 16 up to 256 (cnx_qk_norm_rope_supported). */
+#define CNX_POS_F32 0
+#define CNX_POS_I32 1
+#define CNX_POS_I64 2
+int cnx_qk_norm_rope_supported(int32_t d);
+/* strides: q, k, yq, yk x (sample, token, head) = 12 values */
+int cnx_qk_norm_rope_fwd(const void* q, const void* k, void* yq, void* yk, int dtype, const int64_t* strides, const void* wq,
+                         const void* wk, int w_dtype, const void* positions, int pos_dtype, int64_t pos_batch_stride, int32_t axes,
+                         const int32_t* sections, const float* inv_freq, int64_t B, int64_t N, int32_t Hq, int32_t Hk, int32_t d,
+                         float eps, int32_t norm, int32_t interleaved, void* stream);
+/* Gradients of q, k (dq, dk) and, where dwq / dwk are given, of the weights (fp32 [d], summed over all rows in a fixed order; ws:
+ * cnx_qk_norm_rope_ws_floats(d) floats).  The norm is computed again from q and k (not read, and may be NULL, without norm).
+ * strides: dyq, dyk, q, k, dq, dk x (sample, token, head) = 18 values */
+int64_t cnx_qk_norm_rope_ws_floats(int32_t d);
+int cnx_qk_norm_rope_bwd(const void* dyq, const void* dyk, const void* q, const void* k, void* dq, void* dk, float* dwq, float* dwk,
+                         float* ws, int dtype, const int64_t* strides, const void* wq, const void* wk, int w_dtype, const void* positions,
+                         int pos_dtype, int64_t pos_batch_stride, int32_t axes, const int32_t* sections, const float* inv_freq,
+                         int64_t B, int64_t N, int32_t Hq, int32_t Hk, int32_t d, float eps, int32_t norm, int32_t interleaved,
+                         void* stream);
+
 /* Contraction over the ROW index of two row-major operands (round 5; csrc/wgrad_kernels.hip):
  *     D[N1][N2] = A^T B,   A: bf16 [M, N1] (row stride lda elements), B: bf16 [M, N2] (ldb), D: fp32 [N1, N2] contiguous
  * - the weight gradients of the pointwise convolutions and linears (models/convnext.py:42-46 backward: dW1 = dHpre^T LN(u),

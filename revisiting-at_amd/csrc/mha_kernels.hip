@@ -1,0 +1,788 @@
+// mha_kernels.hip — softmax attention over any number of tokens and its backward pass, on gfx950's matrix cores.
+//
+//   out = softmax(scale q k^T) v                                                      q [B, Nq, H, d], k, v [B, Nk, Hkv, d], H = G Hkv
+//   D = rowsum(dout out),  P = exp(scale q k^T - lse),  dS = P (dout v^T - D)
+//   dv = P^T dout,  dq = scale dS k,  dk = scale dS^T q                               (P and dS summed over the G heads that share a key head)
+// The N x N scores never reach memory: the forward keeps a running maximum and sum per query and saves only lse = log sum exp, the
+// backward forms P again from it.
+//
+// Rows.  The G query heads that share a key head are G rows of one matrix: row r of key head hk is token r / G, head hk G + r % G.  Shared
+// heads then cost no extra reads of k and v, a single token still fills G rows of a tile, and dk / dv are sums inside one workgroup - no
+// atomics, the same bits every time.
+//
+// Orientation.  mfma 32x32x16 leaves, per lane, one COLUMN of its result and 16 rows in registers.
+//   forward, dq:  S^T = K Q^T puts a query on each lane: maxima, sums, lse and D are one register, and P (rounded in registers) is the B
+//                 operand of  O^T = V^T P^T,  dQ^T = K^T dS^T  whose results again have a query per lane - rescaling is one multiply.
+//   dk, dv:       S = Q K^T puts a key on each lane; P and dS are B operands of  dV^T = dO^T P,  dK^T = Q^T dS.
+// Operand images in LDS are row-major as in memory; a product over d reads rows (ds_read_b128), a product over tokens reads columns
+// through the transposing read (ds_read_b64_tr_b16).  16-byte chunk c of row r is stored at chunk c ^ swz(r), which spreads both kinds of
+// read over all banks.
+//
+// Masks.  Each row has an end: keys at or beyond it are not seen (key lengths, causal order, padded queries: end 0).  A row that sees no
+// key gives zeros and lse = -inf, and no gradient.  Rows at or beyond their sample's length are staged as zeros whatever memory holds.
+#include <hip/hip_fp16.h>
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "apgd_hip.h"
+#include "convnext_hip.h"
+
+namespace {
+
+inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
+inline int launch_status() { return static_cast<int>(hipGetLastError()); }
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+typedef __attribute__((ext_vector_type(2))) float f32x2;
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+struct Bf16 {
+  static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const f32x2 v = {lo, hi};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
+  }
+  static __device__ __forceinline__ float lo(uint32_t w) { return __uint_as_float(w << 16); }
+  static __device__ __forceinline__ float hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+};
+struct Fp16 {
+  static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const f32x2 v = {lo, hi};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
+  }
+  static __device__ __forceinline__ float lo(uint32_t w) { return static_cast<float>(__builtin_bit_cast(f16x2, w)[0]); }
+  static __device__ __forceinline__ float hi(uint32_t w) { return static_cast<float>(__builtin_bit_cast(f16x2, w)[1]); }
+};
+
+struct View {                                    // 16-bit [B, N, heads, d], unit stride in d
+  int64_t b, n, h;
+};
+
+struct MhaArgs {
+  const uint16_t *q, *k, *v, *out, *dout;        // out, dout: backward
+  uint16_t *o, *dq, *dk, *dv;                    // o: forward
+  float* lse;                                    // [B, H, Nq]; forward: may be NULL
+  float* dvec;                                   // backward: [B, H, Nq]
+  float* part;                                   // key splits: partial results
+  const int32_t *q_lens, *kv_lens;               // [B] or NULL
+  View vq, vk, vv, vo, vdo, vdq, vdk, vdv;
+  int32_t Nq, Nk, H, Hkv, G, causal;
+  int32_t tiles, splits;                         // row (or key) tiles of a key head, splits of the keys
+  int32_t span;                                  // keys of one split, a multiple of the key tile
+  int64_t B;
+  float scale;
+};
+
+// what a sample allows
+struct Limits {
+  int q_len, kv_len, off;
+  __device__ __forceinline__ Limits(const MhaArgs& a, int64_t b) {
+    q_len = a.q_lens ? min(max(a.q_lens[b], 0), a.Nq) : a.Nq;
+    kv_len = a.kv_lens ? min(max(a.kv_lens[b], 0), a.Nk) : a.Nk;
+    off = kv_len - q_len;                        // causal: the last query sees the last key
+  }
+  // first key that token i does not see
+  __device__ __forceinline__ int end(int i, int causal) const {
+    if (i >= q_len) return 0;
+    return causal ? min(kv_len, max(0, i + off + 1)) : kv_len;
+  }
+};
+
+template <int D> __device__ __forceinline__ int swz(int row) {
+  const int b0 = row & 1, b1 = (row >> 1) & 1, b2 = (row >> 2) & 1, b3 = (row >> 3) & 1;
+  if constexpr (D == 64) return ((b0 ^ b1 ^ b2) << 2) | (b1 << 1) | b0;
+  else return ((b3 ^ b1) << 3) | (b0 << 2) | (b1 << 1) | b2;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t lds_addr(const T* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void*)p));
+}
+__device__ __forceinline__ u32x4 lds_read16(uint32_t addr) {
+  return *reinterpret_cast<const u32x4 __attribute__((address_space(3)))*>(static_cast<uintptr_t>(addr));
+}
+__device__ __forceinline__ u32x2 lds_read_tr(uint32_t addr) {
+  const s16x4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      reinterpret_cast<s16x4 __attribute__((address_space(3)))*>(static_cast<uintptr_t>(addr)));
+  return __builtin_bit_cast(u32x2, r);
+}
+
+// Geometry of a row-major image [rows][D] of 16-bit values in LDS, as one lane reads it.
+template <int D>
+struct Image {
+  static constexpr int ROWB = D * 2, CHUNKS = D / 8, KS = D / 16, DB = D / 32;
+  // operand of a product over d: row l32 of a 32-row block, k-step ks: chunk 2 ks + half
+  static __device__ __forceinline__ uint32_t row_piece(int lane) {
+    const int l32 = lane & 31, half = lane >> 5;
+    return l32 * ROWB + ((half ^ swz<D>(l32)) << 4);
+  }
+  static __device__ __forceinline__ u32x4 row(uint32_t base, uint32_t piece, int blk, int ks) {
+    return lds_read16((base + blk * 32 * ROWB) + (piece ^ (ks << 5)));
+  }
+  // operand of a product over rows: column db * 32 + lane % 32, rows 16 t + {0..3, 8..11} + 4 half of a 32-row block
+  static __device__ __forceinline__ uint32_t col_piece(int lane, int second) {
+    const int g = lane >> 4, i = lane & 15, row = 4 * (g >> 1) + (i >> 2) + 8 * second;
+    const int chunk = 2 * (g & 1) + ((i & 3) >> 1);
+    return row * ROWB + ((chunk ^ swz<D>(row)) << 4) + 8 * (i & 1);
+  }
+  static __device__ __forceinline__ u32x4 col(uint32_t base, uint32_t p0, uint32_t p1, int blk, int t, int db) {
+    const uint32_t at = base + (blk * 32 + t * 16) * ROWB;
+    const u32x2 a = lds_read_tr(at + (p0 ^ (db << 6))), b = lds_read_tr(at + (p1 ^ (db << 6)));
+    return u32x4{a.x, a.y, b.x, b.y};
+  }
+};
+
+// Staging of ROWS rows of a tensor by 256 threads: piece e = (row e / CHUNKS, chunk e % CHUNKS) of thread e % 256.  Loaded to registers one
+// tile ahead, written to LDS when the tile's turn comes.
+template <int D, int ROWS>
+struct Stage {
+  static constexpr int PER = ROWS * (D / 8) / 256;
+  u32x4 r[PER];
+  template <typename Row>                        // Row: row number in the tile -> pointer to the row or nullptr (zeros)
+  __device__ __forceinline__ void load(Row row_of) {
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+      const int e = threadIdx.x + p * 256, row = e / (D / 8), c = e % (D / 8);
+      const uint16_t* src = row_of(row);
+      r[p] = u32x4{0, 0, 0, 0};
+      if (src) r[p] = *reinterpret_cast<const u32x4*>(src + c * 8);
+    }
+  }
+  __device__ __forceinline__ void store(uint32_t base) const {
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+      const int e = threadIdx.x + p * 256, row = e / (D / 8), c = e % (D / 8);
+      *reinterpret_cast<u32x4 __attribute__((address_space(3)))*>(static_cast<uintptr_t>(base + row * D * 2 + ((c ^ swz<D>(row)) << 4))) = r[p];
+    }
+  }
+};
+
+__device__ __forceinline__ f32x16 zeros16() {
+  f32x16 z;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) z[r] = 0.f;
+  return z;
+}
+__device__ __forceinline__ float both_halves_max(float v) { return fmaxf(v, __shfl_xor(v, 32, 64)); }
+__device__ __forceinline__ float both_halves_sum(float v) { return v + __shfl_xor(v, 32, 64); }
+
+// Workgroups go round robin over the 8 XCDs, each with an L2 of its own: a contiguous run of the work per XCD keeps the tiles that read
+// one key head's k and v (or q and dout) on one L2.
+__device__ __forceinline__ int64_t xcd_order(int64_t bid, int64_t total) {
+  const int64_t per = total >> 3, rest = total & 7, x = bid & 7, i = bid >> 3;
+  return x * per + (x < rest ? x : rest) + i;
+}
+
+template <typename T> __device__ __forceinline__ uint2 pack4(float a, float b, float c, float d) { return make_uint2(T::pack(a, b), T::pack(c, d)); }
+
+constexpr int kKT = 64;                          // keys (rows) of a staged tile
+
+// ===================================================================================================================== forward
+// Workgroup: 4 wavefronts x 32 RB rows of one key head, over the keys [split * span, + span).  Row r of the tile: lane.
+template <typename T, int D, int RB>
+__global__ __launch_bounds__(256) void mha_fwd_kernel(const MhaArgs a) {
+  using I = Image<D>;
+  constexpr int KS = I::KS, DB = I::DB, ROWS = 128 * RB;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[2][2][kKT * D * 2];        // [buffer][k, v]
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l32 = lane & 31, half = lane >> 5;
+  const int64_t per_b = static_cast<int64_t>(a.Hkv) * a.tiles * a.splits;
+  int64_t w = xcd_order(blockIdx.x, gridDim.x);
+  const int64_t b = w / per_b;
+  w -= b * per_b;
+  const int hk = static_cast<int>(w / (a.tiles * a.splits));
+  w -= static_cast<int64_t>(hk) * a.tiles * a.splits;
+  const int tile = a.tiles - 1 - static_cast<int>(w / a.splits), split = static_cast<int>(w % a.splits);   // causal: long tiles first
+  const Limits lim(a, b);
+  const int64_t R = static_cast<int64_t>(a.Nq) * a.G, row0 = static_cast<int64_t>(tile) * ROWS;
+  const uint16_t* qb = a.q + b * a.vq.b + static_cast<int64_t>(hk) * a.G * a.vq.h;
+  const uint16_t* kb = a.k + b * a.vk.b + hk * a.vk.h;
+  const uint16_t* vb = a.v + b * a.vv.b + hk * a.vv.h;
+
+  // the lane's rows
+  int tok[RB], end[RB], hd[RB];
+  u32x4 qf[RB][KS];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    const int64_t r = row0 + wave * 32 * RB + rb * 32 + l32;
+    tok[rb] = r < R ? static_cast<int>(r / a.G) : a.Nq;
+    hd[rb] = r < R ? static_cast<int>(r - static_cast<int64_t>(tok[rb]) * a.G) : 0;
+    end[rb] = lim.end(tok[rb], a.causal);
+    const bool live = tok[rb] < lim.q_len;
+    const uint16_t* src = qb + (live ? tok[rb] * a.vq.n + hd[rb] * a.vq.h : 0);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      qf[rb][ks] = u32x4{0, 0, 0, 0};
+      if (live) qf[rb][ks] = *reinterpret_cast<const u32x4*>(src + ks * 16 + half * 8);
+    }
+  }
+  // the workgroup's keys
+  const int64_t last_row = (row0 + ROWS < R ? row0 + ROWS : R) - 1;
+  const int first_tok = static_cast<int>(row0 / a.G), last_tok = min(static_cast<int>(last_row / a.G), lim.q_len - 1);
+  const int k_begin = split * a.span;
+  const int k_end = min(first_tok <= last_tok ? lim.end(last_tok, a.causal) : 0, k_begin + a.span);
+
+  const float c2 = a.scale * kLog2e;
+  float m[RB], l[RB];
+  f32x16 o[RB][DB];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    m[rb] = -INFINITY;
+    l[rb] = 0.f;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) o[rb][db] = zeros16();
+  }
+  Stage<D, kKT> sk, sv;
+  auto fetch = [&](int k0) {
+    sk.load([&](int row) { return k0 + row < lim.kv_len ? kb + (k0 + row) * a.vk.n : nullptr; });
+    sv.load([&](int row) { return k0 + row < lim.kv_len ? vb + (k0 + row) * a.vv.n : nullptr; });
+  };
+  const uint32_t rp = I::row_piece(lane), p0 = I::col_piece(lane, 0), p1 = I::col_piece(lane, 1);
+  if (k_begin < k_end) fetch(k_begin);
+  int buf = 0;
+  for (int k0 = k_begin; k0 < k_end; k0 += kKT, buf ^= 1) {
+    const uint32_t kimg = lds_addr(&lds[buf][0][0]), vimg = lds_addr(&lds[buf][1][0]);
+    sk.store(kimg);
+    sv.store(vimg);
+    __syncthreads();                             // (two buffers: a wavefront writes the next one only after all have left the one before)
+    if (k0 + kKT < k_end) fetch(k0 + kKT);
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      f32x16 s[2];
+#pragma unroll
+      for (int blk = 0; blk < 2; ++blk) {
+        s[blk] = zeros16();
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) s[blk] = T::mfma(I::row(kimg, rp, blk, ks), qf[rb][ks], s[blk]);
+      }
+      if (__any(end[rb] < k0 + kKT)) {
+#pragma unroll
+        for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int key = k0 + blk * 32 + (r & 3) + 8 * (r >> 2) + 4 * half;
+            s[blk][r] = key < end[rb] ? s[blk][r] : -INFINITY;
+          }
+      }
+      float mx = s[0][0];
+#pragma unroll
+      for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[blk][r]);
+      mx = both_halves_max(mx) * c2;             // (c2 > 0: checked on the host)
+      const float mn = fmaxf(m[rb], mx), mu = mn == -INFINITY ? 0.f : mn;
+      const float alpha = __builtin_amdgcn_exp2f(m[rb] - mu);
+      m[rb] = mn;
+      l[rb] *= alpha;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[rb][db][r] *= alpha;
+#pragma unroll
+      for (int blk = 0; blk < 2; ++blk) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[blk][r] = __builtin_amdgcn_exp2f(fmaf(s[blk][r], c2, -mu));
+          l[rb] += s[blk][r];
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          u32x4 p;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) p[j] = T::pack(s[blk][t * 8 + 2 * j], s[blk][t * 8 + 2 * j + 1]);
+#pragma unroll
+          for (int db = 0; db < DB; ++db) o[rb][db] = T::mfma(I::col(vimg, p0, p1, blk, t, db), p, o[rb][db]);
+        }
+      }
+    }
+  }
+  // lane = row: results of the row in registers, d = db * 32 + (r & 3) + 8 (r >> 2) + 4 half
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    const float sum = both_halves_sum(l[rb]);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    if (tok[rb] >= a.Nq) continue;
+    const int h = hk * a.G + hd[rb];
+    const int64_t at = (b * a.H + h) * a.Nq + tok[rb];
+    const float ls = sum == 0.f ? -INFINITY : (m[rb] + __builtin_amdgcn_logf(sum)) * kLn2;
+    if (a.splits > 1) {                          // this split's normalised result in 32 bits and its log sum exp
+      float* po = a.part + (static_cast<int64_t>(split) * a.B * a.H * a.Nq + at) * D;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<float4*>(po + db * 32 + 8 * g + 4 * half) =
+              make_float4(o[rb][db][4 * g] * inv, o[rb][db][4 * g + 1] * inv, o[rb][db][4 * g + 2] * inv, o[rb][db][4 * g + 3] * inv);
+      if (half == 0) a.part[static_cast<int64_t>(a.splits) * a.B * a.H * a.Nq * D + static_cast<int64_t>(split) * a.B * a.H * a.Nq + at] = ls;
+    } else {
+      uint16_t* po = a.o + b * a.vo.b + tok[rb] * a.vo.n + h * a.vo.h;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<uint2*>(po + db * 32 + 8 * g + 4 * half) =
+              pack4<T>(o[rb][db][4 * g] * inv, o[rb][db][4 * g + 1] * inv, o[rb][db][4 * g + 2] * inv, o[rb][db][4 * g + 3] * inv);
+      if (a.lse && half == 0) a.lse[at] = ls;
+    }
+  }
+}
+
+// Joins the splits of the keys: out = sum_s exp(lse_s - lse) out_s.  D / 4 threads per row.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void mha_join_kernel(const MhaArgs a) {
+  constexpr int TPR = D / 4;
+  const int64_t rows = a.B * a.H * a.Nq, at = static_cast<int64_t>(blockIdx.x) * (256 / TPR) + threadIdx.x / TPR;
+  if (at >= rows) return;
+  const int d4 = threadIdx.x % TPR;
+  const float* ls = a.part + static_cast<int64_t>(a.splits) * rows * D;
+  float m = -INFINITY;
+  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, ls[s * rows + at]);
+  const float mu = m == -INFINITY ? 0.f : m;
+  float sum = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < a.splits; ++s) {
+    const float e = __builtin_amdgcn_exp2f((ls[s * rows + at] - mu) * kLog2e);
+    const float4 v = *reinterpret_cast<const float4*>(a.part + (s * rows + at) * D + d4 * 4);
+    sum += e;
+    x[0] = fmaf(e, v.x, x[0]); x[1] = fmaf(e, v.y, x[1]); x[2] = fmaf(e, v.z, x[2]); x[3] = fmaf(e, v.w, x[3]);
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int64_t bh = at / a.Nq, b = bh / a.H;
+  const int i = static_cast<int>(at - bh * a.Nq), h = static_cast<int>(bh - b * a.H);
+  *reinterpret_cast<uint2*>(a.o + b * a.vo.b + i * a.vo.n + h * a.vo.h + d4 * 4) = pack4<T>(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+  if (a.lse && d4 == 0) a.lse[at] = sum == 0.f ? -INFINITY : mu + __builtin_amdgcn_logf(sum) * kLn2;
+}
+
+// ===================================================================================================================== backward
+// dq: workgroup = 4 wavefronts x 32 RB rows, over the keys [split * span, + span).  Also leaves D in dvec.
+template <typename T, int D, int RB>
+__global__ __launch_bounds__(256) void mha_dq_kernel(const MhaArgs a) {
+  using I = Image<D>;
+  constexpr int KS = I::KS, DB = I::DB, ROWS = 128 * RB;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[2][2][kKT * D * 2];        // [buffer][k, v]
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l32 = lane & 31, half = lane >> 5;
+  const int64_t per_b = static_cast<int64_t>(a.Hkv) * a.tiles * a.splits;
+  int64_t w = xcd_order(blockIdx.x, gridDim.x);
+  const int64_t b = w / per_b;
+  w -= b * per_b;
+  const int hk = static_cast<int>(w / (a.tiles * a.splits));
+  w -= static_cast<int64_t>(hk) * a.tiles * a.splits;
+  const int tile = a.tiles - 1 - static_cast<int>(w / a.splits), split = static_cast<int>(w % a.splits);
+  const Limits lim(a, b);
+  const int64_t R = static_cast<int64_t>(a.Nq) * a.G, row0 = static_cast<int64_t>(tile) * ROWS;
+  const uint16_t* qb = a.q + b * a.vq.b + static_cast<int64_t>(hk) * a.G * a.vq.h;
+  const uint16_t* ob = a.out + b * a.vo.b + static_cast<int64_t>(hk) * a.G * a.vo.h;
+  const uint16_t* gb = a.dout + b * a.vdo.b + static_cast<int64_t>(hk) * a.G * a.vdo.h;
+  const uint16_t* kb = a.k + b * a.vk.b + hk * a.vk.h;
+  const uint16_t* vb = a.v + b * a.vv.b + hk * a.vv.h;
+
+  int tok[RB], end[RB], hd[RB];
+  float lse2[RB], dd[RB];
+  u32x4 qf[RB][KS], gf[RB][KS];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    const int64_t r = row0 + wave * 32 * RB + rb * 32 + l32;
+    tok[rb] = r < R ? static_cast<int>(r / a.G) : a.Nq;
+    hd[rb] = r < R ? static_cast<int>(r - static_cast<int64_t>(tok[rb]) * a.G) : 0;
+    end[rb] = lim.end(tok[rb], a.causal);
+    const bool live = end[rb] > 0;               // a row without keys has no gradient
+    const int64_t i = live ? tok[rb] : 0, h = live ? hd[rb] : 0;
+    float part = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      qf[rb][ks] = gf[rb][ks] = u32x4{0, 0, 0, 0};
+      if (live) {
+        qf[rb][ks] = *reinterpret_cast<const u32x4*>(qb + i * a.vq.n + h * a.vq.h + ks * 16 + half * 8);
+        gf[rb][ks] = *reinterpret_cast<const u32x4*>(gb + i * a.vdo.n + h * a.vdo.h + ks * 16 + half * 8);
+        const u32x4 of = *reinterpret_cast<const u32x4*>(ob + i * a.vo.n + h * a.vo.h + ks * 16 + half * 8);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          part = fmaf(T::lo(gf[rb][ks][j]), T::lo(of[j]), fmaf(T::hi(gf[rb][ks][j]), T::hi(of[j]), part));
+      }
+    }
+    dd[rb] = both_halves_sum(part);
+    const int64_t at = (b * a.H + hk * a.G + hd[rb]) * a.Nq + tok[rb];
+    lse2[rb] = live ? a.lse[at] * kLog2e : INFINITY;                 // exp2(s - inf) = 0
+    if (split == 0 && half == 0 && tok[rb] < a.Nq) a.dvec[at] = dd[rb];
+  }
+  const int64_t last_row = (row0 + ROWS < R ? row0 + ROWS : R) - 1;
+  const int first_tok = static_cast<int>(row0 / a.G), last_tok = min(static_cast<int>(last_row / a.G), lim.q_len - 1);
+  const int k_begin = split * a.span;
+  const int k_end = min(first_tok <= last_tok ? lim.end(last_tok, a.causal) : 0, k_begin + a.span);
+
+  const float c2 = a.scale * kLog2e;
+  f32x16 dq[RB][DB];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+    for (int db = 0; db < DB; ++db) dq[rb][db] = zeros16();
+  Stage<D, kKT> sk, sv;
+  auto fetch = [&](int k0) {
+    sk.load([&](int row) { return k0 + row < lim.kv_len ? kb + (k0 + row) * a.vk.n : nullptr; });
+    sv.load([&](int row) { return k0 + row < lim.kv_len ? vb + (k0 + row) * a.vv.n : nullptr; });
+  };
+  const uint32_t rp = I::row_piece(lane), p0 = I::col_piece(lane, 0), p1 = I::col_piece(lane, 1);
+  if (k_begin < k_end) fetch(k_begin);
+  int buf = 0;
+  for (int k0 = k_begin; k0 < k_end; k0 += kKT, buf ^= 1) {
+    const uint32_t kimg = lds_addr(&lds[buf][0][0]), vimg = lds_addr(&lds[buf][1][0]);
+    sk.store(kimg);
+    sv.store(vimg);
+    __syncthreads();
+    if (k0 + kKT < k_end) fetch(k0 + kKT);
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      const bool masked = __any(end[rb] < k0 + kKT);
+#pragma unroll
+      for (int blk = 0; blk < 2; ++blk) {
+        f32x16 s = zeros16(), dp = zeros16();
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          s = T::mfma(I::row(kimg, rp, blk, ks), qf[rb][ks], s);
+          dp = T::mfma(I::row(vimg, rp, blk, ks), gf[rb][ks], dp);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, -lse2[rb])) * (dp[r] - dd[rb]);
+        if (masked) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int key = k0 + blk * 32 + (r & 3) + 8 * (r >> 2) + 4 * half;
+            s[r] = key < end[rb] ? s[r] : 0.f;
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          u32x4 p;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) p[j] = T::pack(s[t * 8 + 2 * j], s[t * 8 + 2 * j + 1]);
+#pragma unroll
+          for (int db = 0; db < DB; ++db) dq[rb][db] = T::mfma(I::col(kimg, p0, p1, blk, t, db), p, dq[rb][db]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    if (tok[rb] >= a.Nq) continue;
+    const int h = hk * a.G + hd[rb];
+    if (a.splits > 1) {
+      float* po = a.part + (static_cast<int64_t>(split) * a.B * a.H * a.Nq + (b * a.H + h) * a.Nq + tok[rb]) * D;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<float4*>(po + db * 32 + 8 * g + 4 * half) =
+              make_float4(dq[rb][db][4 * g], dq[rb][db][4 * g + 1], dq[rb][db][4 * g + 2], dq[rb][db][4 * g + 3]);
+    } else {
+      uint16_t* po = a.dq + b * a.vdq.b + tok[rb] * a.vdq.n + h * a.vdq.h;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<uint2*>(po + db * 32 + 8 * g + 4 * half) =
+              pack4<T>(dq[rb][db][4 * g] * a.scale, dq[rb][db][4 * g + 1] * a.scale, dq[rb][db][4 * g + 2] * a.scale, dq[rb][db][4 * g + 3] * a.scale);
+    }
+  }
+}
+
+// dq = scale * sum of the splits' partial sums, in their order
+template <typename T, int D>
+__global__ __launch_bounds__(256) void mha_dq_join_kernel(const MhaArgs a) {
+  constexpr int TPR = D / 4;
+  const int64_t rows = a.B * a.H * a.Nq, at = static_cast<int64_t>(blockIdx.x) * (256 / TPR) + threadIdx.x / TPR;
+  if (at >= rows) return;
+  const int d4 = threadIdx.x % TPR;
+  float x[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < a.splits; ++s) {
+    const float4 v = *reinterpret_cast<const float4*>(a.part + (s * rows + at) * D + d4 * 4);
+    x[0] += v.x; x[1] += v.y; x[2] += v.z; x[3] += v.w;
+  }
+  const int64_t bh = at / a.Nq, b = bh / a.H;
+  const int i = static_cast<int>(at - bh * a.Nq), h = static_cast<int>(bh - b * a.H);
+  *reinterpret_cast<uint2*>(a.dq + b * a.vdq.b + i * a.vdq.n + h * a.vdq.h + d4 * 4) =
+      pack4<T>(x[0] * a.scale, x[1] * a.scale, x[2] * a.scale, x[3] * a.scale);
+}
+
+// dk, dv: workgroup = 4 wavefronts x 32 KB keys of one key head, over the rows that see them, 64 at a time.
+template <typename T, int D, int KB>
+__global__ __launch_bounds__(256) void mha_dkv_kernel(const MhaArgs a) {
+  using I = Image<D>;
+  constexpr int KS = I::KS, DB = I::DB, KEYS = 128 * KB, RT = kKT;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[2][2][RT * D * 2];         // [buffer][q, dout]
+  __shared__ float stat[2][2][RT];                                                       // [buffer][lse log2(e), D]
+  __shared__ int row_end[2][RT];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l32 = lane & 31, half = lane >> 5;
+  const int64_t per_b = static_cast<int64_t>(a.Hkv) * a.tiles;
+  int64_t w = xcd_order(blockIdx.x, gridDim.x);
+  const int64_t b = w / per_b;
+  w -= b * per_b;
+  const int hk = static_cast<int>(w / a.tiles), tile = static_cast<int>(w - static_cast<int64_t>(hk) * a.tiles);
+  const Limits lim(a, b);
+  const int64_t R = static_cast<int64_t>(lim.q_len) * a.G;             // padded queries are no rows here
+  const uint16_t* qb = a.q + b * a.vq.b + static_cast<int64_t>(hk) * a.G * a.vq.h;
+  const uint16_t* gb = a.dout + b * a.vdo.b + static_cast<int64_t>(hk) * a.G * a.vdo.h;
+  const uint16_t* kb = a.k + b * a.vk.b + hk * a.vk.h;
+  const uint16_t* vb = a.v + b * a.vv.b + hk * a.vv.h;
+  const int key0 = tile * KEYS;
+  int key[KB];
+  u32x4 kf[KB][KS], vf[KB][KS];
+  f32x16 dk[KB][DB], dv[KB][DB];
+#pragma unroll
+  for (int n = 0; n < KB; ++n) {
+    key[n] = key0 + wave * 32 * KB + n * 32 + l32;
+    const bool live = key[n] < lim.kv_len;
+    const int64_t j = live ? key[n] : 0;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      kf[n][ks] = vf[n][ks] = u32x4{0, 0, 0, 0};
+      if (live) {
+        kf[n][ks] = *reinterpret_cast<const u32x4*>(kb + j * a.vk.n + ks * 16 + half * 8);
+        vf[n][ks] = *reinterpret_cast<const u32x4*>(vb + j * a.vv.n + ks * 16 + half * 8);
+      }
+    }
+#pragma unroll
+    for (int db = 0; db < DB; ++db) { dk[n][db] = zeros16(); dv[n][db] = zeros16(); }
+  }
+  // rows that see a key of this tile: all, or (causal) those from token key0 - off on
+  int64_t r_begin = a.causal ? static_cast<int64_t>(max(0, key0 - lim.off)) * a.G : 0;
+  r_begin -= r_begin % RT;
+  const int64_t r_end = key0 < lim.kv_len ? R : 0;
+  const float c2 = a.scale * kLog2e;
+  Stage<D, RT> sq, sg;
+  float st_l = 0.f, st_d = 0.f;
+  int st_e = 0;
+  auto fetch = [&](int64_t r0) {
+    auto at = [&](int row, const uint16_t* base, const View& v) -> const uint16_t* {
+      const int64_t r = r0 + row;
+      if (r >= R) return nullptr;
+      const int64_t i = a.G == 1 ? r : r / a.G;
+      return base + i * v.n + (r - i * a.G) * v.h;
+    };
+    sq.load([&](int row) { return at(row, qb, a.vq); });
+    sg.load([&](int row) { return at(row, gb, a.vdo); });
+    if (threadIdx.x < RT) {
+      const int64_t r = r0 + threadIdx.x;
+      st_l = INFINITY; st_d = 0.f; st_e = 0;
+      if (r < R) {
+        const int64_t i = r / a.G, s = (b * a.H + hk * a.G + (r - i * a.G)) * a.Nq + i;
+        st_e = lim.end(static_cast<int>(i), a.causal);
+        if (st_e > 0) { st_l = a.lse[s] * kLog2e; st_d = a.dvec[s]; }
+      }
+    }
+  };
+  const uint32_t rp = I::row_piece(lane), p0 = I::col_piece(lane, 0), p1 = I::col_piece(lane, 1);
+  if (r_begin < r_end) fetch(r_begin);
+  int buf = 0;
+  const int key_last = min(key0 + KEYS, lim.kv_len) - 1;
+  for (int64_t r0 = r_begin; r0 < r_end; r0 += RT, buf ^= 1) {
+    const uint32_t qimg = lds_addr(&lds[buf][0][0]), gimg = lds_addr(&lds[buf][1][0]);
+    sq.store(qimg);
+    sg.store(gimg);
+    if (threadIdx.x < RT) { stat[buf][0][threadIdx.x] = st_l; stat[buf][1][threadIdx.x] = st_d; row_end[buf][threadIdx.x] = st_e; }
+    __syncthreads();
+    if (r0 + RT < r_end) fetch(r0 + RT);
+    // a tile needs no mask if its first row (the one that sees least) sees the last key; keys beyond kv_len are zeros whose dk, dv are not kept
+    const bool masked = a.causal && row_end[buf][0] <= key_last;
+#pragma unroll
+    for (int blk = 0; blk < RT / 32; ++blk) {
+      u32x4 pf[KB][2], df[KB][2];
+#pragma unroll
+      for (int n = 0; n < KB; ++n) {
+        f32x16 s = zeros16(), dp = zeros16();
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          s = T::mfma(I::row(qimg, rp, blk, ks), kf[n][ks], s);
+          dp = T::mfma(I::row(gimg, rp, blk, ks), vf[n][ks], dp);
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float4 ll = *reinterpret_cast<const float4*>(&stat[buf][0][blk * 32 + 8 * g + 4 * half]);
+          const float4 dl = *reinterpret_cast<const float4*>(&stat[buf][1][blk * 32 + 8 * g + 4 * half]);
+          const float lv[4] = {ll.x, ll.y, ll.z, ll.w}, dv4[4] = {dl.x, dl.y, dl.z, dl.w};
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(s[4 * g + u], c2, -lv[u]));
+            s[4 * g + u] = p;
+            dp[4 * g + u] = p * (dp[4 * g + u] - dv4[u]);
+          }
+        }
+        if (masked) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int4 e4 = *reinterpret_cast<const int4*>(&row_end[buf][blk * 32 + 8 * g + 4 * half]);
+            const int ev[4] = {e4.x, e4.y, e4.z, e4.w};
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              s[4 * g + u] = key[n] < ev[u] ? s[4 * g + u] : 0.f;
+              dp[4 * g + u] = key[n] < ev[u] ? dp[4 * g + u] : 0.f;
+            }
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            pf[n][t][j] = T::pack(s[t * 8 + 2 * j], s[t * 8 + 2 * j + 1]);
+            df[n][t][j] = T::pack(dp[t * 8 + 2 * j], dp[t * 8 + 2 * j + 1]);
+          }
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+          const u32x4 gt = I::col(gimg, p0, p1, blk, t, db), qt = I::col(qimg, p0, p1, blk, t, db);
+#pragma unroll
+          for (int n = 0; n < KB; ++n) {
+            dv[n][db] = T::mfma(gt, pf[n][t], dv[n][db]);
+            dk[n][db] = T::mfma(qt, df[n][t], dk[n][db]);
+          }
+        }
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < KB; ++n) {
+    if (key[n] >= a.Nk) continue;
+    const bool live = key[n] < lim.kv_len;
+    uint16_t* pk = a.dk + b * a.vdk.b + key[n] * a.vdk.n + hk * a.vdk.h;
+    uint16_t* pv = a.dv + b * a.vdv.b + key[n] * a.vdv.n + hk * a.vdv.h;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        float x[4], y[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          x[u] = live ? dk[n][db][4 * g + u] * a.scale : 0.f;
+          y[u] = live ? dv[n][db][4 * g + u] : 0.f;
+        }
+        *reinterpret_cast<uint2*>(pk + db * 32 + 8 * g + 4 * half) = pack4<T>(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<uint2*>(pv + db * 32 + 8 * g + 4 * half) = pack4<T>(y[0], y[1], y[2], y[3]);
+      }
+  }
+}
+
+// ===================================================================================================================== host
+constexpr int kRB = 1, kKB = 1;                  // 32-row (32-key) blocks of a wavefront
+
+// Splits of the keys for `groups` workgroups over Nk keys: enough to give the chip two workgroups per CU, at least 256 keys each.
+int splits_for(int64_t groups, int32_t Nk) {
+  if (groups <= 0 || groups >= 256) return 1;
+  int64_t s = (512 + groups - 1) / groups;
+  const int64_t most = (Nk + 255) / 256;
+  if (s > most) s = most;
+  if (s > 64) s = 64;
+  return s < 1 ? 1 : static_cast<int>(s);
+}
+int64_t row_tiles(int64_t Nq, int64_t G) { return (Nq * G + 128 * kRB - 1) / (128 * kRB); }
+
+int check_args(const MhaArgs& a, int dtype, int32_t head_dim) {
+  if (a.B < 0 || a.Nq < 0 || a.Nk < 0 || a.H < 1 || a.Hkv < 1) return APGD_ERR_SIZE;
+  if (a.H % a.Hkv) return APGD_ERR_ARG;
+  if (!cnx_mha_supported(head_dim)) return APGD_ERR_ARG;
+  if (dtype != APGD_BF16 && dtype != APGD_F16) return APGD_ERR_DTYPE;
+  if (!(a.scale >= 1e-30f) || a.scale > 1e30f) return APGD_ERR_ARG;
+  const int64_t G = a.H / a.Hkv;
+  // row numbers in 31 bits, threads of a launch in 32
+  if (a.Nq * G > 0x7fffffffLL - 1024 || a.Nk > 0x7fffffff - 1024) return APGD_ERR_SIZE;
+  const int64_t tiles = row_tiles(a.Nq, G) > (a.Nk + 127) / 128 ? row_tiles(a.Nq, G) : (a.Nk + 127) / 128;
+  if (a.B > 0 && tiles > 0 && a.B > (1LL << 23) / tiles / a.H) return APGD_ERR_SIZE;
+  return APGD_OK;
+}
+void cut(MhaArgs& a, int64_t tiles, bool split) {
+  a.tiles = static_cast<int32_t>(tiles);
+  a.splits = split ? splits_for(a.B * a.Hkv * tiles, a.Nk) : 1;
+  const int64_t per = ((a.Nk + a.splits - 1) / a.splits + kKT - 1) / kKT * kKT;
+  a.span = static_cast<int32_t>(per < kKT ? kKT : per);
+}
+
+template <typename T, int D>
+int launch_fwd(MhaArgs& a, hipStream_t s) {
+  cut(a, row_tiles(a.Nq, a.G), true);
+  hipLaunchKernelGGL((mha_fwd_kernel<T, D, kRB>), dim3(static_cast<unsigned>(a.B * a.Hkv * a.tiles * a.splits)), dim3(256), 0, s, a);
+  if (a.splits > 1)
+    hipLaunchKernelGGL((mha_join_kernel<T, D>), dim3(static_cast<unsigned>((a.B * a.H * a.Nq * (D / 4) + 255) / 256)), dim3(256), 0, s, a);
+  return launch_status();
+}
+template <typename T, int D>
+int launch_bwd(MhaArgs& a, hipStream_t s) {
+  if (a.Nq > 0) {
+    cut(a, row_tiles(a.Nq, a.G), true);
+    hipLaunchKernelGGL((mha_dq_kernel<T, D, kRB>), dim3(static_cast<unsigned>(a.B * a.Hkv * a.tiles * a.splits)), dim3(256), 0, s, a);
+    if (a.splits > 1)
+      hipLaunchKernelGGL((mha_dq_join_kernel<T, D>), dim3(static_cast<unsigned>((a.B * a.H * a.Nq * (D / 4) + 255) / 256)), dim3(256), 0, s, a);
+  }
+  if (a.Nk > 0) {
+    cut(a, (a.Nk + 128 * kKB - 1) / (128 * kKB), false);
+    hipLaunchKernelGGL((mha_dkv_kernel<T, D, kKB>), dim3(static_cast<unsigned>(a.B * a.Hkv * a.tiles)), dim3(256), 0, s, a);
+  }
+  return launch_status();
+}
+
+View view_of(const int64_t* s) { return View{s[0], s[1], s[2]}; }
+
+}  // namespace
+
+extern "C" {
+
+int cnx_mha_supported(int32_t head_dim) { return head_dim == 64 || head_dim == 128; }
+
+int64_t cnx_mha_ws_floats(int64_t B, int32_t Nq, int32_t Nk, int32_t H, int32_t Hkv, int32_t head_dim) {
+  if (B <= 0 || Nq <= 0 || Nk <= 0 || H < 1 || Hkv < 1 || H % Hkv || !cnx_mha_supported(head_dim)) return 0;
+  const int64_t tiles = row_tiles(Nq, H / Hkv);
+  if (B > INT64_MAX / Hkv / tiles) return 0;
+  const int s = splits_for(B * Hkv * tiles, Nk);
+  return s > 1 ? static_cast<int64_t>(s) * B * H * Nq * (head_dim + 1) : 0;
+}
+
+int cnx_mha_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const int32_t* q_lens, const int32_t* kv_lens, float* ws,
+                const int64_t* strides, int dtype, int64_t B, int32_t Nq, int32_t Nk, int32_t H, int32_t Hkv, int32_t head_dim,
+                int32_t causal, float scale, void* stream) {
+  MhaArgs a = {};
+  a.q = static_cast<const uint16_t*>(q); a.k = static_cast<const uint16_t*>(k); a.v = static_cast<const uint16_t*>(v);
+  a.o = static_cast<uint16_t*>(out); a.lse = lse; a.part = ws; a.q_lens = q_lens; a.kv_lens = kv_lens;
+  a.B = B; a.Nq = Nq; a.Nk = Nk; a.H = H; a.Hkv = Hkv; a.causal = causal != 0; a.scale = scale;
+  if (const int rc = check_args(a, dtype, head_dim)) return rc;
+  if (B == 0 || Nq == 0) return APGD_OK;
+  a.G = H / Hkv;
+  if (!strides || !q || !out || (Nk > 0 && (!k || !v))) return APGD_ERR_NULL;
+  if (cnx_mha_ws_floats(B, Nq, Nk, H, Hkv, head_dim) > 0 && !ws) return APGD_ERR_NULL;
+  a.vq = view_of(strides); a.vk = view_of(strides + 3); a.vv = view_of(strides + 6); a.vo = view_of(strides + 9);
+  hipStream_t s = as_stream(stream);
+  if (dtype == APGD_BF16) return head_dim == 64 ? launch_fwd<Bf16, 64>(a, s) : launch_fwd<Bf16, 128>(a, s);
+  return head_dim == 64 ? launch_fwd<Fp16, 64>(a, s) : launch_fwd<Fp16, 128>(a, s);
+}
+
+int cnx_mha_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse, void* dq, void* dk, void* dv,
+                float* dvec, const int32_t* q_lens, const int32_t* kv_lens, float* ws, const int64_t* strides, int dtype, int64_t B,
+                int32_t Nq, int32_t Nk, int32_t H, int32_t Hkv, int32_t head_dim, int32_t causal, float scale, void* stream) {
+  MhaArgs a = {};
+  a.q = static_cast<const uint16_t*>(q); a.k = static_cast<const uint16_t*>(k); a.v = static_cast<const uint16_t*>(v);
+  a.out = static_cast<const uint16_t*>(out); a.dout = static_cast<const uint16_t*>(dout); a.lse = const_cast<float*>(lse);
+  a.dq = static_cast<uint16_t*>(dq); a.dk = static_cast<uint16_t*>(dk); a.dv = static_cast<uint16_t*>(dv); a.dvec = dvec;
+  a.part = ws; a.q_lens = q_lens; a.kv_lens = kv_lens;
+  a.B = B; a.Nq = Nq; a.Nk = Nk; a.H = H; a.Hkv = Hkv; a.causal = causal != 0; a.scale = scale;
+  if (const int rc = check_args(a, dtype, head_dim)) return rc;
+  if (B == 0 || (Nq == 0 && Nk == 0)) return APGD_OK;
+  a.G = H / Hkv;
+  if (!strides || (Nq > 0 && (!q || !out || !dout || !lse || !dq || !dvec)) || (Nk > 0 && (!k || !v || !dk || !dv))) return APGD_ERR_NULL;
+  if (cnx_mha_ws_floats(B, Nq, Nk, H, Hkv, head_dim) > 0 && !ws) return APGD_ERR_NULL;
+  a.vq = view_of(strides); a.vk = view_of(strides + 3); a.vv = view_of(strides + 6); a.vo = view_of(strides + 9); a.vdo = view_of(strides + 12);
+  a.vdq = view_of(strides + 15); a.vdk = view_of(strides + 18); a.vdv = view_of(strides + 21);
+  hipStream_t s = as_stream(stream);
+  if (dtype == APGD_BF16) return head_dim == 64 ? launch_bwd<Bf16, 64>(a, s) : launch_bwd<Bf16, 128>(a, s);
+  return head_dim == 64 ? launch_bwd<Fp16, 64>(a, s) : launch_bwd<Fp16, 128>(a, s);
+}
+
+}  // extern "C"

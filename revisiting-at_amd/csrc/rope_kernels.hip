@@ -1,0 +1,407 @@
+// rope_kernels.hip — per-head RMS norm of queries and keys and their rotation by positions, one pass each way, for gfx950.
+//
+//   forward   z = x * r * w,  r = (mean(x^2) + eps)^-1/2 over the d values of a head;   y = R(angle) z
+//   backward  dz = R(angle)^T dy;  dw = sum dz * (x r);  dx = r (dz w - (x r) mean(dz w * (x r)))
+// with R the rotation of pair i (dims (i, i + d/2), or (2i, 2i + 1) interleaved) by angle = position[axis(i)] * inv_freq[i]: `sections`
+// gives each axis (time, height, width, ...) its run of pairs.
+//
+// The pass is bound by memory: d values in and out per head, a few operations each.  Layout: a thread owns 8 pairs = 16 values of one
+// head (two 16-byte pieces in 16-bit types), a group of 1, 2, 4, 8 or 16 lanes one head, so the mean of squares is at most four lane
+// exchanges and nothing of a head leaves its group.  The angles belong to a token, not to a head: the workgroup computes the cosines and
+// sines of its tokens once, into LDS, and all heads of q and k read them there.  Angles are products in 64 bits brought to (-1/2, 1/2]
+// turns before they are rounded to 32 (a position of 10^6 at frequency 1 would be off by 0.03 rad in 32 bits).  x r is computed again in the
+// backward instead of kept: it is in registers anyway and would cost as much memory as x.
+// Sums (mean of squares, weight gradients) in 32 bits; one rounding to the output's type at the end.
+#include <hip/hip_fp16.h>
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "apgd_hip.h"
+#include "convnext_hip.h"
+
+namespace {
+
+inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
+inline int launch_status() { return static_cast<int>(hipGetLastError()); }
+
+constexpr int kMaxAxes = 4;
+constexpr int kMaxHead = 256;
+constexpr int kTokens = 8;                      // tokens of a workgroup's tile at most
+constexpr int kFwdGrid = 1 << 20;                // workgroups of the forward at most (they step over the rest)
+constexpr int kBwdGrid = 1024;                  // workgroups (a side) of the backward at most: each leaves one row of partial weight gradients
+
+struct View {                                   // [B, N, H, d] with unit stride in d
+  int64_t b, n, h;
+};
+
+struct Side {                                   // the queries' or the keys' tensors
+  const void *x, *dy;                           // input; backward: the output's gradient
+  void* o;                                      // forward: y; backward: dx
+  const void* w;                                // [d] or NULL
+  View vx, vdy, vo;
+  int32_t heads;
+};
+
+struct RopeArgs {
+  Side q, k;
+  const void* pos;                              // [(B,) N, axes] or NULL
+  const float* inv_freq;                        // [d / 2]
+  float* part;                                  // backward: [2][gridDim.x][d] partial weight gradients or NULL
+  int64_t pos_b;                                // elements between the samples' positions (0: shared)
+  int64_t tokens, N;                            // tokens = B * N
+  int32_t first1, first2, first3;               // first pair of the second, third and fourth axis (d / 2 where there is none)
+  int32_t axes, d, tile, w_dtype, pos_dtype, norm;
+  float eps;
+};
+
+struct bf16_t { uint16_t u; };
+
+template <typename T> struct Io;
+template <> struct Io<float> {
+  static __device__ __forceinline__ void load8(const float* p, float* x) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  }
+  static __device__ __forceinline__ void store8(float* p, const float* x) {
+    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+  }
+};
+template <> struct Io<bf16_t> {
+  typedef __attribute__((ext_vector_type(8))) __bf16 v8;
+  static __device__ __forceinline__ void load8(const bf16_t* p, float* x) {
+    const uint4 a = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+  static __device__ __forceinline__ void store8(bf16_t* p, const float* x) {
+    v8 v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = static_cast<__bf16>(x[i]);
+    *reinterpret_cast<v8*>(p) = v;
+  }
+};
+template <> struct Io<__half> {
+  typedef __attribute__((ext_vector_type(8))) _Float16 v8;
+  static __device__ __forceinline__ void load8(const __half* p, float* x) {
+    const v8 v = *reinterpret_cast<const v8*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(v[i]);
+  }
+  static __device__ __forceinline__ void store8(__half* p, const float* x) {
+    v8 v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = static_cast<_Float16>(x[i]);
+    *reinterpret_cast<v8*>(p) = v;
+  }
+};
+
+// the 16 values of a thread: a = first members of its 8 pairs, b = second members
+template <bool IL, typename T>
+__device__ __forceinline__ void load_pairs(const T* head, int j, int d, float* a, float* b) {
+  if constexpr (IL) {
+    float t[16];
+    Io<T>::load8(head + 16 * j, t);
+    Io<T>::load8(head + 16 * j + 8, t + 8);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { a[i] = t[2 * i]; b[i] = t[2 * i + 1]; }
+  } else {
+    Io<T>::load8(head + 8 * j, a);
+    Io<T>::load8(head + d / 2 + 8 * j, b);
+  }
+}
+template <bool IL, typename T>
+__device__ __forceinline__ void store_pairs(T* head, int j, int d, const float* a, const float* b) {
+  if constexpr (IL) {
+    float t[16];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { t[2 * i] = a[i]; t[2 * i + 1] = b[i]; }
+    Io<T>::store8(head + 16 * j, t);
+    Io<T>::store8(head + 16 * j + 8, t + 8);
+  } else {
+    Io<T>::store8(head + 8 * j, a);
+    Io<T>::store8(head + d / 2 + 8 * j, b);
+  }
+}
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(bf16_t x) { return __uint_as_float(static_cast<uint32_t>(x.u) << 16); }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+template <typename T>
+__device__ __forceinline__ float weight_at(const void* w, int dtype, int at) {
+  if (!w) return 1.f;
+  if (dtype == APGD_F32) return static_cast<const float*>(w)[at];
+  return to_f32(static_cast<const T*>(w)[at]);
+}
+
+// sum over the lanes of a group (a power of two; every lane of the wavefront is here)
+__device__ __forceinline__ float group_sum(float v, int group) {
+  for (int m = 1; m < group; m <<= 1) v += __shfl_xor(v, m, 64);
+  return v;
+}
+
+// cosines and sines of the tile's tokens: cs[t][pair]
+__device__ __forceinline__ void tile_angles(const RopeArgs& a, int64_t t0, int nt, float2* cs) {
+  const int pairs = a.d >> 1;
+  for (int e = threadIdx.x; e < nt * pairs; e += blockDim.x) {
+    const int t = e / pairs, i = e - t * pairs;
+    const int axis = (i >= a.first1) + (i >= a.first2) + (i >= a.first3);
+    const int64_t tok = t0 + t, b = tok / a.N, n = tok - b * a.N;
+    const int64_t at = b * a.pos_b + n * a.axes + axis;
+    double p;
+    if (a.pos_dtype == CNX_POS_F32) p = static_cast<const float*>(a.pos)[at];
+    else if (a.pos_dtype == CNX_POS_I32) p = static_cast<const int32_t*>(a.pos)[at];
+    else p = static_cast<double>(static_cast<const int64_t*>(a.pos)[at]);
+    const double turns = p * static_cast<double>(a.inv_freq[i]) * 0.15915494309189535;      // 1 / (2 pi)
+    const float f = static_cast<float>(turns - rint(turns));
+    cs[t * pairs + i] = make_float2(cospif(2.f * f), sinpif(2.f * f));
+  }
+}
+
+// blockIdx.y: 0 = queries, 1 = keys (so that a thread holds one side's weights and sums: 16 + 16 registers instead of 32 + 32)
+template <typename T, bool BWD, bool IL>
+__global__ __launch_bounds__(256, BWD ? 3 : 4) void qk_norm_rope_kernel(const RopeArgs a) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds_raw[];
+  float2* cs = reinterpret_cast<float2*>(lds_raw);                    // [tile][d / 2]
+  const Side z = blockIdx.y ? a.k : a.q;
+  const int d = a.d, pairs = d >> 1, tph = d >> 4;                    // tph: threads that hold a head
+  int group = 1;
+  while (group < tph) group <<= 1;
+  const int j = threadIdx.x & (group - 1), g0 = threadIdx.x / group, ngroups = 256 / group;
+  const bool here = j < tph;                                          // d / 16 is no power of two: the group's last lanes idle
+  const int jj = here ? j : 0;
+  const float rd = 1.f / static_cast<float>(d);
+  float wa[8], wb[8], sa[8], sb[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int ia = IL ? 16 * jj + 2 * i : 8 * jj + i, ib = IL ? ia + 1 : ia + pairs;
+    wa[i] = weight_at<T>(z.w, a.w_dtype, ia);
+    wb[i] = weight_at<T>(z.w, a.w_dtype, ib);
+    sa[i] = sb[i] = 0.f;                                              // BWD: weight gradients of this thread's dims
+  }
+
+  for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.tile; t0 < a.tokens; t0 += static_cast<int64_t>(gridDim.x) * a.tile) {
+    const int nt = static_cast<int>(a.tokens - t0 < a.tile ? a.tokens - t0 : a.tile);
+    if (a.pos) {
+      __syncthreads();                                                // the last tile's readers are done
+      tile_angles(a, t0, nt, cs);
+      __syncthreads();
+    }
+    const int items = nt * z.heads;
+    for (int it0 = 0; it0 < items; it0 += ngroups) {                  // (uniform trip count: the lane exchanges need whole wavefronts)
+      const int it = it0 + g0;
+      const bool live = here && it < items;
+      const int itc = it < items ? it : items - 1;
+      const int t = itc / z.heads, h = itc - t * z.heads;
+      const int64_t tok = t0 + t, b = tok / a.N, n = tok - b * a.N;
+      float xa[8], xb[8], ga[8], gb[8], c[8], s[8];
+      if (!BWD || a.norm)
+        load_pairs<IL>(static_cast<const T*>(z.x) + b * z.vx.b + n * z.vx.n + h * z.vx.h, jj, d, xa, xb);
+      if constexpr (BWD)
+        load_pairs<IL>(static_cast<const T*>(z.dy) + b * z.vdy.b + n * z.vdy.n + h * z.vdy.h, jj, d, ga, gb);
+      T* o = static_cast<T*>(z.o) + b * z.vo.b + n * z.vo.n + h * z.vo.h;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 v = a.pos ? cs[t * pairs + 8 * jj + i] : make_float2(1.f, 0.f);
+        c[i] = v.x; s[i] = v.y;
+      }
+      if (a.norm) {                                                   // x -> x r
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss = fmaf(xa[i], xa[i], fmaf(xb[i], xb[i], ss));
+        ss = group_sum(here ? ss : 0.f, group);
+        const float r = 1.f / sqrtf(ss * rd + a.eps);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { xa[i] *= r; xb[i] *= r; }
+        if constexpr (BWD) {
+          float dot = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {                               // the rotation's transpose, then the norm's
+            const float u = fmaf(ga[i], c[i], gb[i] * s[i]), v = fmaf(gb[i], c[i], -ga[i] * s[i]);
+            const float ta = u * xa[i], tb = v * xb[i];
+            sa[i] += live ? ta : 0.f;
+            sb[i] += live ? tb : 0.f;
+            dot = fmaf(ta, wa[i], fmaf(tb, wb[i], dot));
+            ga[i] = u * wa[i];
+            gb[i] = v * wb[i];
+          }
+          dot = group_sum(here ? dot : 0.f, group) * rd;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            ga[i] = r * fmaf(-xa[i], dot, ga[i]);
+            gb[i] = r * fmaf(-xb[i], dot, gb[i]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) { xa[i] *= wa[i]; xb[i] *= wb[i]; }
+        }
+      } else if constexpr (BWD) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float u = fmaf(ga[i], c[i], gb[i] * s[i]);
+          gb[i] = fmaf(gb[i], c[i], -ga[i] * s[i]);
+          ga[i] = u;
+        }
+      }
+      if constexpr (!BWD) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          ga[i] = fmaf(xa[i], c[i], -xb[i] * s[i]);
+          gb[i] = fmaf(xb[i], c[i], xa[i] * s[i]);
+        }
+      }
+      if (live) store_pairs<IL>(o, j, d, ga, gb);
+    }
+  }
+  if constexpr (BWD) {
+    if (a.part) {                                                     // (uniform) the workgroup's sums, in the order of its wavefronts
+      float* red = reinterpret_cast<float*>(lds_raw);                 // [4 wavefronts][d]
+      __syncthreads();
+      const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        for (int m = group; m < 64; m <<= 1) {
+          sa[i] += __shfl_xor(sa[i], m, 64);
+          sb[i] += __shfl_xor(sb[i], m, 64);
+        }
+        if (lane < group && here) {
+          const int ia = IL ? 16 * j + 2 * i : 8 * j + i, ib = IL ? ia + 1 : ia + pairs;
+          red[wave * d + ia] = sa[i];
+          red[wave * d + ib] = sb[i];
+        }
+      }
+      __syncthreads();
+      for (int e = threadIdx.x; e < d; e += 256)
+        a.part[(static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * d + e] = ((red[e] + red[d + e]) + red[2 * d + e]) + red[3 * d + e];
+    }
+  }
+}
+
+// dw[e] = sum over the workgroups' rows, in a fixed order: 16 columns x 16 row lanes, every lane its rows one after the other
+__global__ __launch_bounds__(256) void rope_dw_kernel(const float* __restrict__ part, int rows, int d, float* __restrict__ dwq,
+                                                      float* __restrict__ dwk) {
+  __shared__ float red[16][17];
+  float* dw = blockIdx.y ? dwk : dwq;
+  const int col = threadIdx.x & 15, row = threadIdx.x >> 4, e = blockIdx.x * 16 + col;        // d is a multiple of 16
+  float s = 0.f;
+  for (int r = row; r < rows; r += 16) s += part[(static_cast<int64_t>(blockIdx.y) * rows + r) * d + e];
+  red[row][col] = s;
+  __syncthreads();
+  if (row == 0 && dw) {
+    s = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s += red[r][col];
+    dw[e] = s;
+  }
+}
+
+int check_args(RopeArgs& a, int dtype, const int32_t* sections, int64_t B, int64_t N, int32_t Hq, int32_t Hk, int32_t d) {
+  if (B < 0 || N < 0 || Hq < 0 || Hk < 0 || Hq > (1 << 20) || Hk > (1 << 20)) return APGD_ERR_SIZE;
+  if (!cnx_qk_norm_rope_supported(d)) return APGD_ERR_ARG;
+  if (dtype != APGD_F32 && dtype != APGD_BF16 && dtype != APGD_F16) return APGD_ERR_DTYPE;
+  if ((a.q.w || a.k.w) && a.w_dtype != APGD_F32 && a.w_dtype != dtype) return APGD_ERR_DTYPE;
+  if (N > 0 && B > INT64_MAX / N) return APGD_ERR_SIZE;
+  if (a.pos) {
+    if (!a.inv_freq || !sections) return APGD_ERR_NULL;
+    if (a.pos_dtype != CNX_POS_F32 && a.pos_dtype != CNX_POS_I32 && a.pos_dtype != CNX_POS_I64) return APGD_ERR_DTYPE;
+    if (a.axes < 1 || a.axes > kMaxAxes) return APGD_ERR_ARG;
+    int32_t first[kMaxAxes + 1] = {0, d / 2, d / 2, d / 2, d / 2};
+    for (int i = 0; i < a.axes; ++i) {
+      if (sections[i] < 0 || sections[i] > d) return APGD_ERR_ARG;
+      first[i + 1] = first[i] + sections[i];
+    }
+    if (first[a.axes] != d / 2) return APGD_ERR_ARG;
+    a.first1 = first[1]; a.first2 = first[2]; a.first3 = first[3];
+  }
+  a.tokens = B * N;
+  a.N = N;
+  a.q.heads = Hq; a.k.heads = Hk; a.d = d;
+  return APGD_OK;
+}
+
+template <bool BWD, bool IL>
+void launch(const RopeArgs& a, int dtype, unsigned grid, hipStream_t s) {
+  const size_t lds = static_cast<size_t>(a.tile > 4 || !BWD ? a.tile : 4) * a.d * 4;        // tile x d / 2 (cos, sin); BWD: 4 x d sums
+  const dim3 blocks(grid, 2);
+  if (dtype == APGD_F32) hipLaunchKernelGGL((qk_norm_rope_kernel<float, BWD, IL>), blocks, dim3(256), lds, s, a);
+  else if (dtype == APGD_BF16) hipLaunchKernelGGL((qk_norm_rope_kernel<bf16_t, BWD, IL>), blocks, dim3(256), lds, s, a);
+  else hipLaunchKernelGGL((qk_norm_rope_kernel<__half, BWD, IL>), blocks, dim3(256), lds, s, a);
+}
+template <bool BWD>
+void launch(const RopeArgs& a, int dtype, bool interleaved, unsigned grid, hipStream_t s) {
+  if (interleaved) launch<BWD, true>(a, dtype, grid, s);
+  else launch<BWD, false>(a, dtype, grid, s);
+}
+
+// Tokens per workgroup: kTokens where that leaves the chip 512 workgroups a side or more, else fewer (a single token per workgroup for the
+// smallest calls, whose time is one pass through the kernel).
+int tile_for(int64_t tokens) {
+  int t = kTokens;
+  while (t > 1 && (tokens + t - 1) / t < 512) t >>= 1;
+  return t;
+}
+
+View view_of(const int64_t* s) { return View{s[0], s[1], s[2]}; }
+
+}  // namespace
+
+extern "C" {
+
+int cnx_qk_norm_rope_supported(int32_t d) { return d >= 16 && d <= kMaxHead && d % 16 == 0; }
+
+int64_t cnx_qk_norm_rope_ws_floats(int32_t d) { return cnx_qk_norm_rope_supported(d) ? static_cast<int64_t>(kBwdGrid) * 2 * d : 0; }
+
+int cnx_qk_norm_rope_fwd(const void* q, const void* k, void* yq, void* yk, int dtype, const int64_t* strides, const void* wq, const void* wk,
+                         int w_dtype, const void* positions, int pos_dtype, int64_t pos_batch_stride, int32_t axes, const int32_t* sections,
+                         const float* inv_freq, int64_t B, int64_t N, int32_t Hq, int32_t Hk, int32_t d, float eps, int32_t norm,
+                         int32_t interleaved, void* stream) {
+  RopeArgs a = {};
+  a.q.x = q; a.k.x = k; a.q.o = yq; a.k.o = yk;
+  a.q.w = wq; a.k.w = wk; a.w_dtype = w_dtype;
+  a.pos = positions; a.pos_dtype = pos_dtype; a.pos_b = pos_batch_stride; a.axes = axes; a.inv_freq = inv_freq;
+  a.norm = norm != 0; a.eps = eps;
+  if (const int rc = check_args(a, dtype, sections, B, N, Hq, Hk, d)) return rc;
+  if (a.tokens == 0 || Hq + Hk == 0) return APGD_OK;
+  if (!strides || (Hq && (!q || !yq)) || (Hk && (!k || !yk))) return APGD_ERR_NULL;
+  a.q.vx = view_of(strides); a.k.vx = view_of(strides + 3); a.q.vo = view_of(strides + 6); a.k.vo = view_of(strides + 9);
+  a.tile = tile_for(a.tokens);
+  const int64_t grid = (a.tokens + a.tile - 1) / a.tile;
+  launch<false>(a, dtype, interleaved != 0, static_cast<unsigned>(grid < kFwdGrid ? grid : kFwdGrid), as_stream(stream));
+  return launch_status();
+}
+
+int cnx_qk_norm_rope_bwd(const void* dyq, const void* dyk, const void* q, const void* k, void* dq, void* dk, float* dwq, float* dwk, float* ws,
+                         int dtype, const int64_t* strides, const void* wq, const void* wk, int w_dtype, const void* positions, int pos_dtype,
+                         int64_t pos_batch_stride, int32_t axes, const int32_t* sections, const float* inv_freq, int64_t B, int64_t N,
+                         int32_t Hq, int32_t Hk, int32_t d, float eps, int32_t norm, int32_t interleaved, void* stream) {
+  RopeArgs a = {};
+  a.q.x = q; a.k.x = k; a.q.dy = dyq; a.k.dy = dyk; a.q.o = dq; a.k.o = dk;
+  a.q.w = wq; a.k.w = wk; a.w_dtype = w_dtype;
+  a.pos = positions; a.pos_dtype = pos_dtype; a.pos_b = pos_batch_stride; a.axes = axes; a.inv_freq = inv_freq;
+  a.norm = norm != 0; a.eps = eps;
+  if (const int rc = check_args(a, dtype, sections, B, N, Hq, Hk, d)) return rc;
+  const bool want_w = a.norm && (dwq || dwk);
+  if (want_w && !ws) return APGD_ERR_NULL;
+  unsigned grid = 0;
+  if (a.tokens == 0 || Hq + Hk == 0) {
+    if (!want_w) return APGD_OK;                                      // else: the weights' gradients are zeros
+  } else {
+    if (!strides || (Hq && (!dyq || !dq || (norm && !q))) || (Hk && (!dyk || !dk || (norm && !k)))) return APGD_ERR_NULL;
+    a.q.vdy = view_of(strides); a.k.vdy = view_of(strides + 3); a.q.vx = view_of(strides + 6); a.k.vx = view_of(strides + 9);
+    a.q.vo = view_of(strides + 12); a.k.vo = view_of(strides + 15);
+    a.part = want_w ? ws : nullptr;
+    a.tile = tile_for(a.tokens);
+    const int64_t tiles = (a.tokens + a.tile - 1) / a.tile;
+    grid = static_cast<unsigned>(tiles < kBwdGrid ? tiles : kBwdGrid);
+    launch<true>(a, dtype, interleaved != 0, grid, as_stream(stream));
+  }
+  if (want_w)
+    hipLaunchKernelGGL(rope_dw_kernel, dim3(static_cast<unsigned>(d / 16), 2), dim3(256), 0, as_stream(stream), ws, static_cast<int>(grid), d, dwq, dwk);
+  return launch_status();
+}
+
+}  // extern "C"

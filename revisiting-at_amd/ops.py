@@ -15,6 +15,7 @@ The residual stream stays fp32 exactly as in the reference's autocast run (``gam
 from __future__ import annotations
 
 import contextlib
+import ctypes
 import math
 import os
 import weakref
@@ -1971,6 +1972,343 @@ def attention(qkv, num_heads, scale):
     q, k, v = qkv.reshape(B, N, 3, num_heads, C // num_heads).permute(2, 0, 3, 1, 4).unbind(0)
     a = ((q @ k.transpose(-2, -1)) * scale).softmax(dim=-1)
     return (a @ v).transpose(1, 2).reshape(B, N, C)
+
+
+# ------------------------------------------------------------------------------ heads: norm and rotation
+def _on_device(t):
+    """Context in which kernels on ``t`` are launched: its own device, also where another one is current."""
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _check_heads(what, *named):
+    """``named``: (name, tensor or None) - device tensors [B, N, H, d] of one type on one device."""
+    first = named[0][1]
+    for name, t in named:
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{what}: {name} has to be a tensor, not {type(t).__name__}")
+        if t.dim() != 4:
+            raise ValueError(f"{what}: {name} has to be [batch, tokens, heads, head_dim], not {tuple(t.shape)}")
+        if t.dtype != first.dtype:
+            raise TypeError(f"{what}: {name} is {t.dtype}, {named[0][0]} {first.dtype}")
+        if not t.is_cuda:
+            raise _lib.ApgdHipError(f"{what}: {name} has to be a device tensor (no CPU path in the product)")
+        if t.device != first.device:
+            raise ValueError(f"{what}: {name} is on {t.device}, {named[0][0]} on {first.device}")
+        if t.shape[0] != first.shape[0] or t.shape[3] != first.shape[3]:
+            raise ValueError(f"{what}: {name} {tuple(t.shape)} does not go with {named[0][0]} {tuple(first.shape)}")
+
+
+def _head_rows(t):
+    """``t`` [B, N, H, d] itself where the kernels can read it in place (contiguous heads that begin at 16 bytes, any other strides, a
+    stride of zero included), else a contiguous copy."""
+    piece = 16 // t.element_size()
+    st = t.stride()
+    if st[3] == 1 and st[0] % piece == 0 and st[1] % piece == 0 and st[2] % piece == 0 and t.data_ptr() % 16 == 0:
+        return t
+    return torch.empty(t.shape, device=t.device, dtype=t.dtype).copy_(t)
+
+
+def _strides(*tensors):
+    """(sample, token, head) strides of [B, N, H, d] tensors as one host array of the C ABI."""
+    v = [s for t in tensors for s in t.stride()[:3]]
+    return (ctypes.c_int64 * len(v))(*v)
+
+
+class _Rotation:
+    """Checked arguments of the rotation and the norm, as the C entry points take them."""
+    __slots__ = ("positions", "inv_freq", "sections", "axes", "code", "batch_stride", "eps", "norm", "interleaved")
+
+    _CODES = {torch.float32: 0, torch.int32: 1, torch.int64: 2}                # CNX_POS_*
+
+    def __init__(self, what, x, positions, inv_freq, sections, eps, norm, interleaved):
+        d = x.shape[-1]
+        self.eps, self.norm, self.interleaved = float(eps), int(bool(norm)), int(bool(interleaved))
+        if not self.eps >= 0.0:
+            raise ValueError(f"{what}: eps={eps!r}")
+        self.positions, self.inv_freq, self.sections, self.axes, self.code, self.batch_stride = None, None, None, 0, 0, 0
+        if positions is None:
+            if inv_freq is not None or sections is not None:
+                raise ValueError(f"{what}: inv_freq and sections go with positions")
+            return
+        if not isinstance(positions, torch.Tensor) or positions.dtype not in self._CODES:
+            raise TypeError(f"{what}: positions has to be a tensor of float32, int32 or int64")
+        if not isinstance(inv_freq, torch.Tensor) or inv_freq.dtype != torch.float32 or tuple(inv_freq.shape) != (d // 2,):
+            raise ValueError(f"{what}: inv_freq has to be a float32 tensor of head_dim / 2 = {d // 2} frequencies")
+        if positions.device != x.device or inv_freq.device != x.device:
+            raise ValueError(f"{what}: positions and inv_freq have to be on {x.device}")
+        if positions.requires_grad or inv_freq.requires_grad:
+            raise ValueError(f"{what}: positions and inv_freq have no gradient")
+        B, N = x.shape[:2]
+        if positions.dim() not in (2, 3) or positions.shape[-2] != N or (positions.dim() == 3 and positions.shape[0] != B):
+            raise ValueError(f"{what}: positions has to be [tokens, axes] or [batch, tokens, axes] for {B} x {N} tokens, "
+                             f"not {tuple(positions.shape)}")
+        self.axes = positions.shape[-1]
+        sections = (d // 2,) if sections is None else tuple(int(v) for v in sections)
+        if not 1 <= self.axes <= 4 or len(sections) != self.axes or min(sections) < 0 or sum(sections) != d // 2:
+            raise ValueError(f"{what}: sections={sections} has to split the {d // 2} pairs of a head over the {self.axes} axes of positions "
+                             "(1 to 4)")
+        self.positions, self.inv_freq = positions.contiguous(), inv_freq.contiguous()
+        self.sections = (ctypes.c_int32 * self.axes)(*sections)
+        self.code = self._CODES[positions.dtype]
+        self.batch_stride = N * self.axes if positions.dim() == 3 else 0
+
+    def args(self):
+        return _lib.ptr(self.positions), self.code, self.batch_stride, self.axes, self.sections, _lib.ptr(self.inv_freq)
+
+
+def _check_head_weight(what, name, w, x):
+    if w is None:
+        return
+    if not isinstance(w, torch.Tensor) or tuple(w.shape) != (x.shape[-1],):
+        raise ValueError(f"{what}: {name} has to be a tensor of head_dim = {x.shape[-1]} values")
+    if w.dtype not in (torch.float32, x.dtype) or w.device != x.device:
+        raise TypeError(f"{what}: {name} has to be float32 or {x.dtype} on {x.device}, not {w.dtype} on {w.device}")
+
+
+def _rope_forward(q, k, yq, yk, wq, wk, rot):
+    """``qk_norm_rope`` of checked, readable tensors into ``yq`` / ``yk``."""
+    w = wq if wq is not None else wk
+    B, N, Hq, d = q.shape
+    _lib.check(_lib.load().cnx_qk_norm_rope_fwd(
+        q.data_ptr(), k.data_ptr(), yq.data_ptr(), yk.data_ptr(), _code(q), _strides(q, k, yq, yk), _lib.ptr(wq), _lib.ptr(wk),
+        _code(w) if w is not None else 0, *rot.args(), B, N, Hq, k.shape[2], d, rot.eps, rot.norm, rot.interleaved, _stream()),
+        "cnx_qk_norm_rope_fwd")
+
+
+def _rope_backward(dyq, dyk, q, k, dq, dk, wq, wk, rot, want_wq, want_wk):
+    """Gradients of ``qk_norm_rope`` into ``dq`` / ``dk``; returns those of the weights (fp32) or None."""
+    lib = _lib.load()
+    w = wq if wq is not None else wk
+    B, N, Hq, d = dyq.shape
+    dwq = torch.empty(d, device=dyq.device, dtype=torch.float32) if want_wq else None
+    dwk = torch.empty(d, device=dyq.device, dtype=torch.float32) if want_wk else None
+    ws = torch.empty(lib.cnx_qk_norm_rope_ws_floats(d), device=dyq.device, dtype=torch.float32) if want_wq or want_wk else None
+    x = (q, k) if rot.norm else (dyq, dyk)                                      # without norm q and k are not read
+    _lib.check(lib.cnx_qk_norm_rope_bwd(
+        dyq.data_ptr(), dyk.data_ptr(), x[0].data_ptr(), x[1].data_ptr(), dq.data_ptr(), dk.data_ptr(), _lib.ptr(dwq), _lib.ptr(dwk),
+        _lib.ptr(ws), _code(dyq), _strides(dyq, dyk, *x, dq, dk), _lib.ptr(wq), _lib.ptr(wk), _code(w) if w is not None else 0, *rot.args(),
+        B, N, Hq, dyk.shape[2], d, rot.eps, rot.norm, rot.interleaved, _stream()), "cnx_qk_norm_rope_bwd")
+    return dwq, dwk
+
+
+def _head_weights(wq, wk):
+    """Weights of one type: where one is float32 and the other is not, both are."""
+    if wq is not None and wk is not None and wq.dtype != wk.dtype:
+        wq, wk = wq.float(), wk.float()
+    return (None if wq is None else wq.contiguous()), (None if wk is None else wk.contiguous())
+
+
+class _QkNormRope(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, q, k, wq, wk, rot):
+        q, k = _head_rows(q), _head_rows(k)
+        yq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        yk = torch.empty(k.shape, device=k.device, dtype=k.dtype)
+        ctx.w_dtypes = (None if wq is None else wq.dtype), (None if wk is None else wk.dtype)
+        wq, wk = _head_weights(wq, wk)
+        with _on_device(q):
+            _rope_forward(q, k, yq, yk, wq, wk, rot)
+        ctx.save_for_backward(*((q, k) if rot.norm else (None, None)), wq, wk)
+        ctx.rot = rot
+        return yq, yk
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dyq, dyk):
+        q, k, wq, wk = ctx.saved_tensors
+        dyq, dyk = _head_rows(dyq), _head_rows(dyk)
+        dq = torch.empty(dyq.shape, device=dyq.device, dtype=dyq.dtype)
+        dk = torch.empty(dyk.shape, device=dyk.device, dtype=dyk.dtype)
+        want = [ctx.needs_input_grad[i] and not _INPUT_GRAD_ONLY for i in (2, 3)]
+        with _on_device(dyq):
+            dw = _rope_backward(dyq, dyk, q, k, dq, dk, wq, wk, ctx.rot, *want)
+        dwq, dwk = (None if g is None else g.to(dt) for g, dt in zip(dw, ctx.w_dtypes))
+        return dq, dk, dwq, dwk, None
+
+
+def qk_norm_rope(q, k, q_weight=None, k_weight=None, positions=None, inv_freq=None, sections=None, eps=1e-6, norm=True, interleaved=False):
+    """Per-head RMS norm of queries and keys and their rotation by positions, in one pass: ``(q', k')``, contiguous.
+
+    ``q`` [B, N, Hq, d], ``k`` [B, N, Hk, d] (views of a packed projection are read in place), float32, bfloat16 or float16, d a multiple of
+    16 up to 256.  ``norm``: every head is divided by the root of its mean square (+ ``eps``) and multiplied by ``q_weight`` / ``k_weight``
+    [d] (float32 or the heads' type; None: 1).  ``positions`` [N, axes] or [B, N, axes] (float32, int32 or int64; None: no rotation) holds a
+    token's place on 1 to 4 axes (time, height, width ...), ``sections`` how many of the head's d / 2 pairs turn with each axis, in order,
+    ``inv_freq`` [d / 2] the angle of each pair per unit of its axis.  Pairs are (i, i + d / 2), or (2 i, 2 i + 1) if ``interleaved``.
+    Differentiable in q, k and the weights (once)."""
+    what = "qk_norm_rope"
+    _check_heads(what, ("q", q), ("k", k))
+    if q.shape[1] != k.shape[1]:
+        raise ValueError(f"{what}: q has {q.shape[1]} tokens, k {k.shape[1]}")
+    if q.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise TypeError(f"{what}: no kernel for {q.dtype}")
+    if not _lib.load().cnx_qk_norm_rope_supported(q.shape[3]):
+        raise ValueError(f"{what}: head_dim {q.shape[3]} is no multiple of 16 up to 256")
+    if not norm and (q_weight is not None or k_weight is not None):
+        raise ValueError(f"{what}: q_weight and k_weight go with norm=True")
+    _check_head_weight(what, "q_weight", q_weight, q)
+    _check_head_weight(what, "k_weight", k_weight, k)
+    return _QkNormRope.apply(q, k, q_weight, k_weight, _Rotation(what, q, positions, inv_freq, sections, eps, norm, interleaved))
+
+
+# ------------------------------------------------------------------------------ attention over any number of tokens
+def _mha_forward(q, k, v, out, scale, causal, q_lens, kv_lens, want_lse):
+    """``mha`` of checked, readable tensors into ``out``; returns lse [B, H, Nq] or None."""
+    lib = _lib.load()
+    B, Nq, H, d = q.shape
+    Nk, Hkv = k.shape[1], k.shape[2]
+    lse = torch.empty(B, H, Nq, device=q.device, dtype=torch.float32) if want_lse else None
+    n = lib.cnx_mha_ws_floats(B, Nq, Nk, H, Hkv, d)
+    ws = torch.empty(n, device=q.device, dtype=torch.float32) if n else None
+    _lib.check(lib.cnx_mha_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _lib.ptr(lse), _lib.ptr(q_lens), _lib.ptr(kv_lens),
+                               _lib.ptr(ws), _strides(q, k, v, out), _code(q), B, Nq, Nk, H, Hkv, d, causal, scale, _stream()), "cnx_mha_fwd")
+    return lse
+
+
+def _mha_backward(q, k, v, out, dout, lse, dq, dk, dv, scale, causal, q_lens, kv_lens):
+    lib = _lib.load()
+    B, Nq, H, d = q.shape
+    Nk, Hkv = k.shape[1], k.shape[2]
+    dvec = torch.empty(B, H, Nq, device=q.device, dtype=torch.float32)
+    n = lib.cnx_mha_ws_floats(B, Nq, Nk, H, Hkv, d)
+    ws = torch.empty(n, device=q.device, dtype=torch.float32) if n else None
+    _lib.check(lib.cnx_mha_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), lse.data_ptr(), dq.data_ptr(),
+                               dk.data_ptr(), dv.data_ptr(), dvec.data_ptr(), _lib.ptr(q_lens), _lib.ptr(kv_lens), _lib.ptr(ws),
+                               _strides(q, k, v, out, dout, dq, dk, dv), _code(q), B, Nq, Nk, H, Hkv, d, causal, scale, _stream()), "cnx_mha_bwd")
+
+
+class _Mha(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, q, k, v, scale, causal, q_lens, kv_lens):
+        q, k, v = _head_rows(q), _head_rows(k), _head_rows(v)
+        out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        with _on_device(q):
+            lse = _mha_forward(q, k, v, out, scale, causal, q_lens, kv_lens, any(ctx.needs_input_grad[:3]))
+        if lse is not None:
+            ctx.save_for_backward(q, k, v, out, lse, q_lens, kv_lens)
+            ctx.scale, ctx.causal = scale, causal
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse, q_lens, kv_lens = ctx.saved_tensors
+        dout = _head_rows(dout)
+        dq, dk, dv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
+        with _on_device(q):
+            _mha_backward(q, k, v, out, dout, lse, dq, dk, dv, ctx.scale, ctx.causal, q_lens, kv_lens)
+        return dq, dk, dv, None, None, None, None
+
+
+def _check_lens(what, name, lens, q):
+    if lens is None:
+        return None
+    if not isinstance(lens, torch.Tensor) or lens.dtype != torch.int32 or tuple(lens.shape) != (q.shape[0],) or lens.device != q.device:
+        raise ValueError(f"{what}: {name} has to be an int32 tensor of {q.shape[0]} lengths on {q.device}")
+    return lens.contiguous()
+
+
+def _check_scale(what, scale, d):
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not 1e-30 <= scale <= 1e30:
+        raise ValueError(f"{what}: scale={scale!r} has to be positive")
+    return scale
+
+
+def mha(q, k, v, scale=None, causal=False, q_lens=None, kv_lens=None):
+    """Softmax attention over any number of tokens: ``softmax(scale q k^T) v`` -> [B, Nq, H, d], contiguous.
+
+    ``q`` [B, Nq, H, d], ``k`` / ``v`` [B, Nk, Hkv, d] in bfloat16 or float16, d 64 or 128; H a multiple of Hkv (query head h reads key head
+    h // (H / Hkv)).  Views of a packed projection or of a [B, H, N, d] cache are read in place.  ``scale`` defaults to d^-1/2.
+    ``causal``: query i sees the keys up to i + kv_len - q_len (the last query sees the last key).  ``q_lens`` / ``kv_lens`` [B] int32: queries
+    and keys of a padded batch at or beyond these are never used; a padded query, or one that sees no key, gives zeros and no gradient.
+    Differentiable in q, k and v (once); nothing of size Nq x Nk is kept.  ``attention`` is the packed form for up to 416 tokens."""
+    what = "mha"
+    _check_heads(what, ("q", q), ("k", k), ("v", v))
+    if k.shape != v.shape:
+        raise ValueError(f"{what}: k is {tuple(k.shape)}, v {tuple(v.shape)}")
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"{what}: no kernel for {q.dtype}")
+    if not _lib.load().cnx_mha_supported(q.shape[3]):
+        raise ValueError(f"{what}: head_dim {q.shape[3]} is not 64 or 128")
+    if k.shape[2] == 0 or q.shape[2] == 0 or q.shape[2] % k.shape[2]:
+        raise ValueError(f"{what}: {q.shape[2]} query heads over {k.shape[2]} key heads")
+    return _Mha.apply(q, k, v, _check_scale(what, scale, q.shape[3]), int(bool(causal)), _check_lens(what, "q_lens", q_lens, q),
+                      _check_lens(what, "kv_lens", kv_lens, q))
+
+
+class _AttentionRope(torch.autograd.Function):
+    """``qk_norm_rope`` and ``mha`` on a packed projection: q, k, v and their gradients stay slices of it, no copies between the two."""
+
+    @staticmethod
+    def forward(ctx, qkv, wq, wk, num_heads, scale, rot):
+        B, N, C3 = qkv.shape
+        qkv = qkv.contiguous()
+        if qkv.data_ptr() % 16:
+            qkv = qkv.clone()
+        q, k, v = qkv.view(B, N, 3, num_heads, C3 // 3 // num_heads).unbind(2)
+        ctx.w_dtypes = (None if wq is None else wq.dtype), (None if wk is None else wk.dtype)
+        wq, wk = _head_weights(wq, wk)
+        out = torch.empty(q.shape, device=qkv.device, dtype=qkv.dtype)
+        with _on_device(qkv):
+            turned = rot.norm or rot.positions is not None
+            yq, yk = (torch.empty(q.shape, device=qkv.device, dtype=qkv.dtype) for _ in range(2)) if turned else (q, k)
+            if turned:
+                _rope_forward(q, k, yq, yk, wq, wk, rot)
+            lse = _mha_forward(yq, yk, v, out, scale, 0, None, None, any(ctx.needs_input_grad[:3]))
+        if lse is not None:
+            ctx.save_for_backward(qkv, yq if turned else None, yk if turned else None, wq, wk, out, lse)
+            ctx.scale, ctx.rot = scale, rot
+        return out.view(B, N, C3 // 3)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        qkv, yq, yk, wq, wk, out, lse = ctx.saved_tensors
+        B, N, H, d = out.shape
+        q, k, v = qkv.view(B, N, 3, H, d).unbind(2)
+        turned = yq is not None
+        dout = _head_rows(dout.reshape(B, N, H, d))
+        dqkv = torch.empty_like(qkv)
+        dq, dk, dv = dqkv.view(B, N, 3, H, d).unbind(2)
+        dwq = dwk = None
+        with _on_device(qkv):
+            if turned:
+                dyq, dyk = torch.empty_like(yq), torch.empty_like(yk)
+                _mha_backward(yq, yk, v, out, dout, lse, dyq, dyk, dv, ctx.scale, 0, None, None)
+                want = [ctx.needs_input_grad[i] and not _INPUT_GRAD_ONLY for i in (1, 2)]
+                dwq, dwk = _rope_backward(dyq, dyk, q, k, dq, dk, wq, wk, ctx.rot, *want)
+                dwq, dwk = (None if g is None else g.to(dt) for g, dt in zip((dwq, dwk), ctx.w_dtypes))
+            else:
+                _mha_backward(q, k, v, out, dout, lse, dq, dk, dv, ctx.scale, 0, None, None)
+        return dqkv, dwq, dwk, None, None, None
+
+
+def attention_rope(qkv, num_heads, scale=None, q_weight=None, k_weight=None, positions=None, inv_freq=None, sections=None, eps=1e-6,
+                   norm=True, interleaved=False):
+    """``attention`` with normalised heads and rotary positions: ``qk_norm_rope`` of q and k, then ``mha``, from a packed ``[B, N, 3C]``
+    bfloat16 or float16 projection -> ``[B, N, C]``, for any N; head_dim 64 or 128.  The arguments behind ``scale`` are those of
+    ``qk_norm_rope``; with ``norm=False`` and no positions it is ``attention`` without a limit on N.  Differentiable in qkv and the weights."""
+    what = "attention_rope"
+    if not isinstance(qkv, torch.Tensor) or qkv.dim() != 3:
+        raise ValueError(f"{what}: qkv has to be a tensor [batch, tokens, 3 * width]")
+    if not qkv.is_cuda:
+        raise _lib.ApgdHipError(f"{what}: qkv has to be a device tensor (no CPU path in the product)")
+    if qkv.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"{what}: no kernel for {qkv.dtype}")
+    if num_heads < 1 or qkv.shape[2] % (3 * num_heads):
+        raise ValueError(f"{what}: a projection of {qkv.shape[2]} values for {num_heads} heads")
+    d = qkv.shape[2] // 3 // num_heads
+    if not _lib.load().cnx_mha_supported(d):
+        raise ValueError(f"{what}: head_dim {d} is not 64 or 128")
+    if not norm and (q_weight is not None or k_weight is not None):
+        raise ValueError(f"{what}: q_weight and k_weight go with norm=True")
+    x = qkv.detach().unsqueeze(2)[..., :d]                                     # [B, N, 1, d]: what the checks go by
+    _check_head_weight(what, "q_weight", q_weight, x)
+    _check_head_weight(what, "k_weight", k_weight, x)
+    rot = _Rotation(what, x, positions, inv_freq, sections, eps, norm, interleaved)
+    return _AttentionRope.apply(qkv, q_weight, k_weight, num_heads, _check_scale(what, scale, d), rot)
 
 
 # ------------------------------------------------------------------------------ kernel sets (run-time A/B)

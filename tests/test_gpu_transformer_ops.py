@@ -1,0 +1,439 @@
+"""GPU tests of the transformer-block operators (``ops.qk_norm_rope``, ``ops.mha``, ``ops.attention_rope``) against their definitions in 64 bits.
+
+Every bound is derived, element by element, from the roundings the kernels make: ``u`` = half a step of the 16-bit type
+(``torch.finfo(t).eps / 2``), e = 2^-24 for a 32-bit operation; the derivation stands where the bound is formed."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+E = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def R():
+    import revisiting_at_amd as R
+    assert torch.cuda.is_available()
+    R._lib.load()
+    return R
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def inside(got, ref, bound, what=""):
+    got, ref, bound = got.detach().double().cpu(), ref.detach().double().cpu(), bound.detach().double().cpu()
+    assert got.shape == ref.shape, (what, got.shape, ref.shape)
+    off = (got - ref).abs()
+    bad = ~(off <= bound)
+    assert not bool(bad.any()), (what, int(bad.sum()), float((off / bound.clamp(min=1e-300))[bad].max()), float(off[bad].max()))
+
+
+# ------------------------------------------------------------------------------------------------------------------ qk_norm_rope
+def rope_angles(positions, inv_freq, sections):
+    axis = torch.tensor([a for a, n in enumerate(sections) for _ in range(n)])
+    return positions.double().cpu()[..., axis] * inv_freq.double().cpu()          # [(B,) N, d / 2]
+
+
+def split_pairs(x, il):
+    return (x[..., 0::2], x[..., 1::2]) if il else x.chunk(2, -1)
+
+
+def join_pairs(a, b, il):
+    return torch.stack((a, b), -1).flatten(-2) if il else torch.cat((a, b), -1)
+
+
+def rope_ref(x, w, angle, norm, il, eps, dy=None):
+    """(y, bound of y in 32 bits) and, with dy, (dx, its bound, dw, its bound) of one of q, k in 64 bits."""
+    x = x.double().cpu()
+    d = x.shape[-1]
+    w = torch.ones(d, dtype=torch.float64) if w is None else w.detach().double().cpu()
+    r = 1 / torch.sqrt((x * x).mean(-1, keepdim=True) + eps) if norm else torch.ones(x.shape[:-1] + (1,), dtype=torch.float64)
+    xh = x * r
+    z = xh * w
+    c, s = (torch.ones(1).double(), torch.zeros(1).double()) if angle is None else (angle.cos().unsqueeze(-2), angle.sin().unsqueeze(-2))
+    za, zb = split_pairs(z, il)
+    y = join_pairs(za * c - zb * s, zb * c + za * s, il)
+    # r: the mean of d squares (16 in a lane, then at most 4 exchanges), all positive: 21 roundings, halved by the root; + eps, root, quotient,
+    # the factor 1/d: 5;  x r w: 2;  the angle in turns rounded to 24 bits: 2 pi / 4 e, cos and sin: 2 e each;  the turn: 3.  Sum under 32.
+    both = za.abs() + zb.abs()
+    yb = join_pairs(both, both, il) * 32 * E
+    if dy is None:
+        return y, yb
+    dy = dy.double().cpu()
+    ga, gb = split_pairs(dy, il)
+    dz = join_pairs(ga * c + gb * s, gb * c - ga * s, il)
+    mag = join_pairs(ga.abs() + gb.abs(), ga.abs() + gb.abs(), il)                # >= |dz|; dz is 8 e off relative to it
+    t = dz * xh
+    dw, dwb = t.sum((0, 1, 2)), (mag * xh.abs()).sum((0, 1, 2))
+    if norm:
+        dot = (t * w).mean(-1, keepdim=True)
+        tall = (mag * xh.abs() * w.abs()).mean(-1, keepdim=True)
+        dx = r * (dz * w - xh * dot)
+        # dz w: 9; xh: 20; the mean of d products of 30 e each, 21 deep: 52; the last two: 2 + r's 16
+        dxb = r * (mag * w.abs() * 32 + xh.abs() * tall * 96) * E
+    else:
+        dx, dxb = dz, mag * 10 * E
+    # a sum over all rows: 30 e each, as deep as there are rows at most (tested sizes: 2^12 rows' worth at most)
+    rows = x.shape[0] * x.shape[1] * x.shape[2]
+    return y, yb, dx, dxb, dw, dwb * (30 + min(rows, 4096) + 100) * E
+
+
+ROPE = [  # B, N, Hq, Hk, d, axes, norm, interleaved, per-batch positions, far
+    (2, 5, 3, 3, 64, 2, True, False, False, 0),
+    (1, 1, 1, 1, 64, 1, True, False, False, 0),
+    (2, 1, 4, 1, 128, 1, True, False, True, 1_000_000),
+    (1, 197, 6, 6, 64, 2, True, False, False, 0),
+    (3, 50, 12, 4, 128, 3, True, True, True, 1000),
+    (2, 33, 2, 2, 32, 2, True, True, False, 7),
+    (1, 7, 5, 2, 96, 3, True, False, True, 0),
+    (1, 7, 3, 3, 80, 4, True, True, False, 0),
+    (2, 9, 2, 1, 16, 1, True, False, False, 100),
+    (1, 9, 2, 1, 256, 2, True, False, False, 100),
+    (2, 40, 4, 2, 64, 2, False, False, False, 0),
+    (2, 40, 4, 2, 64, 2, False, True, True, 0),
+    (1, 6, 2, 2, 64, 0, True, False, False, 0),
+    (1, 1300, 3, 1, 64, 2, True, False, False, 0),
+    (8, 700, 1, 1, 48, 1, True, False, True, 0),
+]
+
+
+def rope_inputs(R, case, dtype, wdtype, seed):
+    B, N, Hq, Hk, d, axes, norm, il, per, far = case
+    g = torch.Generator().manual_seed(seed)
+    qkv = torch.randn(B, N, Hq + 2 * Hk, d, generator=g).to(dtype).cuda()
+    q, k = qkv[:, :, :Hq].detach().requires_grad_(), qkv[:, :, Hq:Hq + Hk].detach().requires_grad_()
+    wq = wk = pos = inv = sec = None
+    if norm:
+        wq, wk = ((1 + 0.3 * torch.randn(d, generator=g)).to(wdtype).cuda().requires_grad_() for _ in range(2))
+    if axes:
+        sec = [d // 2 // axes + (a < d // 2 % axes) for a in range(axes)]
+        inv = torch.cat([100.0 ** (-torch.arange(n).float() / n) for n in sec]).cuda()
+        pos = torch.randint(0, 60, (B, N, axes) if per else (N, axes), generator=g) + far
+        pos = pos.to([torch.int64, torch.int32, torch.float32][seed % 3]).cuda()
+    dq, dk = (torch.randn(B, N, h, d, generator=g).to(dtype).cuda() for h in (Hq, Hk))
+    return q, k, wq, wk, pos, inv, sec, dq, dk
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("case", ROPE, ids=lambda c: "-".join(str(int(v)) for v in c))
+def test_qk_norm_rope_against_its_definition(R, case, dtype):
+    norm, il = case[6], case[7]
+    wdtype = dtype if case[1] % 2 else torch.float32
+    q, k, wq, wk, pos, inv, sec, dq, dk = rope_inputs(R, case, dtype, wdtype, case[1] + case[4])
+    yq, yk = R.ops.qk_norm_rope(q, k, wq, wk, pos, inv, sec, norm=norm, interleaved=il)
+    leaves = (q, k) + ((wq, wk) if norm else ())
+    grads = torch.autograd.grad((yq, yk), leaves, (dq, dk))
+    angle = None if pos is None else rope_angles(pos, inv, sec)
+    u = 0.0 if dtype == torch.float32 else half_step(dtype)
+    uw = 0.0 if wdtype == torch.float32 else half_step(wdtype)
+    for i, (x, w, dy, y) in enumerate(((q, wq, dq, yq), (k, wk, dk, yk))):
+        ry, by, rx, bx, rw, bw = rope_ref(x, w, angle, norm, il, 1e-6, dy)
+        assert y.dtype == dtype and y.is_contiguous()
+        inside(y, ry, by * (1 + u) + u * ry.abs(), "y")
+        inside(grads[i], rx, bx * (1 + u) + u * rx.abs(), "dx")
+        if norm:
+            assert grads[2 + i].dtype == wdtype
+            inside(grads[2 + i], rw, bw * (1 + uw) + uw * rw.abs(), "dw")
+
+
+def test_qk_norm_rope_gradient_against_differences(R):
+    """d/dh of <y(x + h u), dy> by central differences of the definition in 64 bits: the derivative along a direction through q, k and both weights."""
+    case = (2, 11, 3, 2, 64, 2, True, False, False, 0)
+    q, k, wq, wk, pos, inv, sec, dq, dk = rope_inputs(R, case, torch.float32, torch.float32, 4)
+    grads = torch.autograd.grad(R.ops.qk_norm_rope(q, k, wq, wk, pos, inv, sec), (q, k, wq, wk), (dq, dk))
+    angle = rope_angles(pos, inv, sec)
+    g = torch.Generator().manual_seed(1)
+    dirs = [torch.randn(t.shape, generator=g).double() for t in (q, k, wq, wk)]
+
+    def value(h):
+        xq, xk, vq, vk = (t.detach().double().cpu() + h * u for t, u in zip((q, k, wq, wk), dirs))
+        return sum(float((rope_ref(x, w, angle, True, False, 1e-6)[0] * dy.double().cpu()).sum()) for x, w, dy in ((xq, vq, dq), (xk, vk, dk)))
+    h = 1e-5
+    want = (value(h) - value(-h)) / (2 * h)
+    got = sum(float((t.double().cpu() * u).sum()) for t, u in zip(grads, dirs))
+    # the differences are h^2 of the third derivative off (1e-10 of a value of the sum's size), the gradients 100 e of their sizes
+    size = sum(float((t.double().cpu() * u).abs().sum()) for t, u in zip(grads, dirs))
+    assert abs(got - want) <= 100 * E * size + 1e-7 * size
+
+
+def test_qk_norm_rope_strides_and_shared_inputs(R):
+    """Views that cannot be read in place, broadcast inputs and expanded gradients give what contiguous copies give."""
+    g = torch.Generator().manual_seed(0)
+    pos, inv = torch.arange(10).view(10, 1).cuda(), (100.0 ** (-torch.arange(32).float() / 32)).cuda()
+    wide = torch.randn(2, 10, 3, 130, generator=g).cuda()
+    for q in (wide[..., 1:65], wide[..., ::2][..., :64], wide.permute(0, 1, 2, 3)[..., :64], wide[:1, :, :, :64].expand(2, 10, 3, 64),
+              torch.randn(2, 3, 10, 64, generator=g).cuda().transpose(1, 2)):
+        a = R.ops.qk_norm_rope(q, q, positions=pos, inv_freq=inv)
+        b = R.ops.qk_norm_rope(q.contiguous(), q.contiguous(), positions=pos, inv_freq=inv)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    x = torch.randn(1, 10, 3, 64, generator=g).cuda().requires_grad_()
+    yq, yk = R.ops.qk_norm_rope(x.expand(2, 10, 3, 64), x.expand(2, 10, 3, 64), positions=pos, inv_freq=inv)
+    (gx,) = torch.autograd.grad(yq.sum() + yk.sum(), x)
+    one = x.detach().requires_grad_()
+    y1, _ = R.ops.qk_norm_rope(one, one.detach(), positions=pos, inv_freq=inv)
+    (g1,) = torch.autograd.grad(y1.sum(), one)
+    torch.testing.assert_close(gx, 4 * g1, rtol=4 * E, atol=0)                    # a sum of four equal numbers: two roundings
+    # only one output used; and no tokens at all
+    (g2,) = torch.autograd.grad(R.ops.qk_norm_rope(one, one.detach(), positions=pos, inv_freq=inv)[0].sum(), one)
+    assert torch.equal(g1, g2)
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    none = torch.empty(0, 10, 3, 64, device="cuda", requires_grad=True)
+    y = R.ops.qk_norm_rope(none, none, w, w, pos, inv)[0]
+    gn, gw = torch.autograd.grad(y.sum(), (none, w))
+    assert y.shape == none.shape and gn.shape == none.shape and not bool(gw.any())
+
+
+# ------------------------------------------------------------------------------------------------------------------ mha
+def mha_ref(q, k, v, scale, causal, q_lens, kv_lens, dout, u):
+    """The definition in 64 bits, a sample and head at a time, and how far the kernel's roundings may lead from it:
+    out: P is rounded to 16 bits (u) and the result once more; exp's argument and the sums in 32 bits (t).
+    dv: the same with P^T and dout.   D is formed from the rounded out.   dS is rounded once, the products' results once."""
+    B, Nq, H, d = q.shape
+    Nk, Hkv = k.shape[1], k.shape[2]
+    q, k, v, dout = (x.detach().double().cpu() for x in (q, k, v, dout))
+    out, dq, dk, dv = (torch.zeros_like(x) for x in (q, q, k, v))
+    bo, bq, bk, bv = (torch.zeros_like(x) for x in (q, q, k, v))
+    for b in range(B):
+        ql = Nq if q_lens is None else min(max(int(q_lens[b]), 0), Nq)
+        kl = Nk if kv_lens is None else min(max(int(kv_lens[b]), 0), Nk)
+        i, j = torch.arange(Nq).view(-1, 1), torch.arange(Nk).view(1, -1)
+        ok = (i < ql) & (j < kl)
+        if causal:
+            ok &= j <= i + kl - ql
+        for h in range(H):
+            hk = h // (H // Hkv)
+            Q, K, V, G = q[b, :, h].clone(), k[b, :, hk].clone(), v[b, :, hk].clone(), dout[b, :, h].clone()
+            Q[ql:], G[ql:], K[kl:], V[kl:] = 0, 0, 0, 0
+            S = (Q @ K.T) * scale
+            Sm = S.masked_fill(~ok, -torch.inf)
+            top = Sm.amax(1, keepdim=True) if Nk else torch.full((Nq, 1), -torch.inf).double()
+            P = torch.exp(Sm - torch.where(top == -torch.inf, 0.0, top))
+            Z = P.sum(1, keepdim=True)
+            P = P / torch.where(Z == 0, 1.0, Z)
+            G = torch.where(ok.any(1, keepdim=True), G, 0.0)
+            # 32-bit part, relative to P: a score is d + 2 operations of e of sum |q k| off, twice (against the maximum's or lse's own error),
+            # the sums over keys Nk deep, exp and log themselves 2^-20
+            t = 2 * (d + 4) * E * scale * float((Q.abs() @ K.abs().T).max() if Nk else 0) + (Nk + Nq) * E + 2.0 ** -20
+            O = P @ V
+            eo = (u + t) * (P @ V.abs())
+            out[b, :, h], bo[b, :, h] = O, eo + u * (O.abs() + eo)
+            DP, Dv = G @ V.T, (G * O).sum(1, keepdim=True)
+            DS = P * (DP - Dv)
+            size = G.abs() @ V.abs().T
+            eD = (G.abs() * (eo + u * (O.abs() + eo))).sum(1, keepdim=True) + d * E * (G.abs() * O.abs()).sum(1, keepdim=True)
+            eS = (u + 2 * t) * DS.abs() + (1 + u) * P * (d * E * size + eD)
+            # the 16-bit type's smallest steps (fp16: 2^-25 half a step below 2^-14)
+            tiny = 2.0 ** -25 if u == 2.0 ** -11 else 0.0
+            eP = torch.where(ok, (u + 2 * t) * P + tiny, 0.0)
+            eS = torch.where(ok, eS + tiny, 0.0)
+            for acc, err, x, ex in ((dq[b, :, h], bq[b, :, h], DS @ K, eS @ K.abs()), (dk[b, :, hk], bk[b, :, hk], DS.T @ Q, eS.T @ Q.abs())):
+                acc += x * scale
+                err += (ex + (Nq + Nk) * E * x.abs()) * scale
+            dv[b, :, hk] += P.T @ G
+            bv[b, :, hk] += eP.T @ G.abs()
+    for g, e in ((dq, bq), (dk, bk), (dv, bv)):
+        e += u * (g.abs() + e) + (2.0 ** -25 if u == 2.0 ** -11 else 0.0)
+    bo += 2.0 ** -24 if u == 2.0 ** -11 else 0.0                                   # P's smallest step times v, and out's own
+    return (out, dq, dk, dv), (bo, bq, bk, bv)
+
+
+def heads(B, N, H, d, layout, dtype, g, scale=1.0):
+    x = (torch.randn(B, N, H, d, generator=g) * scale).to(dtype).cuda()
+    if layout == "heads":
+        return x.transpose(1, 2).contiguous().transpose(1, 2)
+    if layout == "packed":
+        return torch.cat((x, x, x), 2)[:, :, H:2 * H]
+    return x
+
+
+MHA = [  # B, Nq, Nk, H, Hkv, d, causal, lens (q, kv) or None, layout
+    (1, 1, 1, 1, 1, 64, False, None, "tokens"),
+    (2, 197, 197, 3, 3, 64, False, None, "packed"),
+    (1, 63, 65, 2, 2, 64, False, None, "heads"),
+    (1, 128, 64, 2, 1, 64, True, None, "tokens"),              # causal with more queries than keys: the first 64 see nothing
+    (1, 129, 257, 4, 2, 64, True, None, "tokens"),
+    (2, 300, 300, 2, 2, 128, True, None, "packed"),
+    (1, 64, 128, 6, 2, 128, False, None, "heads"),
+    (3, 130, 130, 2, 2, 64, False, ([0, 130, 77], [0, 130, 77]), "tokens"),
+    (3, 130, 130, 2, 2, 64, True, ([0, 130, 77], [0, 130, 77]), "heads"),
+    (4, 70, 200, 4, 1, 64, True, ([70, 1, 69, 200], [3, 200, 0, -5]), "tokens"),   # lengths are clamped; some queries see nothing
+    (2, 90, 140, 3, 3, 128, False, (None, [1, 140]), "tokens"),
+    (2, 1, 2000, 8, 2, 64, False, None, "heads"),              # split over the keys
+    (1, 3, 1500, 4, 4, 128, True, None, "tokens"),
+    (2, 17, 900, 2, 1, 64, False, ([17, 3], [900, 5]), "tokens"),                   # splits that hold no key
+    (1, 577, 577, 2, 2, 64, False, None, "packed"),
+    (1, 5, 0, 2, 2, 64, False, None, "tokens"),                # no key at all
+]
+
+
+def mha_case(case, dtype, seed=0, spread=1.0):
+    B, Nq, Nk, H, Hkv, d, causal, lens, layout = case
+    g = torch.Generator().manual_seed(seed + Nq + Nk)
+    q = heads(B, Nq, H, d, layout, dtype, g, spread).detach().requires_grad_()
+    k, v = (heads(B, Nk, Hkv, d, layout, dtype, g).detach().requires_grad_() for _ in range(2))
+    ql, kl = (None, None) if lens is None else (None if x is None else torch.tensor(x, dtype=torch.int32, device="cuda") for x in lens)
+    return q, k, v, torch.randn(B, Nq, H, d, generator=g).to(dtype).cuda(), ql, kl, causal
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("case", MHA, ids=lambda c: "-".join(map(str, c[:6])) + ("-causal" if c[6] else "") + ("-lens" if c[7] else ""))
+def test_mha_against_its_definition(R, case, dtype):
+    q, k, v, dout, ql, kl, causal = mha_case(case, dtype)
+    out = R.ops.mha(q, k, v, causal=causal, q_lens=ql, kv_lens=kl)
+    assert out.dtype == dtype and out.shape == q.shape and out.is_contiguous()
+    got = (out,) + torch.autograd.grad(out, (q, k, v), dout)
+    ref, bound = mha_ref(q, k, v, case[5] ** -0.5, causal, ql, kl, dout, half_step(dtype))
+    for name, a, b, c in zip(("out", "dq", "dk", "dv"), got, ref, bound):
+        inside(a, b, c, name)
+    with torch.no_grad():
+        assert torch.equal(R.ops.mha(q, k, v, causal=causal, q_lens=ql, kv_lens=kl), out)
+
+
+@pytest.mark.parametrize("spread", [8.0, 0.0])
+def test_mha_with_peaked_and_flat_scores(R, spread):
+    """Scores of +-100 (one key takes all) and equal scores."""
+    case = (1, 150, 290, 2, 2, 64, False, None, "tokens")
+    q, k, v, dout, ql, kl, causal = mha_case(case, torch.bfloat16, 3, spread)
+    out = R.ops.mha(q, k, v)
+    got = (out,) + torch.autograd.grad(out, (q, k, v), dout)
+    ref, bound = mha_ref(q, k, v, 0.125, False, None, None, dout, half_step(torch.bfloat16))
+    for name, a, b, c in zip(("out", "dq", "dk", "dv"), got, ref, bound):
+        inside(a, b, c, name)
+
+
+def test_mha_gradient_against_differences(R):
+    """<gradient, direction> against central differences of the definition in 64 bits."""
+    case = (2, 40, 70, 4, 2, 64, True, None, "tokens")
+    q, k, v, dout, _, _, causal = mha_case(case, torch.bfloat16, 5)
+    grads = torch.autograd.grad(R.ops.mha(q, k, v, causal=True), (q, k, v), dout)
+    u = half_step(torch.bfloat16)
+    _, bound = mha_ref(q, k, v, 0.125, True, None, None, dout, u)
+    g = torch.Generator().manual_seed(2)
+    dirs = [torch.randn(t.shape, generator=g).double() for t in (q, k, v)]
+
+    def value(h):
+        x = [t.detach().double().cpu() + h * e for t, e in zip((q, k, v), dirs)]
+        return float((mha_ref(*x, 0.125, True, None, None, dout, u)[0][0] * dout.double().cpu()).sum())
+    h = 1e-4
+    want = (value(h) - value(-h)) / (2 * h)
+    got = sum(float((t.double().cpu() * e).sum()) for t, e in zip(grads, dirs))
+    off = sum(float((b * e.abs()).sum()) for b, e in zip(bound[1:], dirs))
+    assert abs(got - want) <= off + 1e-5 * abs(want) + 1e-4          # the differences' own error: h^2 times a third derivative
+
+
+def test_mha_padding_is_never_used(R):
+    """NaN and infinities behind the lengths change no bit, forward and backward, and padded rows come out as zeros."""
+    case = (3, 130, 130, 4, 2, 64, False, ([0, 130, 77], [0, 130, 77]), "tokens")
+    for causal in (False, True):
+        q, k, v, dout, ql, kl, _ = mha_case(case, torch.bfloat16)
+        clean = R.ops.mha(q, k, v, causal=causal, q_lens=ql, kv_lens=kl)
+        want = (clean,) + torch.autograd.grad(clean, (q, k, v), dout)
+        bad = [t.detach().clone() for t in (q, k, v, dout)]
+        for t, val in zip(bad, (float("nan"), float("inf"), float("nan"), float("-inf"))):
+            t[0], t[2, 77:] = val, val
+        x = [t.requires_grad_() for t in bad[:3]]
+        out = R.ops.mha(*x, causal=causal, q_lens=ql, kv_lens=kl)
+        for name, a, b in zip(("out", "dq", "dk", "dv"), (out,) + torch.autograd.grad(out, x, bad[3]), want):
+            assert torch.equal(a, b), name
+            assert not bool(a[0].any()) and not bool(a[2, 77:].any())
+
+
+def test_mha_same_bits_every_time_on_any_stream_and_in_a_graph(R):
+    for case in (MHA[1], MHA[5], MHA[11]):
+        q, k, v, dout, ql, kl, causal = mha_case(case, torch.bfloat16)
+
+        def both():
+            out = R.ops.mha(q, k, v, causal=causal)
+            return (out.detach(),) + torch.autograd.grad(out, (q, k, v), dout)
+        want = both()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = both()
+        torch.cuda.current_stream().wait_stream(side)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = both()
+        for _ in range(3):
+            for t in got:
+                t.fill_(7)
+            both()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_mha_broadcast_inputs_and_expanded_gradient(R):
+    g = torch.Generator().manual_seed(0)
+    q = torch.randn(3, 40, 4, 64, generator=g).to(torch.bfloat16).cuda()
+    k = torch.randn(1, 50, 2, 64, generator=g).to(torch.bfloat16).cuda().requires_grad_()
+    out = R.ops.mha(q, k.expand(3, 50, 2, 64), k.expand(3, 50, 2, 64))
+    (gk,) = torch.autograd.grad(out.sum(), k)                                      # dout: a zero-stride tensor of ones
+    kk = k.detach().repeat(3, 1, 1, 1).requires_grad_()
+    out2 = R.ops.mha(q, kk, kk)
+    (g2,) = torch.autograd.grad(out2, kk, torch.ones_like(out2))
+    assert torch.equal(out, out2)
+    torch.testing.assert_close(gk.float(), g2.float().sum(0, keepdim=True), rtol=2.0 ** -6, atol=2.0 ** -6)   # sums of three in bf16
+
+
+def test_refusals_name_what_is_wrong(R):
+    bf = dict(device="cuda", dtype=torch.bfloat16)
+    q, k = torch.zeros(2, 5, 4, 64, **bf), torch.zeros(2, 7, 2, 64, **bf)
+    mha, rope, layer = R.ops.mha, R.ops.qk_norm_rope, R.ops.attention_rope
+    for err, f in (
+            (TypeError, lambda: mha(q.float(), k.float(), k.float())), (ValueError, lambda: mha(q, k, k[:, :6])),
+            (ValueError, lambda: mha(q[:, :, :3], k, k)), (ValueError, lambda: mha(q[..., :32], k[..., :32], k[..., :32])),
+            (ValueError, lambda: mha(q, k, k, scale=0.0)), (ValueError, lambda: mha(q, k, k, scale=float("nan"))),
+            (TypeError, lambda: mha(q, k.half(), k.half())), (ValueError, lambda: mha(q[0], k, k)),
+            (ValueError, lambda: mha(q, k, k, kv_lens=torch.tensor([1, 2], device="cuda"))),
+            (ValueError, lambda: mha(q, k, k, kv_lens=torch.tensor([1], dtype=torch.int32, device="cuda"))),
+            (ValueError, lambda: mha(q, k, k, q_lens=torch.tensor([1, 2], dtype=torch.int32))),
+            (R._lib.ApgdHipError, lambda: mha(q.cpu(), k.cpu(), k.cpu())), (TypeError, lambda: mha(q, k, None)),
+            (ValueError, lambda: rope(q, k)), (ValueError, lambda: rope(q[..., :40], q[..., :40])),
+            (ValueError, lambda: rope(q, q, inv_freq=torch.ones(32, device="cuda"))),
+            (ValueError, lambda: rope(q, q, positions=torch.zeros(5, 1, device="cuda"))),
+            (ValueError, lambda: rope(q, q, positions=torch.zeros(4, 1, device="cuda"), inv_freq=torch.ones(32, device="cuda"))),
+            (TypeError, lambda: rope(q, q, positions=torch.zeros(5, 1, device="cuda").half(), inv_freq=torch.ones(32, device="cuda"))),
+            (ValueError, lambda: rope(q, q, positions=torch.zeros(5, 2, device="cuda"), inv_freq=torch.ones(32, device="cuda"), sections=[16, 15])),
+            (ValueError, lambda: rope(q, q, positions=torch.zeros(5, 5, device="cuda"), inv_freq=torch.ones(32, device="cuda"), sections=[8, 8, 8, 8, 0])),
+            (ValueError, lambda: rope(q, q, torch.ones(64, device="cuda"), norm=False)), (ValueError, lambda: rope(q, q, torch.ones(32, device="cuda"))),
+            (TypeError, lambda: rope(q, q, torch.ones(64, device="cuda").half())), (ValueError, lambda: rope(q, q, eps=-1.0)),
+            (ValueError, lambda: layer(torch.zeros(2, 5, 3 * 4 * 32, **bf), 4)), (ValueError, lambda: layer(torch.zeros(2, 5, 100, **bf), 4)),
+            (TypeError, lambda: layer(torch.zeros(2, 5, 768, device="cuda"), 4)), (R._lib.ApgdHipError, lambda: layer(torch.zeros(2, 5, 768), 4))):
+        with pytest.raises(err):
+            f()
+    x = q.clone().requires_grad_()                                                  # once differentiable: a second derivative is refused
+    (gx,) = torch.autograd.grad(mha(x, k, k).float().square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(gx.float().sum(), x)
+
+
+# ------------------------------------------------------------------------------------------------------------------ attention_rope
+@pytest.mark.parametrize("norm,rotate", [(True, True), (True, False), (False, True), (False, False)])
+@pytest.mark.parametrize("B,side,H,d", [(2, 14, 3, 64), (1, 24, 2, 64), (2, 6, 2, 128), (1, 0, 1, 64)])
+def test_attention_rope_is_its_two_operators(R, B, side, H, d, norm, rotate):
+    """Bit for bit ``qk_norm_rope`` then ``mha`` on slices of the projection, in both directions."""
+    N = side * side + 1
+    g = torch.Generator().manual_seed(N)
+    qkv = torch.randn(B, N, 3 * H * d, generator=g).to(torch.bfloat16).cuda().requires_grad_()
+    wq, wk = ((1 + 0.1 * torch.randn(d, generator=g)).cuda().requires_grad_() for _ in range(2)) if norm else (None, None)
+    n = torch.arange(side * side)
+    pos = torch.cat([torch.zeros(1, 2, dtype=torch.int64), torch.stack([n // max(side, 1), n % max(side, 1)], -1) + 1]).cuda() if rotate else None
+    sec = [d // 4, d // 4] if rotate else None
+    inv = torch.cat([100.0 ** (-torch.arange(s).float() / s) for s in sec]).cuda() if rotate else None
+    dout = torch.randn(B, N, H * d, generator=g).to(torch.bfloat16).cuda()
+    out = R.ops.attention_rope(qkv, H, None, wq, wk, pos, inv, sec, norm=norm)
+    leaves = (qkv,) + ((wq, wk) if norm else ())
+    got = (out,) + torch.autograd.grad(out, leaves, dout)
+    x = qkv.detach().requires_grad_()
+    q, k, v = x.view(B, N, 3, H, d).unbind(2)
+    if norm or rotate:
+        q, k = R.ops.qk_norm_rope(q, k, wq, wk, pos, inv, sec, norm=norm)
+    o2 = R.ops.mha(q, k, v).reshape(B, N, H * d)
+    want = (o2,) + torch.autograd.grad(o2, (x,) + ((wq, wk) if norm else ()), dout)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with torch.no_grad():
+        assert torch.equal(R.ops.attention_rope(qkv, H, None, wq, wk, pos, inv, sec, norm=norm), out)
