@@ -330,6 +330,42 @@ int cnx_attention_bwd_supported(int32_t N, int32_t head_dim);
 int cnx_attention_bwd(const void* qkv, const void* out, const void* dout, const float* lse, void* dqkv, float* dvec,
                       int64_t B, int32_t N, int32_t H, int32_t head_dim, float scale, void* stream);
 
+/* The AdamW update (main.py:395-459's optimizer) of many tensors in one launch, moments in 32 or in 8 bits (csrc/optim_kernels.hip):
+ *     p <- p (1 - lr wd);  m <- b1 m + (1 - b1) g;  v <- b2 v + (1 - b2) g^2;  p <- p - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+ * table [n_tensors] and chunks [n_chunks] are DEVICE arrays that the caller builds once: a tensor's parameters (fp32 or bf16, dense, any
+ * address), elements, first element of its moments in their buffers (a multiple of CNX_ADAMW_BLOCK; every tensor's moments are padded with
+ * zeros to whole blocks), width of its moments (32 or 8), dtype, parameter group and step counter; a chunk is part `part` (of
+ * CNX_ADAMW_CHUNK elements) of a tensor, every tensor's parts listed once.  grads (HOST array of device pointers, the parameter's dtype and
+ * layout; NULL: the tensor is left as it is and its step not counted).  hyper (host) [n_groups][5]: lr, beta1, beta2, eps, weight decay;
+ * lr_dev (host array, nullable): device fp32 learning rates that override lr.  steps: fp32 step counters, advanced by the call; coef:
+ * scratch, 8 * n_tensors floats.  m, v: 32-bit moments; m_codes / v_codes (a byte per element), m_scales / v_scales (fp32 per block): 8-bit
+ * ones - a set that no tensor of the table uses may be NULL.  At most CNX_ADAMW_TENSORS tensors and CNX_ADAMW_GROUPS groups a call.
+ * 8-bit moments: code * scale of the block; m: sign bit and 7 bits, v: its root in 8 bits; code c > 0 is the fp32 number whose pattern is
+ * (c + 889) << 20 (m) or (c + 1777) << 19 (root of v), 1.0 the largest, 0 is zero; rounded to nearest even; a root above zero is never
+ * rounded to zero. */
+#define CNX_ADAMW_BLOCK 256
+#define CNX_ADAMW_CHUNK 4096
+#define CNX_ADAMW_TENSORS 440
+#define CNX_ADAMW_GROUPS 8
+typedef struct {
+  void* param;
+  int64_t numel;
+  int64_t state;   /* first element of the moments */
+  int32_t bits;    /* 32 or 8 */
+  int32_t dtype;   /* APGD_F32 or APGD_BF16 */
+  int32_t group;
+  int32_t step;    /* index into steps */
+} cnx_adamw_tensor;
+typedef struct {
+  int32_t tensor, part;
+} cnx_adamw_chunk;
+int cnx_adamw_step(const cnx_adamw_tensor* table, const cnx_adamw_chunk* chunks, int64_t n_chunks, const void* const* grads,
+                   int32_t n_tensors, const double* hyper, const float* const* lr_dev, int32_t n_groups, float* steps, float* coef, float* m,
+                   float* v, uint8_t* m_codes, float* m_scales, uint8_t* v_codes, float* v_scales, void* stream);
+/* The numbers that n elements of 8-bit moments stand for, bf16 m [n] and v [n] (n whole blocks). */
+int cnx_adamw_values(const uint8_t* m_codes, const float* m_scales, const uint8_t* v_codes, const float* v_scales, void* m, void* v, int64_t n,
+                     void* stream);
+
 /* Softmax attention over any number of tokens and its backward pass (csrc/mha_kernels.hip); cnx_attention_fwd / _bwd above are the
  * packed self-attention of up to 416 tokens.
  *     out = softmax(scale * q k^T) v        q, out [B, Nq, H, d], k, v [B, Nk, Hkv, d]; query head h reads key head h / (H / Hkv)

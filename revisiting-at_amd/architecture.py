@@ -356,18 +356,57 @@ class ConvNeXtIsotropic(nn.Module):
 
 
 # ----------------------------------------------------------------------------- ViT (timm 0.8 VisionTransformer)
+class _HeadNorm(nn.Module):
+    """Weight of a per-head RMS norm (``ops.qk_norm_rope``)."""
+
+    def __init__(self, head_dim):
+        super().__init__()
+        self.weight = nn.Parameter(torch.ones(head_dim))
+
+
+def rope_grid(grid_size, head_dim, base=100.0):
+    """``(positions [1 + h w, 2], inv_freq [head_dim / 2], sections)`` of a ViT's tokens: the class token at the origin (not turned), the patches
+    by row and column from (1, 1) on; half of a head's pairs turns with the row, half with the column, at base^(-i / pairs) per patch."""
+    h, w = grid_size
+    n = torch.arange(h * w, dtype=torch.int32)
+    positions = torch.cat((torch.zeros(1, 2, dtype=torch.int32), torch.stack((torch.div(n, w, rounding_mode="floor"), n % w), 1) + 1))
+    sections = (head_dim // 2 - head_dim // 4, head_dim // 4)
+    return positions, torch.cat([base ** (-torch.arange(s, dtype=torch.float32) / s) for s in sections]), sections
+
+
 class Attention(nn.Module):
-    def __init__(self, dim, num_heads):
+    """timm's ``Attention``.  ``qk_norm``: RMS norm of every query and key head (``q_norm.weight``, ``k_norm.weight``); ``rope``: what
+    ``rope_grid`` returns - rotary positions on two axes.  Either takes ``ops.attention_rope`` instead of ``ops.attention``."""
+
+    def __init__(self, dim, num_heads, qk_norm=False, rope=None):
         super().__init__()
         self.num_heads = num_heads
         self.scale = (dim // num_heads) ** -0.5
         self.qkv = nn.Linear(dim, dim * 3, bias=True)
         self.proj = nn.Linear(dim, dim)
+        if qk_norm:
+            self.q_norm, self.k_norm = _HeadNorm(dim // num_heads), _HeadNorm(dim // num_heads)
+        self.qk_norm, self.rope = qk_norm, rope is not None
+        if self.rope:
+            self.register_buffer("positions", rope[0], persistent=False)
+            self.register_buffer("inv_freq", rope[1], persistent=False)
+            self.sections = rope[2]
+
+    def _head_args(self):
+        return ((self.q_norm.weight, self.k_norm.weight) if self.qk_norm else (None, None)) + \
+            ((self.positions, self.inv_freq, self.sections) if self.rope else (None, None, None))
 
     def forward(self, x):
         B, N, C = x.shape
         qkv = ops.linear_lib(x, self.qkv.weight, self.qkv.bias)
-        o = ops.attention(qkv, self.num_heads, self.scale)      # [B, N, C]
+        if not self.qk_norm and not self.rope:
+            o = ops.attention(qkv, self.num_heads, self.scale)      # [B, N, C]
+        elif qkv.dtype in (torch.bfloat16, torch.float16):
+            o = ops.attention_rope(qkv, self.num_heads, self.scale, *self._head_args(), norm=self.qk_norm)
+        else:                                                       # fp32 (evaluation without autocast): library products, as ops.attention
+            q, k, v = qkv.view(B, N, 3, self.num_heads, C // self.num_heads).unbind(2)
+            q, k = ops.qk_norm_rope(q, k, *self._head_args(), norm=self.qk_norm)
+            o = ops.attention(torch.stack((q, k, v), 2).view(B, N, 3 * C), self.num_heads, self.scale)
         return ops.linear_lib(o, self.proj.weight, self.proj.bias)
 
 
@@ -388,10 +427,10 @@ class _RowLayerNorm(nn.LayerNorm):
 
 
 class VitBlock(nn.Module):
-    def __init__(self, dim, num_heads, init_values=None):
+    def __init__(self, dim, num_heads, init_values=None, qk_norm=False, rope=None):
         super().__init__()
         self.norm1 = _RowLayerNorm(dim, eps=1e-6)
-        self.attn = Attention(dim, num_heads)
+        self.attn = Attention(dim, num_heads, qk_norm, rope)
         self.ls1 = _LayerScale(dim, init_values) if init_values else nn.Identity()
         self.norm2 = _RowLayerNorm(dim, eps=1e-6)
         self.mlp = _Mlp(dim, 4 * dim)
@@ -427,16 +466,19 @@ class PatchEmbed(nn.Module):
 
 
 class VisionTransformer(nn.Module):
+    """timm 0.8's ViT.  ``qk_norm`` / ``rope`` (not in the reference's models): per-head norms of queries and keys, rotary positions of the
+    ``img_size`` grid in every block; attention then runs at any resolution."""
 
     def __init__(self, img_size=224, patch_size=16, num_classes=1000, embed_dim=768, depth=12, num_heads=12,
-                 init_values=None, no_embed_class=False):
+                 init_values=None, no_embed_class=False, qk_norm=False, rope=False):
         super().__init__()
         self.num_classes, self.embed_dim, self.no_embed_class = num_classes, embed_dim, no_embed_class
         self.patch_embed = PatchEmbed(img_size, patch_size, 3, embed_dim)
         self.cls_token = nn.Parameter(torch.zeros(1, 1, embed_dim))
         n_pos = self.patch_embed.num_patches + (0 if no_embed_class else 1)
         self.pos_embed = nn.Parameter(torch.randn(1, n_pos, embed_dim) * .02)
-        self.blocks = nn.Sequential(*[VitBlock(embed_dim, num_heads, init_values) for _ in range(depth)])
+        rope = rope_grid(self.patch_embed.grid_size, embed_dim // num_heads) if rope else None
+        self.blocks = nn.Sequential(*[VitBlock(embed_dim, num_heads, init_values, qk_norm, rope) for _ in range(depth)])
         self.norm = _RowLayerNorm(embed_dim, eps=1e-6)
         self.head = nn.Linear(embed_dim, num_classes)
         nn.init.trunc_normal_(self.pos_embed, std=.02)
@@ -482,12 +524,16 @@ def interpolate_pos_encoding(pos_embed, new_img_size, old_img_size: int = 224, p
 
 
 # ----------------------------------------------------------------------------- arch names
-def get_new_model(modelname, pretrained=True, not_original=False, updated=False, img_size=224):
+def get_new_model(modelname, pretrained=True, not_original=False, updated=False, img_size=224, qk_norm=False, rope=False):
     """Arch-name dispatch of ``utils_architecture.py:225-322`` for the ConvNeXt / ViT families.
 
     ``pretrained=True`` needs a network download in the reference; here it raises (load weights with
-    ``load_state_dict`` — key names are timm's).  ``not_original=True`` swaps in the ConvStem.
+    ``load_state_dict`` — key names are timm's).  ``not_original=True`` swaps in the ConvStem.  ``qk_norm`` / ``rope``: ``VisionTransformer``'s,
+    for the ViT names only.
     """
+    if (qk_norm or rope) and not modelname.startswith(('vit_', 'deit_')):
+        raise ValueError(f"qk_norm and rope go with the ViT models, not {modelname!r}")
+    heads = dict(qk_norm=qk_norm, rope=rope)
     if pretrained:
         raise RuntimeError("pretrained=True would download timm weights; pass pretrained=False and load a state dict")
     if modelname == 'convnext_iso':                                    # :235-239 (commented recipe)
@@ -511,16 +557,16 @@ def get_new_model(modelname, pretrained=True, not_original=False, updated=False,
         if not_original:
             model.stem = ConvBlock3(96)
     elif modelname in ('vit_s', 'deit_s'):                             # :271-284
-        model = VisionTransformer(img_size, 16, embed_dim=384, depth=12, num_heads=6)
+        model = VisionTransformer(img_size, 16, embed_dim=384, depth=12, num_heads=6, **heads)
         if not_original:
             model.patch_embed.proj = ConvBlock(48, end_siz=8)
     elif modelname == 'vit_m':                                         # :286-291
         model = VisionTransformer(img_size, 16, embed_dim=512, depth=12, num_heads=8, init_values=1e-6,
-                                  no_embed_class=True)
+                                  no_embed_class=True, **heads)
         if not_original:
             model.patch_embed.proj = ConvBlock2(48)
     elif modelname == 'vit_b':                                         # :297-301
-        model = VisionTransformer(img_size, 16, embed_dim=768, depth=12, num_heads=12)
+        model = VisionTransformer(img_size, 16, embed_dim=768, depth=12, num_heads=12, **heads)
         if not_original:
             model.patch_embed.proj = ConvBlock(48, end_siz=16, fin_dim=None)
     else:

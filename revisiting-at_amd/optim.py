@@ -1,0 +1,242 @@
+"""AdamW over all parameters in two launches, with moments in 32 or in 8 bits (``csrc/optim_kernels.hip``).
+
+The reference steps ``torch.optim.AdamW`` (``main.py:395-459, 993``); ``train_step.create_optimizer`` builds that by default and
+``FusedAdamW`` for ``state_bits=32 | 8``.  Per fp32 parameter a step moves 28 bytes with 32-bit moments and 16 with 8-bit ones, which also
+keep 2 bytes instead of 8 in memory."""
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import torch
+
+from . import _lib, ops
+
+__all__ = ["FusedAdamW"]
+
+BLOCK, CHUNK, MAX_TENSORS, MAX_GROUPS = 256, 4096, 440, 8          # CNX_ADAMW_* of include/convnext_hip.h
+SMALL = 4096                                                       # tensors with fewer elements keep 32-bit moments (norms, biases)
+
+_TENSOR = np.dtype([("param", np.int64), ("numel", np.int64), ("state", np.int64), ("bits", np.int32), ("dtype", np.int32), ("group", np.int32),
+                    ("step", np.int32)])                           # cnx_adamw_tensor
+_CHUNK = np.dtype([("tensor", np.int32), ("part", np.int32)])      # cnx_adamw_chunk
+_KEYS = {32: ("exp_avg", "exp_avg_sq"), 8: ("exp_avg_codes", "exp_avg_scales", "exp_avg_sq_codes", "exp_avg_sq_scales")}
+
+
+def _dense(p):
+    """Elements of ``p`` fill its memory, each once (any order of the dimensions: channels-last weights)."""
+    need = 1
+    for size, stride in sorted(((n, s) for n, s in zip(p.shape, p.stride()) if n > 1), key=lambda v: v[1]):
+        if stride != need:
+            return False
+        need *= size
+    return True
+
+
+class _Plan:
+    """What does not change between steps: the moments' buffers, the device tables of tensors and chunks."""
+
+    def __init__(self, params, groups, bits):
+        dev = params[0].device
+        self.ptrs = [p.data_ptr() for p in params]
+        self.dtypes, self.strides = [p.dtype for p in params], [p.stride() for p in params]
+        self.bits = bits
+        self.at, size = [], {32: 0, 8: 0}
+        for p, b in zip(params, self.bits):
+            self.at.append(size[b])
+            size[b] += -(-p.numel() // BLOCK) * BLOCK
+        self.size = size
+        zeros = lambda n, dt: torch.zeros(n, device=dev, dtype=dt) if n else None                       # noqa: E731
+        self.m, self.v = zeros(size[32], torch.float32), zeros(size[32], torch.float32)
+        self.mc, self.vc = zeros(size[8], torch.uint8), zeros(size[8], torch.uint8)
+        self.ms, self.vs = zeros(size[8] // BLOCK, torch.float32), zeros(size[8] // BLOCK, torch.float32)
+        self.steps = torch.zeros(len(params), device=dev, dtype=torch.float32)
+        self.coef = torch.empty(8 * len(params), device=dev, dtype=torch.float32)
+        self.runs = []                                             # (first tensor, tensors, table, chunks)
+        for first in range(0, len(params), MAX_TENSORS):
+            rows, chunks = [], []
+            for i in range(first, min(first + MAX_TENSORS, len(params))):
+                p = params[i]
+                rows.append((self.ptrs[i], p.numel(), self.at[i], self.bits[i], _lib.dtype_code(p.dtype), groups[i], i))
+                part = np.arange(-(-p.numel() // CHUNK), dtype=np.int32)
+                chunks.append(np.stack((np.full_like(part, i - first), part), 1))
+            table = torch.from_numpy(np.array(rows, dtype=_TENSOR).view(np.uint8).copy()).to(dev)
+            chunks = torch.from_numpy(np.concatenate(chunks)).to(dev)
+            self.runs.append((first, len(rows), table, chunks))
+
+    def moments(self, i, p):
+        """Views of one tensor's moments, by the names they have in a state dict."""
+        a, e = self.at[i], self.at[i] + -(-p.numel() // BLOCK) * BLOCK
+        if self.bits[i] == 32:
+            return {k: t.as_strided(p.shape, p.stride(), a) for k, t in zip(_KEYS[32], (self.m, self.v))}
+        return dict(zip(_KEYS[8], (self.mc[a:e], self.ms[a // BLOCK:e // BLOCK], self.vc[a:e], self.vs[a // BLOCK:e // BLOCK])))
+
+
+class FusedAdamW(torch.optim.Optimizer):
+    """``torch.optim.AdamW`` (decoupled weight decay, bias correction) for fp32 or bf16 parameters on one device: one prepared launch updates
+    them all (at most 8 parameter groups).  ``state_bits=8`` keeps the moments of tensors with 4096 or more elements in a byte each (a
+    scale for every 256 elements; the second moment as its root), the others in 32 bits.
+
+    Step counters live on the device and ``lr`` may be a device tensor, so a step can be captured into a hipGraph after one eager step (or
+    ``load_state_dict``) has built the tables.  Parameters without a gradient are left alone.  ``state_dict`` has torch's layout: ``step`` and
+    ``exp_avg`` / ``exp_avg_sq`` (torch's AdamW loads and is loaded), or ``exp_avg_codes``, ``exp_avg_scales``, ``exp_avg_sq_codes``,
+    ``exp_avg_sq_scales`` where the moments have 8 bits.  ``moments()`` gives all moments as numbers.  The optimizer steps on the stream that
+    is current; its buffers belong to one stream at a time, as the parameters do."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32):
+        if state_bits not in (32, 8):
+            raise ValueError(f"FusedAdamW: state_bits={state_bits!r} is not 32 or 8")
+        if not isinstance(lr, torch.Tensor) and not lr >= 0.0:
+            raise ValueError(f"FusedAdamW: lr={lr!r}")
+        if not 0.0 <= betas[0] < 1.0 or not 0.0 <= betas[1] < 1.0 or not eps >= 0.0 or not weight_decay >= 0.0:
+            raise ValueError(f"FusedAdamW: betas={betas!r}, eps={eps!r}, weight_decay={weight_decay!r}")
+        self.state_bits, self._plan = state_bits, None
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        if len(self.param_groups) > MAX_GROUPS:
+            self.param_groups.pop()
+            raise ValueError(f"FusedAdamW: more than {MAX_GROUPS} parameter groups")
+        self._stale = True
+
+    def _bits(self, p):
+        return 8 if self.state_bits == 8 and p.numel() >= SMALL else 32
+
+    def _params(self):
+        return [p for g in self.param_groups for p in g["params"]]
+
+    def _build(self):
+        """Tables and buffers for the parameters as they are now; moments that exist are kept."""
+        params = self._params()
+        if not params:
+            raise ValueError("FusedAdamW: no parameters")
+        for p in params:
+            if not p.is_cuda:
+                raise _lib.ApgdHipError("FusedAdamW needs device parameters (no CPU path in the product)")
+            if p.device != params[0].device:
+                raise ValueError(f"FusedAdamW: parameters on {params[0].device} and {p.device}")
+            if p.dtype not in (torch.float32, torch.bfloat16):
+                raise TypeError(f"FusedAdamW: no kernel for {p.dtype} parameters")
+            if not _dense(p):
+                raise ValueError(f"FusedAdamW: a parameter with strides {p.stride()} for {tuple(p.shape)} does not fill its memory")
+            if p.numel() > CHUNK * (1 << 22):
+                raise ValueError(f"FusedAdamW: a parameter of {p.numel()} elements")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("FusedAdamW: the first step (and one after parameters were moved or added) has to run outside a graph capture")
+        old = {p: dict(self.state[p]) for p in params if self.state.get(p)}
+        with ops._on_device(params[0]), torch.no_grad():
+            plan = _Plan(params, [i for i, g in enumerate(self.param_groups) for _ in g["params"]], [self._bits(p) for p in params])
+            for i, p in enumerate(params):
+                mine = {"step": plan.steps[i], **plan.moments(i, p)}
+                for k, t in mine.items():
+                    if p in old:
+                        t.copy_(torch.as_tensor(old[p][k]))
+                self.state[p] = mine
+        self._plan, self._stale = plan, False
+        return plan
+
+    def _ready(self, params):
+        plan = self._plan
+        if plan is None or self._stale or any(p.data_ptr() != a for p, a in zip(params, plan.ptrs)):
+            plan = self._build()
+        return plan
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        params = self._params()
+        plan = self._ready(params)
+        grads, keep = [], []
+        for p, dtype, stride in zip(params, plan.dtypes, plan.strides):
+            g = p.grad
+            if g is None:
+                grads.append(None)
+                continue
+            if g.is_sparse:
+                raise RuntimeError("FusedAdamW does not take sparse gradients")
+            if g.dtype != dtype or g.stride() != stride:
+                g = torch.empty_like(p).copy_(g)                   # the parameter's type and order of elements
+                keep.append(g)
+            grads.append(g.data_ptr())
+        n = len(self.param_groups)
+        hyper, lr_dev = (ctypes.c_double * (5 * n))(), (ctypes.c_void_p * n)()
+        for i, g in enumerate(self.param_groups):
+            lr = g["lr"]
+            if isinstance(lr, torch.Tensor):
+                if lr.is_cuda:
+                    if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != params[0].device:
+                        raise ValueError("FusedAdamW: a learning rate in device memory has to be one float32 on the parameters' device")
+                    lr_dev[i] = lr.data_ptr()
+                lr = 0.0 if lr.is_cuda else float(lr)
+            hyper[5 * i:5 * i + 5] = (lr, g["betas"][0], g["betas"][1], g["eps"], g["weight_decay"])
+        if not any(plan.size.values()):                            # only empty parameters
+            return loss
+        lib = _lib.load()
+        with ops._on_device(params[0]):
+            for first, count, table, chunks in plan.runs:
+                _lib.check(lib.cnx_adamw_step(table.data_ptr(), chunks.data_ptr(), chunks.shape[0], (ctypes.c_void_p * count)(*grads[first:first + count]),
+                                              count, hyper, lr_dev, n, plan.steps.data_ptr(), plan.coef.data_ptr() + 32 * first, _lib.ptr(plan.m),
+                                              _lib.ptr(plan.v), _lib.ptr(plan.mc), _lib.ptr(plan.ms), _lib.ptr(plan.vc), _lib.ptr(plan.vs),
+                                              ops._stream()), "cnx_adamw_step")
+        return loss
+
+    @torch.no_grad()
+    def moments(self):
+        """``{32: (exp_avg, exp_avg_sq)}`` and / or ``{8: ...}``: the moments as numbers, flat, the tensors of each width in the order of the
+        groups, each padded with zeros to a multiple of 256 elements.  32 bits: the buffers themselves; 8 bits: bfloat16 copies (a code has
+        4 or 5 significant bits)."""
+        plan = self._ready(self._params())
+        out = {}
+        if plan.m is not None:
+            out[32] = plan.m, plan.v
+        if plan.mc is not None:
+            n = plan.mc.numel()
+            m, v = (torch.empty(n, device=plan.mc.device, dtype=torch.bfloat16) for _ in range(2))
+            with ops._on_device(m):
+                _lib.check(_lib.load().cnx_adamw_values(plan.mc.data_ptr(), plan.ms.data_ptr(), plan.vc.data_ptr(), plan.vs.data_ptr(), m.data_ptr(),
+                                                        v.data_ptr(), n, ops._stream()), "cnx_adamw_values")
+            out[8] = m, v
+        return out
+
+    def state_dict(self):
+        if self._plan is not None:
+            self._ready(self._params())
+        return super().state_dict()
+
+    @torch.no_grad()
+    def load_state_dict(self, state_dict):
+        """A state dict of this class, or (32-bit moments) of ``torch.optim.AdamW``; moments of another width are refused, before anything is
+        changed."""
+        params, ids = self._params(), [i for g in state_dict["param_groups"] for i in g["params"]]
+        for g in state_dict["param_groups"]:
+            if g.get("amsgrad") or g.get("maximize"):
+                raise ValueError("FusedAdamW: no amsgrad, no maximize")
+        for i, (p, at) in enumerate(zip(params, ids)):
+            given = state_dict["state"].get(at)
+            if given is None:                                                                  # never stepped
+                continue
+            bits, blocks = self._bits(p), -(-p.numel() // BLOCK)
+            shapes = dict(zip(_KEYS[bits], [tuple(p.shape)] * 2 if bits == 32 else [(blocks * BLOCK,), (blocks,)] * 2))
+            if {"step", *shapes} - set(given):
+                raise ValueError(f"FusedAdamW: the state of parameter {i} lacks {sorted({'step', *shapes} - set(given))} (state_bits="
+                                 f"{self.state_bits} keeps its moments in {bits} bits)")
+            for k, shape in shapes.items():
+                if tuple(given[k].shape) != shape:
+                    raise ValueError(f"FusedAdamW: {k} of parameter {i} is {tuple(given[k].shape)}, not {shape}")
+        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})     # checks and takes the groups
+        self._build()
+        for p, at in zip(params, ids):
+            for k, x in (state_dict["state"].get(at) or {}).items():
+                if k in self.state[p]:
+                    self.state[p][k].copy_(torch.as_tensor(x))
+
+    def __getstate__(self):
+        return {**super().__getstate__(), "state_bits": self.state_bits}
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._plan, self._stale = None, True

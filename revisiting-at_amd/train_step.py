@@ -20,6 +20,7 @@ import torch.nn as nn
 
 from . import graphed, ops
 from .config import AdvConfig, wrap_model_for_at
+from .optim import FusedAdamW
 
 
 def get_cosine_lr(epoch, lr, epochs, lr_peak_epoch):
@@ -35,13 +36,15 @@ def iteration_lrs(epoch, iters, **kw):
     return np.interp(np.arange(iters), [0, iters], [get_cosine_lr(epoch, **kw), get_cosine_lr(epoch + 1, **kw)])
 
 
-def create_optimizer(model: nn.Module, arch: str, weight_decay: float = 0.05, capturable: bool = False):
+def create_optimizer(model: nn.Module, arch: str, weight_decay: float = 0.05, capturable: bool = False, state_bits: Optional[int] = None):
     """AdamW(betas=(0.9, 0.95)) with the reference's two parameter groups (``main.py:395-459``):
     for convnext/resnet archs the names containing ``bn`` or ``.bias`` are not decayed (LayerNorm
     weights and gammas ARE); otherwise 1-D parameters and biases are not decayed.
 
     ``capturable``: step counters and the learning rate are device tensors, so the update can be part of a hipGraph
-    (``ATTrainStep(graph_train=True)``); the arithmetic is the same."""
+    (``ATTrainStep(graph_train=True)``); the arithmetic is the same.
+
+    ``state_bits``: 32 or 8 - ``optim.FusedAdamW`` with moments of that many bits instead of torch's AdamW (None)."""
     named = [(k, v) for k, v in model.named_parameters() if v.requires_grad]
     if 'convnext' in arch or 'resnet' in arch:
         excluded = ['bn', '.bias']
@@ -51,8 +54,11 @@ def create_optimizer(model: nn.Module, arch: str, weight_decay: float = 0.05, ca
         no_decay = [v for k, v in named if v.ndim <= 1 or k.endswith('.bias')]
         decay = [v for k, v in named if not (v.ndim <= 1 or k.endswith('.bias'))]
     groups = [{'params': no_decay, 'weight_decay': 0.}, {'params': decay, 'weight_decay': weight_decay}]
+    dev = decay[0].device
+    if state_bits is not None:
+        return FusedAdamW(groups, lr=torch.tensor(1e-3, dtype=torch.float32, device=dev) if capturable else 1e-3, betas=(0.9, 0.95),
+                          state_bits=state_bits)
     if capturable:
-        dev = decay[0].device
         return torch.optim.AdamW(groups, lr=torch.tensor(1e-3, dtype=torch.float32, device=dev), betas=(0.9, 0.95), fused=True,
                                  capturable=True)
     return torch.optim.AdamW(groups, betas=(0.9, 0.95), fused=decay[0].is_cuda)
@@ -325,7 +331,9 @@ class ATTrainStep:
     gradient buffers, two asynchronous all-reduces issued between the graph segments of the training pass, so an N > 1 rank runs
     the same replayed step as the single GPU; ``"ddp"``: ``torch.nn.parallel.DistributedDataParallel`` around the wrapped model
     (``main.py:889-890`` literally; its hooks keep the training pass eager).  ``grad_sync="flat"`` with ``distributed=False`` runs
-    the N > 1 code path on one GPU (``bench.py --ddp-path 1``)."""
+    the N > 1 code path on one GPU (``bench.py --ddp-path 1``).
+
+    ``state_bits`` - the optimizer: None = torch's AdamW, 32 or 8 = ``optim.FusedAdamW`` with moments of that many bits."""
 
     # what captures and replays the training pass (a seam for the process-group tests: a rank whose capture failed runs the pass
     # eagerly next to ranks that replay - both issue the same two all-reduces per step, tests/test_ddp_gloo.py)
@@ -335,7 +343,7 @@ class ATTrainStep:
                  weight_decay: float = 0.05, distributed: bool = False, channels_last: bool = True,
                  amp_dtype: Optional[torch.dtype] = torch.bfloat16, ema: bool = True, mixup=None,
                  soft_targets: bool = False, perturb=None, gemm_table: bool = False, ema_decay: float = 0.9999,
-                 graph_train: Optional[bool] = None, grad_sync: Optional[str] = None):
+                 graph_train: Optional[bool] = None, grad_sync: Optional[str] = None, state_bits: Optional[int] = None):
         self.device = torch.device(device)
         self.distributed = bool(distributed)
         if grad_sync not in (None, "flat", "ddp"):
@@ -375,7 +383,7 @@ class ATTrainStep:
             wrapped = nn.parallel.DistributedDataParallel(wrapped, device_ids=ids, broadcast_buffers=False,
                                                           gradient_as_bucket_view=True)
         self.model = wrapped
-        self.optimizer = create_optimizer(self.inner, arch, weight_decay, capturable=self.graph_train)
+        self.optimizer = create_optimizer(self.inner, arch, weight_decay, capturable=self.graph_train, state_bits=state_bits)
         self.loss = (lambda o, t: torch.sum(-t * torch.log_softmax(o.float(), dim=-1), dim=-1).mean()) \
             if soft_targets else nn.CrossEntropyLoss()                     # SoftTargetCrossEntropy / CE (main.py:461-466)
         self.amp_dtype = amp_dtype

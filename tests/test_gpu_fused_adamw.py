@@ -1,0 +1,383 @@
+"""GPU tests of ``optim.FusedAdamW`` (cnx_adamw_step) against the update in 64 bits, of the 8-bit moments' rounding bit by bit, and of the step's
+uses: captured graphs, state dicts, the training step."""
+import copy
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+E = 2.0 ** -24
+LR, BETAS, EPS, WD = 1e-3, (0.9, 0.95), 1e-8, 0.05
+
+
+@pytest.fixture(scope="module")
+def R():
+    import revisiting_at_amd as R
+    assert torch.cuda.is_available()
+    R._lib.load()
+    return R
+
+
+SHAPES = [(1,), (3,), (255,), (256,), (257,), (4095,), (64, 64), (4097,), (5, 1000), (3, 8192), (100, 131), (16, 8, 3, 3), (1, 1, 40)]
+
+
+def make(shapes, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    ps = [torch.nn.Parameter((torch.randn(s, generator=g) * 0.05).to(dtype).cuda()) for s in shapes]
+    return ps, g
+
+
+def set_grads(ps, g, scale=1.0):
+    for i, p in enumerate(ps):
+        p.grad = (torch.randn(p.shape, generator=g) * scale * 10.0 ** (i % 5 - 4)).to(p.dtype).cuda()
+
+
+def exact_step(p, g, m, v, t, wd):
+    """The update in 64 bits."""
+    m, v = BETAS[0] * m + (1 - BETAS[0]) * g, BETAS[1] * v + (1 - BETAS[1]) * g * g
+    move = LR / (1 - BETAS[0] ** t) * m / (v.sqrt() / math.sqrt(1 - BETAS[1] ** t) + EPS)
+    return p * (1 - LR * wd) - move, m, v, move
+
+
+# ---- the 8-bit code, written out: every code's value, and rounding by comparison with the borders between values
+VALUES = {"m": np.array([0.0] + [(1 + (c - 127) % 8 / 8) * 2.0 ** ((c - 127) // 8) for c in range(1, 128)]),
+          "v": np.array([0.0] + [(1 + (c - 255) % 16 / 16) * 2.0 ** ((c - 255) // 16) for c in range(1, 256)])}
+
+
+def to_codes(x, kind):
+    """Nearest code of fp32 x >= 0 (x <= 1 + 1 ulp), ties to the even mantissa = the even code of the full pattern."""
+    val, x = VALUES[kind], x.astype(np.float64)
+    mant = 8 if kind == "m" else 16
+    hi = np.clip(np.searchsorted(val, x), 1, len(val) - 1)
+    lo = hi - 1
+    mid = np.where(lo > 0, (val[lo] + val[hi]) / 2, val[1] * (1 - 1 / (4 * mant)))       # below code 1: the border of the next pattern down
+    even_hi = (hi - (len(val) - 1)) % 2 == 0
+    return np.where((x > mid) | ((x == mid) & even_hi), hi, lo)
+
+
+def decode(state, n):
+    mc, vc = (state[k].cpu().numpy().astype(np.int64) for k in ("exp_avg_codes", "exp_avg_sq_codes"))
+    ms, vs = (state[k].cpu().numpy().repeat(256) for k in ("exp_avg_scales", "exp_avg_sq_scales"))
+    m = (VALUES["m"][mc & 127].astype(np.float32) * ms) * np.where(mc > 127, -1, 1).astype(np.float32)
+    r = VALUES["v"][vc].astype(np.float32) * vs
+    return m[:n], (r * r)[:n], mc, vc, ms, vs
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_steps_in_32_bits(R, dtype):
+    """Four steps; gradients missing at some of them, in another layout at others."""
+    ps, g = make(SHAPES, dtype)
+    ps[11].data = ps[11].data.contiguous(memory_format=torch.channels_last)
+    opt = R.FusedAdamW([{"params": ps[::2], "weight_decay": 0.0}, {"params": ps[1::2]}], lr=LR, betas=BETAS, eps=EPS, weight_decay=WD)
+    ref = {p: [torch.zeros(p.shape).double(), torch.zeros(p.shape).double(), 0] for p in ps}
+    u = 0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
+    for step in range(4):
+        set_grads(ps, g)
+        if step == 1:
+            ps[3].grad = ps[6].grad = None
+        before = [p.detach().double().cpu() for p in ps]
+        opt.step()
+        for i, (p, b) in enumerate(zip(ps, before)):
+            if p.grad is None:
+                assert torch.equal(p.detach().double().cpu(), b)
+                continue
+            r = ref[p]
+            r[2] += 1
+            want, m, v, move = exact_step(b, p.grad.double().cpu(), r[0], r[1], r[2], 0.0 if i % 2 == 0 else WD)
+            st = opt.state[p]
+            assert float(st["step"]) == r[2]
+            # m: its old value times b1, (1 - b1) g, the sum (and both constants rounded): 4 e of the terms' sizes; v likewise, all positive, 5 e
+            mb = 4 * E * (BETAS[0] * r[0].abs() + (1 - BETAS[0]) * p.grad.double().cpu().abs())
+            assert bool(((st["exp_avg"].double().cpu() - m).abs() <= mb + 1e-44).all())
+            assert bool(((st["exp_avg_sq"].double().cpu() - v).abs() <= 5 * E * v + 1e-44).all())
+            # the move: m's error over the root, the root 5/2 + 1, its factor 2, + eps 1, quotient 1, step size 2: 10 e of it; p: 3 e, then its type
+            root = (v.sqrt() / math.sqrt(1 - BETAS[1] ** r[2])) + EPS
+            pb = LR / (1 - BETAS[0] ** r[2]) * mb / root + 10 * E * move.abs() + 3 * E * b.abs()
+            assert bool(((p.detach().double().cpu() - want).abs() <= pb * (1 + u) + u * want.abs() + 1e-44).all()), i
+            r[0], r[1] = st["exp_avg"].double().cpu(), st["exp_avg_sq"].double().cpu()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_steps_in_8_bits(R, dtype):
+    """Moments of tensors of 4096 elements or more: codes and scales bit by bit from the fp32 update of the decoded ones, small ones in 32 bits."""
+    ps, g = make(SHAPES, dtype, 1)
+    opt = R.FusedAdamW(ps, lr=LR, betas=BETAS, eps=EPS, weight_decay=WD, state_bits=8)
+    u = 0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
+    f = np.float32
+    for step in range(1, 5):
+        set_grads(ps, g)
+        if step == 2:
+            for p in ps:
+                p.grad.view(-1)[::7] = 0
+        if step == 4:
+            ps[9].grad[1] = 0                                                       # whole blocks without a gradient
+        before = [p.detach().clone() for p in ps]
+        old = [{k: t.clone() for k, t in opt.state[p].items()} for p in ps] if step > 1 else None
+        opt.step()
+        for i, p in enumerate(ps):
+            st = opt.state[p]
+            assert ("exp_avg_codes" in st) == (p.numel() >= 4096)
+            if p.numel() < 4096:
+                continue
+            n = p.numel()
+            m0, v0 = decode(old[i], n)[:2] if old else (np.zeros(n, f), np.zeros(n, f))
+            gr = p.grad.float().cpu().numpy().reshape(-1)
+            m = m0 * f(BETAS[0]) + gr * f(1 - BETAS[0])
+            v = v0 * f(BETAS[1]) + (gr * gr) * f(1 - BETAS[1])
+            r = np.sqrt(v)
+            want = exact_step(before[i].double().cpu().view(-1), p.grad.double().cpu().view(-1), torch.from_numpy(m0).double(),
+                              torch.from_numpy(v0).double(), step, WD)
+            move = want[3].abs()
+            mb = 4 * E * (BETAS[0] * np.abs(m0) + (1 - BETAS[0]) * np.abs(gr)).astype(np.float64)
+            root = np.sqrt(want[2].numpy() / (1 - BETAS[1] ** step)) + EPS
+            pb = torch.from_numpy(LR / (1 - BETAS[0] ** step) * mb / root) + 10 * E * move + 3 * E * before[i].double().cpu().abs().view(-1)
+            off = (p.detach().double().cpu().view(-1) - want[0]).abs()
+            assert bool((off <= pb * (1 + u) + u * want[0].abs()).all()), (i, step)
+            pad = -n % 256
+            mc, vc, ms, vs = decode(st, n)[2:]
+            for x, codes, scales, kind in ((np.abs(m), mc & 127, ms, "m"), (r, vc, vs, "v")):
+                x = np.pad(x, (0, pad)).reshape(-1, 256)
+                top = x.max(1)
+                assert np.array_equal(scales.reshape(-1, 256)[:, 0], np.where(top < 2.0 ** -126, f(0), top)), (i, step, kind)
+                inv = np.where(top >= 2.0 ** -126, f(1) / np.where(top > 0, top, f(1)), f(0)).astype(f)
+                c = to_codes((x * inv[:, None]).reshape(-1), kind)
+                if kind == "v":
+                    c = np.where((x.reshape(-1) > 0) & (c == 0), 1, c)
+                assert np.array_equal(codes, c), (i, step, kind)
+            assert np.array_equal(mc[:n] > 127, (m < 0))
+
+
+def test_moments_in_8_bits_decay_and_never_divide_by_nothing(R):
+    """Without further gradients the moments fade to nothing as they do in 32 bits, where a fixed 8-bit grid would hold b2 v at v; and a tiny gradient
+    next to a large one moves its parameter by at most lr (its root is not rounded to zero under a moment that is not)."""
+    p = torch.nn.Parameter(torch.zeros(4096, device="cuda"))
+    opt = R.FusedAdamW([p], lr=LR, betas=(0.9, 0.999), weight_decay=0.0, state_bits=8)
+    p.grad = torch.ones_like(p)
+    p.grad[1::2] = 2.0 ** -14
+    opt.step()
+    # each element moves by lr m^ / (sqrt(v^) + eps) = lr up to eps / |g| (1.7e-4 of it), on unrounded moments
+    assert float((p.detach() + LR).abs().max()) <= 2e-4 * LR
+    m, v = opt.moments()[8]
+    top = float(v.max())
+    p.grad = torch.zeros_like(p)
+    for _ in range(700):
+        opt.step()
+    m, v = opt.moments()[8]
+    assert 0 < float(v.max()) <= top * 0.999 ** 700 * (1 + 700 * 4 * E + 2.0 ** -8)       # (bf16 values)
+    assert float(m.abs().max()) <= 0.9 ** 700 and bool(torch.isfinite(p).all())
+
+
+def test_a_moment_that_is_not_finite_stays_visible(R):
+    for bad in (float("nan"), float("inf")):
+        p = torch.nn.Parameter(torch.zeros(8192, device="cuda"))
+        opt = R.FusedAdamW([p], state_bits=8)
+        p.grad = torch.ones_like(p)
+        p.grad[300] = bad
+        opt.step()
+        m, v = opt.moments()[8]
+        assert not bool(torch.isfinite(v[256:512]).any()) and bool(torch.isfinite(v[:256]).all()) and bool(torch.isfinite(v[512:]).all())
+        p.grad = torch.ones_like(p)                                                 # (v infinite: m's zeros times an infinite scale)
+        opt.step()
+        assert bool(torch.isnan(p[256:512]).all()) and bool(torch.isfinite(p[:256]).all()) and bool(torch.isfinite(p[512:]).all())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_unaligned_parameters_and_gradients(R, bits):
+    """Tensors that begin at any element of a flat buffer, as flat gradient buffers hand them out."""
+    g = torch.Generator().manual_seed(3)
+    sizes = [5000, 3, 4096, 70, 8191]
+    flat, gflat = (torch.randn(sum(sizes) + 1, generator=g).cuda() for _ in range(2))
+    apart = [torch.nn.Parameter(x.clone()) for x in flat[1:].split(sizes)]
+    ps = [torch.nn.Parameter(x) for x in flat[1:].split(sizes)]
+    for p, a, x in zip(ps, apart, gflat[1:].split(sizes)):
+        p.grad, a.grad = x, x.clone()
+    first = flat[0].clone()
+    a, b = R.FusedAdamW(ps, state_bits=bits), R.FusedAdamW(apart, state_bits=bits)
+    for _ in range(2):
+        a.step()
+        b.step()
+    assert all(torch.equal(x, y) for x, y in zip(ps, apart)) and torch.equal(flat[0], first)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_captured_step_counts_on(R, bits):
+    """Replays equal eager steps bit for bit, with a learning rate in device memory that changes between them."""
+    def build():
+        ps, g = make([(4096 + 5,), (64, 100), (7,)], torch.float32, 5)
+        set_grads(ps, g)
+        lr = torch.tensor(LR, device="cuda")
+        opt = R.FusedAdamW(ps, lr=lr, betas=BETAS, state_bits=bits)
+        opt.step()
+        return ps, opt, lr
+    (ps, opt, lr), (qs, eager, lr2) = build(), build()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for k in range(4):
+        for rate in (lr, lr2):
+            rate.fill_(LR / (k + 1))
+        graph.replay()
+        eager.step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(ps, qs))
+        assert float(opt.state[ps[0]]["step"]) == float(eager.state[qs[0]]["step"]) == k + 2
+
+
+def test_the_first_step_is_not_captured(R):
+    p = torch.nn.Parameter(torch.zeros(10, device="cuda"))
+    p.grad = torch.zeros_like(p)
+    opt = R.FusedAdamW([p])
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="outside a graph capture"):
+        with torch.cuda.graph(graph):
+            opt.step()
+    opt.step()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_dict_goes_on_where_it_was(R, bits, tmp_path):
+    ps, g = make(SHAPES, torch.float32, 7)
+    opt = R.FusedAdamW(ps, lr=LR, betas=BETAS, state_bits=bits)
+    set_grads(ps, g)
+    opt.step()
+    torch.save(opt.state_dict(), tmp_path / "s.pt")
+    qs = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    other = R.FusedAdamW(qs, state_bits=bits)
+    other.load_state_dict(torch.load(tmp_path / "s.pt", weights_only=True))
+    rs = copy.deepcopy(ps)
+    third = R.FusedAdamW(rs, lr=LR, betas=BETAS, state_bits=bits)
+    third.load_state_dict(opt.state_dict())
+    set_grads(ps, g)
+    for p, q, r in zip(ps, qs, rs):
+        q.grad, r.grad = p.grad, p.grad
+    opt.step(), other.step(), third.step()
+    assert all(torch.equal(p, q) and torch.equal(p, r) for p, q, r in zip(ps, qs, rs))
+    # a parameter that moves, one that joins
+    ps[6].data = ps[6].data.clone()
+    new = torch.nn.Parameter(torch.ones(5000, device="cuda"))
+    opt.add_param_group({"params": [new]})
+    new.grad = torch.ones_like(new)
+    opt.step(), other.step()
+    assert all(torch.equal(p, q) for p, q in zip(ps, qs)) and float(opt.state[new]["step"]) == 1 and float(opt.state[ps[6]]["step"]) == 3
+
+
+def test_torch_adamw_state_loads_and_agrees(R):
+    ps, g = make(SHAPES, torch.float32, 9)
+    qs = copy.deepcopy(ps)
+    lib = torch.optim.AdamW(qs, lr=LR, betas=BETAS, eps=EPS, weight_decay=WD)
+    set_grads(qs, g)
+    lib.step()
+    for p, q in zip(ps, qs):
+        p.data.copy_(q.data)
+    opt = R.FusedAdamW(ps)
+    opt.load_state_dict(lib.state_dict())
+    set_grads(qs, g)
+    for p, q in zip(ps, qs):
+        p.grad = q.grad.clone()
+    opt.step(), lib.step()
+    for p, q in zip(ps, qs):
+        # both are the same formula in 32 bits: 10 e of the move (at most 10 lr here: one step after the first) and 3 e of p each
+        assert bool(((p - q).abs() <= 2 * (10 * E * 10 * LR + 3 * E * q.abs())).all())
+    torch.optim.AdamW(copy.deepcopy(qs)).load_state_dict(opt.state_dict())
+
+
+def test_refusals(R):
+    p = torch.nn.Parameter(torch.zeros(5000, device="cuda"))
+    O = R.FusedAdamW
+    for bad in (dict(state_bits=4), dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(betas=(0.9, -0.1)), dict(eps=-1.0), dict(weight_decay=-1.0)):
+        with pytest.raises(ValueError):
+            O([p], **bad)
+
+    def step(q, grad=None, **kw):
+        q.grad = torch.zeros_like(q) if grad is None else grad
+        O([q], **kw).step()
+    with pytest.raises(R._lib.ApgdHipError):
+        step(torch.nn.Parameter(torch.zeros(3)))
+    with pytest.raises(TypeError):
+        step(torch.nn.Parameter(torch.zeros(3, device="cuda").half()))
+    with pytest.raises(ValueError):
+        step(torch.nn.Parameter(torch.zeros(6, device="cuda")[::2]))
+    with pytest.raises(ValueError):
+        step(torch.nn.Parameter(torch.zeros(6, device="cuda")), lr=torch.zeros(2, device="cuda"))
+    with pytest.raises(RuntimeError):
+        step(torch.nn.Parameter(torch.zeros(3, 2, device="cuda")), torch.zeros(3, 2, device="cuda").to_sparse())
+    with pytest.raises(ValueError):
+        O([{"params": [torch.nn.Parameter(torch.zeros(3, device="cuda"))]} for _ in range(9)])
+    p.grad = torch.zeros_like(p)
+    a, b = O([p], state_bits=8), O([p])
+    a.step(), b.step()
+    for x, y in ((a, b), (b, a)):
+        with pytest.raises(ValueError, match="lacks"):
+            x.load_state_dict(y.state_dict())
+    sd = b.state_dict()
+    sd["param_groups"][0]["amsgrad"] = True
+    with pytest.raises(ValueError, match="amsgrad"):
+        b.load_state_dict(sd)
+
+
+def test_more_tensors_than_one_launch_takes(R):
+    g = torch.Generator().manual_seed(11)
+    ps = [torch.nn.Parameter(torch.randn(3 + i % 9, generator=g).cuda()) for i in range(1000)]
+    qs = copy.deepcopy(ps)
+    for p, q in zip(ps, qs):
+        p.grad = torch.randn(p.shape, generator=g).cuda()
+        q.grad = p.grad
+    opt, lib = R.FusedAdamW(ps, lr=LR), torch.optim.AdamW(qs, lr=LR)
+    opt.step(), lib.step()
+    for p, q in zip(ps, qs):
+        assert bool(((p - q).abs() <= 2 * (10 * E * LR + 3 * E * q.abs())).all())
+
+
+# ------------------------------------------------------------------------------------------------------------------ together
+@pytest.mark.parametrize("bits", [None, 32, 8])
+@pytest.mark.parametrize("graph", [0, 1])
+def test_training_step_of_a_vit_with_rope_and_head_norms(R, bits, graph):
+    """attention_rope, its gradients and the optimizer in adversarial training steps, eager and replayed: finite losses, every parameter updated, and
+    a replayed run that follows the eager one."""
+    def run(graph):
+        torch.manual_seed(0)
+        model = R.architecture.VisionTransformer(img_size=64, patch_size=16, num_classes=10, embed_dim=128, depth=2, num_heads=2, qk_norm=True, rope=True)
+        step = R.ATTrainStep(model, "vit_s", R.AdvConfig(attack="apgd", n_iter=2, graph=graph), "cuda:0", lr=1e-3, state_bits=bits)
+        g = torch.Generator().manual_seed(1)
+        x, y = torch.rand(8, 3, 64, 64, generator=g).cuda(), torch.randint(0, 10, (8,), generator=g).cuda()
+        before = [p.detach().clone() for p in model.parameters()]
+        losses = [float(step.step(x, y)) for _ in range(6)]
+        assert all(np.isfinite(losses))
+        assert all(not torch.equal(a, p) for a, p in zip(before, model.parameters()))
+        return losses, type(step.optimizer).__name__, [p.detach().clone() for p in model.parameters()]
+    losses, name, ps = run(graph)
+    assert name == ("AdamW" if bits is None else "FusedAdamW")
+    if graph:
+        eager, _, qs = run(0)
+        assert abs(losses[0] - eager[0]) <= 1e-6 * abs(eager[0])                 # the first step is the same program; later ones see library noise
+
+
+def test_vit_with_rope_gradients_follow_its_definition(R):
+    """A whole model under autocast against the same weights in fp32 (ops.qk_norm_rope in 32 bits, library products): the input gradient's direction."""
+    torch.manual_seed(0)
+    model = R.architecture.VisionTransformer(img_size=64, patch_size=16, num_classes=10, embed_dim=128, depth=2, num_heads=2, qk_norm=True, rope=True).cuda()
+    x = torch.rand(4, 3, 64, 64, device="cuda", requires_grad=True)
+    ref = model(x)
+    cot = torch.randn_like(ref)
+    names = [n for n, _ in model.named_parameters()]
+    gr = torch.autograd.grad(ref, [x] + list(model.parameters()), cot)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        out = model(x)
+    gd = torch.autograd.grad(out, [x] + list(model.parameters()), cot.to(out.dtype))
+    # some 30 roundings to bf16 on the way through two blocks, u = 2^-8 each, adding up like independent ones: sqrt(30) u = 2.2 %; twice that
+    assert float((out.float() - ref).norm() / ref.norm()) < 0.045
+    for name, a, b in zip(["x"] + names, gd, gr):
+        assert float((a.float() - b).norm() / b.norm().clamp(min=1e-12)) < 0.09, name    # the way back as well
+
+
+def test_vit_options_leave_the_plain_model_alone(R):
+    A = R.architecture
+    torch.manual_seed(0)
+    a = A.get_new_model("vit_s", pretrained=False, img_size=64)
+    b = A.get_new_model("vit_s", pretrained=False, img_size=64, qk_norm=True, rope=True)
+    extra = set(b.state_dict()) - set(a.state_dict())
+    assert extra == {f"blocks.{i}.attn.{n}_norm.weight" for i in range(12) for n in "qk"} and not set(a.state_dict()) - set(b.state_dict())
+    with pytest.raises(ValueError):
+        A.get_new_model("convnext_tiny", pretrained=False, rope=True)
