@@ -43,6 +43,8 @@ typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
 typedef __attribute__((ext_vector_type(4))) short s16x4;
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int kKT = 64;                          // keys (rows) of a staged tile
+constexpr float kSlack = 8.f;                    // see mha_fwd_kernel
 
 struct Bf16 {
   static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
@@ -120,55 +122,74 @@ __device__ __forceinline__ u32x2 lds_read_tr(uint32_t addr) {
   return __builtin_bit_cast(u32x2, r);
 }
 
-// Geometry of a row-major image [rows][D] of 16-bit values in LDS, as one lane reads it.
+// How one lane reads row-major images [rows][D] of 16-bit values in LDS.  Addresses are made once; what changes - image, buffer, block - is a
+// constant that the read's own offset field takes.
 template <int D>
-struct Image {
-  static constexpr int ROWB = D * 2, CHUNKS = D / 8, KS = D / 16, DB = D / 32;
-  // operand of a product over d: row l32 of a 32-row block, k-step ks: chunk 2 ks + half
-  static __device__ __forceinline__ uint32_t row_piece(int lane) {
-    const int l32 = lane & 31, half = lane >> 5;
-    return l32 * ROWB + ((half ^ swz<D>(l32)) << 4);
+struct Lane {
+  static constexpr int ROWB = D * 2, KS = D / 16, DB = D / 32;
+  uint32_t ra[KS];                               // row l32 of a 32-row block, chunk 2 ks + half
+  uint32_t ca[2][DB];                            // column db * 32 + lane % 32, rows {0..3} + 4 half and {8..11} + 4 half of 16 rows
+  __device__ __forceinline__ Lane(uint32_t base) {
+    const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5, g = lane >> 4, i = lane & 15;
+    const uint32_t r = base + l32 * ROWB + ((half ^ swz<D>(l32)) << 4);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) ra[ks] = r ^ (ks << 5);           // (the base is a multiple of a row: only chunk bits change)
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const int row = 4 * (g >> 1) + (i >> 2) + 8 * n, chunk = 2 * (g & 1) + ((i & 3) >> 1);
+      const uint32_t c = base + row * ROWB + ((chunk ^ swz<D>(row)) << 4) + 8 * (i & 1);
+#pragma unroll
+      for (int db = 0; db < DB; ++db) ca[n][db] = c ^ (db << 6);
+    }
   }
-  static __device__ __forceinline__ u32x4 row(uint32_t base, uint32_t piece, int blk, int ks) {
-    return lds_read16((base + blk * 32 * ROWB) + (piece ^ (ks << 5)));
-  }
-  // operand of a product over rows: column db * 32 + lane % 32, rows 16 t + {0..3, 8..11} + 4 half of a 32-row block
-  static __device__ __forceinline__ uint32_t col_piece(int lane, int second) {
-    const int g = lane >> 4, i = lane & 15, row = 4 * (g >> 1) + (i >> 2) + 8 * second;
-    const int chunk = 2 * (g & 1) + ((i & 3) >> 1);
-    return row * ROWB + ((chunk ^ swz<D>(row)) << 4) + 8 * (i & 1);
-  }
-  static __device__ __forceinline__ u32x4 col(uint32_t base, uint32_t p0, uint32_t p1, int blk, int t, int db) {
-    const uint32_t at = base + (blk * 32 + t * 16) * ROWB;
-    const u32x2 a = lds_read_tr(at + (p0 ^ (db << 6))), b = lds_read_tr(at + (p1 ^ (db << 6)));
+  // operand of a product over d: rows of 32-row block blk
+  __device__ __forceinline__ u32x4 row(uint32_t image, int blk, int ks) const { return lds_read16(ra[ks] + (image + blk * 32 * ROWB)); }
+  // operand of a product over rows: a column of rows 16 t .. 16 t + 15 of block blk
+  __device__ __forceinline__ u32x4 col(uint32_t image, int blk, int t, int db) const {
+    const uint32_t at = image + (blk * 32 + t * 16) * ROWB;
+    const u32x2 a = lds_read_tr(ca[0][db] + at), b = lds_read_tr(ca[1][db] + at);
     return u32x4{a.x, a.y, b.x, b.y};
   }
 };
 
-// Staging of ROWS rows of a tensor by 256 threads: piece e = (row e / CHUNKS, chunk e % CHUNKS) of thread e % 256.  Loaded to registers one
-// tile ahead, written to LDS when the tile's turn comes.
-template <int D, int ROWS>
+// Staging of a 64-row tile by 256 threads straight from memory to LDS (no registers in between): instruction p of a wavefront fills the
+// 16-byte pieces e = (4 p + wave) * 64 + lane, row e / CHUNKS, chunk position e % CHUNKS, which holds chunk position ^ swz(row).  Rows that do
+// not exist have an offset beyond the buffer's end and come out as zeros.
+constexpr uint32_t kNoRow = 0xfffffff0u;
+template <int D>
 struct Stage {
-  static constexpr int PER = ROWS * (D / 8) / 256;
-  u32x4 r[PER];
-  template <typename Row>                        // Row: row number in the tile -> pointer to the row or nullptr (zeros)
-  __device__ __forceinline__ void load(Row row_of) {
+  static constexpr int CHUNKS = D / 8, PER = kKT * CHUNKS / 256;
+  static __device__ __forceinline__ int row(int p) { return ((4 * p + (threadIdx.x >> 6)) * 64 + (threadIdx.x & 63)) / CHUNKS; }
+  static __device__ __forceinline__ uint32_t chunk(int p) { return ((threadIdx.x & (CHUNKS - 1)) ^ swz<D>(row(p))) << 4; }
+  uint32_t off[PER];                             // byte offset of the thread's pieces from the tile's first row
+  __device__ __forceinline__ void rows_apart(int64_t stride) {
 #pragma unroll
-    for (int p = 0; p < PER; ++p) {
-      const int e = threadIdx.x + p * 256, row = e / (D / 8), c = e % (D / 8);
-      const uint16_t* src = row_of(row);
-      r[p] = u32x4{0, 0, 0, 0};
-      if (src) r[p] = *reinterpret_cast<const u32x4*>(src + c * 8);
+    for (int p = 0; p < PER; ++p) off[p] = static_cast<uint32_t>(row(p) * stride * 2) + chunk(p);
+  }
+  // the tile at `base` (uniform), its first `rows` rows, to LDS address `dst`
+  __device__ __forceinline__ void load(const uint16_t* base, int rows, uint32_t dst) const {
+    const uint64_t p64 = reinterpret_cast<uint64_t>(base);
+    const u32x4 rs = {static_cast<uint32_t>(p64), static_cast<uint32_t>(p64 >> 32) & 0xffffu, 0x80000000u, 0x00020000u};      // raw buffer of 2 GiB
+    const uint32_t at = __builtin_amdgcn_readfirstlane(dst + (threadIdx.x >> 6) * 1024);
+    if (rows >= kKT) {
+#pragma unroll
+      for (int p = 0; p < PER; ++p) piece(rs, at + p * 4096, off[p]);
+    } else {
+#pragma unroll
+      for (int p = 0; p < PER; ++p) piece(rs, at + p * 4096, row(p) < rows ? off[p] : kNoRow);
     }
   }
-  __device__ __forceinline__ void store(uint32_t base) const {
-#pragma unroll
-    for (int p = 0; p < PER; ++p) {
-      const int e = threadIdx.x + p * 256, row = e / (D / 8), c = e % (D / 8);
-      *reinterpret_cast<u32x4 __attribute__((address_space(3)))*>(static_cast<uintptr_t>(base + row * D * 2 + ((c ^ swz<D>(row)) << 4))) = r[p];
-    }
+  // 64 lanes x 16 bytes to LDS addresses dst + 16 lane.  Inline, because the compiler waits for the builtin's load before any LDS read that it
+  // cannot tell apart - the other buffer's; tile_barrier() waits instead.  (No destination registers.)
+  static __device__ __forceinline__ void piece(u32x4 rs, uint32_t dst, uint32_t off) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(dst), "v"(off), "s"(rs) : "memory");
   }
 };
+// this wavefront's pieces have landed, then everybody's
+__device__ __forceinline__ void tile_barrier() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
 
 __device__ __forceinline__ f32x16 zeros16() {
   f32x16 z;
@@ -188,16 +209,15 @@ __device__ __forceinline__ int64_t xcd_order(int64_t bid, int64_t total) {
 
 template <typename T> __device__ __forceinline__ uint2 pack4(float a, float b, float c, float d) { return make_uint2(T::pack(a, b), T::pack(c, d)); }
 
-constexpr int kKT = 64;                          // keys (rows) of a staged tile
-
 // ===================================================================================================================== forward
 // Workgroup: 4 wavefronts x 32 RB rows of one key head, over the keys [split * span, + span).  Row r of the tile: lane.
+// The running maximum of a row moves only when a tile exceeds it by more than 2^kSlack: until then P grows to at most 2^8, which costs
+// neither type any accuracy (both are relative) and saves the rescaling of the result's registers.
 template <typename T, int D, int RB>
-__global__ __launch_bounds__(256) void mha_fwd_kernel(const MhaArgs a) {
-  using I = Image<D>;
-  constexpr int KS = I::KS, DB = I::DB, ROWS = 128 * RB;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[2][2][kKT * D * 2];        // [buffer][k, v]
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l32 = lane & 31, half = lane >> 5;
+__global__ __launch_bounds__(256, 2) void mha_fwd_kernel(const MhaArgs a) {
+  constexpr int KS = D / 16, DB = D / 32, ROWS = 128 * RB, IMG = kKT * D * 2;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * 2 * IMG];              // [buffer][k, v]
+  const int wave = threadIdx.x >> 6, l32 = threadIdx.x & 31, half = (threadIdx.x >> 5) & 1;
   const int64_t per_b = static_cast<int64_t>(a.Hkv) * a.tiles * a.splits;
   int64_t w = xcd_order(blockIdx.x, gridDim.x);
   const int64_t b = w / per_b;
@@ -210,6 +230,21 @@ __global__ __launch_bounds__(256) void mha_fwd_kernel(const MhaArgs a) {
   const uint16_t* qb = a.q + b * a.vq.b + static_cast<int64_t>(hk) * a.G * a.vq.h;
   const uint16_t* kb = a.k + b * a.vk.b + hk * a.vk.h;
   const uint16_t* vb = a.v + b * a.vv.b + hk * a.vv.h;
+
+  // the workgroup's keys
+  const int64_t last_row = (row0 + ROWS < R ? row0 + ROWS : R) - 1;
+  const int first_tok = static_cast<int>(row0 / a.G), last_tok = min(static_cast<int>(last_row / a.G), lim.q_len - 1);
+  const int k_begin = split * a.span;
+  const int k_end = min(first_tok <= last_tok ? lim.end(last_tok, a.causal) : 0, k_begin + a.span);
+  Stage<D> sk, sv;
+  sk.rows_apart(a.vk.n);
+  sv.rows_apart(a.vv.n);
+  const uint32_t base = lds_addr(&lds[0]);
+  auto fetch = [&](int k0, uint32_t buffer) {
+    sk.load(kb + k0 * a.vk.n, lim.kv_len - k0, base + buffer);
+    sv.load(vb + k0 * a.vv.n, lim.kv_len - k0, base + buffer + IMG);
+  };
+  if (k_begin < k_end) fetch(k_begin, 0);
 
   // the lane's rows
   int tok[RB], end[RB], hd[RB];
@@ -228,12 +263,6 @@ __global__ __launch_bounds__(256) void mha_fwd_kernel(const MhaArgs a) {
       if (live) qf[rb][ks] = *reinterpret_cast<const u32x4*>(src + ks * 16 + half * 8);
     }
   }
-  // the workgroup's keys
-  const int64_t last_row = (row0 + ROWS < R ? row0 + ROWS : R) - 1;
-  const int first_tok = static_cast<int>(row0 / a.G), last_tok = min(static_cast<int>(last_row / a.G), lim.q_len - 1);
-  const int k_begin = split * a.span;
-  const int k_end = min(first_tok <= last_tok ? lim.end(last_tok, a.causal) : 0, k_begin + a.span);
-
   const float c2 = a.scale * kLog2e;
   float m[RB], l[RB];
   f32x16 o[RB][DB];
@@ -244,20 +273,11 @@ __global__ __launch_bounds__(256) void mha_fwd_kernel(const MhaArgs a) {
 #pragma unroll
     for (int db = 0; db < DB; ++db) o[rb][db] = zeros16();
   }
-  Stage<D, kKT> sk, sv;
-  auto fetch = [&](int k0) {
-    sk.load([&](int row) { return k0 + row < lim.kv_len ? kb + (k0 + row) * a.vk.n : nullptr; });
-    sv.load([&](int row) { return k0 + row < lim.kv_len ? vb + (k0 + row) * a.vv.n : nullptr; });
-  };
-  const uint32_t rp = I::row_piece(lane), p0 = I::col_piece(lane, 0), p1 = I::col_piece(lane, 1);
-  if (k_begin < k_end) fetch(k_begin);
-  int buf = 0;
-  for (int k0 = k_begin; k0 < k_end; k0 += kKT, buf ^= 1) {
-    const uint32_t kimg = lds_addr(&lds[buf][0][0]), vimg = lds_addr(&lds[buf][1][0]);
-    sk.store(kimg);
-    sv.store(vimg);
-    __syncthreads();                             // (two buffers: a wavefront writes the next one only after all have left the one before)
-    if (k0 + kKT < k_end) fetch(k0 + kKT);
+  const Lane<D> L(base);
+  auto step = [&](int k0, uint32_t kimg, uint32_t next) {
+    const uint32_t vimg = kimg + IMG;
+    tile_barrier();                              // the tile is there, and nobody reads the other buffer any more
+    if (k0 + kKT < k_end) fetch(k0 + kKT, next);
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
       f32x16 s[2];
@@ -265,7 +285,7 @@ __global__ __launch_bounds__(256) void mha_fwd_kernel(const MhaArgs a) {
       for (int blk = 0; blk < 2; ++blk) {
         s[blk] = zeros16();
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s[blk] = T::mfma(I::row(kimg, rp, blk, ks), qf[rb][ks], s[blk]);
+        for (int ks = 0; ks < KS; ++ks) s[blk] = T::mfma(L.row(kimg, blk, ks), qf[rb][ks], s[blk]);
       }
       if (__any(end[rb] < k0 + kKT)) {
 #pragma unroll
@@ -282,14 +302,18 @@ __global__ __launch_bounds__(256) void mha_fwd_kernel(const MhaArgs a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[blk][r]);
       mx = both_halves_max(mx) * c2;             // (c2 > 0: checked on the host)
-      const float mn = fmaxf(m[rb], mx), mu = mn == -INFINITY ? 0.f : mn;
-      const float alpha = __builtin_amdgcn_exp2f(m[rb] - mu);
-      m[rb] = mn;
-      l[rb] *= alpha;
+      if (__any(mx > m[rb] + kSlack)) {          // (uniform) lanes below keep their maximum: alpha = 1
+        const float mn = mx > m[rb] + kSlack ? mx : m[rb];
+        const float alpha = __builtin_amdgcn_exp2f(m[rb] - mn);       // m = -inf: 0
+        const float al = mn == m[rb] ? 1.f : alpha;
+        m[rb] = mn;
+        l[rb] *= al;
 #pragma unroll
-      for (int db = 0; db < DB; ++db)
+        for (int db = 0; db < DB; ++db)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[rb][db][r] *= alpha;
+          for (int r = 0; r < 16; ++r) o[rb][db][r] *= al;
+      }
+      const float mu = m[rb] == -INFINITY ? 0.f : m[rb];
 #pragma unroll
       for (int blk = 0; blk < 2; ++blk) {
 #pragma unroll
@@ -303,10 +327,14 @@ __global__ __launch_bounds__(256) void mha_fwd_kernel(const MhaArgs a) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) p[j] = T::pack(s[blk][t * 8 + 2 * j], s[blk][t * 8 + 2 * j + 1]);
 #pragma unroll
-          for (int db = 0; db < DB; ++db) o[rb][db] = T::mfma(I::col(vimg, p0, p1, blk, t, db), p, o[rb][db]);
+          for (int db = 0; db < DB; ++db) o[rb][db] = T::mfma(L.col(vimg, blk, t, db), p, o[rb][db]);
         }
       }
     }
+  };
+  for (int k0 = k_begin; k0 < k_end; k0 += 2 * kKT) {
+    step(k0, 0, 2 * IMG);
+    if (k0 + kKT < k_end) step(k0 + kKT, 2 * IMG, 0);
   }
   // lane = row: results of the row in registers, d = db * 32 + (r & 3) + 8 (r >> 2) + 4 half
 #pragma unroll
@@ -367,11 +395,10 @@ __global__ __launch_bounds__(256) void mha_join_kernel(const MhaArgs a) {
 // ===================================================================================================================== backward
 // dq: workgroup = 4 wavefronts x 32 RB rows, over the keys [split * span, + span).  Also leaves D in dvec.
 template <typename T, int D, int RB>
-__global__ __launch_bounds__(256) void mha_dq_kernel(const MhaArgs a) {
-  using I = Image<D>;
-  constexpr int KS = I::KS, DB = I::DB, ROWS = 128 * RB;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[2][2][kKT * D * 2];        // [buffer][k, v]
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l32 = lane & 31, half = lane >> 5;
+__global__ __launch_bounds__(256, 2) void mha_dq_kernel(const MhaArgs a) {
+  constexpr int KS = D / 16, DB = D / 32, ROWS = 128 * RB, IMG = kKT * D * 2;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * 2 * IMG];              // [buffer][k, v]
+  const int wave = threadIdx.x >> 6, l32 = threadIdx.x & 31, half = (threadIdx.x >> 5) & 1;
   const int64_t per_b = static_cast<int64_t>(a.Hkv) * a.tiles * a.splits;
   int64_t w = xcd_order(blockIdx.x, gridDim.x);
   const int64_t b = w / per_b;
@@ -386,6 +413,20 @@ __global__ __launch_bounds__(256) void mha_dq_kernel(const MhaArgs a) {
   const uint16_t* gb = a.dout + b * a.vdo.b + static_cast<int64_t>(hk) * a.G * a.vdo.h;
   const uint16_t* kb = a.k + b * a.vk.b + hk * a.vk.h;
   const uint16_t* vb = a.v + b * a.vv.b + hk * a.vv.h;
+
+  const int64_t last_row = (row0 + ROWS < R ? row0 + ROWS : R) - 1;
+  const int first_tok = static_cast<int>(row0 / a.G), last_tok = min(static_cast<int>(last_row / a.G), lim.q_len - 1);
+  const int k_begin = split * a.span;
+  const int k_end = min(first_tok <= last_tok ? lim.end(last_tok, a.causal) : 0, k_begin + a.span);
+  Stage<D> sk, sv;
+  sk.rows_apart(a.vk.n);
+  sv.rows_apart(a.vv.n);
+  const uint32_t base = lds_addr(&lds[0]);
+  auto fetch = [&](int k0, uint32_t buffer) {
+    sk.load(kb + k0 * a.vk.n, lim.kv_len - k0, base + buffer);
+    sv.load(vb + k0 * a.vv.n, lim.kv_len - k0, base + buffer + IMG);
+  };
+  if (k_begin < k_end) fetch(k_begin, 0);
 
   int tok[RB], end[RB], hd[RB];
   float lse2[RB], dd[RB];
@@ -416,31 +457,17 @@ __global__ __launch_bounds__(256) void mha_dq_kernel(const MhaArgs a) {
     lse2[rb] = live ? a.lse[at] * kLog2e : INFINITY;                 // exp2(s - inf) = 0
     if (split == 0 && half == 0 && tok[rb] < a.Nq) a.dvec[at] = dd[rb];
   }
-  const int64_t last_row = (row0 + ROWS < R ? row0 + ROWS : R) - 1;
-  const int first_tok = static_cast<int>(row0 / a.G), last_tok = min(static_cast<int>(last_row / a.G), lim.q_len - 1);
-  const int k_begin = split * a.span;
-  const int k_end = min(first_tok <= last_tok ? lim.end(last_tok, a.causal) : 0, k_begin + a.span);
-
   const float c2 = a.scale * kLog2e;
   f32x16 dq[RB][DB];
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
     for (int db = 0; db < DB; ++db) dq[rb][db] = zeros16();
-  Stage<D, kKT> sk, sv;
-  auto fetch = [&](int k0) {
-    sk.load([&](int row) { return k0 + row < lim.kv_len ? kb + (k0 + row) * a.vk.n : nullptr; });
-    sv.load([&](int row) { return k0 + row < lim.kv_len ? vb + (k0 + row) * a.vv.n : nullptr; });
-  };
-  const uint32_t rp = I::row_piece(lane), p0 = I::col_piece(lane, 0), p1 = I::col_piece(lane, 1);
-  if (k_begin < k_end) fetch(k_begin);
-  int buf = 0;
-  for (int k0 = k_begin; k0 < k_end; k0 += kKT, buf ^= 1) {
-    const uint32_t kimg = lds_addr(&lds[buf][0][0]), vimg = lds_addr(&lds[buf][1][0]);
-    sk.store(kimg);
-    sv.store(vimg);
-    __syncthreads();
-    if (k0 + kKT < k_end) fetch(k0 + kKT);
+  const Lane<D> L(base);
+  auto step = [&](int k0, uint32_t kimg, uint32_t next) {
+    const uint32_t vimg = kimg + IMG;
+    tile_barrier();
+    if (k0 + kKT < k_end) fetch(k0 + kKT, next);
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
       const bool masked = __any(end[rb] < k0 + kKT);
@@ -449,8 +476,8 @@ __global__ __launch_bounds__(256) void mha_dq_kernel(const MhaArgs a) {
         f32x16 s = zeros16(), dp = zeros16();
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-          s = T::mfma(I::row(kimg, rp, blk, ks), qf[rb][ks], s);
-          dp = T::mfma(I::row(vimg, rp, blk, ks), gf[rb][ks], dp);
+          s = T::mfma(L.row(kimg, blk, ks), qf[rb][ks], s);
+          dp = T::mfma(L.row(vimg, blk, ks), gf[rb][ks], dp);
         }
 #pragma unroll
         for (int r = 0; r < 16; ++r)
@@ -468,10 +495,14 @@ __global__ __launch_bounds__(256) void mha_dq_kernel(const MhaArgs a) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) p[j] = T::pack(s[t * 8 + 2 * j], s[t * 8 + 2 * j + 1]);
 #pragma unroll
-          for (int db = 0; db < DB; ++db) dq[rb][db] = T::mfma(I::col(kimg, p0, p1, blk, t, db), p, dq[rb][db]);
+          for (int db = 0; db < DB; ++db) dq[rb][db] = T::mfma(L.col(kimg, blk, t, db), p, dq[rb][db]);
         }
       }
     }
+  };
+  for (int k0 = k_begin; k0 < k_end; k0 += 2 * kKT) {
+    step(k0, 0, 2 * IMG);
+    if (k0 + kKT < k_end) step(k0 + kKT, 2 * IMG, 0);
   }
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
@@ -517,13 +548,12 @@ __global__ __launch_bounds__(256) void mha_dq_join_kernel(const MhaArgs a) {
 
 // dk, dv: workgroup = 4 wavefronts x 32 KB keys of one key head, over the rows that see them, 64 at a time.
 template <typename T, int D, int KB>
-__global__ __launch_bounds__(256) void mha_dkv_kernel(const MhaArgs a) {
-  using I = Image<D>;
-  constexpr int KS = I::KS, DB = I::DB, KEYS = 128 * KB, RT = kKT;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[2][2][RT * D * 2];         // [buffer][q, dout]
-  __shared__ float stat[2][2][RT];                                                       // [buffer][lse log2(e), D]
-  __shared__ int row_end[2][RT];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l32 = lane & 31, half = lane >> 5;
+__global__ __launch_bounds__(256, 2) void mha_dkv_kernel(const MhaArgs a) {
+  constexpr int KS = D / 16, DB = D / 32, KEYS = 128 * KB, RT = kKT, IMG = RT * D * 2;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * 2 * IMG];              // [buffer][q, dout]
+  __shared__ __attribute__((aligned(16))) float stat[2][2][RT];                          // [buffer][lse log2(e), D]
+  __shared__ __attribute__((aligned(16))) int row_end[2][RT];
+  const int wave = threadIdx.x >> 6, l32 = threadIdx.x & 31, half = (threadIdx.x >> 5) & 1;
   const int64_t per_b = static_cast<int64_t>(a.Hkv) * a.tiles;
   int64_t w = xcd_order(blockIdx.x, gridDim.x);
   const int64_t b = w / per_b;
@@ -536,6 +566,54 @@ __global__ __launch_bounds__(256) void mha_dkv_kernel(const MhaArgs a) {
   const uint16_t* kb = a.k + b * a.vk.b + hk * a.vk.h;
   const uint16_t* vb = a.v + b * a.vv.b + hk * a.vv.h;
   const int key0 = tile * KEYS;
+  // rows that see a key of this tile: all, or (causal) those from token key0 - off on
+  int64_t r_begin = a.causal ? static_cast<int64_t>(max(0, key0 - lim.off)) * a.G : 0;
+  r_begin -= r_begin % RT;
+  const int64_t r_end = key0 < lim.kv_len ? R : 0;
+  // Row r0 + row of a tile lies (row / G) tokens and row % G heads behind row r0 if G divides the tile; otherwise its place is found again for
+  // every tile.
+  const bool even = RT % a.G == 0;
+  Stage<D> sq, sg;
+#pragma unroll
+  for (int p = 0; p < Stage<D>::PER; ++p) {
+    const int row = Stage<D>::row(p), i = row / a.G, j = row - i * a.G;
+    sq.off[p] = static_cast<uint32_t>((i * a.vq.n + j * a.vq.h) * 2) + Stage<D>::chunk(p);
+    sg.off[p] = static_cast<uint32_t>((i * a.vdo.n + j * a.vdo.h) * 2) + Stage<D>::chunk(p);
+  }
+  const uint32_t base = lds_addr(&lds[0]);
+  float st_l = 0.f, st_d = 0.f;
+  int st_e = 0;
+  auto fetch = [&](int64_t r0, uint32_t buffer) {
+    const int64_t i0 = r0 / a.G;
+    const int rows = static_cast<int>(R - r0 < RT ? R - r0 : RT);
+    if (!even) {
+      const int j0 = static_cast<int>(r0 - i0 * a.G);
+#pragma unroll
+      for (int p = 0; p < Stage<D>::PER; ++p) {
+        const int row = Stage<D>::row(p), i = (j0 + row) / a.G, j = j0 + row - i * a.G;
+        sq.off[p] = static_cast<uint32_t>((i * a.vq.n + j * a.vq.h) * 2) + Stage<D>::chunk(p);
+        sg.off[p] = static_cast<uint32_t>((i * a.vdo.n + j * a.vdo.h) * 2) + Stage<D>::chunk(p);
+      }
+    }
+    sq.load(qb + i0 * a.vq.n, rows, base + buffer);
+    sg.load(gb + i0 * a.vdo.n, rows, base + buffer + IMG);
+    if (threadIdx.x < RT) {
+      const int64_t r = r0 + threadIdx.x;
+      st_l = INFINITY; st_d = 0.f; st_e = 0;
+      if (r < R) {
+        const int64_t i = r / a.G, s = (b * a.H + hk * a.G + (r - i * a.G)) * a.Nq + i;
+        st_e = lim.end(static_cast<int>(i), a.causal);
+        if (st_e > 0) { st_l = a.lse[s] * kLog2e; st_d = a.dvec[s]; }
+      }
+    }
+  };
+  auto keep = [&](int buf) {
+    if (threadIdx.x < RT) { stat[buf][0][threadIdx.x] = st_l; stat[buf][1][threadIdx.x] = st_d; row_end[buf][threadIdx.x] = st_e; }
+  };
+  if (r_begin < r_end) {
+    fetch(r_begin, 0);
+    keep(0);
+  }
   int key[KB];
   u32x4 kf[KB][KS], vf[KB][KS];
   f32x16 dk[KB][DB], dv[KB][DB];
@@ -555,44 +633,14 @@ __global__ __launch_bounds__(256) void mha_dkv_kernel(const MhaArgs a) {
 #pragma unroll
     for (int db = 0; db < DB; ++db) { dk[n][db] = zeros16(); dv[n][db] = zeros16(); }
   }
-  // rows that see a key of this tile: all, or (causal) those from token key0 - off on
-  int64_t r_begin = a.causal ? static_cast<int64_t>(max(0, key0 - lim.off)) * a.G : 0;
-  r_begin -= r_begin % RT;
-  const int64_t r_end = key0 < lim.kv_len ? R : 0;
   const float c2 = a.scale * kLog2e;
-  Stage<D, RT> sq, sg;
-  float st_l = 0.f, st_d = 0.f;
-  int st_e = 0;
-  auto fetch = [&](int64_t r0) {
-    auto at = [&](int row, const uint16_t* base, const View& v) -> const uint16_t* {
-      const int64_t r = r0 + row;
-      if (r >= R) return nullptr;
-      const int64_t i = a.G == 1 ? r : r / a.G;
-      return base + i * v.n + (r - i * a.G) * v.h;
-    };
-    sq.load([&](int row) { return at(row, qb, a.vq); });
-    sg.load([&](int row) { return at(row, gb, a.vdo); });
-    if (threadIdx.x < RT) {
-      const int64_t r = r0 + threadIdx.x;
-      st_l = INFINITY; st_d = 0.f; st_e = 0;
-      if (r < R) {
-        const int64_t i = r / a.G, s = (b * a.H + hk * a.G + (r - i * a.G)) * a.Nq + i;
-        st_e = lim.end(static_cast<int>(i), a.causal);
-        if (st_e > 0) { st_l = a.lse[s] * kLog2e; st_d = a.dvec[s]; }
-      }
-    }
-  };
-  const uint32_t rp = I::row_piece(lane), p0 = I::col_piece(lane, 0), p1 = I::col_piece(lane, 1);
-  if (r_begin < r_end) fetch(r_begin);
-  int buf = 0;
+  const Lane<D> L(base);
   const int key_last = min(key0 + KEYS, lim.kv_len) - 1;
-  for (int64_t r0 = r_begin; r0 < r_end; r0 += RT, buf ^= 1) {
-    const uint32_t qimg = lds_addr(&lds[buf][0][0]), gimg = lds_addr(&lds[buf][1][0]);
-    sq.store(qimg);
-    sg.store(gimg);
-    if (threadIdx.x < RT) { stat[buf][0][threadIdx.x] = st_l; stat[buf][1][threadIdx.x] = st_d; row_end[buf][threadIdx.x] = st_e; }
-    __syncthreads();
-    if (r0 + RT < r_end) fetch(r0 + RT);
+  auto step = [&](int64_t r0, int buf) {
+    const uint32_t qimg = buf * 2 * IMG, gimg = qimg + IMG;
+    tile_barrier();
+    const bool more = r0 + RT < r_end;
+    if (more) fetch(r0 + RT, (buf ^ 1) * 2 * IMG);
     // a tile needs no mask if its first row (the one that sees least) sees the last key; keys beyond kv_len are zeros whose dk, dv are not kept
     const bool masked = a.causal && row_end[buf][0] <= key_last;
 #pragma unroll
@@ -603,8 +651,8 @@ __global__ __launch_bounds__(256) void mha_dkv_kernel(const MhaArgs a) {
         f32x16 s = zeros16(), dp = zeros16();
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-          s = T::mfma(I::row(qimg, rp, blk, ks), kf[n][ks], s);
-          dp = T::mfma(I::row(gimg, rp, blk, ks), vf[n][ks], dp);
+          s = T::mfma(L.row(qimg, blk, ks), kf[n][ks], s);
+          dp = T::mfma(L.row(gimg, blk, ks), vf[n][ks], dp);
         }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
@@ -642,7 +690,7 @@ __global__ __launch_bounds__(256) void mha_dkv_kernel(const MhaArgs a) {
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
-          const u32x4 gt = I::col(gimg, p0, p1, blk, t, db), qt = I::col(qimg, p0, p1, blk, t, db);
+          const u32x4 gt = L.col(gimg, blk, t, db), qt = L.col(qimg, blk, t, db);
 #pragma unroll
           for (int n = 0; n < KB; ++n) {
             dv[n][db] = T::mfma(gt, pf[n][t], dv[n][db]);
@@ -650,6 +698,11 @@ __global__ __launch_bounds__(256) void mha_dkv_kernel(const MhaArgs a) {
           }
         }
     }
+    if (more) keep(buf ^ 1);
+  };
+  for (int64_t r0 = r_begin; r0 < r_end; r0 += 2 * RT) {
+    step(r0, 0);
+    if (r0 + RT < r_end) step(r0 + RT, 1);
   }
 #pragma unroll
   for (int n = 0; n < KB; ++n) {
@@ -731,6 +784,10 @@ int launch_bwd(MhaArgs& a, hipStream_t s) {
 }
 
 View view_of(const int64_t* s) { return View{s[0], s[1], s[2]}; }
+// a staged tile's rows lie within 31 bits of bytes of its first: 64 tokens and the heads that share a key head
+bool near_enough(const View& v, int64_t G) {
+  return v.n >= 0 && v.h >= 0 && v.n < (1LL << 30) / 128 && v.h < (1LL << 30) / (2 * G);
+}
 
 }  // namespace
 
@@ -759,6 +816,7 @@ int cnx_mha_fwd(const void* q, const void* k, const void* v, void* out, float* l
   if (!strides || !q || !out || (Nk > 0 && (!k || !v))) return APGD_ERR_NULL;
   if (cnx_mha_ws_floats(B, Nq, Nk, H, Hkv, head_dim) > 0 && !ws) return APGD_ERR_NULL;
   a.vq = view_of(strides); a.vk = view_of(strides + 3); a.vv = view_of(strides + 6); a.vo = view_of(strides + 9);
+  if (!near_enough(a.vk, 1) || !near_enough(a.vv, 1)) return APGD_ERR_ARG;
   hipStream_t s = as_stream(stream);
   if (dtype == APGD_BF16) return head_dim == 64 ? launch_fwd<Bf16, 64>(a, s) : launch_fwd<Bf16, 128>(a, s);
   return head_dim == 64 ? launch_fwd<Fp16, 64>(a, s) : launch_fwd<Fp16, 128>(a, s);
@@ -780,6 +838,7 @@ int cnx_mha_bwd(const void* q, const void* k, const void* v, const void* out, co
   if (cnx_mha_ws_floats(B, Nq, Nk, H, Hkv, head_dim) > 0 && !ws) return APGD_ERR_NULL;
   a.vq = view_of(strides); a.vk = view_of(strides + 3); a.vv = view_of(strides + 6); a.vo = view_of(strides + 9); a.vdo = view_of(strides + 12);
   a.vdq = view_of(strides + 15); a.vdk = view_of(strides + 18); a.vdv = view_of(strides + 21);
+  if (!near_enough(a.vq, a.G) || !near_enough(a.vk, 1) || !near_enough(a.vv, 1) || !near_enough(a.vdo, a.G)) return APGD_ERR_ARG;
   hipStream_t s = as_stream(stream);
   if (dtype == APGD_BF16) return head_dim == 64 ? launch_bwd<Bf16, 64>(a, s) : launch_bwd<Bf16, 128>(a, s);
   return head_dim == 64 ? launch_bwd<Fp16, 64>(a, s) : launch_bwd<Fp16, 128>(a, s);

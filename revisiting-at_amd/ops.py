@@ -1999,11 +1999,12 @@ def _check_heads(what, *named):
 
 
 def _head_rows(t):
-    """``t`` [B, N, H, d] itself where the kernels can read it in place (contiguous heads that begin at 16 bytes, any other strides, a
-    stride of zero included), else a contiguous copy."""
+    """``t`` [B, N, H, d] itself where the kernels can read it in place (contiguous heads that begin at 16 bytes, any other strides up to 2^22
+    elements between tokens and 2^28 over a token's heads, zero included), else a contiguous copy."""
     piece = 16 // t.element_size()
     st = t.stride()
-    if st[3] == 1 and st[0] % piece == 0 and st[1] % piece == 0 and st[2] % piece == 0 and t.data_ptr() % 16 == 0:
+    if (st[3] == 1 and st[0] % piece == 0 and st[1] % piece == 0 and st[2] % piece == 0 and t.data_ptr() % 16 == 0
+            and st[1] < 1 << 22 and st[2] * t.shape[2] < 1 << 28):
         return t
     return torch.empty(t.shape, device=t.device, dtype=t.dtype).copy_(t)
 
