@@ -103,10 +103,12 @@ struct Limits {
   }
 };
 
+// Spreads both kinds of read over the 64 banks: the 16 lanes that a 16-byte read serves at a time (rows 0 - 15, or 0 - 3, 12 - 15, 20 - 27 and
+// so on) fall on 16 different pieces of 256 bytes, and the four rows x 64 bytes of a transposing read on its four quarters.
 template <int D> __device__ __forceinline__ int swz(int row) {
   const int b0 = row & 1, b1 = (row >> 1) & 1, b2 = (row >> 2) & 1, b3 = (row >> 3) & 1;
-  if constexpr (D == 64) return ((b0 ^ b1 ^ b2) << 2) | (b1 << 1) | b0;
-  else return ((b3 ^ b1) << 3) | (b0 << 2) | (b1 << 1) | b2;
+  if constexpr (D == 64) return (b1 << 2) | (b3 << 1) | b2;            // (rows of 128 bytes: b0 is the half already)
+  else return (b1 << 3) | (b0 << 2) | (b3 << 1) | b2;
 }
 
 template <typename T>
@@ -548,7 +550,7 @@ __global__ __launch_bounds__(256) void mha_dq_join_kernel(const MhaArgs a) {
 
 // dk, dv: workgroup = 4 wavefronts x 32 KB keys of one key head, over the rows that see them, 64 at a time.
 template <typename T, int D, int KB>
-__global__ __launch_bounds__(256, 2) void mha_dkv_kernel(const MhaArgs a) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 1) void mha_dkv_kernel(const MhaArgs a) {
   constexpr int KS = D / 16, DB = D / 32, KEYS = 128 * KB, RT = kKT, IMG = RT * D * 2;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * 2 * IMG];              // [buffer][q, dout]
   __shared__ __attribute__((aligned(16))) float stat[2][2][RT];                          // [buffer][lse log2(e), D]
