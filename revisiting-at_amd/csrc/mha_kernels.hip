@@ -170,8 +170,7 @@ struct Stage {
   }
   // the tile at `base` (uniform), its first `rows` rows, to LDS address `dst`
   __device__ __forceinline__ void load(const uint16_t* base, int rows, uint32_t dst) const {
-    const uint64_t p64 = reinterpret_cast<uint64_t>(base);
-    const u32x4 rs = {static_cast<uint32_t>(p64), static_cast<uint32_t>(p64 >> 32) & 0xffffu, 0x80000000u, 0x00020000u};      // raw buffer of 2 GiB
+    const u32x4 rs = buffer(base);
     const uint32_t at = __builtin_amdgcn_readfirstlane(dst + (threadIdx.x >> 6) * 1024);
     if (rows >= kKT) {
 #pragma unroll
@@ -180,6 +179,17 @@ struct Stage {
 #pragma unroll
       for (int p = 0; p < PER; ++p) piece(rs, at + p * 4096, row(p) < rows ? off[p] : kNoRow);
     }
+  }
+  template <typename Live>                       // Live: number of the thread's piece -> whether its row exists
+  __device__ __forceinline__ void load(const uint16_t* base, uint32_t dst, Live live) const {
+    const u32x4 rs = buffer(base);
+    const uint32_t at = __builtin_amdgcn_readfirstlane(dst + (threadIdx.x >> 6) * 1024);
+#pragma unroll
+    for (int p = 0; p < PER; ++p) piece(rs, at + p * 4096, live(p) ? off[p] : kNoRow);
+  }
+  static __device__ __forceinline__ u32x4 buffer(const uint16_t* base) {                       // raw buffer of 2 GiB
+    const uint64_t p64 = reinterpret_cast<uint64_t>(base);
+    return u32x4{static_cast<uint32_t>(p64), static_cast<uint32_t>(p64 >> 32) & 0xffffu, 0x80000000u, 0x00020000u};
   }
   // 64 lanes x 16 bytes to LDS addresses dst + 16 lane.  Inline, because the compiler waits for the builtin's load before any LDS read that it
   // cannot tell apart - the other buffer's; tile_barrier() waits instead.  (No destination registers.)
@@ -209,6 +219,8 @@ __device__ __forceinline__ int64_t xcd_order(int64_t bid, int64_t total) {
   return x * per + (x < rest ? x : rest) + i;
 }
 
+__device__ __forceinline__ int over(int r, int G) { return G == 1 ? r : static_cast<int>(static_cast<uint32_t>(r) / static_cast<uint32_t>(G)); }
+
 template <typename T> __device__ __forceinline__ uint2 pack4(float a, float b, float c, float d) { return make_uint2(T::pack(a, b), T::pack(c, d)); }
 
 // ===================================================================================================================== forward
@@ -228,14 +240,13 @@ __global__ __launch_bounds__(256, 2) void mha_fwd_kernel(const MhaArgs a) {
   w -= static_cast<int64_t>(hk) * a.tiles * a.splits;
   const int tile = a.tiles - 1 - static_cast<int>(w / a.splits), split = static_cast<int>(w % a.splits);   // causal: long tiles first
   const Limits lim(a, b);
-  const int64_t R = static_cast<int64_t>(a.Nq) * a.G, row0 = static_cast<int64_t>(tile) * ROWS;
+  const int R = a.Nq * a.G, row0 = tile * ROWS;                        // (31 bits: checked on the host)
   const uint16_t* qb = a.q + b * a.vq.b + static_cast<int64_t>(hk) * a.G * a.vq.h;
   const uint16_t* kb = a.k + b * a.vk.b + hk * a.vk.h;
   const uint16_t* vb = a.v + b * a.vv.b + hk * a.vv.h;
 
   // the workgroup's keys
-  const int64_t last_row = (row0 + ROWS < R ? row0 + ROWS : R) - 1;
-  const int first_tok = static_cast<int>(row0 / a.G), last_tok = min(static_cast<int>(last_row / a.G), lim.q_len - 1);
+  const int first_tok = over(row0, a.G), last_tok = min(over(min(row0 + ROWS, R) - 1, a.G), lim.q_len - 1);
   const int k_begin = split * a.span;
   const int k_end = min(first_tok <= last_tok ? lim.end(last_tok, a.causal) : 0, k_begin + a.span);
   Stage<D> sk, sv;
@@ -253,9 +264,9 @@ __global__ __launch_bounds__(256, 2) void mha_fwd_kernel(const MhaArgs a) {
   u32x4 qf[RB][KS];
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
-    const int64_t r = row0 + wave * 32 * RB + rb * 32 + l32;
-    tok[rb] = r < R ? static_cast<int>(r / a.G) : a.Nq;
-    hd[rb] = r < R ? static_cast<int>(r - static_cast<int64_t>(tok[rb]) * a.G) : 0;
+    const int r = row0 + wave * 32 * RB + rb * 32 + l32;
+    tok[rb] = r < R ? over(r, a.G) : a.Nq;
+    hd[rb] = r < R ? r - tok[rb] * a.G : 0;
     end[rb] = lim.end(tok[rb], a.causal);
     const bool live = tok[rb] < lim.q_len;
     const uint16_t* src = qb + (live ? tok[rb] * a.vq.n + hd[rb] * a.vq.h : 0);
@@ -409,15 +420,14 @@ __global__ __launch_bounds__(256, 2) void mha_dq_kernel(const MhaArgs a) {
   w -= static_cast<int64_t>(hk) * a.tiles * a.splits;
   const int tile = a.tiles - 1 - static_cast<int>(w / a.splits), split = static_cast<int>(w % a.splits);
   const Limits lim(a, b);
-  const int64_t R = static_cast<int64_t>(a.Nq) * a.G, row0 = static_cast<int64_t>(tile) * ROWS;
+  const int R = a.Nq * a.G, row0 = tile * ROWS;                        // (31 bits: checked on the host)
   const uint16_t* qb = a.q + b * a.vq.b + static_cast<int64_t>(hk) * a.G * a.vq.h;
   const uint16_t* ob = a.out + b * a.vo.b + static_cast<int64_t>(hk) * a.G * a.vo.h;
   const uint16_t* gb = a.dout + b * a.vdo.b + static_cast<int64_t>(hk) * a.G * a.vdo.h;
   const uint16_t* kb = a.k + b * a.vk.b + hk * a.vk.h;
   const uint16_t* vb = a.v + b * a.vv.b + hk * a.vv.h;
 
-  const int64_t last_row = (row0 + ROWS < R ? row0 + ROWS : R) - 1;
-  const int first_tok = static_cast<int>(row0 / a.G), last_tok = min(static_cast<int>(last_row / a.G), lim.q_len - 1);
+  const int first_tok = over(row0, a.G), last_tok = min(over(min(row0 + ROWS, R) - 1, a.G), lim.q_len - 1);
   const int k_begin = split * a.span;
   const int k_end = min(first_tok <= last_tok ? lim.end(last_tok, a.causal) : 0, k_begin + a.span);
   Stage<D> sk, sv;
@@ -435,9 +445,9 @@ __global__ __launch_bounds__(256, 2) void mha_dq_kernel(const MhaArgs a) {
   u32x4 qf[RB][KS], gf[RB][KS];
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
-    const int64_t r = row0 + wave * 32 * RB + rb * 32 + l32;
-    tok[rb] = r < R ? static_cast<int>(r / a.G) : a.Nq;
-    hd[rb] = r < R ? static_cast<int>(r - static_cast<int64_t>(tok[rb]) * a.G) : 0;
+    const int r = row0 + wave * 32 * RB + rb * 32 + l32;
+    tok[rb] = r < R ? over(r, a.G) : a.Nq;
+    hd[rb] = r < R ? r - tok[rb] * a.G : 0;
     end[rb] = lim.end(tok[rb], a.causal);
     const bool live = end[rb] > 0;               // a row without keys has no gradient
     const int64_t i = live ? tok[rb] : 0, h = live ? hd[rb] : 0;
@@ -548,13 +558,16 @@ __global__ __launch_bounds__(256) void mha_dq_join_kernel(const MhaArgs a) {
       pack4<T>(x[0] * a.scale, x[1] * a.scale, x[2] * a.scale, x[3] * a.scale);
 }
 
-// dk, dv: workgroup = 4 wavefronts x 32 KB keys of one key head, over the rows that see them, 64 at a time.
-template <typename T, int D, int KB>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 1) void mha_dkv_kernel(const MhaArgs a) {
-  constexpr int KS = D / 16, DB = D / 32, KEYS = 128 * KB, RT = kKT, IMG = RT * D * 2;
+// dk, dv: workgroup = 4 wavefronts x 32 keys of one key head, over the rows that see them, a tile of up to 64 at a time: the 64 / G tokens
+// that fill one (or, with more than 64 heads on a key head, 64 heads of a token), so that a row's place in its tile never changes.
+// Here a lane is a key and lse and D belong to registers.  They enter as the products' initial values instead: lane l32 of the lower half
+// holds -lse / scale of row l32, of the upper half -D, as three bf16 terms (24 bits) in its first three k-slots, and one product with
+// ones in the lower (upper) half's slots leaves -lse / scale (-D) in the accumulators of S (of dout v^T): exp2 of S times scale log2(e) is P.
+template <typename T, int D>
+__global__ __launch_bounds__(256, D == 64 ? 2 : 1) void mha_dkv_kernel(const MhaArgs a) {
+  constexpr int KS = D / 16, DB = D / 32, KEYS = 128, RT = kKT, IMG = RT * D * 2;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * 2 * IMG];              // [buffer][q, dout]
-  __shared__ __attribute__((aligned(16))) float stat[2][2][RT];                          // [buffer][lse log2(e), D]
-  __shared__ __attribute__((aligned(16))) int row_end[2][RT];
+  __shared__ __attribute__((aligned(16))) int row_tok[RT];                               // token of a tile's row, from the tile's first
   const int wave = threadIdx.x >> 6, l32 = threadIdx.x & 31, half = (threadIdx.x >> 5) & 1;
   const int64_t per_b = static_cast<int64_t>(a.Hkv) * a.tiles;
   int64_t w = xcd_order(blockIdx.x, gridDim.x);
@@ -562,174 +575,179 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 1) void mha_dkv_kernel(const Mha
   w -= b * per_b;
   const int hk = static_cast<int>(w / a.tiles), tile = static_cast<int>(w - static_cast<int64_t>(hk) * a.tiles);
   const Limits lim(a, b);
-  const int64_t R = static_cast<int64_t>(lim.q_len) * a.G;             // padded queries are no rows here
   const uint16_t* qb = a.q + b * a.vq.b + static_cast<int64_t>(hk) * a.G * a.vq.h;
   const uint16_t* gb = a.dout + b * a.vdo.b + static_cast<int64_t>(hk) * a.G * a.vdo.h;
   const uint16_t* kb = a.k + b * a.vk.b + hk * a.vk.h;
   const uint16_t* vb = a.v + b * a.vv.b + hk * a.vv.h;
-  const int key0 = tile * KEYS;
-  // rows that see a key of this tile: all, or (causal) those from token key0 - off on
-  int64_t r_begin = a.causal ? static_cast<int64_t>(max(0, key0 - lim.off)) * a.G : 0;
-  r_begin -= r_begin % RT;
-  const int64_t r_end = key0 < lim.kv_len ? R : 0;
-  // Row r0 + row of a tile lies (row / G) tokens and row % G heads behind row r0 if G divides the tile; otherwise its place is found again for
-  // every tile.
-  const bool even = RT % a.G == 0;
+  const int key0 = tile * KEYS, key = key0 + wave * 32 + l32;
+
+  const int gt = min(a.G, RT), tt = RT / gt;                           // heads and tokens of a row tile
+  // first token that sees a key of this tile; every row from there on sees one
+  const int t_begin = a.causal ? max(0, key0 - lim.off) : 0, t_end = key0 < lim.kv_len ? lim.q_len : 0;
   Stage<D> sq, sg;
+  int tk[Stage<D>::PER], hd[Stage<D>::PER];
 #pragma unroll
   for (int p = 0; p < Stage<D>::PER; ++p) {
-    const int row = Stage<D>::row(p), i = row / a.G, j = row - i * a.G;
-    sq.off[p] = static_cast<uint32_t>((i * a.vq.n + j * a.vq.h) * 2) + Stage<D>::chunk(p);
-    sg.off[p] = static_cast<uint32_t>((i * a.vdo.n + j * a.vdo.h) * 2) + Stage<D>::chunk(p);
+    const int row = Stage<D>::row(p);
+    tk[p] = row / gt;
+    hd[p] = row - tk[p] * gt;
+    sq.off[p] = static_cast<uint32_t>((tk[p] * a.vq.n + hd[p] * a.vq.h) * 2) + Stage<D>::chunk(p);
+    sg.off[p] = static_cast<uint32_t>((tk[p] * a.vdo.n + hd[p] * a.vdo.h) * 2) + Stage<D>::chunk(p);
   }
+  if (threadIdx.x < RT) row_tok[threadIdx.x] = threadIdx.x / gt;
+  // the lane's rows' lse (lower half) or D (upper half)
+  int st_t[2], st_h[2];
+#pragma unroll
+  for (int blk = 0; blk < 2; ++blk) {
+    st_t[blk] = (blk * 32 + l32) / gt;
+    st_h[blk] = blk * 32 + l32 - st_t[blk] * gt;
+  }
+  const float* st_base = (half ? a.dvec : a.lse) + (b * a.H + static_cast<int64_t>(hk) * a.G) * a.Nq;
+  const float st_mul = half ? -1.f : -1.f / a.scale, st_none = half ? 0.f : -3e38f;
+  float st[2] = {0.f, 0.f};
   const uint32_t base = lds_addr(&lds[0]);
-  float st_l = 0.f, st_d = 0.f;
-  int st_e = 0;
-  auto fetch = [&](int64_t r0, uint32_t buffer) {
-    const int64_t i0 = r0 / a.G;
-    const int rows = static_cast<int>(R - r0 < RT ? R - r0 : RT);
-    if (!even) {
-      const int j0 = static_cast<int>(r0 - i0 * a.G);
-#pragma unroll
-      for (int p = 0; p < Stage<D>::PER; ++p) {
-        const int row = Stage<D>::row(p), i = (j0 + row) / a.G, j = j0 + row - i * a.G;
-        sq.off[p] = static_cast<uint32_t>((i * a.vq.n + j * a.vq.h) * 2) + Stage<D>::chunk(p);
-        sg.off[p] = static_cast<uint32_t>((i * a.vdo.n + j * a.vdo.h) * 2) + Stage<D>::chunk(p);
-      }
+  auto fetch = [&](int t0, int h0, uint32_t buffer) {
+    const int tokens = min(tt, t_end - t0), heads = a.G - h0;
+    const uint16_t *pq = qb + t0 * a.vq.n + h0 * a.vq.h, *pg = gb + t0 * a.vdo.n + h0 * a.vdo.h;
+    if (tokens * gt >= RT && heads >= gt) {
+      sq.load(pq, RT, base + buffer);
+      sg.load(pg, RT, base + buffer + IMG);
+    } else {
+      sq.load(pq, base + buffer, [&](int p) { return tk[p] < tokens && hd[p] < heads; });
+      sg.load(pg, base + buffer + IMG, [&](int p) { return tk[p] < tokens && hd[p] < heads; });
     }
-    sq.load(qb + i0 * a.vq.n, rows, base + buffer);
-    sg.load(gb + i0 * a.vdo.n, rows, base + buffer + IMG);
-    if (threadIdx.x < RT) {
-      const int64_t r = r0 + threadIdx.x;
-      st_l = INFINITY; st_d = 0.f; st_e = 0;
-      if (r < R) {
-        const int64_t i = r / a.G, s = (b * a.H + hk * a.G + (r - i * a.G)) * a.Nq + i;
-        st_e = lim.end(static_cast<int>(i), a.causal);
-        if (st_e > 0) { st_l = a.lse[s] * kLog2e; st_d = a.dvec[s]; }
-      }
+#pragma unroll
+    for (int blk = 0; blk < 2; ++blk) {
+      st[blk] = st_none;
+      if (st_t[blk] < tokens && st_h[blk] < heads) st[blk] = st_base[static_cast<int64_t>(h0 + st_h[blk]) * a.Nq + (t0 + st_t[blk])] * st_mul;
     }
   };
-  auto keep = [&](int buf) {
-    if (threadIdx.x < RT) { stat[buf][0][threadIdx.x] = st_l; stat[buf][1][threadIdx.x] = st_d; row_end[buf][threadIdx.x] = st_e; }
+  int t0 = t_begin, h0 = 0;                                            // the tile that is computed; the one after it:
+  auto after = [&](int& t, int& h) {
+    h += gt;
+    if (h >= a.G) { h = 0; t += tt; }
   };
-  if (r_begin < r_end) {
-    fetch(r_begin, 0);
-    keep(0);
-  }
-  int key[KB];
-  u32x4 kf[KB][KS], vf[KB][KS];
-  f32x16 dk[KB][DB], dv[KB][DB];
-#pragma unroll
-  for (int n = 0; n < KB; ++n) {
-    key[n] = key0 + wave * 32 * KB + n * 32 + l32;
-    const bool live = key[n] < lim.kv_len;
-    const int64_t j = live ? key[n] : 0;
+  if (t0 < t_end) fetch(t0, h0, 0);
+
+  u32x4 kf[KS], vf[KS];
+  f32x16 dk[DB], dv[DB];
+  {
+    const bool live = key < lim.kv_len;
+    const int64_t j = live ? key : 0;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      kf[n][ks] = vf[n][ks] = u32x4{0, 0, 0, 0};
+      kf[ks] = vf[ks] = u32x4{0, 0, 0, 0};
       if (live) {
-        kf[n][ks] = *reinterpret_cast<const u32x4*>(kb + j * a.vk.n + ks * 16 + half * 8);
-        vf[n][ks] = *reinterpret_cast<const u32x4*>(vb + j * a.vv.n + ks * 16 + half * 8);
+        kf[ks] = *reinterpret_cast<const u32x4*>(kb + j * a.vk.n + ks * 16 + half * 8);
+        vf[ks] = *reinterpret_cast<const u32x4*>(vb + j * a.vv.n + ks * 16 + half * 8);
       }
     }
-#pragma unroll
-    for (int db = 0; db < DB; ++db) { dk[n][db] = zeros16(); dv[n][db] = zeros16(); }
   }
+#pragma unroll
+  for (int db = 0; db < DB; ++db) { dk[db] = zeros16(); dv[db] = zeros16(); }
   const float c2 = a.scale * kLog2e;
   const Lane<D> L(base);
+  const uint32_t one2 = 0x3f803f80u, one1 = 0x00003f80u;               // bf16 (1, 1) and (1, 0)
+  const u32x4 ones_s = half ? u32x4{0, 0, 0, 0} : u32x4{one2, one1, 0, 0}, ones_d = half ? u32x4{one2, one1, 0, 0} : u32x4{0, 0, 0, 0};
   const int key_last = min(key0 + KEYS, lim.kv_len) - 1;
-  auto step = [&](int64_t r0, int buf) {
+  auto step = [&](int buf) {
     const uint32_t qimg = buf * 2 * IMG, gimg = qimg + IMG;
     tile_barrier();
-    const bool more = r0 + RT < r_end;
-    if (more) fetch(r0 + RT, (buf ^ 1) * 2 * IMG);
-    // a tile needs no mask if its first row (the one that sees least) sees the last key; keys beyond kv_len are zeros whose dk, dv are not kept
-    const bool masked = a.causal && row_end[buf][0] <= key_last;
+    u32x4 init[2];
+#pragma unroll
+    for (int blk = 0; blk < 2; ++blk) {
+      const float x = st[blk];
+      const uint32_t hi = __float_as_uint(x) & 0xffff0000u;            // truncated: the rest keeps its sign and 16 bits
+      const float y = x - __uint_as_float(hi);
+      const uint32_t mid = __float_as_uint(y) & 0xffff0000u;
+      const float z = y - __uint_as_float(mid);
+      init[blk] = u32x4{(hi >> 16) | mid, __float_as_uint(z) >> 16, 0, 0};
+    }
+    // a tile needs no mask if its first token sees the last key; keys beyond kv_len are zeros whose dk, dv are not kept
+    const bool masked = a.causal && t0 + lim.off < key_last;
+    const int lim_tok = key - t0 - lim.off;                            // masked: the row's token in the tile has to be at least this
+    after(t0, h0);
+    if (t0 < t_end) fetch(t0, h0, (buf ^ 1) * 2 * IMG);
 #pragma unroll
     for (int blk = 0; blk < RT / 32; ++blk) {
-      u32x4 pf[KB][2], df[KB][2];
+      u32x4 qr[KS], gr[KS];
 #pragma unroll
-      for (int n = 0; n < KB; ++n) {
-        f32x16 s = zeros16(), dp = zeros16();
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          s = T::mfma(L.row(qimg, blk, ks), kf[n][ks], s);
-          dp = T::mfma(L.row(gimg, blk, ks), vf[n][ks], dp);
-        }
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const float4 ll = *reinterpret_cast<const float4*>(&stat[buf][0][blk * 32 + 8 * g + 4 * half]);
-          const float4 dl = *reinterpret_cast<const float4*>(&stat[buf][1][blk * 32 + 8 * g + 4 * half]);
-          const float lv[4] = {ll.x, ll.y, ll.z, ll.w}, dv4[4] = {dl.x, dl.y, dl.z, dl.w};
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const float p = __builtin_amdgcn_exp2f(fmaf(s[4 * g + u], c2, -lv[u]));
-            s[4 * g + u] = p;
-            dp[4 * g + u] = p * (dp[4 * g + u] - dv4[u]);
-          }
-        }
-        if (masked) {
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const int4 e4 = *reinterpret_cast<const int4*>(&row_end[buf][blk * 32 + 8 * g + 4 * half]);
-            const int ev[4] = {e4.x, e4.y, e4.z, e4.w};
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              s[4 * g + u] = key[n] < ev[u] ? s[4 * g + u] : 0.f;
-              dp[4 * g + u] = key[n] < ev[u] ? dp[4 * g + u] : 0.f;
-            }
-          }
-        }
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            pf[n][t][j] = T::pack(s[t * 8 + 2 * j], s[t * 8 + 2 * j + 1]);
-            df[n][t][j] = T::pack(dp[t * 8 + 2 * j], dp[t * 8 + 2 * j + 1]);
-          }
+      for (int ks = 0; ks < KS; ++ks) {
+        qr[ks] = L.row(qimg, blk, ks);
+        gr[ks] = L.row(gimg, blk, ks);
       }
+      f32x16 s = Bf16::mfma(init[blk], ones_s, zeros16()), dp = Bf16::mfma(init[blk], ones_d, zeros16());
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        s = T::mfma(qr[ks], kf[ks], s);
+        dp = T::mfma(gr[ks], vf[ks], dp);
+      }
+      u32x4 gc[2][DB], qc[2][DB];
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
-          const u32x4 gt = L.col(gimg, blk, t, db), qt = L.col(qimg, blk, t, db);
+          gc[t][db] = L.col(gimg, blk, t, db);
+          qc[t][db] = L.col(qimg, blk, t, db);
+        }
 #pragma unroll
-          for (int n = 0; n < KB; ++n) {
-            dv[n][db] = T::mfma(gt, pf[n][t], dv[n][db]);
-            dk[n][db] = T::mfma(qt, df[n][t], dk[n][db]);
+      for (int r = 0; r < 16; ++r) {
+        s[r] = __builtin_amdgcn_exp2f(s[r] * c2);
+        dp[r] = s[r] * dp[r];
+      }
+      if (masked) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int4 e4 = *reinterpret_cast<const int4*>(&row_tok[blk * 32 + 8 * g + 4 * half]);
+          const int ev[4] = {e4.x, e4.y, e4.z, e4.w};
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            s[4 * g + u] = ev[u] >= lim_tok ? s[4 * g + u] : 0.f;
+            dp[4 * g + u] = ev[u] >= lim_tok ? dp[4 * g + u] : 0.f;
           }
         }
-    }
-    if (more) keep(buf ^ 1);
-  };
-  for (int64_t r0 = r_begin; r0 < r_end; r0 += 2 * RT) {
-    step(r0, 0);
-    if (r0 + RT < r_end) step(r0 + RT, 1);
-  }
-#pragma unroll
-  for (int n = 0; n < KB; ++n) {
-    if (key[n] >= a.Nk) continue;
-    const bool live = key[n] < lim.kv_len;
-    uint16_t* pk = a.dk + b * a.vdk.b + key[n] * a.vdk.n + hk * a.vdk.h;
-    uint16_t* pv = a.dv + b * a.vdv.b + key[n] * a.vdv.n + hk * a.vdv.h;
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        float x[4], y[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          x[u] = live ? dk[n][db][4 * g + u] * a.scale : 0.f;
-          y[u] = live ? dv[n][db][4 * g + u] : 0.f;
-        }
-        *reinterpret_cast<uint2*>(pk + db * 32 + 8 * g + 4 * half) = pack4<T>(x[0], x[1], x[2], x[3]);
-        *reinterpret_cast<uint2*>(pv + db * 32 + 8 * g + 4 * half) = pack4<T>(y[0], y[1], y[2], y[3]);
       }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        u32x4 pf, df;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          pf[j] = T::pack(s[t * 8 + 2 * j], s[t * 8 + 2 * j + 1]);
+          df[j] = T::pack(dp[t * 8 + 2 * j], dp[t * 8 + 2 * j + 1]);
+        }
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+          dv[db] = T::mfma(gc[t][db], pf, dv[db]);
+          dk[db] = T::mfma(qc[t][db], df, dk[db]);
+        }
+      }
+    }
+  };
+  while (t0 < t_end) {
+    step(0);
+    if (t0 < t_end) step(1);
   }
+  if (key >= a.Nk) return;
+  const bool live = key < lim.kv_len;
+  uint16_t* pk = a.dk + b * a.vdk.b + key * a.vdk.n + hk * a.vdk.h;
+  uint16_t* pv = a.dv + b * a.vdv.b + key * a.vdv.n + hk * a.vdv.h;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      float x[4], y[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        x[u] = live ? dk[db][4 * g + u] * a.scale : 0.f;
+        y[u] = live ? dv[db][4 * g + u] : 0.f;
+      }
+      *reinterpret_cast<uint2*>(pk + db * 32 + 8 * g + 4 * half) = pack4<T>(x[0], x[1], x[2], x[3]);
+      *reinterpret_cast<uint2*>(pv + db * 32 + 8 * g + 4 * half) = pack4<T>(y[0], y[1], y[2], y[3]);
+    }
 }
 
 // ===================================================================================================================== host
-constexpr int kRB = 1, kKB = 1;                  // 32-row (32-key) blocks of a wavefront
+constexpr int kRB = 1;                           // 32-row blocks of a wavefront
 
 // Splits of the keys for `groups` workgroups over Nk keys: enough to give the chip two workgroups per CU, at least 256 keys each.
 int splits_for(int64_t groups, int32_t Nk) {
@@ -779,8 +797,8 @@ int launch_bwd(MhaArgs& a, hipStream_t s) {
       hipLaunchKernelGGL((mha_dq_join_kernel<T, D>), dim3(static_cast<unsigned>((a.B * a.H * a.Nq * (D / 4) + 255) / 256)), dim3(256), 0, s, a);
   }
   if (a.Nk > 0) {
-    cut(a, (a.Nk + 128 * kKB - 1) / (128 * kKB), false);
-    hipLaunchKernelGGL((mha_dkv_kernel<T, D, kKB>), dim3(static_cast<unsigned>(a.B * a.Hkv * a.tiles)), dim3(256), 0, s, a);
+    cut(a, (a.Nk + 127) / 128, false);
+    hipLaunchKernelGGL((mha_dkv_kernel<T, D>), dim3(static_cast<unsigned>(a.B * a.Hkv * a.tiles)), dim3(256), 0, s, a);
   }
   return launch_status();
 }
