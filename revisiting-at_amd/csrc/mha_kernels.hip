@@ -604,7 +604,8 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void mha_dkv_kernel(const Mha
   }
   const float* st_base = (half ? a.dvec : a.lse) + (b * a.H + static_cast<int64_t>(hk) * a.G) * a.Nq;
   const float st_mul = half ? -1.f : -1.f / a.scale, st_none = half ? 0.f : -3e38f;
-  float st[2] = {0.f, 0.f};
+  float st[2] = {0.f, 0.f};                                            // as loaded: nothing waits for them before the next tile
+  bool st_ok[2] = {false, false};
   const uint32_t base = lds_addr(&lds[0]);
   auto fetch = [&](int t0, int h0, uint32_t buffer) {
     const int tokens = min(tt, t_end - t0), heads = a.G - h0;
@@ -618,8 +619,8 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void mha_dkv_kernel(const Mha
     }
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk) {
-      st[blk] = st_none;
-      if (st_t[blk] < tokens && st_h[blk] < heads) st[blk] = st_base[static_cast<int64_t>(h0 + st_h[blk]) * a.Nq + (t0 + st_t[blk])] * st_mul;
+      st_ok[blk] = st_t[blk] < tokens && st_h[blk] < heads;
+      if (st_ok[blk]) st[blk] = st_base[static_cast<int64_t>(h0 + st_h[blk]) * a.Nq + (t0 + st_t[blk])];
     }
   };
   int t0 = t_begin, h0 = 0;                                            // the tile that is computed; the one after it:
@@ -656,7 +657,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void mha_dkv_kernel(const Mha
     u32x4 init[2];
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk) {
-      const float x = st[blk];
+      const float x = st_ok[blk] ? st[blk] * st_mul : st_none;
       const uint32_t hi = __float_as_uint(x) & 0xffff0000u;            // truncated: the rest keeps its sign and 16 bits
       const float y = x - __uint_as_float(hi);
       const uint32_t mid = __float_as_uint(y) & 0xffff0000u;
