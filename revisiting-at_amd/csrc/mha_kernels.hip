@@ -197,9 +197,10 @@ struct Stage {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(dst), "v"(off), "s"(rs) : "memory");
   }
 };
-// this wavefront's pieces have landed, then everybody's
+// This wavefront's pieces have landed, then everybody's.  (The builtin, so that the compiler knows of the wait: it would wait once more, for
+// loads in front of the loop, behind the next tile's pieces.)
 __device__ __forceinline__ void tile_barrier() {
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0f70);            // vmcnt(0)
   __syncthreads();
 }
 
@@ -221,162 +222,193 @@ __device__ __forceinline__ int64_t xcd_order(int64_t bid, int64_t total) {
 
 __device__ __forceinline__ int over(int r, int G) { return G == 1 ? r : static_cast<int>(static_cast<uint32_t>(r) / static_cast<uint32_t>(G)); }
 
+// sum of a row's three bf16 terms (k-slots 0 .. 2 of its half) times ones: the product of four k-slots per half
+__device__ __forceinline__ f32x16 first_terms(u32x2 terms, u32x2 ones) {
+  return __builtin_amdgcn_mfma_f32_32x32x8bf16_1k(__builtin_bit_cast(s16x4, terms), __builtin_bit_cast(s16x4, ones), zeros16(), 0, 0, 0);
+}
+
 template <typename T> __device__ __forceinline__ uint2 pack4(float a, float b, float c, float d) { return make_uint2(T::pack(a, b), T::pack(c, d)); }
 
+// A workgroup of the forward or of dq: 128 rows of one key head against the keys [k_begin, k_end), tile by tile.
+template <int D>
+struct Tile {
+  static constexpr int IMG = kKT * D * 2;
+  Stage<D> sk, sv;
+  const uint16_t *kp, *vp;                       // the key head's first key
+  Limits lim;
+  int64_t b;
+  int hk, split;
+  int tok, hd, end;                              // this lane's row: token (Nq where there is none), head of the key head, first key it does not see
+  int wave_end;                                  // the same of the wavefront's rows together
+  int k_begin, k_end;
+  uint32_t base;
+
+  __device__ __forceinline__ Tile(const MhaArgs& a, uint32_t lds) : Tile(a, lds, xcd_order(blockIdx.x, gridDim.x)) {}
+  __device__ __forceinline__ Tile(const MhaArgs& a, uint32_t lds, int64_t w) : lim(a, w / (static_cast<int64_t>(a.Hkv) * a.tiles * a.splits)) {
+    const int per_h = a.tiles * a.splits;
+    b = w / (static_cast<int64_t>(a.Hkv) * per_h);
+    int rest = static_cast<int>(w - b * a.Hkv * per_h);
+    hk = rest / per_h;
+    rest -= hk * per_h;
+    const int tile = a.tiles - 1 - rest / a.splits;                    // causal: the long tiles first
+    split = rest % a.splits;
+    base = lds;
+    kp = a.k + b * a.vk.b + hk * a.vk.h;
+    vp = a.v + b * a.vv.b + hk * a.vv.h;
+    const int R = a.Nq * a.G, row0 = tile * 128, wave = threadIdx.x >> 6;                     // (31 bits: checked on the host)
+    // what the rows from `first` to `last` see of the keys
+    auto end_of = [&](int first, int last) {
+      const int t0 = over(first, a.G), t1 = min(over(min(last, R - 1), a.G), lim.q_len - 1);
+      return first < R && t0 <= t1 ? lim.end(t1, a.causal) : 0;
+    };
+    k_begin = split * a.span;
+    k_end = min(end_of(row0, row0 + 127), k_begin + a.span);
+    wave_end = __builtin_amdgcn_readfirstlane(min(end_of(row0 + wave * 32, row0 + wave * 32 + 31), k_end));
+    const int r = row0 + wave * 32 + (threadIdx.x & 31);
+    tok = r < R ? over(r, a.G) : a.Nq;
+    hd = r < R ? r - tok * a.G : 0;
+    end = lim.end(tok, a.causal);
+    sk.rows_apart(a.vk.n);
+    sv.rows_apart(a.vv.n);
+    if (k_begin < k_end) fetch(a, k_begin, 0);
+  }
+  __device__ __forceinline__ void fetch(const MhaArgs& a, int k0, uint32_t buffer) const {
+    sk.load(kp + k0 * a.vk.n, lim.kv_len - k0, base + buffer);
+    sv.load(vp + k0 * a.vv.n, lim.kv_len - k0, base + buffer + IMG);
+  }
+  // compute(first key, image) for every tile that the wavefront's rows see a key of
+  template <typename F>
+  __device__ __forceinline__ void walk(const MhaArgs& a, F compute) const {
+    auto step = [&](int k0, uint32_t image, uint32_t next) {
+      tile_barrier();                            // the tile is there, and nobody reads the other buffer any more
+      if (k0 + kKT < k_end) fetch(a, k0 + kKT, next);
+      if (wave_end > k0) compute(k0, image);
+    };
+    for (int k0 = k_begin; k0 < k_end; k0 += 2 * kKT) {
+      step(k0, 0, 2 * IMG);
+      if (k0 + kKT < k_end) step(k0 + kKT, 2 * IMG, 0);
+    }
+  }
+};
+
 // ===================================================================================================================== forward
-// Workgroup: 4 wavefronts x 32 RB rows of one key head, over the keys [split * span, + span).  Row r of the tile: lane.
+// Workgroup: 4 wavefronts x 32 rows of one key head, over the keys [split * span, + span).  A row is a lane.
 // The running maximum of a row moves only when a tile exceeds it by more than 2^kSlack: until then P grows to at most 2^8, which costs
 // neither type any accuracy (both are relative) and saves the rescaling of the result's registers.
-template <typename T, int D, int RB>
-__global__ __launch_bounds__(256, 2) void mha_fwd_kernel(const MhaArgs a) {
-  constexpr int KS = D / 16, DB = D / 32, ROWS = 128 * RB, IMG = kKT * D * 2;
+// What bounds it: per 32 x 32 block 8 (d = 64) products of 32 cycles and about 75 other instructions, 16 exponentials among them; the two
+// share the issue slots of a SIMD (a product takes about half its cycles from the others), at the clock that the power limit leaves.
+template <typename T, int D>
+#ifndef WF
+#define WF 2
+#endif
+#ifndef WQ
+#define WQ 2
+#endif
+#ifndef WK
+#define WK 2
+#endif
+__global__ __launch_bounds__(256, D == 64 ? WF : 2) void mha_fwd_kernel(const MhaArgs a) {
+  constexpr int KS = D / 16, DB = D / 32, IMG = kKT * D * 2;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * 2 * IMG];              // [buffer][k, v]
-  const int wave = threadIdx.x >> 6, l32 = threadIdx.x & 31, half = (threadIdx.x >> 5) & 1;
-  const int64_t per_b = static_cast<int64_t>(a.Hkv) * a.tiles * a.splits;
-  int64_t w = xcd_order(blockIdx.x, gridDim.x);
-  const int64_t b = w / per_b;
-  w -= b * per_b;
-  const int hk = static_cast<int>(w / (a.tiles * a.splits));
-  w -= static_cast<int64_t>(hk) * a.tiles * a.splits;
-  const int tile = a.tiles - 1 - static_cast<int>(w / a.splits), split = static_cast<int>(w % a.splits);   // causal: long tiles first
-  const Limits lim(a, b);
-  const int R = a.Nq * a.G, row0 = tile * ROWS;                        // (31 bits: checked on the host)
-  const uint16_t* qb = a.q + b * a.vq.b + static_cast<int64_t>(hk) * a.G * a.vq.h;
-  const uint16_t* kb = a.k + b * a.vk.b + hk * a.vk.h;
-  const uint16_t* vb = a.v + b * a.vv.b + hk * a.vv.h;
-
-  // the workgroup's keys
-  const int first_tok = over(row0, a.G), last_tok = min(over(min(row0 + ROWS, R) - 1, a.G), lim.q_len - 1);
-  const int k_begin = split * a.span;
-  const int k_end = min(first_tok <= last_tok ? lim.end(last_tok, a.causal) : 0, k_begin + a.span);
-  Stage<D> sk, sv;
-  sk.rows_apart(a.vk.n);
-  sv.rows_apart(a.vv.n);
-  const uint32_t base = lds_addr(&lds[0]);
-  auto fetch = [&](int k0, uint32_t buffer) {
-    sk.load(kb + k0 * a.vk.n, lim.kv_len - k0, base + buffer);
-    sv.load(vb + k0 * a.vv.n, lim.kv_len - k0, base + buffer + IMG);
-  };
-  if (k_begin < k_end) fetch(k_begin, 0);
-
-  // the lane's rows
-  int tok[RB], end[RB], hd[RB];
-  u32x4 qf[RB][KS];
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    const int r = row0 + wave * 32 * RB + rb * 32 + l32;
-    tok[rb] = r < R ? over(r, a.G) : a.Nq;
-    hd[rb] = r < R ? r - tok[rb] * a.G : 0;
-    end[rb] = lim.end(tok[rb], a.causal);
-    const bool live = tok[rb] < lim.q_len;
-    const uint16_t* src = qb + (live ? tok[rb] * a.vq.n + hd[rb] * a.vq.h : 0);
+  const Tile<D> w(a, lds_addr(&lds[0]));
+  const int half = (threadIdx.x >> 5) & 1;
+  u32x4 qf[KS];
+  {
+    const bool live = w.tok < w.lim.q_len;
+    const uint16_t* src = a.q + w.b * a.vq.b + (static_cast<int64_t>(w.hk) * a.G + w.hd) * a.vq.h + (live ? w.tok : 0) * a.vq.n;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      qf[rb][ks] = u32x4{0, 0, 0, 0};
-      if (live) qf[rb][ks] = *reinterpret_cast<const u32x4*>(src + ks * 16 + half * 8);
+      qf[ks] = u32x4{0, 0, 0, 0};
+      if (live) qf[ks] = *reinterpret_cast<const u32x4*>(src + ks * 16 + half * 8);
     }
   }
   const float c2 = a.scale * kLog2e;
-  float m[RB], l[RB];
-  f32x16 o[RB][DB];
+  float m = -INFINITY, l = 0.f;
+  f32x16 o[DB];
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    m[rb] = -INFINITY;
-    l[rb] = 0.f;
-#pragma unroll
-    for (int db = 0; db < DB; ++db) o[rb][db] = zeros16();
-  }
-  const Lane<D> L(base);
-  auto step = [&](int k0, uint32_t kimg, uint32_t next) {
+  for (int db = 0; db < DB; ++db) o[db] = zeros16();
+  const Lane<D> L(w.base);
+  auto compute = [&](int k0, uint32_t kimg) {
+    constexpr int NB = kKT / 32;
     const uint32_t vimg = kimg + IMG;
-    tile_barrier();                              // the tile is there, and nobody reads the other buffer any more
-    if (k0 + kKT < k_end) fetch(k0 + kKT, next);
+    f32x16 s[NB];
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      f32x16 s[2];
+    for (int blk = 0; blk < NB; ++blk) {
+      s[blk] = zeros16();
 #pragma unroll
-      for (int blk = 0; blk < 2; ++blk) {
-        s[blk] = zeros16();
+      for (int ks = 0; ks < KS; ++ks) s[blk] = T::mfma(L.row(kimg, blk, ks), qf[ks], s[blk]);
+    }
+    if (__any(w.end < k0 + kKT)) {
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s[blk] = T::mfma(L.row(kimg, blk, ks), qf[rb][ks], s[blk]);
-      }
-      if (__any(end[rb] < k0 + kKT)) {
-#pragma unroll
-        for (int blk = 0; blk < 2; ++blk)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int key = k0 + blk * 32 + (r & 3) + 8 * (r >> 2) + 4 * half;
-            s[blk][r] = key < end[rb] ? s[blk][r] : -INFINITY;
-          }
-      }
-      float mx = s[0][0];
-#pragma unroll
-      for (int blk = 0; blk < 2; ++blk)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[blk][r]);
-      mx = both_halves_max(mx) * c2;             // (c2 > 0: checked on the host)
-      if (__any(mx > m[rb] + kSlack)) {          // (uniform) lanes below keep their maximum: alpha = 1
-        const float mn = mx > m[rb] + kSlack ? mx : m[rb];
-        const float alpha = __builtin_amdgcn_exp2f(m[rb] - mn);       // m = -inf: 0
-        const float al = mn == m[rb] ? 1.f : alpha;
-        m[rb] = mn;
-        l[rb] *= al;
-#pragma unroll
-        for (int db = 0; db < DB; ++db)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) o[rb][db][r] *= al;
-      }
-      const float mu = m[rb] == -INFINITY ? 0.f : m[rb];
-#pragma unroll
-      for (int blk = 0; blk < 2; ++blk) {
+      for (int blk = 0; blk < NB; ++blk)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          s[blk][r] = __builtin_amdgcn_exp2f(fmaf(s[blk][r], c2, -mu));
-          l[rb] += s[blk][r];
+          const int key = k0 + blk * 32 + (r & 3) + 8 * (r >> 2) + 4 * half;
+          s[blk][r] = key < w.end ? s[blk][r] : -INFINITY;
         }
+    }
+    float mx = s[0][0];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          u32x4 p;
+    for (int blk = 0; blk < NB; ++blk)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) p[j] = T::pack(s[blk][t * 8 + 2 * j], s[blk][t * 8 + 2 * j + 1]);
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[blk][r]);
+    mx = both_halves_max(mx) * c2;               // (c2 > 0: checked on the host)
+    if (__any(mx > m + kSlack)) {                // lanes below keep their maximum
+      const bool up = mx > m + kSlack;
+      const float al = up ? __builtin_amdgcn_exp2f(m - mx) : 1.f;      // m = -inf: 0
+      m = up ? mx : m;
+      l *= al;
 #pragma unroll
-          for (int db = 0; db < DB; ++db) o[rb][db] = T::mfma(L.col(vimg, blk, t, db), p, o[rb][db]);
-        }
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[db][r] *= al;
+    }
+    const float mu = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int blk = 0; blk < NB; ++blk) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[blk][r] = __builtin_amdgcn_exp2f(fmaf(s[blk][r], c2, -mu));
+        l += s[blk][r];
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        u32x4 p;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[j] = T::pack(s[blk][t * 8 + 2 * j], s[blk][t * 8 + 2 * j + 1]);
+#pragma unroll
+        for (int db = 0; db < DB; ++db) o[db] = T::mfma(L.col(vimg, blk, t, db), p, o[db]);
       }
     }
   };
-  for (int k0 = k_begin; k0 < k_end; k0 += 2 * kKT) {
-    step(k0, 0, 2 * IMG);
-    if (k0 + kKT < k_end) step(k0 + kKT, 2 * IMG, 0);
-  }
+  w.walk(a, compute);
+
   // lane = row: results of the row in registers, d = db * 32 + (r & 3) + 8 (r >> 2) + 4 half
+  const float sum = both_halves_sum(l);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  if (w.tok >= a.Nq) return;
+  const int h = w.hk * a.G + w.hd;
+  const int64_t at = (w.b * a.H + h) * a.Nq + w.tok;
+  const float ls = sum == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(sum)) * kLn2;
+  if (a.splits > 1) {                            // this split's normalised result in 32 bits and its log sum exp
+    const int64_t rows = a.B * a.H * a.Nq;
+    float* po = a.part + (w.split * rows + at) * D;
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    const float sum = both_halves_sum(l[rb]);
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    if (tok[rb] >= a.Nq) continue;
-    const int h = hk * a.G + hd[rb];
-    const int64_t at = (b * a.H + h) * a.Nq + tok[rb];
-    const float ls = sum == 0.f ? -INFINITY : (m[rb] + __builtin_amdgcn_logf(sum)) * kLn2;
-    if (a.splits > 1) {                          // this split's normalised result in 32 bits and its log sum exp
-      float* po = a.part + (static_cast<int64_t>(split) * a.B * a.H * a.Nq + at) * D;
+    for (int db = 0; db < DB; ++db)
 #pragma unroll
-      for (int db = 0; db < DB; ++db)
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<float4*>(po + db * 32 + 8 * g + 4 * half) =
+            make_float4(o[db][4 * g] * inv, o[db][4 * g + 1] * inv, o[db][4 * g + 2] * inv, o[db][4 * g + 3] * inv);
+    if (half == 0) a.part[a.splits * rows * D + w.split * rows + at] = ls;
+  } else {
+    uint16_t* po = a.o + w.b * a.vo.b + w.tok * a.vo.n + h * a.vo.h;
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
-          *reinterpret_cast<float4*>(po + db * 32 + 8 * g + 4 * half) =
-              make_float4(o[rb][db][4 * g] * inv, o[rb][db][4 * g + 1] * inv, o[rb][db][4 * g + 2] * inv, o[rb][db][4 * g + 3] * inv);
-      if (half == 0) a.part[static_cast<int64_t>(a.splits) * a.B * a.H * a.Nq * D + static_cast<int64_t>(split) * a.B * a.H * a.Nq + at] = ls;
-    } else {
-      uint16_t* po = a.o + b * a.vo.b + tok[rb] * a.vo.n + h * a.vo.h;
+    for (int db = 0; db < DB; ++db)
 #pragma unroll
-      for (int db = 0; db < DB; ++db)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-          *reinterpret_cast<uint2*>(po + db * 32 + 8 * g + 4 * half) =
-              pack4<T>(o[rb][db][4 * g] * inv, o[rb][db][4 * g + 1] * inv, o[rb][db][4 * g + 2] * inv, o[rb][db][4 * g + 3] * inv);
-      if (a.lse && half == 0) a.lse[at] = ls;
-    }
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<uint2*>(po + db * 32 + 8 * g + 4 * half) =
+            pack4<T>(o[db][4 * g] * inv, o[db][4 * g + 1] * inv, o[db][4 * g + 2] * inv, o[db][4 * g + 3] * inv);
+    if (a.lse && half == 0) a.lse[at] = ls;
   }
 }
 
@@ -406,137 +438,91 @@ __global__ __launch_bounds__(256) void mha_join_kernel(const MhaArgs a) {
 }
 
 // ===================================================================================================================== backward
-// dq: workgroup = 4 wavefronts x 32 RB rows, over the keys [split * span, + span).  Also leaves D in dvec.
-template <typename T, int D, int RB>
-__global__ __launch_bounds__(256, 2) void mha_dq_kernel(const MhaArgs a) {
-  constexpr int KS = D / 16, DB = D / 32, ROWS = 128 * RB, IMG = kKT * D * 2;
+// dq: workgroup = 4 wavefronts x 32 rows, over the keys [split * span, + span).  Also leaves D in dvec.
+template <typename T, int D>
+__global__ __launch_bounds__(256, D == 64 ? WQ : 2) void mha_dq_kernel(const MhaArgs a) {
+  constexpr int KS = D / 16, DB = D / 32, IMG = kKT * D * 2;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * 2 * IMG];              // [buffer][k, v]
-  const int wave = threadIdx.x >> 6, l32 = threadIdx.x & 31, half = (threadIdx.x >> 5) & 1;
-  const int64_t per_b = static_cast<int64_t>(a.Hkv) * a.tiles * a.splits;
-  int64_t w = xcd_order(blockIdx.x, gridDim.x);
-  const int64_t b = w / per_b;
-  w -= b * per_b;
-  const int hk = static_cast<int>(w / (a.tiles * a.splits));
-  w -= static_cast<int64_t>(hk) * a.tiles * a.splits;
-  const int tile = a.tiles - 1 - static_cast<int>(w / a.splits), split = static_cast<int>(w % a.splits);
-  const Limits lim(a, b);
-  const int R = a.Nq * a.G, row0 = tile * ROWS;                        // (31 bits: checked on the host)
-  const uint16_t* qb = a.q + b * a.vq.b + static_cast<int64_t>(hk) * a.G * a.vq.h;
-  const uint16_t* ob = a.out + b * a.vo.b + static_cast<int64_t>(hk) * a.G * a.vo.h;
-  const uint16_t* gb = a.dout + b * a.vdo.b + static_cast<int64_t>(hk) * a.G * a.vdo.h;
-  const uint16_t* kb = a.k + b * a.vk.b + hk * a.vk.h;
-  const uint16_t* vb = a.v + b * a.vv.b + hk * a.vv.h;
-
-  const int first_tok = over(row0, a.G), last_tok = min(over(min(row0 + ROWS, R) - 1, a.G), lim.q_len - 1);
-  const int k_begin = split * a.span;
-  const int k_end = min(first_tok <= last_tok ? lim.end(last_tok, a.causal) : 0, k_begin + a.span);
-  Stage<D> sk, sv;
-  sk.rows_apart(a.vk.n);
-  sv.rows_apart(a.vv.n);
-  const uint32_t base = lds_addr(&lds[0]);
-  auto fetch = [&](int k0, uint32_t buffer) {
-    sk.load(kb + k0 * a.vk.n, lim.kv_len - k0, base + buffer);
-    sv.load(vb + k0 * a.vv.n, lim.kv_len - k0, base + buffer + IMG);
-  };
-  if (k_begin < k_end) fetch(k_begin, 0);
-
-  int tok[RB], end[RB], hd[RB];
-  float lse2[RB], dd[RB];
-  u32x4 qf[RB][KS], gf[RB][KS];
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    const int r = row0 + wave * 32 * RB + rb * 32 + l32;
-    tok[rb] = r < R ? over(r, a.G) : a.Nq;
-    hd[rb] = r < R ? r - tok[rb] * a.G : 0;
-    end[rb] = lim.end(tok[rb], a.causal);
-    const bool live = end[rb] > 0;               // a row without keys has no gradient
-    const int64_t i = live ? tok[rb] : 0, h = live ? hd[rb] : 0;
+  const Tile<D> w(a, lds_addr(&lds[0]));
+  const int half = (threadIdx.x >> 5) & 1, h = w.hk * a.G + w.hd;
+  const int64_t at = (w.b * a.H + h) * a.Nq + w.tok;
+  u32x4 qf[KS], gf[KS];
+  float lse2, dd;
+  {
+    const bool live = w.end > 0;                 // a row without keys has no gradient
+    const int64_t i = live ? w.tok : 0;
+    const uint16_t* pq = a.q + w.b * a.vq.b + h * a.vq.h + i * a.vq.n + half * 8;
+    const uint16_t* pg = a.dout + w.b * a.vdo.b + h * a.vdo.h + i * a.vdo.n + half * 8;
+    const uint16_t* po = a.out + w.b * a.vo.b + h * a.vo.h + i * a.vo.n + half * 8;
     float part = 0.f;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      qf[rb][ks] = gf[rb][ks] = u32x4{0, 0, 0, 0};
+      qf[ks] = gf[ks] = u32x4{0, 0, 0, 0};
       if (live) {
-        qf[rb][ks] = *reinterpret_cast<const u32x4*>(qb + i * a.vq.n + h * a.vq.h + ks * 16 + half * 8);
-        gf[rb][ks] = *reinterpret_cast<const u32x4*>(gb + i * a.vdo.n + h * a.vdo.h + ks * 16 + half * 8);
-        const u32x4 of = *reinterpret_cast<const u32x4*>(ob + i * a.vo.n + h * a.vo.h + ks * 16 + half * 8);
+        qf[ks] = *reinterpret_cast<const u32x4*>(pq + ks * 16);
+        gf[ks] = *reinterpret_cast<const u32x4*>(pg + ks * 16);
+        const u32x4 of = *reinterpret_cast<const u32x4*>(po + ks * 16);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          part = fmaf(T::lo(gf[rb][ks][j]), T::lo(of[j]), fmaf(T::hi(gf[rb][ks][j]), T::hi(of[j]), part));
+        for (int j = 0; j < 4; ++j) part = fmaf(T::lo(gf[ks][j]), T::lo(of[j]), fmaf(T::hi(gf[ks][j]), T::hi(of[j]), part));
       }
     }
-    dd[rb] = both_halves_sum(part);
-    const int64_t at = (b * a.H + hk * a.G + hd[rb]) * a.Nq + tok[rb];
-    lse2[rb] = live ? a.lse[at] * kLog2e : INFINITY;                 // exp2(s - inf) = 0
-    if (split == 0 && half == 0 && tok[rb] < a.Nq) a.dvec[at] = dd[rb];
+    dd = both_halves_sum(part);
+    lse2 = live ? a.lse[at] * kLog2e : INFINITY;                       // exp2(s - inf) = 0
+    if (w.split == 0 && half == 0 && w.tok < a.Nq) a.dvec[at] = dd;
   }
   const float c2 = a.scale * kLog2e;
-  f32x16 dq[RB][DB];
+  f32x16 dq[DB];
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-    for (int db = 0; db < DB; ++db) dq[rb][db] = zeros16();
-  const Lane<D> L(base);
-  auto step = [&](int k0, uint32_t kimg, uint32_t next) {
+  for (int db = 0; db < DB; ++db) dq[db] = zeros16();
+  const Lane<D> L(w.base);
+  auto compute = [&](int k0, uint32_t kimg) {
     const uint32_t vimg = kimg + IMG;
-    tile_barrier();
-    if (k0 + kKT < k_end) fetch(k0 + kKT, next);
+    const bool masked = __any(w.end < k0 + kKT);
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      const bool masked = __any(end[rb] < k0 + kKT);
+    for (int blk = 0; blk < kKT / 32; ++blk) {
+      f32x16 s = zeros16(), dp = zeros16();
 #pragma unroll
-      for (int blk = 0; blk < 2; ++blk) {
-        f32x16 s = zeros16(), dp = zeros16();
+      for (int ks = 0; ks < KS; ++ks) {
+        s = T::mfma(L.row(kimg, blk, ks), qf[ks], s);
+        dp = T::mfma(L.row(vimg, blk, ks), gf[ks], dp);
+      }
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          s = T::mfma(L.row(kimg, blk, ks), qf[rb][ks], s);
-          dp = T::mfma(L.row(vimg, blk, ks), gf[rb][ks], dp);
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, -lse2)) * (dp[r] - dd);
+      if (masked) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = k0 + blk * 32 + (r & 3) + 8 * (r >> 2) + 4 * half;
+          s[r] = key < w.end ? s[r] : 0.f;
         }
+      }
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, -lse2[rb])) * (dp[r] - dd[rb]);
-        if (masked) {
+      for (int t = 0; t < 2; ++t) {
+        u32x4 p;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int key = k0 + blk * 32 + (r & 3) + 8 * (r >> 2) + 4 * half;
-            s[r] = key < end[rb] ? s[r] : 0.f;
-          }
-        }
+        for (int j = 0; j < 4; ++j) p[j] = T::pack(s[t * 8 + 2 * j], s[t * 8 + 2 * j + 1]);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          u32x4 p;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) p[j] = T::pack(s[t * 8 + 2 * j], s[t * 8 + 2 * j + 1]);
-#pragma unroll
-          for (int db = 0; db < DB; ++db) dq[rb][db] = T::mfma(L.col(kimg, blk, t, db), p, dq[rb][db]);
-        }
+        for (int db = 0; db < DB; ++db) dq[db] = T::mfma(L.col(kimg, blk, t, db), p, dq[db]);
       }
     }
   };
-  for (int k0 = k_begin; k0 < k_end; k0 += 2 * kKT) {
-    step(k0, 0, 2 * IMG);
-    if (k0 + kKT < k_end) step(k0 + kKT, 2 * IMG, 0);
-  }
+  w.walk(a, compute);
+  if (w.tok >= a.Nq) return;
+  if (a.splits > 1) {
+    float* po = a.part + (w.split * a.B * a.H * a.Nq + at) * D;
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    if (tok[rb] >= a.Nq) continue;
-    const int h = hk * a.G + hd[rb];
-    if (a.splits > 1) {
-      float* po = a.part + (static_cast<int64_t>(split) * a.B * a.H * a.Nq + (b * a.H + h) * a.Nq + tok[rb]) * D;
+    for (int db = 0; db < DB; ++db)
 #pragma unroll
-      for (int db = 0; db < DB; ++db)
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<float4*>(po + db * 32 + 8 * g + 4 * half) =
+            make_float4(dq[db][4 * g], dq[db][4 * g + 1], dq[db][4 * g + 2], dq[db][4 * g + 3]);
+  } else {
+    uint16_t* po = a.dq + w.b * a.vdq.b + w.tok * a.vdq.n + h * a.vdq.h;
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
-          *reinterpret_cast<float4*>(po + db * 32 + 8 * g + 4 * half) =
-              make_float4(dq[rb][db][4 * g], dq[rb][db][4 * g + 1], dq[rb][db][4 * g + 2], dq[rb][db][4 * g + 3]);
-    } else {
-      uint16_t* po = a.dq + b * a.vdq.b + tok[rb] * a.vdq.n + h * a.vdq.h;
+    for (int db = 0; db < DB; ++db)
 #pragma unroll
-      for (int db = 0; db < DB; ++db)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-          *reinterpret_cast<uint2*>(po + db * 32 + 8 * g + 4 * half) =
-              pack4<T>(dq[rb][db][4 * g] * a.scale, dq[rb][db][4 * g + 1] * a.scale, dq[rb][db][4 * g + 2] * a.scale, dq[rb][db][4 * g + 3] * a.scale);
-    }
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<uint2*>(po + db * 32 + 8 * g + 4 * half) =
+            pack4<T>(dq[db][4 * g] * a.scale, dq[db][4 * g + 1] * a.scale, dq[db][4 * g + 2] * a.scale, dq[db][4 * g + 3] * a.scale);
   }
 }
 
@@ -564,7 +550,7 @@ __global__ __launch_bounds__(256) void mha_dq_join_kernel(const MhaArgs a) {
 // holds -lse / scale of row l32, of the upper half -D, as three bf16 terms (24 bits) in its first three k-slots, and one product with
 // ones in the lower (upper) half's slots leaves -lse / scale (-D) in the accumulators of S (of dout v^T): exp2 of S times scale log2(e) is P.
 template <typename T, int D>
-__global__ __launch_bounds__(256, D == 64 ? 2 : 1) void mha_dkv_kernel(const MhaArgs a) {
+__global__ __launch_bounds__(256, D == 64 ? WK : 1) void mha_dkv_kernel(const MhaArgs a) {
   constexpr int KS = D / 16, DB = D / 32, KEYS = 128, RT = kKT, IMG = RT * D * 2;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * 2 * IMG];              // [buffer][q, dout]
   __shared__ __attribute__((aligned(16))) int row_tok[RT];                               // token of a tile's row, from the tile's first
@@ -585,50 +571,34 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void mha_dkv_kernel(const Mha
   // first token that sees a key of this tile; every row from there on sees one
   const int t_begin = a.causal ? max(0, key0 - lim.off) : 0, t_end = key0 < lim.kv_len ? lim.q_len : 0;
   Stage<D> sq, sg;
-  int tk[Stage<D>::PER], hd[Stage<D>::PER];
 #pragma unroll
   for (int p = 0; p < Stage<D>::PER; ++p) {
-    const int row = Stage<D>::row(p);
-    tk[p] = row / gt;
-    hd[p] = row - tk[p] * gt;
-    sq.off[p] = static_cast<uint32_t>((tk[p] * a.vq.n + hd[p] * a.vq.h) * 2) + Stage<D>::chunk(p);
-    sg.off[p] = static_cast<uint32_t>((tk[p] * a.vdo.n + hd[p] * a.vdo.h) * 2) + Stage<D>::chunk(p);
+    const int row = Stage<D>::row(p), i = row / gt, j = row - i * gt;
+    sq.off[p] = static_cast<uint32_t>((i * a.vq.n + j * a.vq.h) * 2) + Stage<D>::chunk(p);
+    sg.off[p] = static_cast<uint32_t>((i * a.vdo.n + j * a.vdo.h) * 2) + Stage<D>::chunk(p);
   }
   if (threadIdx.x < RT) row_tok[threadIdx.x] = threadIdx.x / gt;
   // the lane's rows' lse (lower half) or D (upper half)
-  int st_t[2], st_h[2];
+  int st_off[2];
 #pragma unroll
   for (int blk = 0; blk < 2; ++blk) {
-    st_t[blk] = (blk * 32 + l32) / gt;
-    st_h[blk] = blk * 32 + l32 - st_t[blk] * gt;
+    const int row = blk * 32 + l32, i = row / gt;
+    st_off[blk] = (row - i * gt) * a.Nq + i;
   }
   const float* st_base = (half ? a.dvec : a.lse) + (b * a.H + static_cast<int64_t>(hk) * a.G) * a.Nq;
-  const float st_mul = half ? -1.f : -1.f / a.scale, st_none = half ? 0.f : -3e38f;
   float st[2] = {0.f, 0.f};                                            // as loaded: nothing waits for them before the next tile
-  bool st_ok[2] = {false, false};
   const uint32_t base = lds_addr(&lds[0]);
-  auto fetch = [&](int t0, int h0, uint32_t buffer) {
-    const int tokens = min(tt, t_end - t0), heads = a.G - h0;
-    const uint16_t *pq = qb + t0 * a.vq.n + h0 * a.vq.h, *pg = gb + t0 * a.vdo.n + h0 * a.vdo.h;
-    if (tokens * gt >= RT && heads >= gt) {
-      sq.load(pq, RT, base + buffer);
-      sg.load(pg, RT, base + buffer + IMG);
-    } else {
-      sq.load(pq, base + buffer, [&](int p) { return tk[p] < tokens && hd[p] < heads; });
-      sg.load(pg, base + buffer + IMG, [&](int p) { return tk[p] < tokens && hd[p] < heads; });
-    }
-#pragma unroll
-    for (int blk = 0; blk < 2; ++blk) {
-      st_ok[blk] = st_t[blk] < tokens && st_h[blk] < heads;
-      if (st_ok[blk]) st[blk] = st_base[static_cast<int64_t>(h0 + st_h[blk]) * a.Nq + (t0 + st_t[blk])];
-    }
+  int t0 = t_begin, h0 = 0;                                            // the tile that is fetched next
+  int rows = 0;                                                        // its rows (tokens of all G heads, or heads of a token: always the first ones)
+  auto fetch = [&](uint32_t buffer) {
+    rows = min(tt, t_end - t0) * min(gt, a.G - h0);
+    sq.load(qb + t0 * a.vq.n + h0 * a.vq.h, rows, base + buffer);
+    sg.load(gb + t0 * a.vdo.n + h0 * a.vdo.h, rows, base + buffer + IMG);
+    const float* ps = st_base + static_cast<int64_t>(h0) * a.Nq + t0;
+    st[0] = ps[l32 < rows ? st_off[0] : 0];
+    st[1] = ps[32 + l32 < rows ? st_off[1] : 0];
   };
-  int t0 = t_begin, h0 = 0;                                            // the tile that is computed; the one after it:
-  auto after = [&](int& t, int& h) {
-    h += gt;
-    if (h >= a.G) { h = 0; t += tt; }
-  };
-  if (t0 < t_end) fetch(t0, h0, 0);
+  if (t0 < t_end) fetch(0);
 
   u32x4 kf[KS], vf[KS];
   f32x16 dk[DB], dv[DB];
@@ -648,36 +618,42 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void mha_dkv_kernel(const Mha
   for (int db = 0; db < DB; ++db) { dk[db] = zeros16(); dv[db] = zeros16(); }
   const float c2 = a.scale * kLog2e;
   const Lane<D> L(base);
-  const uint32_t one2 = 0x3f803f80u, one1 = 0x00003f80u;               // bf16 (1, 1) and (1, 0)
-  const u32x4 ones_s = half ? u32x4{0, 0, 0, 0} : u32x4{one2, one1, 0, 0}, ones_d = half ? u32x4{one2, one1, 0, 0} : u32x4{0, 0, 0, 0};
-  const int key_last = min(key0 + KEYS, lim.kv_len) - 1;
+  const u32x2 ones = {0x3f803f80u, 0x00003f80u};                       // bf16 (1, 1, 1, 0)
+  const u32x2 ones_s = half ? u32x2{0, 0} : ones, ones_d = half ? ones : u32x2{0, 0};
+  const float st_mul = half ? -1.f : -1.f / a.scale;
+  const int last_tok[2] = {31 / gt, 63 / gt};                          // token in the tile of a block's last row
+  const int wave_key = key0 + wave * 32, wave_last = min(wave_key + 32, lim.kv_len) - 1;       // the wavefront's keys
   auto step = [&](int buf) {
     const uint32_t qimg = buf * 2 * IMG, gimg = qimg + IMG;
     tile_barrier();
-    u32x4 init[2];
+    const int t = t0, here = rows;
+    u32x2 init[2];
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk) {
-      const float x = st_ok[blk] ? st[blk] * st_mul : st_none;
+      const float x = blk * 32 + l32 < here ? st[blk] * st_mul : half ? 0.f : -3e38f;        // no row: P = exp2(-huge) = 0
       const uint32_t hi = __float_as_uint(x) & 0xffff0000u;            // truncated: the rest keeps its sign and 16 bits
       const float y = x - __uint_as_float(hi);
       const uint32_t mid = __float_as_uint(y) & 0xffff0000u;
       const float z = y - __uint_as_float(mid);
-      init[blk] = u32x4{(hi >> 16) | mid, __float_as_uint(z) >> 16, 0, 0};
+      init[blk] = u32x2{(hi >> 16) | mid, __float_as_uint(z) >> 16};
     }
-    // a tile needs no mask if its first token sees the last key; keys beyond kv_len are zeros whose dk, dv are not kept
-    const bool masked = a.causal && t0 + lim.off < key_last;
-    const int lim_tok = key - t0 - lim.off;                            // masked: the row's token in the tile has to be at least this
-    after(t0, h0);
-    if (t0 < t_end) fetch(t0, h0, (buf ^ 1) * 2 * IMG);
+    h0 += gt;
+    if (h0 >= a.G) { h0 = 0; t0 += tt; }
+    if (t0 < t_end) fetch((buf ^ 1) * 2 * IMG);
+    if (wave_last < wave_key) return;                                  // all its keys are padding
+    // a tile needs no mask if its first token sees the wavefront's last key; keys beyond kv_len are zeros whose dk, dv are not kept
+    const bool masked = a.causal && t + lim.off < wave_last;
+    const int lim_tok = key - t - lim.off;                             // masked: the row's token in the tile has to be at least this
 #pragma unroll
     for (int blk = 0; blk < RT / 32; ++blk) {
+      if (blk * 32 >= here || (a.causal && t + last_tok[blk] + lim.off < wave_key)) continue;    // no row, or none that sees a key
       u32x4 qr[KS], gr[KS];
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         qr[ks] = L.row(qimg, blk, ks);
         gr[ks] = L.row(gimg, blk, ks);
       }
-      f32x16 s = Bf16::mfma(init[blk], ones_s, zeros16()), dp = Bf16::mfma(init[blk], ones_d, zeros16());
+      f32x16 s = first_terms(init[blk], ones_s), dp = first_terms(init[blk], ones_d);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         s = T::mfma(qr[ks], kf[ks], s);
@@ -748,8 +724,6 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void mha_dkv_kernel(const Mha
 }
 
 // ===================================================================================================================== host
-constexpr int kRB = 1;                           // 32-row blocks of a wavefront
-
 // Splits of the keys for `groups` workgroups over Nk keys: enough to give the chip two workgroups per CU, at least 256 keys each.
 int splits_for(int64_t groups, int32_t Nk) {
   if (groups <= 0 || groups >= 256) return 1;
@@ -759,7 +733,7 @@ int splits_for(int64_t groups, int32_t Nk) {
   if (s > 64) s = 64;
   return s < 1 ? 1 : static_cast<int>(s);
 }
-int64_t row_tiles(int64_t Nq, int64_t G) { return (Nq * G + 128 * kRB - 1) / (128 * kRB); }
+int64_t row_tiles(int64_t Nq, int64_t G) { return (Nq * G + 127) / 128; }
 
 int check_args(const MhaArgs& a, int dtype, int32_t head_dim) {
   if (a.B < 0 || a.Nq < 0 || a.Nk < 0 || a.H < 1 || a.Hkv < 1) return APGD_ERR_SIZE;
@@ -784,7 +758,7 @@ void cut(MhaArgs& a, int64_t tiles, bool split) {
 template <typename T, int D>
 int launch_fwd(MhaArgs& a, hipStream_t s) {
   cut(a, row_tiles(a.Nq, a.G), true);
-  hipLaunchKernelGGL((mha_fwd_kernel<T, D, kRB>), dim3(static_cast<unsigned>(a.B * a.Hkv * a.tiles * a.splits)), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((mha_fwd_kernel<T, D>), dim3(static_cast<unsigned>(a.B * a.Hkv * a.tiles * a.splits)), dim3(256), 0, s, a);
   if (a.splits > 1)
     hipLaunchKernelGGL((mha_join_kernel<T, D>), dim3(static_cast<unsigned>((a.B * a.H * a.Nq * (D / 4) + 255) / 256)), dim3(256), 0, s, a);
   return launch_status();
@@ -793,7 +767,7 @@ template <typename T, int D>
 int launch_bwd(MhaArgs& a, hipStream_t s) {
   if (a.Nq > 0) {
     cut(a, row_tiles(a.Nq, a.G), true);
-    hipLaunchKernelGGL((mha_dq_kernel<T, D, kRB>), dim3(static_cast<unsigned>(a.B * a.Hkv * a.tiles * a.splits)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((mha_dq_kernel<T, D>), dim3(static_cast<unsigned>(a.B * a.Hkv * a.tiles * a.splits)), dim3(256), 0, s, a);
     if (a.splits > 1)
       hipLaunchKernelGGL((mha_dq_join_kernel<T, D>), dim3(static_cast<unsigned>((a.B * a.H * a.Nq * (D / 4) + 255) / 256)), dim3(256), 0, s, a);
   }
