@@ -1975,14 +1975,26 @@ def attention(qkv, num_heads, scale):
 
 
 # ------------------------------------------------------------------------------ heads: norm and rotation
+_NO_SWITCH = contextlib.nullcontext()
+
+
 def _on_device(t):
     """Context in which kernels on ``t`` are launched: its own device, also where another one is current."""
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _NO_SWITCH if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
+
+
+def _raw_stream():
+    """``_stream()`` without building a Stream object (3 us of the 20 that a small call takes)."""
+    return _SIDE.handle if _SIDE is not None else torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _check_heads(what, *named):
     """``named``: (name, tensor or None) - device tensors [B, N, H, d] of one type on one device."""
     first = named[0][1]
+    if all(isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 4 for _, t in named):
+        B, _, _, d = first.shape
+        if all(t.dtype is first.dtype and t.device == first.device and t.shape[0] == B and t.shape[3] == d for _, t in named[1:]):
+            return
     for name, t in named:
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{what}: {name} has to be a tensor, not {type(t).__name__}")
@@ -2013,6 +2025,13 @@ def _strides(*tensors):
     """(sample, token, head) strides of [B, N, H, d] tensors as one host array of the C ABI."""
     v = [s for t in tensors for s in t.stride()[:3]]
     return (ctypes.c_int64 * len(v))(*v)
+
+
+def _backward_once(gradients, ctx, grads):
+    """A backward that has no derivative of its own: where a graph of the gradient is recorded, using it raises."""
+    if torch.is_grad_enabled():
+        return torch.autograd.function.once_differentiable(gradients)(ctx, *grads)
+    return gradients(ctx, *grads)
 
 
 class _Rotation:
@@ -2072,7 +2091,7 @@ def _rope_forward(q, k, yq, yk, wq, wk, rot):
     B, N, Hq, d = q.shape
     _lib.check(_lib.load().cnx_qk_norm_rope_fwd(
         q.data_ptr(), k.data_ptr(), yq.data_ptr(), yk.data_ptr(), _code(q), _strides(q, k, yq, yk), _lib.ptr(wq), _lib.ptr(wk),
-        _code(w) if w is not None else 0, *rot.args(), B, N, Hq, k.shape[2], d, rot.eps, rot.norm, rot.interleaved, _stream()),
+        _code(w) if w is not None else 0, *rot.args(), B, N, Hq, k.shape[2], d, rot.eps, rot.norm, rot.interleaved, _raw_stream()),
         "cnx_qk_norm_rope_fwd")
 
 
@@ -2088,7 +2107,7 @@ def _rope_backward(dyq, dyk, q, k, dq, dk, wq, wk, rot, want_wq, want_wk):
     _lib.check(lib.cnx_qk_norm_rope_bwd(
         dyq.data_ptr(), dyk.data_ptr(), x[0].data_ptr(), x[1].data_ptr(), dq.data_ptr(), dk.data_ptr(), _lib.ptr(dwq), _lib.ptr(dwk),
         _lib.ptr(ws), _code(dyq), _strides(dyq, dyk, *x, dq, dk), _lib.ptr(wq), _lib.ptr(wk), _code(w) if w is not None else 0, *rot.args(),
-        B, N, Hq, dyk.shape[2], d, rot.eps, rot.norm, rot.interleaved, _stream()), "cnx_qk_norm_rope_bwd")
+        B, N, Hq, dyk.shape[2], d, rot.eps, rot.norm, rot.interleaved, _raw_stream()), "cnx_qk_norm_rope_bwd")
     return dwq, dwk
 
 
@@ -2115,8 +2134,11 @@ class _QkNormRope(torch.autograd.Function):
         return yq, yk
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dyq, dyk):
+    def backward(ctx, *grads):
+        return _backward_once(_QkNormRope._gradients, ctx, grads)
+
+    @staticmethod
+    def _gradients(ctx, dyq, dyk):
         q, k, wq, wk = ctx.saved_tensors
         dyq, dyk = _head_rows(dyq), _head_rows(dyk)
         dq = torch.empty(dyq.shape, device=dyq.device, dtype=dyq.dtype)
@@ -2162,7 +2184,7 @@ def _mha_forward(q, k, v, out, scale, causal, q_lens, kv_lens, want_lse):
     n = lib.cnx_mha_ws_floats(B, Nq, Nk, H, Hkv, d)
     ws = torch.empty(n, device=q.device, dtype=torch.float32) if n else None
     _lib.check(lib.cnx_mha_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _lib.ptr(lse), _lib.ptr(q_lens), _lib.ptr(kv_lens),
-                               _lib.ptr(ws), _strides(q, k, v, out), _code(q), B, Nq, Nk, H, Hkv, d, causal, scale, _stream()), "cnx_mha_fwd")
+                               _lib.ptr(ws), _strides(q, k, v, out), _code(q), B, Nq, Nk, H, Hkv, d, causal, scale, _raw_stream()), "cnx_mha_fwd")
     return lse
 
 
@@ -2175,7 +2197,7 @@ def _mha_backward(q, k, v, out, dout, lse, dq, dk, dv, scale, causal, q_lens, kv
     ws = torch.empty(n, device=q.device, dtype=torch.float32) if n else None
     _lib.check(lib.cnx_mha_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), lse.data_ptr(), dq.data_ptr(),
                                dk.data_ptr(), dv.data_ptr(), dvec.data_ptr(), _lib.ptr(q_lens), _lib.ptr(kv_lens), _lib.ptr(ws),
-                               _strides(q, k, v, out, dout, dq, dk, dv), _code(q), B, Nq, Nk, H, Hkv, d, causal, scale, _stream()), "cnx_mha_bwd")
+                               _strides(q, k, v, out, dout, dq, dk, dv), _code(q), B, Nq, Nk, H, Hkv, d, causal, scale, _raw_stream()), "cnx_mha_bwd")
 
 
 class _Mha(torch.autograd.Function):
@@ -2192,8 +2214,11 @@ class _Mha(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dout):
+    def backward(ctx, *grads):
+        return _backward_once(_Mha._gradients, ctx, grads)
+
+    @staticmethod
+    def _gradients(ctx, dout):
         q, k, v, out, lse, q_lens, kv_lens = ctx.saved_tensors
         dout = _head_rows(dout)
         dq, dk, dv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
@@ -2264,8 +2289,11 @@ class _AttentionRope(torch.autograd.Function):
         return out.view(B, N, C3 // 3)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dout):
+    def backward(ctx, *grads):
+        return _backward_once(_AttentionRope._gradients, ctx, grads)
+
+    @staticmethod
+    def _gradients(ctx, dout):
         qkv, yq, yk, wq, wk, out, lse = ctx.saved_tensors
         B, N, H, d = out.shape
         q, k, v = qkv.view(B, N, 3, H, d).unbind(2)
