@@ -412,7 +412,7 @@ __global__ __launch_bounds__(256, D == 64 ? WF : 2) void mha_fwd_kernel(const Mh
   }
 }
 
-// Joins the splits of the keys: out = sum_s exp(lse_s - lse) out_s.  D / 4 threads per row.
+// Joins the splits of the keys: out = sum_s exp(lse_s - lse) out_s.  D / 4 threads per row; eight splits' values are in flight at a time.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void mha_join_kernel(const MhaArgs a) {
   constexpr int TPR = D / 4;
@@ -420,21 +420,39 @@ __global__ __launch_bounds__(256) void mha_join_kernel(const MhaArgs a) {
   if (at >= rows) return;
   const int d4 = threadIdx.x % TPR;
   const float* ls = a.part + static_cast<int64_t>(a.splits) * rows * D;
-  float m = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, ls[s * rows + at]);
-  const float mu = m == -INFINITY ? 0.f : m;
-  float sum = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < a.splits; ++s) {
-    const float e = __builtin_amdgcn_exp2f((ls[s * rows + at] - mu) * kLog2e);
-    const float4 v = *reinterpret_cast<const float4*>(a.part + (s * rows + at) * D + d4 * 4);
-    sum += e;
-    x[0] = fmaf(e, v.x, x[0]); x[1] = fmaf(e, v.y, x[1]); x[2] = fmaf(e, v.z, x[2]); x[3] = fmaf(e, v.w, x[3]);
+  float m = -INFINITY, sum = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < a.splits; s0 += 8) {
+    float e[8];
+    float4 v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int64_t s = min(s0 + u, a.splits - 1);
+      e[u] = ls[s * rows + at];
+      v[u] = *reinterpret_cast<const float4*>(a.part + (s * rows + at) * D + d4 * 4);
+    }
+    float mn = m;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      if (s0 + u >= a.splits) e[u] = -INFINITY;
+      mn = fmaxf(mn, e[u]);
+    }
+    const float mu = mn == -INFINITY ? 0.f : mn, al = __builtin_amdgcn_exp2f((m - mu) * kLog2e);
+    m = mn;
+    sum *= al;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] *= al;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const float g = __builtin_amdgcn_exp2f((e[u] - mu) * kLog2e);
+      sum += g;
+      x[0] = fmaf(g, v[u].x, x[0]); x[1] = fmaf(g, v[u].y, x[1]); x[2] = fmaf(g, v[u].z, x[2]); x[3] = fmaf(g, v[u].w, x[3]);
+    }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int64_t bh = at / a.Nq, b = bh / a.H;
   const int i = static_cast<int>(at - bh * a.Nq), h = static_cast<int>(bh - b * a.H);
   *reinterpret_cast<uint2*>(a.o + b * a.vo.b + i * a.vo.n + h * a.vo.h + d4 * 4) = pack4<T>(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-  if (a.lse && d4 == 0) a.lse[at] = sum == 0.f ? -INFINITY : mu + __builtin_amdgcn_logf(sum) * kLn2;
+  if (a.lse && d4 == 0) a.lse[at] = sum == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(sum) * kLn2;
 }
 
 // ===================================================================================================================== backward
@@ -534,9 +552,13 @@ __global__ __launch_bounds__(256) void mha_dq_join_kernel(const MhaArgs a) {
   if (at >= rows) return;
   const int d4 = threadIdx.x % TPR;
   float x[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < a.splits; ++s) {
-    const float4 v = *reinterpret_cast<const float4*>(a.part + (s * rows + at) * D + d4 * 4);
-    x[0] += v.x; x[1] += v.y; x[2] += v.z; x[3] += v.w;
+  for (int s0 = 0; s0 < a.splits; s0 += 8) {
+    float4 v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = *reinterpret_cast<const float4*>(a.part + (min(s0 + u, a.splits - 1) * rows + at) * D + d4 * 4);
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (s0 + u < a.splits) { x[0] += v[u].x; x[1] += v[u].y; x[2] += v[u].z; x[3] += v[u].w; }
   }
   const int64_t bh = at / a.Nq, b = bh / a.H;
   const int i = static_cast<int>(at - bh * a.Nq), h = static_cast<int>(bh - b * a.H);
