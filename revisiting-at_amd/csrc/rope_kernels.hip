@@ -7,10 +7,11 @@
 //
 // The pass is bound by memory: d values in and out per head, a few operations each.  Layout: a thread owns 8 pairs = 16 values of one
 // head (two 16-byte pieces in 16-bit types), a group of 1, 2, 4, 8 or 16 lanes one head, so the mean of squares is at most four lane
-// exchanges and nothing of a head leaves its group.  The angles belong to a token, not to a head: the workgroup computes the cosines and
-// sines of its tokens once, into LDS, and all heads of q and k read them there.  Angles are products in 64 bits brought to (-1/2, 1/2]
-// turns before they are rounded to 32 (a position of 10^6 at frequency 1 would be off by 0.03 rad in 32 bits).  x r is computed again in the
-// backward instead of kept: it is in registers anyway and would cost as much memory as x.
+// exchanges and nothing of a head leaves its group.  The angles belong to a token, not to a head: a workgroup takes a few tokens of - where the
+// samples share their positions - several samples, computes the cosines and sines once into LDS, and all heads read them there; the next
+// head's pieces are in flight while one is worked on.  Angles are products in 64 bits brought to (-1/2, 1/2] turns before they are rounded to
+// 32 (a position of 10^6 at frequency 1 would be off by 0.03 rad in 32 bits).  x r is computed again in the backward instead of kept: it is in
+// registers anyway and would cost as much memory as x.
 // Sums (mean of squares, weight gradients) in 32 bits; one rounding to the output's type at the end.
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
@@ -26,8 +27,8 @@ inline int launch_status() { return static_cast<int>(hipGetLastError()); }
 
 constexpr int kMaxAxes = 4;
 constexpr int kMaxHead = 256;
-constexpr int kTokens = 8;                      // tokens of a workgroup's tile at most
-constexpr int kFwdGrid = 1 << 20;                // workgroups of the forward at most (they step over the rest)
+constexpr int kHeads = 4096;
+constexpr int kFwdGrid = 1 << 20;               // workgroups (a side) of the forward at most: they step over the rest
 constexpr int kBwdGrid = 1024;                  // workgroups (a side) of the backward at most: each leaves one row of partial weight gradients
 
 struct View {                                   // [B, N, H, d] with unit stride in d
@@ -40,6 +41,7 @@ struct Side {                                   // the queries' or the keys' ten
   const void* w;                                // [d] or NULL
   View vx, vdy, vo;
   int32_t heads;
+  uint32_t magic;                               // ceil(2^32 / heads): i / heads = mulhi(i, magic) for i * heads < 2^32
 };
 
 struct RopeArgs {
@@ -48,19 +50,21 @@ struct RopeArgs {
   const float* inv_freq;                        // [d / 2]
   float* part;                                  // backward: [2][gridDim.x][d] partial weight gradients or NULL
   int64_t pos_b;                                // elements between the samples' positions (0: shared)
-  int64_t tokens, N;                            // tokens = B * N
+  int64_t B, N, tiles;                          // tiles: of `tile` tokens x `samples` samples
   int32_t first1, first2, first3;               // first pair of the second, third and fourth axis (d / 2 where there is none)
-  int32_t axes, d, tile, w_dtype, pos_dtype, norm;
+  int32_t axes, d, tile, log_tile, samples, sample_tiles, w_dtype, pos_dtype, norm;
   float eps;
 };
 
 struct bf16_t { uint16_t u; };
 
+// 8 consecutive values as loaded and as 32-bit numbers
 template <typename T> struct Io;
 template <> struct Io<float> {
-  static __device__ __forceinline__ void load8(const float* p, float* x) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  struct Raw { float4 a, b; };
+  static __device__ __forceinline__ Raw raw8(const float* p) { return Raw{*reinterpret_cast<const float4*>(p), *reinterpret_cast<const float4*>(p + 4)}; }
+  static __device__ __forceinline__ void widen(const Raw& r, float* x) {
+    x[0] = r.a.x; x[1] = r.a.y; x[2] = r.a.z; x[3] = r.a.w; x[4] = r.b.x; x[5] = r.b.y; x[6] = r.b.z; x[7] = r.b.w;
   }
   static __device__ __forceinline__ void store8(float* p, const float* x) {
     *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
@@ -69,8 +73,9 @@ template <> struct Io<float> {
 };
 template <> struct Io<bf16_t> {
   typedef __attribute__((ext_vector_type(8))) __bf16 v8;
-  static __device__ __forceinline__ void load8(const bf16_t* p, float* x) {
-    const uint4 a = *reinterpret_cast<const uint4*>(p);
+  using Raw = uint4;
+  static __device__ __forceinline__ Raw raw8(const bf16_t* p) { return *reinterpret_cast<const uint4*>(p); }
+  static __device__ __forceinline__ void widen(const Raw& a, float* x) {
     const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -87,8 +92,9 @@ template <> struct Io<bf16_t> {
 };
 template <> struct Io<__half> {
   typedef __attribute__((ext_vector_type(8))) _Float16 v8;
-  static __device__ __forceinline__ void load8(const __half* p, float* x) {
-    const v8 v = *reinterpret_cast<const v8*>(p);
+  using Raw = v8;
+  static __device__ __forceinline__ Raw raw8(const __half* p) { return *reinterpret_cast<const v8*>(p); }
+  static __device__ __forceinline__ void widen(const Raw& v, float* x) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(v[i]);
   }
@@ -101,17 +107,22 @@ template <> struct Io<__half> {
 };
 
 // the 16 values of a thread: a = first members of its 8 pairs, b = second members
+template <typename T> struct Pairs { typename Io<T>::Raw lo, hi; };
 template <bool IL, typename T>
-__device__ __forceinline__ void load_pairs(const T* head, int j, int d, float* a, float* b) {
+__device__ __forceinline__ Pairs<T> raw_pairs(const T* head, int j, int d) {
+  return IL ? Pairs<T>{Io<T>::raw8(head + 16 * j), Io<T>::raw8(head + 16 * j + 8)} : Pairs<T>{Io<T>::raw8(head + 8 * j), Io<T>::raw8(head + d / 2 + 8 * j)};
+}
+template <bool IL, typename T>
+__device__ __forceinline__ void widen(const Pairs<T>& r, float* a, float* b) {
   if constexpr (IL) {
     float t[16];
-    Io<T>::load8(head + 16 * j, t);
-    Io<T>::load8(head + 16 * j + 8, t + 8);
+    Io<T>::widen(r.lo, t);
+    Io<T>::widen(r.hi, t + 8);
 #pragma unroll
     for (int i = 0; i < 8; ++i) { a[i] = t[2 * i]; b[i] = t[2 * i + 1]; }
   } else {
-    Io<T>::load8(head + 8 * j, a);
-    Io<T>::load8(head + d / 2 + 8 * j, b);
+    Io<T>::widen(r.lo, a);
+    Io<T>::widen(r.hi, b);
   }
 }
 template <bool IL, typename T>
@@ -144,14 +155,13 @@ __device__ __forceinline__ float group_sum(float v, int group) {
   return v;
 }
 
-// cosines and sines of the tile's tokens: cs[t][pair]
-__device__ __forceinline__ void tile_angles(const RopeArgs& a, int64_t t0, int nt, float2* cs) {
+// cosines and sines of tokens n0 .. n0 + nt - 1 of sample b: cs[t][pair]
+__device__ __forceinline__ void tile_angles(const RopeArgs& a, int64_t b, int64_t n0, int nt, float2* cs) {
   const int pairs = a.d >> 1;
   for (int e = threadIdx.x; e < nt * pairs; e += blockDim.x) {
     const int t = e / pairs, i = e - t * pairs;
     const int axis = (i >= a.first1) + (i >= a.first2) + (i >= a.first3);
-    const int64_t tok = t0 + t, b = tok / a.N, n = tok - b * a.N;
-    const int64_t at = b * a.pos_b + n * a.axes + axis;
+    const int64_t at = b * a.pos_b + (n0 + t) * a.axes + axis;
     double p;
     if (a.pos_dtype == CNX_POS_F32) p = static_cast<const float*>(a.pos)[at];
     else if (a.pos_dtype == CNX_POS_I32) p = static_cast<const int32_t*>(a.pos)[at];
@@ -162,11 +172,12 @@ __device__ __forceinline__ void tile_angles(const RopeArgs& a, int64_t t0, int n
   }
 }
 
-// blockIdx.y: 0 = queries, 1 = keys (so that a thread holds one side's weights and sums: 16 + 16 registers instead of 32 + 32)
+// blockIdx.y: 0 = queries, 1 = keys (so that a thread holds one side's sums)
 template <typename T, bool BWD, bool IL>
 __global__ __launch_bounds__(256, BWD ? 3 : 4) void qk_norm_rope_kernel(const RopeArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char lds_raw[];
-  float2* cs = reinterpret_cast<float2*>(lds_raw);                    // [tile][d / 2]
+  float* wl = reinterpret_cast<float*>(lds_raw);                      // [2][d / 2] weights of the pairs' first and second members
+  float2* cs = reinterpret_cast<float2*>(wl + a.d);                   // [tile][d / 2] cosines, sines
   const Side z = blockIdx.y ? a.k : a.q;
   const int d = a.d, pairs = d >> 1, tph = d >> 4;                    // tph: threads that hold a head
   int group = 1;
@@ -175,38 +186,59 @@ __global__ __launch_bounds__(256, BWD ? 3 : 4) void qk_norm_rope_kernel(const Ro
   const bool here = j < tph;                                          // d / 16 is no power of two: the group's last lanes idle
   const int jj = here ? j : 0;
   const float rd = 1.f / static_cast<float>(d);
-  float wa[8], wb[8], sa[8], sb[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int ia = IL ? 16 * jj + 2 * i : 8 * jj + i, ib = IL ? ia + 1 : ia + pairs;
-    wa[i] = weight_at<T>(z.w, a.w_dtype, ia);
-    wb[i] = weight_at<T>(z.w, a.w_dtype, ib);
-    sa[i] = sb[i] = 0.f;                                              // BWD: weight gradients of this thread's dims
+  if (a.norm) {
+    for (int e = threadIdx.x; e < d; e += 256) {
+      const int member = IL ? e & 1 : e >= pairs, pair = IL ? e >> 1 : member ? e - pairs : e;
+      wl[member * pairs + pair] = weight_at<T>(z.w, a.w_dtype, e);
+    }
   }
+  __syncthreads();
+  float sa[8], sb[8];                                                 // BWD: weight gradients of this thread's dims
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sa[i] = sb[i] = 0.f;
 
-  for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.tile; t0 < a.tokens; t0 += static_cast<int64_t>(gridDim.x) * a.tile) {
-    const int nt = static_cast<int>(a.tokens - t0 < a.tile ? a.tokens - t0 : a.tile);
+  for (int64_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
+    const int64_t nt0 = tile / a.sample_tiles, n0 = nt0 * a.tile, b0 = (tile - nt0 * a.sample_tiles) * a.samples;
+    const int nt = static_cast<int>(a.N - n0 < a.tile ? a.N - n0 : a.tile), ns = static_cast<int>(a.B - b0 < a.samples ? a.B - b0 : a.samples);
+    const T* px = static_cast<const T*>(z.x) + b0 * z.vx.b + n0 * z.vx.n;
+    const T* pg = static_cast<const T*>(z.dy) + b0 * z.vdy.b + n0 * z.vdy.n;
+    T* po = static_cast<T*>(z.o) + b0 * z.vo.b + n0 * z.vo.n;
+    // item = (sample, token, head): places past the tile's last token are passed over
+    const int items = (ns << a.log_tile) * z.heads;
+    struct Item { int s, t, h; bool live; };
+    auto item = [&](int it) {
+      const int i = it < items ? it : items - 1;
+      const int q = z.heads == 1 ? i : static_cast<int>(__umulhi(static_cast<uint32_t>(i), z.magic));
+      Item r = {q >> a.log_tile, q & (a.tile - 1), i - q * z.heads, it < items};
+      if (r.t >= nt) { r.t = nt - 1; r.live = false; }
+      return r;
+    };
+    Item cur = item(g0);
+    Pairs<T> rx, rg;
+    auto load = [&](const Item& i) {
+      if (!BWD || a.norm) rx = raw_pairs<IL>(px + i.s * z.vx.b + i.t * z.vx.n + i.h * z.vx.h, jj, d);
+      if constexpr (BWD) rg = raw_pairs<IL>(pg + i.s * z.vdy.b + i.t * z.vdy.n + i.h * z.vdy.h, jj, d);
+    };
+    if (items > 0) load(cur);
     if (a.pos) {
       __syncthreads();                                                // the last tile's readers are done
-      tile_angles(a, t0, nt, cs);
+      tile_angles(a, b0, n0, nt, cs);
       __syncthreads();
     }
-    const int items = nt * z.heads;
+#pragma unroll 1
     for (int it0 = 0; it0 < items; it0 += ngroups) {                  // (uniform trip count: the lane exchanges need whole wavefronts)
-      const int it = it0 + g0;
-      const bool live = here && it < items;
-      const int itc = it < items ? it : items - 1;
-      const int t = itc / z.heads, h = itc - t * z.heads;
-      const int64_t tok = t0 + t, b = tok / a.N, n = tok - b * a.N;
       float xa[8], xb[8], ga[8], gb[8], c[8], s[8];
-      if (!BWD || a.norm)
-        load_pairs<IL>(static_cast<const T*>(z.x) + b * z.vx.b + n * z.vx.n + h * z.vx.h, jj, d, xa, xb);
-      if constexpr (BWD)
-        load_pairs<IL>(static_cast<const T*>(z.dy) + b * z.vdy.b + n * z.vdy.n + h * z.vdy.h, jj, d, ga, gb);
-      T* o = static_cast<T*>(z.o) + b * z.vo.b + n * z.vo.n + h * z.vo.h;
+      if (!BWD || a.norm) widen<IL, T>(rx, xa, xb);
+      if constexpr (BWD) widen<IL, T>(rg, ga, gb);
+      const Item now = cur;
+      if (it0 + ngroups < items) {                                    // the next item's pieces
+        cur = item(it0 + ngroups + g0);
+        load(cur);
+      }
+      const bool live = here && now.live;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float2 v = a.pos ? cs[t * pairs + 8 * jj + i] : make_float2(1.f, 0.f);
+        const float2 v = a.pos ? cs[now.t * pairs + 8 * jj + i] : make_float2(1.f, 0.f);
         c[i] = v.x; s[i] = v.y;
       }
       if (a.norm) {                                                   // x -> x r
@@ -223,11 +255,12 @@ __global__ __launch_bounds__(256, BWD ? 3 : 4) void qk_norm_rope_kernel(const Ro
           for (int i = 0; i < 8; ++i) {                               // the rotation's transpose, then the norm's
             const float u = fmaf(ga[i], c[i], gb[i] * s[i]), v = fmaf(gb[i], c[i], -ga[i] * s[i]);
             const float ta = u * xa[i], tb = v * xb[i];
+            const float wa = wl[8 * jj + i], wb = wl[pairs + 8 * jj + i];
             sa[i] += live ? ta : 0.f;
             sb[i] += live ? tb : 0.f;
-            dot = fmaf(ta, wa[i], fmaf(tb, wb[i], dot));
-            ga[i] = u * wa[i];
-            gb[i] = v * wb[i];
+            dot = fmaf(ta, wa, fmaf(tb, wb, dot));
+            ga[i] = u * wa;
+            gb[i] = v * wb;
           }
           dot = group_sum(here ? dot : 0.f, group) * rd;
 #pragma unroll
@@ -237,7 +270,7 @@ __global__ __launch_bounds__(256, BWD ? 3 : 4) void qk_norm_rope_kernel(const Ro
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) { xa[i] *= wa[i]; xb[i] *= wb[i]; }
+          for (int i = 0; i < 8; ++i) { xa[i] *= wl[8 * jj + i]; xb[i] *= wl[pairs + 8 * jj + i]; }
         }
       } else if constexpr (BWD) {
 #pragma unroll
@@ -254,7 +287,7 @@ __global__ __launch_bounds__(256, BWD ? 3 : 4) void qk_norm_rope_kernel(const Ro
           gb[i] = fmaf(xb[i], c[i], xa[i] * s[i]);
         }
       }
-      if (live) store_pairs<IL>(o, j, d, ga, gb);
+      if (live) store_pairs<IL>(po + now.s * z.vo.b + now.t * z.vo.n + now.h * z.vo.h, j, d, ga, gb);
     }
   }
   if constexpr (BWD) {
@@ -281,26 +314,35 @@ __global__ __launch_bounds__(256, BWD ? 3 : 4) void qk_norm_rope_kernel(const Ro
   }
 }
 
-// dw[e] = sum over the workgroups' rows, in a fixed order: 16 columns x 16 row lanes, every lane its rows one after the other
-__global__ __launch_bounds__(256) void rope_dw_kernel(const float* __restrict__ part, int rows, int d, float* __restrict__ dwq,
-                                                      float* __restrict__ dwk) {
-  __shared__ float red[16][17];
+// dw[e] = sum over the workgroups' rows, in a fixed order: 16 columns x 64 row lanes, every lane its rows one after the other
+__global__ __launch_bounds__(1024) void rope_dw_kernel(const float* __restrict__ part, int rows, int d, float* __restrict__ dwq,
+                                                       float* __restrict__ dwk) {
+  __shared__ float red[64][17];
   float* dw = blockIdx.y ? dwk : dwq;
   const int col = threadIdx.x & 15, row = threadIdx.x >> 4, e = blockIdx.x * 16 + col;        // d is a multiple of 16
   float s = 0.f;
-  for (int r = row; r < rows; r += 16) s += part[(static_cast<int64_t>(blockIdx.y) * rows + r) * d + e];
+  for (int r0 = 0; r0 < rows; r0 += 512) {                            // eight loads at a time
+    float v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int r = r0 + u * 64 + row;
+      v[u] = r < rows ? part[(static_cast<int64_t>(blockIdx.y) * rows + r) * d + e] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) s += v[u];
+  }
   red[row][col] = s;
   __syncthreads();
   if (row == 0 && dw) {
     s = 0.f;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s += red[r][col];
+    for (int r = 0; r < 64; ++r) s += red[r][col];
     dw[e] = s;
   }
 }
 
 int check_args(RopeArgs& a, int dtype, const int32_t* sections, int64_t B, int64_t N, int32_t Hq, int32_t Hk, int32_t d) {
-  if (B < 0 || N < 0 || Hq < 0 || Hk < 0 || Hq > (1 << 20) || Hk > (1 << 20)) return APGD_ERR_SIZE;
+  if (B < 0 || N < 0 || Hq < 0 || Hk < 0 || Hq > kHeads || Hk > kHeads) return APGD_ERR_SIZE;
   if (!cnx_qk_norm_rope_supported(d)) return APGD_ERR_ARG;
   if (dtype != APGD_F32 && dtype != APGD_BF16 && dtype != APGD_F16) return APGD_ERR_DTYPE;
   if ((a.q.w || a.k.w) && a.w_dtype != APGD_F32 && a.w_dtype != dtype) return APGD_ERR_DTYPE;
@@ -317,15 +359,30 @@ int check_args(RopeArgs& a, int dtype, const int32_t* sections, int64_t B, int64
     if (first[a.axes] != d / 2) return APGD_ERR_ARG;
     a.first1 = first[1]; a.first2 = first[2]; a.first3 = first[3];
   }
-  a.tokens = B * N;
+  a.B = B;
   a.N = N;
   a.q.heads = Hq; a.k.heads = Hk; a.d = d;
+  a.q.magic = Hq > 1 ? static_cast<uint32_t>((0x100000000ULL + Hq - 1) / Hq) : 0;
+  a.k.magic = Hk > 1 ? static_cast<uint32_t>((0x100000000ULL + Hk - 1) / Hk) : 0;
   return APGD_OK;
+}
+
+// Tiles: up to 8 tokens of one sample, or - where the samples share their positions - of up to 8 samples, as long as that leaves the
+// chip 512 workgroups a side (fewer tokens for the smallest calls, whose time is one pass through the kernel).
+void cut(RopeArgs& a) {
+  a.log_tile = 3;
+  while (a.log_tile > 0 && ((a.N + (1 << a.log_tile) - 1) >> a.log_tile) * a.B < 512) --a.log_tile;
+  a.tile = 1 << a.log_tile;
+  const int64_t token_tiles = (a.N + a.tile - 1) / a.tile;
+  a.samples = 1;
+  while (a.pos_b == 0 && a.samples < 8 && a.samples < a.B && token_tiles * ((a.B + 2 * a.samples - 1) / (2 * a.samples)) >= 512) a.samples *= 2;
+  a.sample_tiles = static_cast<int32_t>((a.B + a.samples - 1) / a.samples);
+  a.tiles = token_tiles * a.sample_tiles;
 }
 
 template <bool BWD, bool IL>
 void launch(const RopeArgs& a, int dtype, unsigned grid, hipStream_t s) {
-  const size_t lds = static_cast<size_t>(a.tile > 4 || !BWD ? a.tile : 4) * a.d * 4;        // tile x d / 2 (cos, sin); BWD: 4 x d sums
+  const size_t lds = static_cast<size_t>(BWD && a.tile < 3 ? 4 : a.tile + 1) * a.d * 4;     // d weights and tile x d / 2 (cos, sin); BWD: 4 x d sums
   const dim3 blocks(grid, 2);
   if (dtype == APGD_F32) hipLaunchKernelGGL((qk_norm_rope_kernel<float, BWD, IL>), blocks, dim3(256), lds, s, a);
   else if (dtype == APGD_BF16) hipLaunchKernelGGL((qk_norm_rope_kernel<bf16_t, BWD, IL>), blocks, dim3(256), lds, s, a);
@@ -335,14 +392,6 @@ template <bool BWD>
 void launch(const RopeArgs& a, int dtype, bool interleaved, unsigned grid, hipStream_t s) {
   if (interleaved) launch<BWD, true>(a, dtype, grid, s);
   else launch<BWD, false>(a, dtype, grid, s);
-}
-
-// Tokens per workgroup: kTokens where that leaves the chip 512 workgroups a side or more, else fewer (a single token per workgroup for the
-// smallest calls, whose time is one pass through the kernel).
-int tile_for(int64_t tokens) {
-  int t = kTokens;
-  while (t > 1 && (tokens + t - 1) / t < 512) t >>= 1;
-  return t;
 }
 
 View view_of(const int64_t* s) { return View{s[0], s[1], s[2]}; }
@@ -365,12 +414,11 @@ int cnx_qk_norm_rope_fwd(const void* q, const void* k, void* yq, void* yk, int d
   a.pos = positions; a.pos_dtype = pos_dtype; a.pos_b = pos_batch_stride; a.axes = axes; a.inv_freq = inv_freq;
   a.norm = norm != 0; a.eps = eps;
   if (const int rc = check_args(a, dtype, sections, B, N, Hq, Hk, d)) return rc;
-  if (a.tokens == 0 || Hq + Hk == 0) return APGD_OK;
+  if (B == 0 || N == 0 || Hq + Hk == 0) return APGD_OK;
   if (!strides || (Hq && (!q || !yq)) || (Hk && (!k || !yk))) return APGD_ERR_NULL;
   a.q.vx = view_of(strides); a.k.vx = view_of(strides + 3); a.q.vo = view_of(strides + 6); a.k.vo = view_of(strides + 9);
-  a.tile = tile_for(a.tokens);
-  const int64_t grid = (a.tokens + a.tile - 1) / a.tile;
-  launch<false>(a, dtype, interleaved != 0, static_cast<unsigned>(grid < kFwdGrid ? grid : kFwdGrid), as_stream(stream));
+  cut(a);
+  launch<false>(a, dtype, interleaved != 0, static_cast<unsigned>(a.tiles < kFwdGrid ? a.tiles : kFwdGrid), as_stream(stream));
   return launch_status();
 }
 
@@ -387,20 +435,19 @@ int cnx_qk_norm_rope_bwd(const void* dyq, const void* dyk, const void* q, const 
   const bool want_w = a.norm && (dwq || dwk);
   if (want_w && !ws) return APGD_ERR_NULL;
   unsigned grid = 0;
-  if (a.tokens == 0 || Hq + Hk == 0) {
+  if (B == 0 || N == 0 || Hq + Hk == 0) {
     if (!want_w) return APGD_OK;                                      // else: the weights' gradients are zeros
   } else {
     if (!strides || (Hq && (!dyq || !dq || (norm && !q))) || (Hk && (!dyk || !dk || (norm && !k)))) return APGD_ERR_NULL;
     a.q.vdy = view_of(strides); a.k.vdy = view_of(strides + 3); a.q.vx = view_of(strides + 6); a.k.vx = view_of(strides + 9);
     a.q.vo = view_of(strides + 12); a.k.vo = view_of(strides + 15);
     a.part = want_w ? ws : nullptr;
-    a.tile = tile_for(a.tokens);
-    const int64_t tiles = (a.tokens + a.tile - 1) / a.tile;
-    grid = static_cast<unsigned>(tiles < kBwdGrid ? tiles : kBwdGrid);
+    cut(a);
+    grid = static_cast<unsigned>(a.tiles < kBwdGrid ? a.tiles : kBwdGrid);
     launch<true>(a, dtype, interleaved != 0, grid, as_stream(stream));
   }
   if (want_w)
-    hipLaunchKernelGGL(rope_dw_kernel, dim3(static_cast<unsigned>(d / 16), 2), dim3(256), 0, as_stream(stream), ws, static_cast<int>(grid), d, dwq, dwk);
+    hipLaunchKernelGGL(rope_dw_kernel, dim3(static_cast<unsigned>(d / 16), 2), dim3(1024), 0, as_stream(stream), ws, static_cast<int>(grid), d, dwq, dwk);
   return launch_status();
 }
 
