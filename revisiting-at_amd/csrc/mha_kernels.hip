@@ -298,16 +298,7 @@ struct Tile {
 // What bounds it: per 32 x 32 block 8 (d = 64) products of 32 cycles and about 75 other instructions, 16 exponentials among them; the two
 // share the issue slots of a SIMD (a product takes about half its cycles from the others), at the clock that the power limit leaves.
 template <typename T, int D>
-#ifndef WF
-#define WF 2
-#endif
-#ifndef WQ
-#define WQ 2
-#endif
-#ifndef WK
-#define WK 2
-#endif
-__global__ __launch_bounds__(256, D == 64 ? WF : 2) void mha_fwd_kernel(const MhaArgs a) {
+__global__ __launch_bounds__(256, 2) void mha_fwd_kernel(const MhaArgs a) {
   constexpr int KS = D / 16, DB = D / 32, IMG = kKT * D * 2;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * 2 * IMG];              // [buffer][k, v]
   const Tile<D> w(a, lds_addr(&lds[0]));
@@ -458,7 +449,7 @@ __global__ __launch_bounds__(256) void mha_join_kernel(const MhaArgs a) {
 // ===================================================================================================================== backward
 // dq: workgroup = 4 wavefronts x 32 rows, over the keys [split * span, + span).  Also leaves D in dvec.
 template <typename T, int D>
-__global__ __launch_bounds__(256, D == 64 ? WQ : 2) void mha_dq_kernel(const MhaArgs a) {
+__global__ __launch_bounds__(256, 2) void mha_dq_kernel(const MhaArgs a) {
   constexpr int KS = D / 16, DB = D / 32, IMG = kKT * D * 2;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * 2 * IMG];              // [buffer][k, v]
   const Tile<D> w(a, lds_addr(&lds[0]));
@@ -572,7 +563,7 @@ __global__ __launch_bounds__(256) void mha_dq_join_kernel(const MhaArgs a) {
 // holds -lse / scale of row l32, of the upper half -D, as three bf16 terms (24 bits) in its first three k-slots, and one product with
 // ones in the lower (upper) half's slots leaves -lse / scale (-D) in the accumulators of S (of dout v^T): exp2 of S times scale log2(e) is P.
 template <typename T, int D>
-__global__ __launch_bounds__(256, D == 64 ? WK : 1) void mha_dkv_kernel(const MhaArgs a) {
+__global__ __launch_bounds__(256, D == 64 ? 2 : 1) void mha_dkv_kernel(const MhaArgs a) {
   constexpr int KS = D / 16, DB = D / 32, KEYS = 128, RT = kKT, IMG = RT * D * 2;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * 2 * IMG];              // [buffer][q, dout]
   __shared__ __attribute__((aligned(16))) int row_tok[RT];                               // token of a tile's row, from the tile's first
