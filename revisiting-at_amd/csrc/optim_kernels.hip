@@ -16,7 +16,7 @@
 //      the update divides by it (rounded to zero it would make m / eps)
 // Rounding is to nearest, ties to even, by an integer addition.  Scaling by the block's maximum lets a block decay as a whole: the largest
 // element is always exact, which a fixed grid would keep from shrinking when b v rounds back to v.  A wavefront holds a block (4 elements per
-// lane): its maximum is six lane exchanges.  Maxima are taken of bit patterns, so that a NaN or infinite moment makes its block's scale (and
+// lane): its maximum is six steps through the lanes' neighbours (DPP).  Maxima are taken of bit patterns, so that a NaN or infinite moment makes its block's scale (and
 // with it the block) non-finite instead of vanishing.  The update uses the moments before they are rounded.
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -120,13 +120,21 @@ __device__ __forceinline__ uint32_t value_code(float x) {                       
   b -= one - TOP;
   return static_cast<uint32_t>(b < 0 ? 0 : b > TOP ? TOP : b);
 }
+// the wavefront's largest value, by shifts within rows of 16 lanes and two broadcasts across them (a lane exchange through LDS would cost more
+// than the rest of the block's arithmetic); the last lane has it, and all get it as a scalar
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t max_shifted(uint32_t v) {
+  const uint32_t o = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xf, false));
+  return o > v ? o : v;
+}
 __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-#pragma unroll
-  for (int m = 32; m > 0; m >>= 1) {
-    const uint32_t o = static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), m, 64));
-    v = o > v ? o : v;
-  }
-  return v;
+  v = max_shifted<0x111, 0xf>(v);                // row_shr:1, 2, 4, 8
+  v = max_shifted<0x112, 0xf>(v);
+  v = max_shifted<0x114, 0xf>(v);
+  v = max_shifted<0x118, 0xf>(v);
+  v = max_shifted<0x142, 0xa>(v);                // row_bcast:15 into rows 1 and 3
+  v = max_shifted<0x143, 0xc>(v);                // row_bcast:31 into rows 2 and 3
+  return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 63));
 }
 // a block's scale from the pattern of its largest magnitude: values too small to be divided by are no scale
 __device__ __forceinline__ float scale_of(uint32_t top) {
@@ -134,6 +142,7 @@ __device__ __forceinline__ float scale_of(uint32_t top) {
   return s < 1.17549435e-38f ? 0.f : s;
 }
 
+// (the quotient by v_rcp_f32, off by at most 1 ulp: a division's twelve instructions per element made the 8-bit step bound by them)
 __device__ __forceinline__ void update(const Coef& c, f32x4& p, f32x4 g, f32x4& m, f32x4& v, f32x4& root) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -141,7 +150,7 @@ __device__ __forceinline__ void update(const Coef& c, f32x4& p, f32x4 g, f32x4& 
     m[i] = m[i] * c.b1 + g[i] * c.nb1;
     v[i] = v[i] * c.b2 + (g[i] * g[i]) * c.nb2;
     root[i] = sqrtf(v[i]);
-    p[i] = p[i] - (m[i] / (root[i] * c.inv_root + c.eps)) * c.step_size;
+    p[i] = p[i] - (m[i] * __builtin_amdgcn_rcpf(root[i] * c.inv_root + c.eps)) * c.step_size;
   }
 }
 
@@ -157,7 +166,7 @@ __global__ void adamw_prepare_kernel(const cnx_adamw_tensor* __restrict__ table,
     c.decay = static_cast<float>(1.0 - lr * h.wd);
     c.b1 = static_cast<float>(h.b1); c.nb1 = static_cast<float>(1.0 - h.b1);
     c.b2 = static_cast<float>(h.b2); c.nb2 = static_cast<float>(1.0 - h.b2);
-    c.eps = static_cast<float>(h.eps);
+    c.eps = h.eps > 0.0 ? fmaxf(static_cast<float>(h.eps), 1.17549435e-38f) : 0.f;             // (v_rcp_f32 takes no subnormals)
     c.step_size = static_cast<float>(lr / (1.0 - pow(h.b1, static_cast<double>(t))));
     c.inv_root = static_cast<float>(1.0 / sqrt(1.0 - pow(h.b2, static_cast<double>(t))));
     coef[i] = c;
