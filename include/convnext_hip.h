@@ -375,10 +375,12 @@ int cnx_adamw_values(const uint8_t* m_codes, const float* m_scales, const uint8_
  * them are padding: never used, padded queries give zeros (lse -inf), padded rows of every gradient are zeros.  causal: query i sees keys
  * j <= i + kv_len - q_len (the last query sees the last key).  A query that sees no key gives zeros and no gradient.  A masked key's own
  * values have no influence, except that causal order needs finite v: the tile that holds a row's last key may hold later ones.
- * lse [B, H, Nq] (nullable in the forward) = log sum exp of the scaled scores.  ws: cnx_mha_ws_floats(...) floats (0 = none: NULL is
- * fine), for calls with few rows, whose keys are split over workgroups; dvec: B * H * Nq floats.  scale > 0.  Deterministic. */
+ * lse [B, H, Nq] (nullable in the forward) = log sum exp of the scaled scores.  ws: cnx_mha_ws_floats(...) floats for the forward,
+ * cnx_mha_bwd_ws_floats(...) for the backward (0 = none: NULL is fine), for calls with few rows or key tiles, which are split over
+ * workgroups and joined in a fixed order; dvec: B * H * Nq floats.  scale > 0.  Deterministic. */
 int cnx_mha_supported(int32_t head_dim);
 int64_t cnx_mha_ws_floats(int64_t B, int32_t Nq, int32_t Nk, int32_t H, int32_t Hkv, int32_t head_dim);
+int64_t cnx_mha_bwd_ws_floats(int64_t B, int32_t Nq, int32_t Nk, int32_t H, int32_t Hkv, int32_t head_dim, int32_t causal);
 /* strides: q, k, v, out x (sample, token, head) = 12 values */
 int cnx_mha_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const int32_t* q_lens, const int32_t* kv_lens, float* ws,
                 const int64_t* strides, int dtype, int64_t B, int32_t Nq, int32_t Nk, int32_t H, int32_t Hkv, int32_t head_dim,

@@ -98,6 +98,7 @@ PROTOTYPES = {
     "cnx_adamw_values": (C.c_int, [_p, _p, _p, _p, _p, _p, _i64, _p]),
     "cnx_mha_supported": (C.c_int, [_i32]),
     "cnx_mha_ws_floats": (C.c_int64, [_i64, _i32, _i32, _i32, _i32, _i32]),
+    "cnx_mha_bwd_ws_floats": (C.c_int64, [_i64, _i32, _i32, _i32, _i32, _i32, _i32]),
     "cnx_mha_fwd": (C.c_int, [_p, _p, _p, _p, _p, _p, _p, _p, _p, C.c_int, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _f, _p]),
     "cnx_mha_bwd": (C.c_int, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, C.c_int, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _f, _p]),
     "cnx_qk_norm_rope_supported": (C.c_int, [_i32]),

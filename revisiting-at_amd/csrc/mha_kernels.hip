@@ -24,6 +24,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "apgd_hip.h"
 #include "convnext_hip.h"
 
@@ -568,11 +570,13 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void mha_dkv_kernel(const Mha
   __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * 2 * IMG];              // [buffer][q, dout]
   __shared__ __attribute__((aligned(16))) int row_tok[RT];                               // token of a tile's row, from the tile's first
   const int wave = threadIdx.x >> 6, l32 = threadIdx.x & 31, half = (threadIdx.x >> 5) & 1;
-  const int64_t per_b = static_cast<int64_t>(a.Hkv) * a.tiles;
+  const int64_t per_h = static_cast<int64_t>(a.tiles) * a.splits, per_b = a.Hkv * per_h;
   int64_t w = xcd_order(blockIdx.x, gridDim.x);
   const int64_t b = w / per_b;
   w -= b * per_b;
-  const int hk = static_cast<int>(w / a.tiles), tile = static_cast<int>(w - static_cast<int64_t>(hk) * a.tiles);
+  const int hk = static_cast<int>(w / per_h);
+  w -= hk * per_h;
+  const int tile = static_cast<int>(w / a.splits), split = static_cast<int>(w - static_cast<int64_t>(tile) * a.splits);    // causal: long ones first
   const Limits lim(a, b);
   const uint16_t* qb = a.q + b * a.vq.b + static_cast<int64_t>(hk) * a.G * a.vq.h;
   const uint16_t* gb = a.dout + b * a.vdo.b + static_cast<int64_t>(hk) * a.G * a.vdo.h;
@@ -581,8 +585,10 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void mha_dkv_kernel(const Mha
   const int key0 = tile * KEYS, key = key0 + wave * 32 + l32;
 
   const int gt = min(a.G, RT), tt = RT / gt;                           // heads and tokens of a row tile
-  // first token that sees a key of this tile; every row from there on sees one
-  const int t_begin = a.causal ? max(0, key0 - lim.off) : 0, t_end = key0 < lim.kv_len ? lim.q_len : 0;
+  // first token that sees a key of this tile; every row from there on sees one.  The splits share these tokens equally.
+  const int t_first = a.causal ? max(0, key0 - lim.off) : 0, t_last = key0 < lim.kv_len ? lim.q_len : 0;
+  const int share = (max(0, t_last - t_first) + a.splits * tt - 1) / (a.splits * tt) * tt;
+  const int t_begin = min(t_first + split * share, max(t_first, t_last)), t_end = min(t_begin + share, t_last);
   Stage<D> sq, sg;
 #pragma unroll
   for (int p = 0; p < Stage<D>::PER; ++p) {
@@ -719,6 +725,20 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void mha_dkv_kernel(const Mha
   }
   if (key >= a.Nk) return;
   const bool live = key < lim.kv_len;
+  if (a.splits > 1) {                            // [split][dk, dv][sample, head, key][D] in 32 bits
+    const int64_t keys = a.B * a.Hkv * a.Nk, at = (b * a.Hkv + hk) * a.Nk + key;
+    float* pk = a.part + (2 * split * keys + at) * D + 4 * half;
+    float* pv = pk + keys * D;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int r = 4 * g, e = db * 32 + 8 * g;
+        *reinterpret_cast<float4*>(pk + e) = live ? make_float4(dk[db][r], dk[db][r + 1], dk[db][r + 2], dk[db][r + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+        *reinterpret_cast<float4*>(pv + e) = live ? make_float4(dv[db][r], dv[db][r + 1], dv[db][r + 2], dv[db][r + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    return;
+  }
   uint16_t* pk = a.dk + b * a.vdk.b + key * a.vdk.n + hk * a.vdk.h;
   uint16_t* pv = a.dv + b * a.vdv.b + key * a.vdv.n + hk * a.vdv.h;
 #pragma unroll
@@ -736,6 +756,30 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void mha_dkv_kernel(const Mha
     }
 }
 
+// dk = scale * sum of the splits' partial sums, dv = their sum, in their order
+template <typename T, int D>
+__global__ __launch_bounds__(256) void mha_dkv_join_kernel(const MhaArgs a) {
+  constexpr int TPR = D / 4;
+  const int64_t keys = a.B * a.Hkv * a.Nk, at = static_cast<int64_t>(blockIdx.x) * (256 / TPR) + threadIdx.x / TPR;
+  if (at >= keys) return;
+  const int d4 = threadIdx.x % TPR, is_v = blockIdx.y;
+  float x[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < a.splits; s0 += 4) {
+    float4 v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      v[u] = *reinterpret_cast<const float4*>(a.part + ((2 * static_cast<int64_t>(min(s0 + u, a.splits - 1)) + is_v) * keys + at) * D + d4 * 4);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (s0 + u < a.splits) { x[0] += v[u].x; x[1] += v[u].y; x[2] += v[u].z; x[3] += v[u].w; }
+  }
+  const int64_t bh = at / a.Nk, b = bh / a.Hkv;
+  const int j = static_cast<int>(at - bh * a.Nk), h = static_cast<int>(bh - b * a.Hkv);
+  const float mul = is_v ? 1.f : a.scale;
+  uint16_t* po = is_v ? a.dv + b * a.vdv.b + j * a.vdv.n + h * a.vdv.h : a.dk + b * a.vdk.b + j * a.vdk.n + h * a.vdk.h;
+  *reinterpret_cast<uint2*>(po + d4 * 4) = pack4<T>(x[0] * mul, x[1] * mul, x[2] * mul, x[3] * mul);
+}
+
 // ===================================================================================================================== host
 // Splits of the keys for `groups` workgroups over Nk keys: enough to give the chip two workgroups per CU, at least 256 keys each.
 int splits_for(int64_t groups, int32_t Nk) {
@@ -745,6 +789,26 @@ int splits_for(int64_t groups, int32_t Nk) {
   if (s > most) s = most;
   if (s > 64) s = 64;
   return s < 1 ? 1 : static_cast<int>(s);
+}
+// Splits of the rows that a tile of 128 keys meets in dk/dv: the count, 1 to 8, whose estimated time is least.  A workgroup takes about 2.3 us
+// per 64 rows, and the chip runs 512 of them at a time (256 at head dim 128); whole rounds of them are counted, causal ones as half the work
+// (long ones go first) at the lower clock of a chip that is busy throughout.  Against that stand a launch more and the splits' sums in 32 bits,
+// written and read.  Measured, us with the join: 2 x 4096 tokens, causal, 16 heads on 4, d = 128: 1 split 611, 2: 423, 3: 448, 4: 444, 6: 472;
+// 32 x 577 tokens, 12 heads, d = 64: 106, 186, 231, 299.
+int dkv_splits(int64_t B, int64_t Nq, int64_t Nk, int64_t Hkv, int64_t G, int d, bool causal) {
+  const double tiles = static_cast<double>(Nk + 127) / 128 * B * Hkv, slots = d == 64 ? 512 : 256, rows = static_cast<double>(Nq) * G;
+  if (tiles >= 8 * slots) return 1;
+  int best = 1;
+  double least = 0;
+  for (int s = 1; s <= 8 && (s == 1 || rows >= 256.0 * s); ++s) {
+    const double one = rows / 64 * 2.3 / s, groups = tiles * s;       // a workgroup that meets all its rows
+    double t;
+    if (causal) t = one * std::max(1.0, 0.625 * groups / slots);
+    else t = one * static_cast<double>(static_cast<int64_t>((groups + slots - 1) / slots));
+    if (s > 1) t += 5 + s * (static_cast<double>(B) * Nk * Hkv * d * 16) / 4e6;
+    if (s == 1 || t < least) { best = s; least = t; }
+  }
+  return best;
 }
 int64_t row_tiles(int64_t Nq, int64_t G) { return (Nq * G + 127) / 128; }
 
@@ -761,16 +825,16 @@ int check_args(const MhaArgs& a, int dtype, int32_t head_dim) {
   if (a.B > 0 && tiles > 0 && a.B > (1LL << 23) / tiles / a.H) return APGD_ERR_SIZE;
   return APGD_OK;
 }
-void cut(MhaArgs& a, int64_t tiles, bool split) {
+void cut(MhaArgs& a, int64_t tiles) {
   a.tiles = static_cast<int32_t>(tiles);
-  a.splits = split ? splits_for(a.B * a.Hkv * tiles, a.Nk) : 1;
+  a.splits = splits_for(a.B * a.Hkv * tiles, a.Nk);
   const int64_t per = ((a.Nk + a.splits - 1) / a.splits + kKT - 1) / kKT * kKT;
   a.span = static_cast<int32_t>(per < kKT ? kKT : per);
 }
 
 template <typename T, int D>
 int launch_fwd(MhaArgs& a, hipStream_t s) {
-  cut(a, row_tiles(a.Nq, a.G), true);
+  cut(a, row_tiles(a.Nq, a.G));
   hipLaunchKernelGGL((mha_fwd_kernel<T, D>), dim3(static_cast<unsigned>(a.B * a.Hkv * a.tiles * a.splits)), dim3(256), 0, s, a);
   if (a.splits > 1)
     hipLaunchKernelGGL((mha_join_kernel<T, D>), dim3(static_cast<unsigned>((a.B * a.H * a.Nq * (D / 4) + 255) / 256)), dim3(256), 0, s, a);
@@ -779,14 +843,17 @@ int launch_fwd(MhaArgs& a, hipStream_t s) {
 template <typename T, int D>
 int launch_bwd(MhaArgs& a, hipStream_t s) {
   if (a.Nq > 0) {
-    cut(a, row_tiles(a.Nq, a.G), true);
+    cut(a, row_tiles(a.Nq, a.G));
     hipLaunchKernelGGL((mha_dq_kernel<T, D>), dim3(static_cast<unsigned>(a.B * a.Hkv * a.tiles * a.splits)), dim3(256), 0, s, a);
     if (a.splits > 1)
       hipLaunchKernelGGL((mha_dq_join_kernel<T, D>), dim3(static_cast<unsigned>((a.B * a.H * a.Nq * (D / 4) + 255) / 256)), dim3(256), 0, s, a);
   }
   if (a.Nk > 0) {
-    cut(a, (a.Nk + 127) / 128, false);
-    hipLaunchKernelGGL((mha_dkv_kernel<T, D>), dim3(static_cast<unsigned>(a.B * a.Hkv * a.tiles)), dim3(256), 0, s, a);
+    a.tiles = (a.Nk + 127) / 128;
+    a.splits = dkv_splits(a.B, a.Nq, a.Nk, a.Hkv, a.G, D, a.causal != 0);
+    hipLaunchKernelGGL((mha_dkv_kernel<T, D>), dim3(static_cast<unsigned>(a.B * a.Hkv * a.tiles * a.splits)), dim3(256), 0, s, a);
+    if (a.splits > 1)
+      hipLaunchKernelGGL((mha_dkv_join_kernel<T, D>), dim3(static_cast<unsigned>((a.B * a.Hkv * a.Nk * (D / 4) + 255) / 256), 2), dim3(256), 0, s, a);
   }
   return launch_status();
 }
@@ -809,6 +876,14 @@ int64_t cnx_mha_ws_floats(int64_t B, int32_t Nq, int32_t Nk, int32_t H, int32_t 
   if (B > INT64_MAX / Hkv / tiles) return 0;
   const int s = splits_for(B * Hkv * tiles, Nk);
   return s > 1 ? static_cast<int64_t>(s) * B * H * Nq * (head_dim + 1) : 0;
+}
+
+int64_t cnx_mha_bwd_ws_floats(int64_t B, int32_t Nq, int32_t Nk, int32_t H, int32_t Hkv, int32_t head_dim, int32_t causal) {
+  const int64_t dq = cnx_mha_ws_floats(B, Nq, Nk, H, Hkv, head_dim);
+  if (B <= 0 || Nq <= 0 || Nk <= 0 || H < 1 || Hkv < 1 || H % Hkv || !cnx_mha_supported(head_dim)) return 0;
+  const int s = dkv_splits(B, Nq, Nk, Hkv, H / Hkv, head_dim, causal != 0);
+  const int64_t dkv = s > 1 ? static_cast<int64_t>(s) * 2 * B * Nk * Hkv * head_dim : 0;
+  return dq > dkv ? dq : dkv;
 }
 
 int cnx_mha_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const int32_t* q_lens, const int32_t* kv_lens, float* ws,
@@ -843,7 +918,7 @@ int cnx_mha_bwd(const void* q, const void* k, const void* v, const void* out, co
   if (B == 0 || (Nq == 0 && Nk == 0)) return APGD_OK;
   a.G = H / Hkv;
   if (!strides || (Nq > 0 && (!q || !out || !dout || !lse || !dq || !dvec)) || (Nk > 0 && (!k || !v || !dk || !dv))) return APGD_ERR_NULL;
-  if (cnx_mha_ws_floats(B, Nq, Nk, H, Hkv, head_dim) > 0 && !ws) return APGD_ERR_NULL;
+  if (cnx_mha_bwd_ws_floats(B, Nq, Nk, H, Hkv, head_dim, causal) > 0 && !ws) return APGD_ERR_NULL;
   a.vq = view_of(strides); a.vk = view_of(strides + 3); a.vv = view_of(strides + 6); a.vo = view_of(strides + 9); a.vdo = view_of(strides + 12);
   a.vdq = view_of(strides + 15); a.vdk = view_of(strides + 18); a.vdv = view_of(strides + 21);
   if (!near_enough(a.vq, a.G) || !near_enough(a.vk, 1) || !near_enough(a.vv, 1) || !near_enough(a.vdo, a.G)) return APGD_ERR_ARG;

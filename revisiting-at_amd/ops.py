@@ -2193,7 +2193,7 @@ def _mha_backward(q, k, v, out, dout, lse, dq, dk, dv, scale, causal, q_lens, kv
     B, Nq, H, d = q.shape
     Nk, Hkv = k.shape[1], k.shape[2]
     dvec = torch.empty(B, H, Nq, device=q.device, dtype=torch.float32)
-    n = lib.cnx_mha_ws_floats(B, Nq, Nk, H, Hkv, d)
+    n = lib.cnx_mha_bwd_ws_floats(B, Nq, Nk, H, Hkv, d, causal)
     ws = torch.empty(n, device=q.device, dtype=torch.float32) if n else None
     _lib.check(lib.cnx_mha_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), lse.data_ptr(), dq.data_ptr(),
                                dk.data_ptr(), dv.data_ptr(), dvec.data_ptr(), _lib.ptr(q_lens), _lib.ptr(kv_lens), _lib.ptr(ws),

@@ -265,6 +265,10 @@ MHA = [  # B, Nq, Nk, H, Hkv, d, causal, lens (q, kv) or None, layout
     (2, 17, 900, 2, 1, 64, False, ([17, 3], [900, 5]), "tokens"),                   # splits that hold no key
     (1, 577, 577, 2, 2, 64, False, None, "packed"),
     (1, 5, 0, 2, 2, 64, False, None, "tokens"),                # no key at all
+    (1, 700, 150, 4, 1, 64, True, None, "tokens"),             # few key tiles: dk and dv split over the rows
+    (2, 1100, 70, 2, 1, 128, False, ([1100, 9], [70, 33]), "heads"),
+    (1, 20, 140, 70, 1, 64, True, None, "packed"),             # more heads on a key head than rows in a tile
+    (2, 600, 600, 2, 1, 128, True, ([600, 5], [600, 300]), "tokens"),
 ]
 
 

@@ -22,8 +22,8 @@ def mha_fwd(lib, q=P, k=P, v=P, out=P, ws=P, strides=S12, dtype=1, B=1, Nq=4, Nk
     return lib.cnx_mha_fwd(q, k, v, out, None, None, None, ws, strides, dtype, B, Nq, Nk, H, Hkv, d, 0, scale, None)
 
 
-def mha_bwd(lib, q=P, dq=P, lse=P, dvec=P, dk=P, strides=S24, dtype=1, B=1, Nq=4, Nk=4, H=2, Hkv=1, d=64, scale=0.125):
-    return lib.cnx_mha_bwd(q, P, P, P, P, lse, dq, dk, P, dvec, None, None, P, strides, dtype, B, Nq, Nk, H, Hkv, d, 0, scale, None)
+def mha_bwd(lib, q=P, dq=P, lse=P, dvec=P, dk=P, ws=P, strides=S24, dtype=1, B=1, Nq=4, Nk=4, H=2, Hkv=1, d=64, scale=0.125):
+    return lib.cnx_mha_bwd(q, P, P, P, P, lse, dq, dk, P, dvec, None, None, ws, strides, dtype, B, Nq, Nk, H, Hkv, d, 0, scale, None)
 
 
 @pytest.mark.parametrize("kw,code", [
@@ -43,6 +43,9 @@ def test_mha_refuses_missing_outputs_and_workspace(R):
     assert mha_bwd(lib, dq=None) == NULL and mha_bwd(lib, lse=None) == NULL and mha_bwd(lib, dvec=None) == NULL and mha_bwd(lib, dk=None) == NULL
     assert lib.cnx_mha_ws_floats(1, 1, 5000, 2, 1, 64) > 0                     # few rows: the keys are split
     assert mha_fwd(lib, ws=None, Nq=1, Nk=5000) == NULL
+    assert lib.cnx_mha_bwd_ws_floats(1, 5000, 100, 2, 1, 64, 0) > 0 == lib.cnx_mha_ws_floats(1, 5000, 100, 2, 1, 64)     # few key tiles: the rows
+    assert mha_bwd(lib, ws=None, Nq=5000, Nk=100, H=2, Hkv=1) == NULL
+    assert lib.cnx_mha_bwd_ws_floats(1, 5000, 100, 2, 1, 80, 0) == 0 and lib.cnx_mha_bwd_ws_floats(64, 1025, 1025, 6, 6, 64, 0) == 0
     assert lib.cnx_mha_ws_floats(1, 1, 5000, 2, 1, 80) == 0 and lib.cnx_mha_ws_floats(0, 1, 1, 1, 1, 64) == 0
     assert mha_fwd(lib, Nq=0) == 0 and mha_bwd(lib, Nq=0, Nk=0) == 0
     assert [lib.cnx_mha_supported(d) for d in (0, 32, 64, 96, 128, 256)] == [0, 0, 1, 0, 1, 0]
