@@ -420,6 +420,18 @@ int cnx_qk_norm_rope_bwd(const void* dyq, const void* dyk, const void* q, const 
                          int64_t B, int64_t N, int32_t Hq, int32_t Hk, int32_t d, float eps, int32_t norm, int32_t interleaved,
                          void* stream);
 
+/* Backward pass of the two chained on a packed projection in one: mha's of q', k' and v, whose dq' and dk' go through the rotation and the
+ * norm where they are summed, in fp32, without a pass of their own.  qkv, dqkv [B, N, 3, H, d], yq, yk (q', k' as cnx_qk_norm_rope_fwd left
+ * them), out [B, N, H, d]: contiguous; dout: `dout_strides` (sample, token, head).  No lengths, not causal; wq, wk fp32 [d] or NULL; dwq, dwk
+ * fp32 [d] or NULL; the rest as above.  ws: cnx_attention_rope_bwd_ws_floats(...) floats (own_positions: the samples have their own);
+ * 0 = not in this form (few rows, which are split over workgroups: cnx_mha_bwd and cnx_qk_norm_rope_bwd). */
+int64_t cnx_attention_rope_bwd_ws_floats(int64_t B, int32_t N, int32_t H, int32_t head_dim, int32_t own_positions);
+int cnx_attention_rope_bwd(const void* qkv, const void* yq, const void* yk, const void* out, const void* dout, const float* lse, void* dqkv,
+                           float* dwq, float* dwk, float* ws, const int64_t* dout_strides, int dtype, const float* wq, const float* wk,
+                           const void* positions, int pos_dtype, int64_t pos_batch_stride, int32_t axes, const int32_t* sections,
+                           const float* inv_freq, int64_t B, int32_t N, int32_t H, int32_t head_dim, float eps, int32_t norm,
+                           int32_t interleaved, float scale, void* stream);
+
 /* Contraction over the ROW index of two row-major operands (round 5; csrc/wgrad_kernels.hip):
  *     D[N1][N2] = A^T B,   A: bf16 [M, N1] (row stride lda elements), B: bf16 [M, N2] (ldb), D: fp32 [N1, N2] contiguous
  * - the weight gradients of the pointwise convolutions and linears (models/convnext.py:42-46 backward: dW1 = dHpre^T LN(u),

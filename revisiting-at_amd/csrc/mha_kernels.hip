@@ -28,6 +28,7 @@
 
 #include "apgd_hip.h"
 #include "convnext_hip.h"
+#include "rope_internal.h"
 
 namespace {
 
@@ -43,6 +44,7 @@ typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
 typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
 typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((ext_vector_type(4), aligned(4))) float f32x4u;   // at any address of a float
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kKT = 64;                          // keys (rows) of a staged tile
@@ -75,6 +77,14 @@ struct View {                                    // 16-bit [B, N, heads, d], uni
   int64_t b, n, h;
 };
 
+// attention_rope's backward: the way back from q' (k') to q (k), at the end of dq (dk/dv)
+struct Turn {
+  const uint16_t* x;                             // q (k) as it was
+  View vx;
+  const float* w;                                // [D] or NULL
+  float* part;                                   // [workgroup][D] partial weight gradients or NULL
+};
+
 struct MhaArgs {
   const uint16_t *q, *k, *v, *out, *dout;        // out, dout: backward
   uint16_t *o, *dq, *dk, *dv;                    // o: forward
@@ -88,6 +98,11 @@ struct MhaArgs {
   int32_t span;                                  // keys of one split, a multiple of the key tile
   int64_t B;
   float scale;
+  Turn tq, tk;                                   // TURN: G = 1, no key splits, no lengths
+  const float2* cs;                              // cosines and sines [(B,) N][D / 2] or NULL
+  int64_t cs_b;                                  // pairs between the samples' (0: shared)
+  float eps;
+  int32_t norm, il;
 };
 
 // what a sample allows
@@ -449,8 +464,110 @@ __global__ __launch_bounds__(256) void mha_join_kernel(const MhaArgs a) {
 }
 
 // ===================================================================================================================== backward
-// dq: workgroup = 4 wavefronts x 32 rows, over the keys [split * span, + span).  Also leaves D in dvec.
+// The gradient g of a row of q' (k') becomes that of q (k) in the accumulators it is in: lane = row, d = db * 32 + (r & 3) + 8 (r >> 2) + 4 half,
+// so both members of a pair are one lane's, and a row's sums need one exchange of the two halves.  With z = x r w the normalised row, R its
+// rotation:  dz = R^T g,  dw = sum over the rows of dz * (x r),  dx = r (dz w - (x r) mean(dz w * (x r))).  Nothing is rounded in between.
 template <typename T, int D>
+__device__ __forceinline__ void turn_back(const MhaArgs& a, const Turn& t, f32x16 (&g)[D / 32], int64_t b, int tok, int h, bool live, unsigned char* lds) {
+  constexpr int DB = D / 32;
+  const int half = (threadIdx.x >> 5) & 1;
+  const int64_t i = live ? tok : 0;
+  if (a.cs) {
+    const float2* cs = a.cs + b * a.cs_b + i * (D / 2);
+    if (a.il) {
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float4 p = *reinterpret_cast<const float4*>(cs + db * 16 + 4 * q + 2 * half);  // (cos, sin) of two pairs
+          const float g0 = g[db][4 * q], g1 = g[db][4 * q + 1], g2 = g[db][4 * q + 2], g3 = g[db][4 * q + 3];
+          g[db][4 * q] = fmaf(g0, p.x, g1 * p.y);
+          g[db][4 * q + 1] = fmaf(g1, p.x, -g0 * p.y);
+          g[db][4 * q + 2] = fmaf(g2, p.z, g3 * p.w);
+          g[db][4 * q + 3] = fmaf(g3, p.z, -g2 * p.w);
+        }
+    } else {
+#pragma unroll
+      for (int db = 0; db < DB / 2; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+          const float4 p = *reinterpret_cast<const float4*>(cs + db * 32 + 8 * (r >> 2) + 4 * half + (r & 3));
+          const float g0 = g[db][r], g1 = g[db][r + 1], e0 = g[db + DB / 2][r], e1 = g[db + DB / 2][r + 1];
+          g[db][r] = fmaf(g0, p.x, e0 * p.y);
+          g[db + DB / 2][r] = fmaf(e0, p.x, -g0 * p.y);
+          g[db][r + 1] = fmaf(g1, p.z, e1 * p.w);
+          g[db + DB / 2][r + 1] = fmaf(e1, p.z, -g1 * p.w);
+        }
+    }
+  }
+  if (!a.norm) return;
+  const uint16_t* px = t.x + b * t.vx.b + i * t.vx.n + h * t.vx.h + 4 * half;
+  float x[DB][16], ss = 0.f;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint2 v = *reinterpret_cast<const uint2*>(px + db * 32 + 8 * q);
+      x[db][4 * q] = T::lo(v.x); x[db][4 * q + 1] = T::hi(v.x); x[db][4 * q + 2] = T::lo(v.y); x[db][4 * q + 3] = T::hi(v.y);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) ss = fmaf(x[db][4 * q + u], x[db][4 * q + u], ss);
+    }
+  const float rn = 1.f / sqrtf(both_halves_sum(ss) * (1.f / D) + a.eps);
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[db][r] *= rn;
+  if (t.part) {                                  // (uniform) the workgroup's 128 rows, through LDS: pieces of 16 bytes, spread over the banks by the row
+    float* rows = reinterpret_cast<float*>(lds);
+    const int row = (threadIdx.x >> 6) * 32 + (threadIdx.x & 31);
+    __syncthreads();                             // nobody reads tiles any more
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float e[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) e[u] = live ? g[db][4 * q + u] * x[db][4 * q + u] : 0.f;
+        *reinterpret_cast<float4*>(rows + row * D + (((db * 8 + 2 * q + half) ^ (row & (D / 4 - 1))) << 2)) = make_float4(e[0], e[1], e[2], e[3]);
+      }
+    __syncthreads();
+    constexpr int PARTS = 256 / D;
+    const int e = threadIdx.x % D, part = threadIdx.x / D;
+    float s = 0.f;
+#pragma unroll 8
+    for (int k = 0; k < 128 / PARTS; ++k) {
+      const int rr = part * (128 / PARTS) + k;
+      s += rows[rr * D + (((e >> 2) ^ (rr & (D / 4 - 1))) << 2) + (e & 3)];
+    }
+    __syncthreads();
+    rows[threadIdx.x] = s;
+    __syncthreads();
+    if (threadIdx.x < D) {
+#pragma unroll
+      for (int k = 1; k < PARTS; ++k) s += rows[k * D + e];
+      t.part[static_cast<int64_t>(blockIdx.x) * D + e] = s;
+    }
+  }
+  float dot = 0.f;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      f32x4u w = {1.f, 1.f, 1.f, 1.f};
+      if (t.w) w = *reinterpret_cast<const f32x4u*>(t.w + db * 32 + 8 * q + 4 * half);
+      g[db][4 * q] *= w.x; g[db][4 * q + 1] *= w.y; g[db][4 * q + 2] *= w.z; g[db][4 * q + 3] *= w.w;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) dot = fmaf(g[db][4 * q + u], x[db][4 * q + u], dot);
+    }
+  dot = both_halves_sum(dot) * (1.f / D);
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) g[db][r] = rn * fmaf(-x[db][r], dot, g[db][r]);
+}
+
+// dq: workgroup = 4 wavefronts x 32 rows, over the keys [split * span, + span).  Also leaves D in dvec.
+template <typename T, int D, bool TURN>
 __global__ __launch_bounds__(256, 2) void mha_dq_kernel(const MhaArgs a) {
   constexpr int KS = D / 16, DB = D / 32, IMG = kKT * D * 2;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * 2 * IMG];              // [buffer][k, v]
@@ -517,8 +634,17 @@ __global__ __launch_bounds__(256, 2) void mha_dq_kernel(const MhaArgs a) {
     }
   };
   w.walk(a, compute);
+  float mul = a.scale;
+  if constexpr (TURN) {
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dq[db][r] *= mul;
+    mul = 1.f;
+    turn_back<T, D>(a, a.tq, dq, w.b, w.tok, h, w.tok < a.Nq, lds);
+  }
   if (w.tok >= a.Nq) return;
-  if (a.splits > 1) {
+  if (!TURN && a.splits > 1) {
     float* po = a.part + (w.split * a.B * a.H * a.Nq + at) * D;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
@@ -533,7 +659,7 @@ __global__ __launch_bounds__(256, 2) void mha_dq_kernel(const MhaArgs a) {
 #pragma unroll
       for (int g = 0; g < 4; ++g)
         *reinterpret_cast<uint2*>(po + db * 32 + 8 * g + 4 * half) =
-            pack4<T>(dq[db][4 * g] * a.scale, dq[db][4 * g + 1] * a.scale, dq[db][4 * g + 2] * a.scale, dq[db][4 * g + 3] * a.scale);
+            pack4<T>(dq[db][4 * g] * mul, dq[db][4 * g + 1] * mul, dq[db][4 * g + 2] * mul, dq[db][4 * g + 3] * mul);
   }
 }
 
@@ -564,7 +690,7 @@ __global__ __launch_bounds__(256) void mha_dq_join_kernel(const MhaArgs a) {
 // Here a lane is a key and lse and D belong to registers.  They enter as the products' initial values instead: lane l32 of the lower half
 // holds -lse / scale of row l32, of the upper half -D, as three bf16 terms (24 bits) in its first three k-slots, and one product with
 // ones in the lower (upper) half's slots leaves -lse / scale (-D) in the accumulators of S (of dout v^T): exp2 of S times scale log2(e) is P.
-template <typename T, int D>
+template <typename T, int D, bool TURN>
 __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void mha_dkv_kernel(const MhaArgs a) {
   constexpr int KS = D / 16, DB = D / 32, KEYS = 128, RT = kKT, IMG = RT * D * 2;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * 2 * IMG];              // [buffer][q, dout]
@@ -723,6 +849,30 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void mha_dkv_kernel(const Mha
     step(0);
     if (t0 < t_end) step(1);
   }
+  if constexpr (TURN) {
+    const bool live = key < a.Nk;
+    if (live) {
+      uint16_t* pv = a.dv + b * a.vdv.b + key * a.vdv.n + hk * a.vdv.h;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<uint2*>(pv + db * 32 + 8 * g + 4 * half) = pack4<T>(dv[db][4 * g], dv[db][4 * g + 1], dv[db][4 * g + 2], dv[db][4 * g + 3]);
+    }
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dk[db][r] *= a.scale;
+    turn_back<T, D>(a, a.tk, dk, b, key, hk, live, lds);
+    if (!live) return;
+    uint16_t* pk = a.dk + b * a.vdk.b + key * a.vdk.n + hk * a.vdk.h;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<uint2*>(pk + db * 32 + 8 * g + 4 * half) = pack4<T>(dk[db][4 * g], dk[db][4 * g + 1], dk[db][4 * g + 2], dk[db][4 * g + 3]);
+    return;
+  }
   if (key >= a.Nk) return;
   const bool live = key < lim.kv_len;
   if (a.splits > 1) {                            // [split][dk, dv][sample, head, key][D] in 32 bits
@@ -840,22 +990,28 @@ int launch_fwd(MhaArgs& a, hipStream_t s) {
     hipLaunchKernelGGL((mha_join_kernel<T, D>), dim3(static_cast<unsigned>((a.B * a.H * a.Nq * (D / 4) + 255) / 256)), dim3(256), 0, s, a);
   return launch_status();
 }
-template <typename T, int D>
+template <typename T, int D, bool TURN>
 int launch_bwd(MhaArgs& a, hipStream_t s) {
   if (a.Nq > 0) {
     cut(a, row_tiles(a.Nq, a.G));
-    hipLaunchKernelGGL((mha_dq_kernel<T, D>), dim3(static_cast<unsigned>(a.B * a.Hkv * a.tiles * a.splits)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((mha_dq_kernel<T, D, TURN>), dim3(static_cast<unsigned>(a.B * a.Hkv * a.tiles * a.splits)), dim3(256), 0, s, a);
     if (a.splits > 1)
       hipLaunchKernelGGL((mha_dq_join_kernel<T, D>), dim3(static_cast<unsigned>((a.B * a.H * a.Nq * (D / 4) + 255) / 256)), dim3(256), 0, s, a);
   }
   if (a.Nk > 0) {
     a.tiles = (a.Nk + 127) / 128;
     a.splits = dkv_splits(a.B, a.Nq, a.Nk, a.Hkv, a.G, D, a.causal != 0);
-    hipLaunchKernelGGL((mha_dkv_kernel<T, D>), dim3(static_cast<unsigned>(a.B * a.Hkv * a.tiles * a.splits)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((mha_dkv_kernel<T, D, TURN>), dim3(static_cast<unsigned>(a.B * a.Hkv * a.tiles * a.splits)), dim3(256), 0, s, a);
     if (a.splits > 1)
       hipLaunchKernelGGL((mha_dkv_join_kernel<T, D>), dim3(static_cast<unsigned>((a.B * a.Hkv * a.Nk * (D / 4) + 255) / 256), 2), dim3(256), 0, s, a);
   }
   return launch_status();
+}
+
+template <bool TURN>
+int launch_bwd(MhaArgs& a, int dtype, int32_t head_dim, hipStream_t s) {
+  if (dtype == APGD_BF16) return head_dim == 64 ? launch_bwd<Bf16, 64, TURN>(a, s) : launch_bwd<Bf16, 128, TURN>(a, s);
+  return head_dim == 64 ? launch_bwd<Fp16, 64, TURN>(a, s) : launch_bwd<Fp16, 128, TURN>(a, s);
 }
 
 View view_of(const int64_t* s) { return View{s[0], s[1], s[2]}; }
@@ -923,8 +1079,54 @@ int cnx_mha_bwd(const void* q, const void* k, const void* v, const void* out, co
   a.vdq = view_of(strides + 15); a.vdk = view_of(strides + 18); a.vdv = view_of(strides + 21);
   if (!near_enough(a.vq, a.G) || !near_enough(a.vk, 1) || !near_enough(a.vv, 1) || !near_enough(a.vdo, a.G)) return APGD_ERR_ARG;
   hipStream_t s = as_stream(stream);
-  if (dtype == APGD_BF16) return head_dim == 64 ? launch_bwd<Bf16, 64>(a, s) : launch_bwd<Bf16, 128>(a, s);
-  return head_dim == 64 ? launch_bwd<Fp16, 64>(a, s) : launch_bwd<Fp16, 128>(a, s);
+  return launch_bwd<false>(a, dtype, head_dim, s);
+}
+
+int64_t cnx_attention_rope_bwd_ws_floats(int64_t B, int32_t N, int32_t H, int32_t head_dim, int32_t own_positions) {
+  if (B <= 0 || N <= 0 || H < 1 || !cnx_mha_supported(head_dim) || cnx_mha_bwd_ws_floats(B, N, N, H, H, head_dim, 0) > 0) return 0;
+  const int64_t tiles = (N + 127) / 128;         // D; cosines and sines; weight gradients of the workgroups
+  return (B * H * N + 3) / 4 * 4 + (own_positions ? B : 1) * N * head_dim + 2 * B * H * tiles * head_dim;
+}
+
+int cnx_attention_rope_bwd(const void* qkv, const void* yq, const void* yk, const void* out, const void* dout, const float* lse, void* dqkv,
+                           float* dwq, float* dwk, float* ws, const int64_t* dout_strides, int dtype, const float* wq, const float* wk,
+                           const void* positions, int pos_dtype, int64_t pos_batch_stride, int32_t axes, const int32_t* sections,
+                           const float* inv_freq, int64_t B, int32_t N, int32_t H, int32_t head_dim, float eps, int32_t norm,
+                           int32_t interleaved, float scale, void* stream) {
+  MhaArgs a = {};
+  const int64_t D = head_dim, C = H * D;
+  a.q = static_cast<const uint16_t*>(yq); a.k = static_cast<const uint16_t*>(yk);
+  a.out = static_cast<const uint16_t*>(out); a.dout = static_cast<const uint16_t*>(dout); a.lse = const_cast<float*>(lse);
+  a.B = B; a.Nq = a.Nk = N; a.H = a.Hkv = H; a.G = 1; a.scale = scale;
+  a.eps = eps; a.norm = norm != 0; a.il = interleaved != 0;
+  if (const int rc = check_args(a, dtype, head_dim)) return rc;
+  if ((dwq || dwk) && !norm) return APGD_ERR_ARG;
+  if (B == 0 || N == 0) return APGD_ERR_SIZE;
+  const int64_t need = cnx_attention_rope_bwd_ws_floats(B, N, H, head_dim, pos_batch_stride != 0);
+  if (need == 0) return APGD_ERR_SIZE;           // few rows: the two operators' own backward passes
+  if (!qkv || !yq || !yk || !out || !dout || !lse || !dqkv || !ws || !dout_strides) return APGD_ERR_NULL;
+  const View packed = {N * 3 * C, 3 * C, D}, dense = {N * C, C, D};
+  a.v = static_cast<const uint16_t*>(qkv) + 2 * C;
+  a.dq = static_cast<uint16_t*>(dqkv); a.dk = a.dq + C; a.dv = a.dk + C;
+  a.vq = a.vk = a.vo = dense;
+  a.vv = a.vdq = a.vdk = a.vdv = packed;
+  a.vdo = view_of(dout_strides);
+  if (!near_enough(a.vk, 1) || !near_enough(a.vv, 1) || !near_enough(a.vdo, 1)) return APGD_ERR_ARG;
+  hipStream_t s = as_stream(stream);
+  a.dvec = ws;
+  float* table = ws + (B * H * N + 3) / 4 * 4;
+  float* part = table + (pos_batch_stride ? B : 1) * N * D;
+  const int64_t groups = B * H * ((N + 127) / 128);
+  a.tq = Turn{static_cast<const uint16_t*>(qkv), packed, wq, dwq || dwk ? part : nullptr};
+  a.tk = Turn{static_cast<const uint16_t*>(qkv) + C, packed, wk, dwq || dwk ? part + groups * D : nullptr};
+  if (positions) {
+    a.cs = reinterpret_cast<const float2*>(table);
+    a.cs_b = pos_batch_stride ? N * D / 2 : 0;
+    if (const int rc = rope_table(positions, pos_dtype, pos_batch_stride, axes, sections, inv_freq, B, N, head_dim, reinterpret_cast<float2*>(table), s))
+      return rc;
+  }
+  if (const int rc = launch_bwd<true>(a, dtype, head_dim, s)) return rc;
+  return dwq || dwk ? rope_dw(part, static_cast<int>(groups), head_dim, dwq, dwk, s) : APGD_OK;
 }
 
 }  // extern "C"

@@ -19,6 +19,7 @@
 
 #include "apgd_hip.h"
 #include "convnext_hip.h"
+#include "rope_internal.h"
 
 namespace {
 
@@ -155,20 +156,31 @@ __device__ __forceinline__ float group_sum(float v, int group) {
   return v;
 }
 
-// cosines and sines of tokens n0 .. n0 + nt - 1 of sample b: cs[t][pair]
+// cosine and sine of pair i of token n of sample b
+__device__ __forceinline__ float2 cos_sin(const RopeArgs& a, int64_t b, int64_t n, int i) {
+  const int axis = (i >= a.first1) + (i >= a.first2) + (i >= a.first3);
+  const int64_t at = b * a.pos_b + n * a.axes + axis;
+  double p;
+  if (a.pos_dtype == CNX_POS_F32) p = static_cast<const float*>(a.pos)[at];
+  else if (a.pos_dtype == CNX_POS_I32) p = static_cast<const int32_t*>(a.pos)[at];
+  else p = static_cast<double>(static_cast<const int64_t*>(a.pos)[at]);
+  const double turns = p * static_cast<double>(a.inv_freq[i]) * 0.15915494309189535;        // 1 / (2 pi)
+  const float f = static_cast<float>(turns - rint(turns));
+  return make_float2(cospif(2.f * f), sinpif(2.f * f));
+}
+// those of tokens n0 .. n0 + nt - 1 of sample b: cs[t][pair]
 __device__ __forceinline__ void tile_angles(const RopeArgs& a, int64_t b, int64_t n0, int nt, float2* cs) {
   const int pairs = a.d >> 1;
   for (int e = threadIdx.x; e < nt * pairs; e += blockDim.x) {
     const int t = e / pairs, i = e - t * pairs;
-    const int axis = (i >= a.first1) + (i >= a.first2) + (i >= a.first3);
-    const int64_t at = b * a.pos_b + (n0 + t) * a.axes + axis;
-    double p;
-    if (a.pos_dtype == CNX_POS_F32) p = static_cast<const float*>(a.pos)[at];
-    else if (a.pos_dtype == CNX_POS_I32) p = static_cast<const int32_t*>(a.pos)[at];
-    else p = static_cast<double>(static_cast<const int64_t*>(a.pos)[at]);
-    const double turns = p * static_cast<double>(a.inv_freq[i]) * 0.15915494309189535;      // 1 / (2 pi)
-    const float f = static_cast<float>(turns - rint(turns));
-    cs[t * pairs + i] = make_float2(cospif(2.f * f), sinpif(2.f * f));
+    cs[t * pairs + i] = cos_sin(a, b, n0 + t, i);
+  }
+}
+__global__ __launch_bounds__(256) void rope_table_kernel(const RopeArgs a, float2* __restrict__ cs, int64_t rows) {
+  const int pairs = a.d >> 1;
+  for (int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; e < rows * pairs; e += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t row = e / pairs, b = a.pos_b ? row / a.N : 0;
+    cs[e] = cos_sin(a, b, row - b * a.N, static_cast<int>(e - row * pairs));
   }
 }
 
@@ -398,6 +410,20 @@ View view_of(const int64_t* s) { return View{s[0], s[1], s[2]}; }
 
 }  // namespace
 
+int rope_table(const void* positions, int pos_dtype, int64_t pos_b, int32_t axes, const int32_t* sections, const float* inv_freq, int64_t B,
+               int64_t N, int32_t d, float2* cs, hipStream_t s) {
+  RopeArgs a = {};
+  a.pos = positions; a.pos_dtype = pos_dtype; a.pos_b = pos_b; a.axes = axes; a.inv_freq = inv_freq;
+  if (const int rc = check_args(a, APGD_F32, sections, B, N, 0, 0, d)) return rc;
+  const int64_t rows = pos_b ? B * N : N, blocks = (rows * (d / 2) + 255) / 256;
+  hipLaunchKernelGGL(rope_table_kernel, dim3(static_cast<unsigned>(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s, a, cs, rows);
+  return launch_status();
+}
+int rope_dw(const float* part, int rows, int32_t d, float* dwq, float* dwk, hipStream_t s) {
+  hipLaunchKernelGGL(rope_dw_kernel, dim3(static_cast<unsigned>(d / 16), 2), dim3(1024), 0, s, part, rows, d, dwq, dwk);
+  return launch_status();
+}
+
 extern "C" {
 
 int cnx_qk_norm_rope_supported(int32_t d) { return d >= 16 && d <= kMaxHead && d % 16 == 0; }
@@ -446,9 +472,7 @@ int cnx_qk_norm_rope_bwd(const void* dyq, const void* dyk, const void* q, const 
     grid = static_cast<unsigned>(a.tiles < kBwdGrid ? a.tiles : kBwdGrid);
     launch<true>(a, dtype, interleaved != 0, grid, as_stream(stream));
   }
-  if (want_w)
-    hipLaunchKernelGGL(rope_dw_kernel, dim3(static_cast<unsigned>(d / 16), 2), dim3(1024), 0, as_stream(stream), ws, static_cast<int>(grid), d, dwq, dwk);
-  return launch_status();
+  return want_w ? rope_dw(ws, static_cast<int>(grid), d, dwq, dwk, as_stream(stream)) : launch_status();
 }
 
 }  // extern "C"

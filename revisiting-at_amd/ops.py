@@ -2303,10 +2303,20 @@ class _AttentionRope(torch.autograd.Function):
         dq, dk, dv = dqkv.view(B, N, 3, H, d).unbind(2)
         dwq = dwk = None
         with _on_device(qkv):
-            if turned:
+            want = [ctx.needs_input_grad[i] and not _INPUT_GRAD_ONLY for i in (1, 2)]
+            n = _lib.load().cnx_attention_rope_bwd_ws_floats(B, N, H, d, ctx.rot.batch_stride != 0) if turned else 0
+            if n:
+                ws = torch.empty(n, device=qkv.device, dtype=torch.float32)
+                dwq, dwk = (torch.empty(d, device=qkv.device, dtype=torch.float32) if w else None for w in want)
+                fq, fk = (None if w is None else w.float() for w in (wq, wk))
+                _lib.check(_lib.load().cnx_attention_rope_bwd(
+                    qkv.data_ptr(), yq.data_ptr(), yk.data_ptr(), out.data_ptr(), dout.data_ptr(), lse.data_ptr(), dqkv.data_ptr(), _lib.ptr(dwq),
+                    _lib.ptr(dwk), ws.data_ptr(), _strides(dout), _code(qkv), _lib.ptr(fq), _lib.ptr(fk), *ctx.rot.args(), B, N, H, d, ctx.rot.eps,
+                    ctx.rot.norm, ctx.rot.interleaved, ctx.scale, _raw_stream()), "cnx_attention_rope_bwd")
+                dwq, dwk = (None if g is None else g.to(dt) for g, dt in zip((dwq, dwk), ctx.w_dtypes))
+            elif turned:
                 dyq, dyk = torch.empty_like(yq), torch.empty_like(yk)
                 _mha_backward(yq, yk, v, out, dout, lse, dyq, dyk, dv, ctx.scale, 0, None, None)
-                want = [ctx.needs_input_grad[i] and not _INPUT_GRAD_ONLY for i in (1, 2)]
                 dwq, dwk = _rope_backward(dyq, dyk, q, k, dq, dk, wq, wk, ctx.rot, *want)
                 dwq, dwk = (None if g is None else g.to(dt) for g, dt in zip((dwq, dwk), ctx.w_dtypes))
             else:

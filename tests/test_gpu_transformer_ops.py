@@ -186,7 +186,7 @@ def test_qk_norm_rope_strides_and_shared_inputs(R):
 
 
 # ------------------------------------------------------------------------------------------------------------------ mha
-def mha_ref(q, k, v, scale, causal, q_lens, kv_lens, dout, u):
+def mha_ref(q, k, v, scale, causal, q_lens, kv_lens, dout, u, rounded=True):
     """The definition in 64 bits, a sample and head at a time, and how far the kernel's roundings may lead from it:
     out: P is rounded to 16 bits (u) and the result once more; exp's argument and the sums in 32 bits (t).
     dv: the same with P^T and dout.   D is formed from the rounded out.   dS is rounded once, the products' results once."""
@@ -233,7 +233,7 @@ def mha_ref(q, k, v, scale, causal, q_lens, kv_lens, dout, u):
                 err += (ex + (Nq + Nk) * E * x.abs()) * scale
             dv[b, :, hk] += P.T @ G
             bv[b, :, hk] += eP.T @ G.abs()
-    for g, e in ((dq, bq), (dk, bk), (dv, bv)):
+    for g, e in ((dq, bq), (dk, bk), (dv, bv)) if rounded else ((dv, bv),):        # not rounded: dq and dk as they are in 32 bits
         e += u * (g.abs() + e) + (2.0 ** -25 if u == 2.0 ** -11 else 0.0)
     bo += 2.0 ** -24 if u == 2.0 ** -11 else 0.0                                   # P's smallest step times v, and out's own
     return (out, dq, dk, dv), (bo, bq, bk, bv)
@@ -419,7 +419,8 @@ def test_refusals_name_what_is_wrong(R):
 @pytest.mark.parametrize("norm,rotate", [(True, True), (True, False), (False, True), (False, False)])
 @pytest.mark.parametrize("B,side,H,d", [(2, 14, 3, 64), (1, 24, 2, 64), (2, 6, 2, 128), (1, 0, 1, 64)])
 def test_attention_rope_is_its_two_operators(R, B, side, H, d, norm, rotate):
-    """Bit for bit ``qk_norm_rope`` then ``mha`` on slices of the projection, in both directions."""
+    """Bit for bit ``qk_norm_rope`` then ``mha`` on slices of the projection, forward and dv; all gradients where the rows are split over workgroups or
+    nothing is turned (elsewhere dq' and dk' are not rounded in between)."""
     N = side * side + 1
     g = torch.Generator().manual_seed(N)
     qkv = torch.randn(B, N, 3 * H * d, generator=g).to(torch.bfloat16).cuda().requires_grad_()
@@ -438,6 +439,73 @@ def test_attention_rope_is_its_two_operators(R, B, side, H, d, norm, rotate):
         q, k = R.ops.qk_norm_rope(q, k, wq, wk, pos, inv, sec, norm=norm)
     o2 = R.ops.mha(q, k, v).reshape(B, N, H * d)
     want = (o2,) + torch.autograd.grad(o2, (x,) + ((wq, wk) if norm else ()), dout)
-    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1][..., 2 * H * d:], want[1][..., 2 * H * d:])
+    fused = R._lib.load().cnx_attention_rope_bwd_ws_floats(B, N, H, d, 0) > 0 and (norm or rotate)
+    assert fused == (N != 577 and (norm or rotate))
+    if not fused:
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
     with torch.no_grad():
         assert torch.equal(R.ops.attention_rope(qkv, H, None, wq, wk, pos, inv, sec, norm=norm), out)
+
+
+ATTN = [  # B, N, H, d, norm, rotate, interleaved, per-batch positions, weights' type (None: none), dout
+    (2, 17, 2, 64, True, True, False, False, torch.float32, "whole"),
+    (1, 1, 1, 64, True, True, False, False, torch.float32, "whole"),
+    (2, 130, 2, 64, True, True, True, True, torch.float32, "whole"),
+    (1, 200, 2, 128, True, True, False, True, None, "part"),
+    (2, 129, 1, 128, True, True, True, False, torch.float32, "whole"),
+    (1, 64, 3, 64, True, False, False, False, "x", "expanded"),
+    (1, 65, 2, 64, False, True, False, True, None, "whole"),
+    (43, 257, 2, 64, True, True, False, False, torch.float32, "whole"),          # more than 256 keys: enough samples that no row is split
+    (29, 260, 3, 128, False, True, True, False, None, "part"),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("case", ATTN, ids=lambda c: "-".join(str(v).split(".")[-1] for v in c))
+def test_attention_rope_gradients_against_their_definition(R, case, dtype):
+    """The backward pass in one: dq' and dk' of q' and k' as they were rounded, through the rotation and the norm, rounded once at the end."""
+    B, N, H, d, norm, rotate, il, per_batch, wt, part = case
+    assert R._lib.load().cnx_attention_rope_bwd_ws_floats(B, N, H, d, per_batch) > 0
+    g = torch.Generator().manual_seed(N + d)
+    u = half_step(dtype)
+    qkv = torch.randn(B, N, 3 * H * d, generator=g).to(dtype).cuda().requires_grad_()
+    wt = dtype if wt == "x" else wt
+    wq, wk = (None, None) if wt is None else ((1 + 0.1 * torch.randn(d + 1, generator=g)).to(wt).cuda()[1:].requires_grad_() for _ in range(2))
+    pos = torch.randint(-5, 40, (B, N, 2) if per_batch else (N, 2), generator=g).cuda() if rotate else None
+    sec = [d // 2 - d // 8, d // 8] if rotate else None
+    inv = torch.cat([100.0 ** (-torch.arange(s).float() / s) for s in sec]).cuda() if rotate else None
+    dout = torch.randn(B, N, 2 * H * d, generator=g).to(dtype).cuda()
+    dout = dout[..., H * d:] if part == "part" else dout[:, :1, :H * d].expand(B, N, H * d) if part == "expanded" else dout[..., :H * d].contiguous()
+    out = R.ops.attention_rope(qkv, H, None, wq, wk, pos, inv, sec, norm=norm, interleaved=il)
+    leaves = (qkv,) + (() if wt is None else (wq, wk))
+    got = torch.autograd.grad(out, leaves, dout)
+    q, k, v = qkv.detach().view(B, N, 3, H, d).unbind(2)
+    with torch.no_grad():
+        yq, yk = R.ops.qk_norm_rope(q, k, wq, wk, pos, inv, sec, norm=norm, interleaved=il)
+    (_, dq, dk, dv), (_, bq, bk, bv) = mha_ref(yq, yk, v, d ** -0.5, False, None, None, dout.reshape(B, N, H, d), u, rounded=False)
+    angle = rope_angles(pos, inv, sec) if rotate else None
+    mine = got[0].view(B, N, 3, H, d).unbind(2)
+    inside(mine[2], dv, bv, "dv")
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    for i, (name, x, w, dy, b) in enumerate((("dq", q, wq, dq, bq), ("dk", k, wk, dk, bk))):
+        _, _, dx, dxb, dw, dwb = rope_ref(x, w, angle, norm, il, 1e-6, dy)
+        # b is carried through the rotation (each member takes part of both) and the norm's linear map, each term by its size
+        ea, eb = split_pairs(b, il)
+        c, s = (1.0, 0.0) if angle is None else (angle.cos().abs().unsqueeze(-2), angle.sin().abs().unsqueeze(-2))
+        eb = join_pairs(ea * c + eb * s, eb * c + ea * s, il)
+        if norm:
+            x64 = x.double().cpu()
+            r = 1 / torch.sqrt((x64 * x64).mean(-1, keepdim=True) + 1e-6)
+            xh, wa = (x64 * r).abs(), torch.ones(d).double() if w is None else w.detach().double().cpu().abs()
+            dwb = dwb + (eb * xh).sum((0, 1, 2))
+            eb = r * (eb * wa + xh * (eb * xh * wa).mean(-1, keepdim=True))
+        e = eb + 1.01 * dxb                                                         # (32-bit part: of dy's size with its own error)
+        inside(mine[i], dx, e + u * (dx.abs() + e) + tiny, name)
+        if w is not None:
+            last = u if w.dtype == dtype else 0.0
+            inside(got[1 + i], dw, 1.01 * dwb + last * (dw.abs() + 1.01 * dwb) + (2.0 ** -25 if w.dtype == torch.float16 else 0.0), "d" + name[1] + " weight")
+    x2 = qkv.detach().requires_grad_()                                              # without weight gradients: the same bits
+    (again,) = torch.autograd.grad(R.ops.attention_rope(x2, H, None, None if wq is None else wq.detach(), None if wk is None else wk.detach(), pos, inv, sec,
+                                                        norm=norm, interleaved=il), (x2,), dout)
+    assert torch.equal(again, got[0])
