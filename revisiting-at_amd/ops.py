@@ -2027,6 +2027,15 @@ def _strides(*tensors):
     return (ctypes.c_int64 * len(v))(*v)
 
 
+def _put_strides(array, at, t):
+    """``t``'s strides as the ``at``-th tensor's of ``array``, in a copy where they differ."""
+    v = t.stride()[:3]
+    if v != tuple(array[3 * at:3 * at + 3]):
+        array = type(array)(*array)
+        array[3 * at:3 * at + 3] = v
+    return array
+
+
 def _backward_once(gradients, ctx, grads):
     """A backward that has no derivative of its own: where a graph of the gradient is recorded, using it raises."""
     if torch.is_grad_enabled():
@@ -2085,17 +2094,17 @@ def _check_head_weight(what, name, w, x):
         raise TypeError(f"{what}: {name} has to be float32 or {x.dtype} on {x.device}, not {w.dtype} on {w.device}")
 
 
-def _rope_forward(q, k, yq, yk, wq, wk, rot):
+def _rope_forward(q, k, yq, yk, wq, wk, rot, strides=None):
     """``qk_norm_rope`` of checked, readable tensors into ``yq`` / ``yk``."""
     w = wq if wq is not None else wk
     B, N, Hq, d = q.shape
     _lib.check(_lib.load().cnx_qk_norm_rope_fwd(
-        q.data_ptr(), k.data_ptr(), yq.data_ptr(), yk.data_ptr(), _code(q), _strides(q, k, yq, yk), _lib.ptr(wq), _lib.ptr(wk),
+        q.data_ptr(), k.data_ptr(), yq.data_ptr(), yk.data_ptr(), _code(q), strides or _strides(q, k, yq, yk), _lib.ptr(wq), _lib.ptr(wk),
         _code(w) if w is not None else 0, *rot.args(), B, N, Hq, k.shape[2], d, rot.eps, rot.norm, rot.interleaved, _raw_stream()),
         "cnx_qk_norm_rope_fwd")
 
 
-def _rope_backward(dyq, dyk, q, k, dq, dk, wq, wk, rot, want_wq, want_wk):
+def _rope_backward(dyq, dyk, q, k, dq, dk, wq, wk, rot, want_wq, want_wk, strides=None):
     """Gradients of ``qk_norm_rope`` into ``dq`` / ``dk``; returns those of the weights (fp32) or None."""
     lib = _lib.load()
     w = wq if wq is not None else wk
@@ -2106,7 +2115,7 @@ def _rope_backward(dyq, dyk, q, k, dq, dk, wq, wk, rot, want_wq, want_wk):
     x = (q, k) if rot.norm else (dyq, dyk)                                      # without norm q and k are not read
     _lib.check(lib.cnx_qk_norm_rope_bwd(
         dyq.data_ptr(), dyk.data_ptr(), x[0].data_ptr(), x[1].data_ptr(), dq.data_ptr(), dk.data_ptr(), _lib.ptr(dwq), _lib.ptr(dwk),
-        _lib.ptr(ws), _code(dyq), _strides(dyq, dyk, *x, dq, dk), _lib.ptr(wq), _lib.ptr(wk), _code(w) if w is not None else 0, *rot.args(),
+        _lib.ptr(ws), _code(dyq), strides or _strides(dyq, dyk, *x, dq, dk), _lib.ptr(wq), _lib.ptr(wk), _code(w) if w is not None else 0, *rot.args(),
         B, N, Hq, dyk.shape[2], d, rot.eps, rot.norm, rot.interleaved, _raw_stream()), "cnx_qk_norm_rope_bwd")
     return dwq, dwk
 
@@ -2125,10 +2134,11 @@ class _QkNormRope(torch.autograd.Function):
         q, k = _head_rows(q), _head_rows(k)
         yq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
         yk = torch.empty(k.shape, device=k.device, dtype=k.dtype)
+        ctx.strides = _strides(yq, yk, q, k, yq, yk)               # dyq, dyk, q, k, dq, dk of the backward; from q on the forward's four
         ctx.w_dtypes = (None if wq is None else wq.dtype), (None if wk is None else wk.dtype)
         wq, wk = _head_weights(wq, wk)
         with _on_device(q):
-            _rope_forward(q, k, yq, yk, wq, wk, rot)
+            _rope_forward(q, k, yq, yk, wq, wk, rot, (ctypes.c_int64 * 12).from_buffer(ctx.strides, 48))
         ctx.save_for_backward(*((q, k) if rot.norm else (None, None)), wq, wk)
         ctx.rot = rot
         return yq, yk
@@ -2141,13 +2151,15 @@ class _QkNormRope(torch.autograd.Function):
     def _gradients(ctx, dyq, dyk):
         q, k, wq, wk = ctx.saved_tensors
         dyq, dyk = _head_rows(dyq), _head_rows(dyk)
-        dq = torch.empty(dyq.shape, device=dyq.device, dtype=dyq.dtype)
-        dk = torch.empty(dyk.shape, device=dyk.device, dtype=dyk.dtype)
-        want = [ctx.needs_input_grad[i] and not _INPUT_GRAD_ONLY for i in (2, 3)]
+        dq, dk = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (dyq, dyk))
+        strides = _put_strides(_put_strides(ctx.strides, 0, dyq), 1, dyk)
+        if not ctx.rot.norm:                                       # q and k are not read: their places are taken by dyq and dyk
+            strides = _put_strides(_put_strides(strides, 2, dyq), 3, dyk)
+        need = ctx.needs_input_grad
         with _on_device(dyq):
-            dw = _rope_backward(dyq, dyk, q, k, dq, dk, wq, wk, ctx.rot, *want)
-        dwq, dwk = (None if g is None else g.to(dt) for g, dt in zip(dw, ctx.w_dtypes))
-        return dq, dk, dwq, dwk, None
+            dwq, dwk = _rope_backward(dyq, dyk, q, k, dq, dk, wq, wk, ctx.rot, need[2] and not _INPUT_GRAD_ONLY, need[3] and not _INPUT_GRAD_ONLY,
+                                      strides)
+        return dq, dk, None if dwq is None else dwq.to(ctx.w_dtypes[0]), None if dwk is None else dwk.to(ctx.w_dtypes[1]), None
 
 
 def qk_norm_rope(q, k, q_weight=None, k_weight=None, positions=None, inv_freq=None, sections=None, eps=1e-6, norm=True, interleaved=False):
@@ -2175,7 +2187,7 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, positions=None, inv_freq=No
 
 
 # ------------------------------------------------------------------------------ attention over any number of tokens
-def _mha_forward(q, k, v, out, scale, causal, q_lens, kv_lens, want_lse):
+def _mha_forward(q, k, v, out, scale, causal, q_lens, kv_lens, want_lse, strides=None):
     """``mha`` of checked, readable tensors into ``out``; returns lse [B, H, Nq] or None."""
     lib = _lib.load()
     B, Nq, H, d = q.shape
@@ -2184,11 +2196,11 @@ def _mha_forward(q, k, v, out, scale, causal, q_lens, kv_lens, want_lse):
     n = lib.cnx_mha_ws_floats(B, Nq, Nk, H, Hkv, d)
     ws = torch.empty(n, device=q.device, dtype=torch.float32) if n else None
     _lib.check(lib.cnx_mha_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _lib.ptr(lse), _lib.ptr(q_lens), _lib.ptr(kv_lens),
-                               _lib.ptr(ws), _strides(q, k, v, out), _code(q), B, Nq, Nk, H, Hkv, d, causal, scale, _raw_stream()), "cnx_mha_fwd")
+                               _lib.ptr(ws), strides or _strides(q, k, v, out), _code(q), B, Nq, Nk, H, Hkv, d, causal, scale, _raw_stream()), "cnx_mha_fwd")
     return lse
 
 
-def _mha_backward(q, k, v, out, dout, lse, dq, dk, dv, scale, causal, q_lens, kv_lens):
+def _mha_backward(q, k, v, out, dout, lse, dq, dk, dv, scale, causal, q_lens, kv_lens, strides=None):
     lib = _lib.load()
     B, Nq, H, d = q.shape
     Nk, Hkv = k.shape[1], k.shape[2]
@@ -2197,7 +2209,7 @@ def _mha_backward(q, k, v, out, dout, lse, dq, dk, dv, scale, causal, q_lens, kv
     ws = torch.empty(n, device=q.device, dtype=torch.float32) if n else None
     _lib.check(lib.cnx_mha_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), lse.data_ptr(), dq.data_ptr(),
                                dk.data_ptr(), dv.data_ptr(), dvec.data_ptr(), _lib.ptr(q_lens), _lib.ptr(kv_lens), _lib.ptr(ws),
-                               _strides(q, k, v, out, dout, dq, dk, dv), _code(q), B, Nq, Nk, H, Hkv, d, causal, scale, _raw_stream()), "cnx_mha_bwd")
+                               strides or _strides(q, k, v, out, dout, dq, dk, dv), _code(q), B, Nq, Nk, H, Hkv, d, causal, scale, _raw_stream()), "cnx_mha_bwd")
 
 
 class _Mha(torch.autograd.Function):
@@ -2206,11 +2218,18 @@ class _Mha(torch.autograd.Function):
     def forward(ctx, q, k, v, scale, causal, q_lens, kv_lens):
         q, k, v = _head_rows(q), _head_rows(k), _head_rows(v)
         out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        need = ctx.needs_input_grad
+        want, strides = need[0] or need[1] or need[2], None
+        if want:                                                   # q, k, v, out and, contiguous, dout, dq, dk, dv: the backward thread's work is the slower
+            _, n, h, d = k.shape
+            like_k = n * h * d, h * d, d
+            like_q = out.stride()[:3]
+            strides = (ctypes.c_int64 * 24)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *like_q, *like_q, *like_q, *like_k, *like_k)
         with _on_device(q):
-            lse = _mha_forward(q, k, v, out, scale, causal, q_lens, kv_lens, any(ctx.needs_input_grad[:3]))
-        if lse is not None:
+            lse = _mha_forward(q, k, v, out, scale, causal, q_lens, kv_lens, want, strides)
+        if want:
             ctx.save_for_backward(q, k, v, out, lse, q_lens, kv_lens)
-            ctx.scale, ctx.causal = scale, causal
+            ctx.scale, ctx.causal, ctx.strides = scale, causal, strides
         return out
 
     @staticmethod
@@ -2221,9 +2240,9 @@ class _Mha(torch.autograd.Function):
     def _gradients(ctx, dout):
         q, k, v, out, lse, q_lens, kv_lens = ctx.saved_tensors
         dout = _head_rows(dout)
-        dq, dk, dv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
+        dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
         with _on_device(q):
-            _mha_backward(q, k, v, out, dout, lse, dq, dk, dv, ctx.scale, ctx.causal, q_lens, kv_lens)
+            _mha_backward(q, k, v, out, dout, lse, dq, dk, dv, ctx.scale, ctx.causal, q_lens, kv_lens, _put_strides(ctx.strides, 4, dout))
         return dq, dk, dv, None, None, None, None
 
 
