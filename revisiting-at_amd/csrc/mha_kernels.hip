@@ -464,11 +464,34 @@ __global__ __launch_bounds__(256) void mha_join_kernel(const MhaArgs a) {
 }
 
 // ===================================================================================================================== backward
+// Sums of 32 values over the 32 lanes of a half: lane l32 gets the sum of value l32.  Every step halves the values that a lane still holds; lanes
+// of opposite bit trade what the other one keeps, across rows of 16 lanes, then within them.
+template <int CTRL>
+__device__ __forceinline__ float traded(bool upper, float lo, float hi) {
+  const float keep = upper ? hi : lo, give = upper ? lo : hi;
+  return keep + __uint_as_float(static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(__float_as_uint(give)), CTRL, 0xf, 0xf, true)));
+}
+__device__ __forceinline__ float rows_sum(float (&v)[32]) {
+  const int lane = threadIdx.x;
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[k]), __float_as_uint(v[k + 16]), false, false);
+    v[k] = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = traded<0x140>(lane & 8, v[k], v[k + 8]);                  // row_mirror: lane 15 - i
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v[k] = traded<0x141>(lane & 4, v[k], v[k + 4]);                  // row_half_mirror: lane 7 - i
+#pragma unroll
+  for (int k = 0; k < 2; ++k) v[k] = traded<0x1b>(lane & 2, v[k], v[k + 2]);                   // quad_perm: lane 3 - i
+  return traded<0xb1>(lane & 1, v[0], v[1]);                                                   // quad_perm: lane i ^ 1
+}
+
 // The gradient g of a row of q' (k') becomes that of q (k) in the accumulators it is in: lane = row, d = db * 32 + (r & 3) + 8 (r >> 2) + 4 half,
 // so both members of a pair are one lane's, and a row's sums need one exchange of the two halves.  With z = x r w the normalised row, R its
 // rotation:  dz = R^T g,  dw = sum over the rows of dz * (x r),  dx = r (dz w - (x r) mean(dz w * (x r))).  Nothing is rounded in between.
 template <typename T, int D>
-__device__ __forceinline__ void turn_back(const MhaArgs& a, const Turn& t, f32x16 (&g)[D / 32], int64_t b, int tok, int h, bool live, unsigned char* lds) {
+__device__ __forceinline__ void turn_back(const MhaArgs& a, const Turn& t, f32x16 (&g)[D / 32], int64_t b, int tok, int h, bool live) {
   constexpr int DB = D / 32;
   const int half = (threadIdx.x >> 5) & 1;
   const int64_t i = live ? tok : 0;
@@ -517,35 +540,21 @@ __device__ __forceinline__ void turn_back(const MhaArgs& a, const Turn& t, f32x1
   for (int db = 0; db < DB; ++db)
 #pragma unroll
     for (int r = 0; r < 16; ++r) x[db][r] *= rn;
-  if (t.part) {                                  // (uniform) the workgroup's 128 rows, through LDS: pieces of 16 bytes, spread over the banks by the row
-    float* rows = reinterpret_cast<float*>(lds);
-    const int row = (threadIdx.x >> 6) * 32 + (threadIdx.x & 31);
-    __syncthreads();                             // nobody reads tiles any more
+  if (t.part) {                                  // (uniform) over the workgroup's 128 rows
+    __shared__ float red[4 * D];
+    const int l32 = threadIdx.x & 31, wave = threadIdx.x >> 6;
 #pragma unroll
-    for (int db = 0; db < DB; ++db)
+    for (int db = 0; db < DB; db += 2) {
+      float e[32];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        float e[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) e[u] = live ? g[db][4 * q + u] * x[db][4 * q + u] : 0.f;
-        *reinterpret_cast<float4*>(rows + row * D + (((db * 8 + 2 * q + half) ^ (row & (D / 4 - 1))) << 2)) = make_float4(e[0], e[1], e[2], e[3]);
-      }
-    __syncthreads();
-    constexpr int PARTS = 256 / D;
-    const int e = threadIdx.x % D, part = threadIdx.x / D;
-    float s = 0.f;
-#pragma unroll 8
-    for (int k = 0; k < 128 / PARTS; ++k) {
-      const int rr = part * (128 / PARTS) + k;
-      s += rows[rr * D + (((e >> 2) ^ (rr & (D / 4 - 1))) << 2) + (e & 3)];
+      for (int k = 0; k < 32; ++k) e[k] = live ? g[db + (k >> 4)][k & 15] * x[db + (k >> 4)][k & 15] : 0.f;
+      const int r = l32 & 15;
+      red[wave * D + (db + (l32 >> 4)) * 32 + (r & 3) + 8 * (r >> 2) + 4 * half] = rows_sum(e);
     }
     __syncthreads();
-    rows[threadIdx.x] = s;
-    __syncthreads();
     if (threadIdx.x < D) {
-#pragma unroll
-      for (int k = 1; k < PARTS; ++k) s += rows[k * D + e];
-      t.part[static_cast<int64_t>(blockIdx.x) * D + e] = s;
+      const int e = threadIdx.x;
+      t.part[static_cast<int64_t>(blockIdx.x) * D + e] = ((red[e] + red[D + e]) + red[2 * D + e]) + red[3 * D + e];
     }
   }
   float dot = 0.f;
@@ -641,7 +650,7 @@ __global__ __launch_bounds__(256, 2) void mha_dq_kernel(const MhaArgs a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) dq[db][r] *= mul;
     mul = 1.f;
-    turn_back<T, D>(a, a.tq, dq, w.b, w.tok, h, w.tok < a.Nq, lds);
+    turn_back<T, D>(a, a.tq, dq, w.b, w.tok, h, w.tok < a.Nq);
   }
   if (w.tok >= a.Nq) return;
   if (!TURN && a.splits > 1) {
@@ -863,7 +872,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void mha_dkv_kernel(const Mha
     for (int db = 0; db < DB; ++db)
 #pragma unroll
       for (int r = 0; r < 16; ++r) dk[db][r] *= a.scale;
-    turn_back<T, D>(a, a.tk, dk, b, key, hk, live, lds);
+    turn_back<T, D>(a, a.tk, dk, b, key, hk, live);
     if (!live) return;
     uint16_t* pk = a.dk + b * a.vdk.b + key * a.vdk.n + hk * a.vdk.h;
 #pragma unroll
