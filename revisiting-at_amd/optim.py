@@ -33,6 +33,18 @@ def _dense(p):
     return True
 
 
+def _copy(pairs):
+    """``dst.copy_(src)`` of each pair, those of one type and device together."""
+    groups = {}
+    for dst, src in pairs:
+        src = torch.as_tensor(src)
+        dsts, srcs = groups.setdefault((dst.dtype, src.dtype, src.device), ([], []))
+        dsts.append(dst)
+        srcs.append(src)
+    for dsts, srcs in groups.values():
+        torch._foreach_copy_(dsts, srcs)
+
+
 class _Plan:
     """What does not change between steps: the moments' buffers, the device tables of tensors and chunks."""
 
@@ -127,12 +139,12 @@ class FusedAdamW(torch.optim.Optimizer):
         old = {p: dict(self.state[p]) for p in params if self.state.get(p)}
         with ops._on_device(params[0]), torch.no_grad():
             plan = _Plan(params, [i for i, g in enumerate(self.param_groups) for _ in g["params"]], [self._bits(p) for p in params])
-            for i, p in enumerate(params):
-                mine = {"step": plan.steps[i], **plan.moments(i, p)}
-                for k, t in mine.items():
-                    if p in old:
-                        t.copy_(torch.as_tensor(old[p][k]))
-                self.state[p] = mine
+            pairs = []
+            for i, (p, step) in enumerate(zip(params, plan.steps.unbind())):
+                self.state[p] = {"step": step, **plan.moments(i, p)}
+                if p in old:
+                    pairs += [(t, old[p][k]) for k, t in self.state[p].items()]
+            _copy(pairs)
         self._plan, self._stale = plan, False
         return plan
 
@@ -229,10 +241,8 @@ class FusedAdamW(torch.optim.Optimizer):
                     raise ValueError(f"FusedAdamW: {k} of parameter {i} is {tuple(given[k].shape)}, not {shape}")
         super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})     # checks and takes the groups
         self._build()
-        for p, at in zip(params, ids):
-            for k, x in (state_dict["state"].get(at) or {}).items():
-                if k in self.state[p]:
-                    self.state[p][k].copy_(torch.as_tensor(x))
+        with ops._on_device(params[0]):
+            _copy([(self.state[p][k], x) for p, at in zip(params, ids) for k, x in (state_dict["state"].get(at) or {}).items() if k in self.state[p]])
 
     def __getstate__(self):
         return {**super().__getstate__(), "state_bits": self.state_bits}
