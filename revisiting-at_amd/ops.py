@@ -2043,6 +2043,11 @@ def _backward_once(gradients, ctx, grads):
     return gradients(ctx, *grads)
 
 
+def _wants_grad(*tensors):
+    """Whether autograd has to see the call; without it the kernels are launched directly (a recorded call costs the host 5 us more)."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 class _Rotation:
     """Checked arguments of the rotation and the norm, as the C entry points take them."""
     __slots__ = ("positions", "inv_freq", "sections", "axes", "code", "batch_stride", "eps", "norm", "interleaved")
@@ -2183,7 +2188,14 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, positions=None, inv_freq=No
         raise ValueError(f"{what}: q_weight and k_weight go with norm=True")
     _check_head_weight(what, "q_weight", q_weight, q)
     _check_head_weight(what, "k_weight", k_weight, k)
-    return _QkNormRope.apply(q, k, q_weight, k_weight, _Rotation(what, q, positions, inv_freq, sections, eps, norm, interleaved))
+    rot = _Rotation(what, q, positions, inv_freq, sections, eps, norm, interleaved)
+    if _wants_grad(q, k, q_weight, k_weight):
+        return _QkNormRope.apply(q, k, q_weight, k_weight, rot)
+    q, k = _head_rows(q), _head_rows(k)
+    yq, yk = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k))
+    with _on_device(q):
+        _rope_forward(q, k, yq, yk, *_head_weights(q_weight, k_weight), rot)
+    return yq, yk
 
 
 # ------------------------------------------------------------------------------ attention over any number of tokens
@@ -2218,18 +2230,15 @@ class _Mha(torch.autograd.Function):
     def forward(ctx, q, k, v, scale, causal, q_lens, kv_lens):
         q, k, v = _head_rows(q), _head_rows(k), _head_rows(v)
         out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        need = ctx.needs_input_grad
-        want, strides = need[0] or need[1] or need[2], None
-        if want:                                                   # q, k, v, out and, contiguous, dout, dq, dk, dv: the backward thread's work is the slower
-            _, n, h, d = k.shape
-            like_k = n * h * d, h * d, d
-            like_q = out.stride()[:3]
-            strides = (ctypes.c_int64 * 24)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *like_q, *like_q, *like_q, *like_k, *like_k)
+        # q, k, v, out and, contiguous, dout, dq, dk, dv: made here because the backward's thread takes twice as long for the same
+        _, n, h, d = k.shape
+        like_k = n * h * d, h * d, d
+        like_q = out.stride()[:3]
+        ctx.strides = (ctypes.c_int64 * 24)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *like_q, *like_q, *like_q, *like_k, *like_k)
         with _on_device(q):
-            lse = _mha_forward(q, k, v, out, scale, causal, q_lens, kv_lens, want, strides)
-        if want:
-            ctx.save_for_backward(q, k, v, out, lse, q_lens, kv_lens)
-            ctx.scale, ctx.causal, ctx.strides = scale, causal, strides
+            lse = _mha_forward(q, k, v, out, scale, causal, q_lens, kv_lens, True, ctx.strides)
+        ctx.save_for_backward(q, k, v, out, lse, q_lens, kv_lens)
+        ctx.scale, ctx.causal = scale, causal
         return out
 
     @staticmethod
@@ -2279,8 +2288,32 @@ def mha(q, k, v, scale=None, causal=False, q_lens=None, kv_lens=None):
         raise ValueError(f"{what}: head_dim {q.shape[3]} is not 64 or 128")
     if k.shape[2] == 0 or q.shape[2] == 0 or q.shape[2] % k.shape[2]:
         raise ValueError(f"{what}: {q.shape[2]} query heads over {k.shape[2]} key heads")
-    return _Mha.apply(q, k, v, _check_scale(what, scale, q.shape[3]), int(bool(causal)), _check_lens(what, "q_lens", q_lens, q),
-                      _check_lens(what, "kv_lens", kv_lens, q))
+    scale, causal = _check_scale(what, scale, q.shape[3]), int(bool(causal))
+    q_lens, kv_lens = _check_lens(what, "q_lens", q_lens, q), _check_lens(what, "kv_lens", kv_lens, q)
+    if _wants_grad(q, k, v):
+        return _Mha.apply(q, k, v, scale, causal, q_lens, kv_lens)
+    q, k, v = _head_rows(q), _head_rows(k), _head_rows(v)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    with _on_device(q):
+        _mha_forward(q, k, v, out, scale, causal, q_lens, kv_lens, False)
+    return out
+
+
+def _attention_rope_forward(qkv, wq, wk, num_heads, scale, rot, want_lse):
+    """(qkv as it is read, q', k' or None, out [B, N, H, d], lse or None) of checked arguments."""
+    B, N, C3 = qkv.shape
+    qkv = qkv.contiguous()
+    if qkv.data_ptr() % 16:
+        qkv = qkv.clone()
+    q, k, v = qkv.view(B, N, 3, num_heads, C3 // 3 // num_heads).unbind(2)
+    turned = rot.norm or rot.positions is not None
+    out, yq, yk = (torch.empty_like(q, memory_format=torch.contiguous_format) if i == 0 or turned else None for i in range(3))
+    with _on_device(qkv):
+        if turned:
+            _rope_forward(q, k, yq, yk, wq, wk, rot)
+            q, k = yq, yk
+        lse = _mha_forward(q, k, v, out, scale, 0, None, None, want_lse)
+    return qkv, yq, yk, out, lse
 
 
 class _AttentionRope(torch.autograd.Function):
@@ -2288,24 +2321,12 @@ class _AttentionRope(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, qkv, wq, wk, num_heads, scale, rot):
-        B, N, C3 = qkv.shape
-        qkv = qkv.contiguous()
-        if qkv.data_ptr() % 16:
-            qkv = qkv.clone()
-        q, k, v = qkv.view(B, N, 3, num_heads, C3 // 3 // num_heads).unbind(2)
         ctx.w_dtypes = (None if wq is None else wq.dtype), (None if wk is None else wk.dtype)
         wq, wk = _head_weights(wq, wk)
-        out = torch.empty(q.shape, device=qkv.device, dtype=qkv.dtype)
-        with _on_device(qkv):
-            turned = rot.norm or rot.positions is not None
-            yq, yk = (torch.empty(q.shape, device=qkv.device, dtype=qkv.dtype) for _ in range(2)) if turned else (q, k)
-            if turned:
-                _rope_forward(q, k, yq, yk, wq, wk, rot)
-            lse = _mha_forward(yq, yk, v, out, scale, 0, None, None, any(ctx.needs_input_grad[:3]))
-        if lse is not None:
-            ctx.save_for_backward(qkv, yq if turned else None, yk if turned else None, wq, wk, out, lse)
-            ctx.scale, ctx.rot = scale, rot
-        return out.view(B, N, C3 // 3)
+        qkv, yq, yk, out, lse = _attention_rope_forward(qkv, wq, wk, num_heads, scale, rot, True)
+        ctx.save_for_backward(qkv, yq, yk, wq, wk, out, lse)
+        ctx.scale, ctx.rot = scale, rot
+        return out.flatten(2)
 
     @staticmethod
     def backward(ctx, *grads):
@@ -2366,7 +2387,10 @@ def attention_rope(qkv, num_heads, scale=None, q_weight=None, k_weight=None, pos
     _check_head_weight(what, "q_weight", q_weight, x)
     _check_head_weight(what, "k_weight", k_weight, x)
     rot = _Rotation(what, x, positions, inv_freq, sections, eps, norm, interleaved)
-    return _AttentionRope.apply(qkv, q_weight, k_weight, num_heads, _check_scale(what, scale, d), rot)
+    scale = _check_scale(what, scale, d)
+    if _wants_grad(qkv, q_weight, k_weight):
+        return _AttentionRope.apply(qkv, q_weight, k_weight, num_heads, scale, rot)
+    return _attention_rope_forward(qkv, *_head_weights(q_weight, k_weight), num_heads, scale, rot, False)[3].flatten(2)
 
 
 # ------------------------------------------------------------------------------ kernel sets (run-time A/B)
