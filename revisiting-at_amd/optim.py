@@ -50,8 +50,7 @@ class _Plan:
 
     def __init__(self, params, groups, bits):
         dev = params[0].device
-        self.ptrs = [p.data_ptr() for p in params]
-        self.dtypes, self.strides = [p.dtype for p in params], [p.stride() for p in params]
+        self.layout = [(p.data_ptr(), p.dtype, p.shape, p.stride()) for p in params]
         self.bits = bits
         self.at, size = [], {32: 0, 8: 0}
         for p, b in zip(params, self.bits):
@@ -69,7 +68,7 @@ class _Plan:
             rows, chunks = [], []
             for i in range(first, min(first + MAX_TENSORS, len(params))):
                 p = params[i]
-                rows.append((self.ptrs[i], p.numel(), self.at[i], self.bits[i], _lib.dtype_code(p.dtype), groups[i], i))
+                rows.append((p.data_ptr(), p.numel(), self.at[i], self.bits[i], _lib.dtype_code(p.dtype), groups[i], i))
                 part = np.arange(-(-p.numel() // CHUNK), dtype=np.int32)
                 chunks.append(np.stack((np.full_like(part, i - first), part), 1))
             table = torch.from_numpy(np.array(rows, dtype=_TENSOR).view(np.uint8).copy()).to(dev)
@@ -134,6 +133,9 @@ class FusedAdamW(torch.optim.Optimizer):
                 raise ValueError(f"FusedAdamW: a parameter with strides {p.stride()} for {tuple(p.shape)} does not fill its memory")
             if p.numel() > CHUNK * (1 << 22):
                 raise ValueError(f"FusedAdamW: a parameter of {p.numel()} elements")
+        spans = sorted((p.data_ptr(), p.numel() * p.element_size()) for p in params if p.numel())
+        if any(a + n > b for (a, n), (b, _) in zip(spans, spans[1:])):
+            raise ValueError("FusedAdamW: two parameters share memory")                        # (their updates would race)
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("FusedAdamW: the first step (and one after parameters were moved or added) has to run outside a graph capture")
         old = {p: dict(self.state[p]) for p in params if self.state.get(p)}
@@ -150,7 +152,8 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def _ready(self, params):
         plan = self._plan
-        if plan is None or self._stale or any(p.data_ptr() != a for p, a in zip(params, plan.ptrs)):
+        # (the address alone does not tell: memory that was given back comes again for other sizes and types)
+        if plan is None or self._stale or [(p.data_ptr(), p.dtype, p.shape, p.stride()) for p in params] != plan.layout:
             plan = self._build()
         return plan
 
@@ -163,7 +166,7 @@ class FusedAdamW(torch.optim.Optimizer):
         params = self._params()
         plan = self._ready(params)
         grads, keep = [], []
-        for p, dtype, stride in zip(params, plan.dtypes, plan.strides):
+        for p, (_, dtype, _, stride) in zip(params, plan.layout):
             g = p.grad
             if g is None:
                 grads.append(None)

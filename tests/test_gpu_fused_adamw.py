@@ -263,6 +263,38 @@ def test_state_dict_goes_on_where_it_was(R, bits, tmp_path):
     assert all(torch.equal(p, q) for p, q in zip(ps, qs)) and float(opt.state[new]["step"]) == 1 and float(opt.state[ps[6]]["step"]) == 3
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_parameters_that_change_in_place(R, bits):
+    """Memory at the same address with another type, order or size."""
+    base = torch.randn(64, 128, generator=torch.Generator().manual_seed(4)).cuda()
+    p = torch.nn.Parameter(base)
+    opt = R.FusedAdamW([p], lr=LR, state_bits=bits)
+    p.grad = torch.ones_like(p)
+    opt.step()
+    for data in (base.view(128, 64).t(), base.view(-1).view(torch.bfloat16)[:8192].view(64, 128)):
+        p.grad, p.data = None, data
+        q = torch.nn.Parameter(data.clone())
+        other = R.FusedAdamW([q], lr=LR, state_bits=bits)
+        other.load_state_dict(copy.deepcopy(opt.state_dict()))
+        p.grad = torch.linspace(-1, 1, 8192, device="cuda").to(data.dtype).view(64, 128)
+        q.grad = p.grad
+        opt.step(), other.step()
+        bits_of = torch.int32 if data.dtype == torch.float32 else torch.int16       # (half of an fp32 number may be a NaN: bits, not values)
+        assert torch.equal(p.data.view(bits_of), q.data.view(bits_of)) and p.data_ptr() == base.data_ptr()
+    p.grad, p.data = None, p.data.view(-1)[:5000]
+    p.grad = torch.ones_like(p)
+    with pytest.raises(RuntimeError):                                               # its moments have another size
+        opt.step()
+
+
+def test_parameters_that_share_memory_are_refused(R):
+    base = torch.zeros(100, device="cuda")
+    a, b = torch.nn.Parameter(base[:60]), torch.nn.Parameter(base[50:])
+    a.grad, b.grad = torch.ones_like(a), torch.ones_like(b)
+    with pytest.raises(ValueError, match="share memory"):
+        R.FusedAdamW([a, b]).step()
+
+
 def test_torch_adamw_state_loads_and_agrees(R):
     ps, g = make(SHAPES, torch.float32, 9)
     qs = copy.deepcopy(ps)

@@ -509,3 +509,49 @@ def test_attention_rope_gradients_against_their_definition(R, case, dtype):
     (again,) = torch.autograd.grad(R.ops.attention_rope(x2, H, None, None if wq is None else wq.detach(), None if wk is None else wk.detach(), pos, inv, sec,
                                                         norm=norm, interleaved=il), (x2,), dout)
     assert torch.equal(again, got[0])
+
+
+@pytest.mark.parametrize("B,N,H", [(0, 5, 2), (2, 0, 2)])
+def test_empty_calls(R, B, N, H):
+    """No sample or no token: empty results and gradients, zeros for the weights'."""
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    q, k = (torch.zeros(B, N, H, 64, device="cuda", dtype=torch.bfloat16, requires_grad=True) for _ in range(2))
+    pos, inv = torch.zeros(N, 1, device="cuda", dtype=torch.int32), torch.ones(32, device="cuda")
+    y = R.ops.qk_norm_rope(q, k, w, w, pos, inv)
+    gq, gw = torch.autograd.grad(y, (q, w), [torch.zeros_like(t) for t in y])
+    assert y[0].shape == gq.shape == q.shape and not bool(gw.any())
+    out = R.ops.mha(q, k, k)
+    assert out.shape == q.shape and torch.autograd.grad(out, q, torch.zeros_like(out))[0].shape == q.shape
+    qkv = torch.zeros(B, N, 3 * H * 64, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    out = R.ops.attention_rope(qkv, H, None, w, w, pos, inv)
+    gq, gw = torch.autograd.grad(out, (qkv, w), torch.zeros_like(out))
+    assert out.shape == (B, N, H * 64) and gq.shape == qkv.shape and not bool(gw.any())
+
+
+def test_attention_rope_backward_in_a_graph(R):
+    """Forward and backward captured, replayed with eager work in between."""
+    g = torch.Generator().manual_seed(5)
+    qkv = torch.randn(2, 150, 3 * 128, generator=g).to(torch.bfloat16).cuda().requires_grad_()
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    pos, inv = torch.arange(150, device="cuda").view(-1, 1), 100.0 ** (-torch.arange(32, device="cuda") / 32)
+    dout = torch.randn(2, 150, 128, generator=g).to(torch.bfloat16).cuda()
+
+    def both():
+        out = R.ops.attention_rope(qkv, 2, None, w, w, pos, inv)
+        return (out.detach(),) + torch.autograd.grad(out, (qkv, w), dout)
+    want = both()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = both()
+    for _ in range(3):
+        for t in got:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert all(torch.equal(a, b) for a, b in zip(both(), want))

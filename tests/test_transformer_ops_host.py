@@ -51,6 +51,28 @@ def test_mha_refuses_missing_outputs_and_workspace(R):
     assert [lib.cnx_mha_supported(d) for d in (0, 32, 64, 96, 128, 256)] == [0, 0, 1, 0, 1, 0]
 
 
+def attn_bwd(lib, qkv=P, out=P, dqkv=P, ws=P, strides=S24, dtype=1, pos=P, pos_dtype=2, axes=2, sections=(16, 16), inv=P, B=1, N=4, H=2, d=64, dw=None,
+             norm=1, scale=0.125):
+    sec = None if sections is None else (ctypes.c_int32 * len(sections))(*sections)
+    return lib.cnx_attention_rope_bwd(qkv, P, P, out, P, P, dqkv, dw, dw, ws, strides, dtype, None, None, pos, pos_dtype, 0, axes, sec, inv, B, N, H, d,
+                                      1e-6, norm, 0, scale, None)
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(qkv=None), NULL), (dict(out=None), NULL), (dict(dqkv=None), NULL), (dict(ws=None), NULL), (dict(strides=None), NULL), (dict(dtype=0), DTYPE),
+    (dict(d=32), ARG), (dict(H=0), SIZE), (dict(B=0), SIZE), (dict(N=0), SIZE), (dict(N=-1), SIZE), (dict(B=1, N=1000), SIZE), (dict(scale=0.0), ARG),
+    (dict(dw=P, norm=0), ARG), (dict(inv=None), NULL), (dict(sections=None), NULL), (dict(pos_dtype=3), DTYPE), (dict(axes=5), ARG),
+    (dict(sections=(16, 17)), ARG), (dict(B=2 ** 40), SIZE)])
+def test_attention_rope_backward_refuses(R, kw, code):
+    assert attn_bwd(R._lib.load(), **kw) == code
+
+
+def test_attention_rope_backward_workspace(R):
+    size = R._lib.load().cnx_attention_rope_bwd_ws_floats
+    assert size(2, 17, 2, 64, 0) == 68 + 17 * 64 + 2 * 4 * 64 and size(2, 17, 2, 64, 1) == 68 + 2 * 17 * 64 + 2 * 4 * 64
+    assert size(1, 1000, 2, 64, 0) == 0 and size(1, 17, 2, 96, 0) == 0 and size(0, 17, 2, 64, 0) == 0     # rows split, no such head, empty
+
+
 def rope(lib, fwd=True, q=P, out=P, strides=S24, dtype=1, w=None, w_dtype=0, pos=P, pos_dtype=2, axes=2, sections=(16, 16), inv=P, B=1, N=4, Hq=2,
          Hk=2, d=64, dw=None, ws=None, norm=1):
     sec = None if sections is None else (ctypes.c_int32 * len(sections))(*sections)
