@@ -32,6 +32,7 @@ MODE = os.environ.get("APGD_OPS", "hip")
 # torch's own ops get this from the engine's per-call output mask; Python Functions only see the
 # static ctx.needs_input_grad, so the fused operators consult this flag to skip parameter gradients.
 _INPUT_GRAD_ONLY = False
+_INPUT_GRAD_ONLY_NATIVE = ctypes.c_int32(0)                        # the same for the C++ nodes
 
 
 class input_grad_only:
@@ -41,11 +42,13 @@ class input_grad_only:
         global _INPUT_GRAD_ONLY
         self._prev = _INPUT_GRAD_ONLY
         _INPUT_GRAD_ONLY = True
+        _INPUT_GRAD_ONLY_NATIVE.value = 1
         return self
 
     def __exit__(self, *exc):
         global _INPUT_GRAD_ONLY
         _INPUT_GRAD_ONLY = self._prev
+        _INPUT_GRAD_ONLY_NATIVE.value = int(self._prev)
         return False
 
 
@@ -1974,18 +1977,28 @@ def attention(qkv, num_heads, scale):
     return (a @ v).transpose(1, 2).reshape(B, N, C)
 
 
-# ------------------------------------------------------------------------------ heads: norm and rotation
-_NO_SWITCH = contextlib.nullcontext()
+# ------------------------------------------------------------------------------ heads: norm and rotation, attention of any length
+# Autograd nodes and launches of the three operators are C++ (csrc/heads_binding.cpp); what a call may be is checked here.
+_HEADS = None
+
+
+def _heads():
+    """The extension, bound to the library that ``_lib`` has loaded and to the flag of ``input_grad_only``."""
+    global _HEADS
+    if _HEADS is None:
+        try:
+            from . import _heads as module
+        except ImportError as e:
+            raise _lib.ApgdHipError(f"revisiting-at_amd/_heads.so cannot be loaded ({e}): build it with `python -c 'import __graft_entry__ as g; "
+                                    "g.build()'` or `make -C revisiting-at_amd/csrc`") from e
+        module.bind(_lib.load()._handle, ctypes.addressof(_INPUT_GRAD_ONLY_NATIVE))
+        _HEADS = module
+    return _HEADS
 
 
 def _on_device(t):
     """Context in which kernels on ``t`` are launched: its own device, also where another one is current."""
-    return _NO_SWITCH if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
-
-
-def _raw_stream():
-    """``_stream()`` without building a Stream object (3 us of the 20 that a small call takes)."""
-    return _SIDE.handle if _SIDE is not None else torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+    return contextlib.nullcontext() if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
 def _check_heads(what, *named):
@@ -2010,84 +2023,37 @@ def _check_heads(what, *named):
             raise ValueError(f"{what}: {name} {tuple(t.shape)} does not go with {named[0][0]} {tuple(first.shape)}")
 
 
-def _head_rows(t):
-    """``t`` [B, N, H, d] itself where the kernels can read it in place (contiguous heads that begin at 16 bytes, any other strides up to 2^22
-    elements between tokens and 2^28 over a token's heads, zero included), else a contiguous copy."""
-    piece = 16 // t.element_size()
-    st = t.stride()
-    if (st[3] == 1 and st[0] % piece == 0 and st[1] % piece == 0 and st[2] % piece == 0 and t.data_ptr() % 16 == 0
-            and st[1] < 1 << 22 and st[2] * t.shape[2] < 1 << 28):
-        return t
-    return torch.empty(t.shape, device=t.device, dtype=t.dtype).copy_(t)
+_POSITIONS = {torch.float32: 0, torch.int32: 1, torch.int64: 2}                # CNX_POS_*
 
 
-def _strides(*tensors):
-    """(sample, token, head) strides of [B, N, H, d] tensors as one host array of the C ABI."""
-    v = [s for t in tensors for s in t.stride()[:3]]
-    return (ctypes.c_int64 * len(v))(*v)
-
-
-def _put_strides(array, at, t):
-    """``t``'s strides as the ``at``-th tensor's of ``array``, in a copy where they differ."""
-    v = t.stride()[:3]
-    if v != tuple(array[3 * at:3 * at + 3]):
-        array = type(array)(*array)
-        array[3 * at:3 * at + 3] = v
-    return array
-
-
-def _backward_once(gradients, ctx, grads):
-    """A backward that has no derivative of its own: where a graph of the gradient is recorded, using it raises."""
-    if torch.is_grad_enabled():
-        return torch.autograd.function.once_differentiable(gradients)(ctx, *grads)
-    return gradients(ctx, *grads)
-
-
-def _wants_grad(*tensors):
-    """Whether autograd has to see the call; without it the kernels are launched directly (a recorded call costs the host 5 us more)."""
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-class _Rotation:
-    """Checked arguments of the rotation and the norm, as the C entry points take them."""
-    __slots__ = ("positions", "inv_freq", "sections", "axes", "code", "batch_stride", "eps", "norm", "interleaved")
-
-    _CODES = {torch.float32: 0, torch.int32: 1, torch.int64: 2}                # CNX_POS_*
-
-    def __init__(self, what, x, positions, inv_freq, sections, eps, norm, interleaved):
-        d = x.shape[-1]
-        self.eps, self.norm, self.interleaved = float(eps), int(bool(norm)), int(bool(interleaved))
-        if not self.eps >= 0.0:
-            raise ValueError(f"{what}: eps={eps!r}")
-        self.positions, self.inv_freq, self.sections, self.axes, self.code, self.batch_stride = None, None, None, 0, 0, 0
-        if positions is None:
-            if inv_freq is not None or sections is not None:
-                raise ValueError(f"{what}: inv_freq and sections go with positions")
-            return
-        if not isinstance(positions, torch.Tensor) or positions.dtype not in self._CODES:
-            raise TypeError(f"{what}: positions has to be a tensor of float32, int32 or int64")
-        if not isinstance(inv_freq, torch.Tensor) or inv_freq.dtype != torch.float32 or tuple(inv_freq.shape) != (d // 2,):
-            raise ValueError(f"{what}: inv_freq has to be a float32 tensor of head_dim / 2 = {d // 2} frequencies")
-        if positions.device != x.device or inv_freq.device != x.device:
-            raise ValueError(f"{what}: positions and inv_freq have to be on {x.device}")
-        if positions.requires_grad or inv_freq.requires_grad:
-            raise ValueError(f"{what}: positions and inv_freq have no gradient")
-        B, N = x.shape[:2]
-        if positions.dim() not in (2, 3) or positions.shape[-2] != N or (positions.dim() == 3 and positions.shape[0] != B):
-            raise ValueError(f"{what}: positions has to be [tokens, axes] or [batch, tokens, axes] for {B} x {N} tokens, "
-                             f"not {tuple(positions.shape)}")
-        self.axes = positions.shape[-1]
-        sections = (d // 2,) if sections is None else tuple(int(v) for v in sections)
-        if not 1 <= self.axes <= 4 or len(sections) != self.axes or min(sections) < 0 or sum(sections) != d // 2:
-            raise ValueError(f"{what}: sections={sections} has to split the {d // 2} pairs of a head over the {self.axes} axes of positions "
-                             "(1 to 4)")
-        self.positions, self.inv_freq = positions.contiguous(), inv_freq.contiguous()
-        self.sections = (ctypes.c_int32 * self.axes)(*sections)
-        self.code = self._CODES[positions.dtype]
-        self.batch_stride = N * self.axes if positions.dim() == 3 else 0
-
-    def args(self):
-        return _lib.ptr(self.positions), self.code, self.batch_stride, self.axes, self.sections, _lib.ptr(self.inv_freq)
+def _rotation(what, x, positions, inv_freq, sections, eps, norm, interleaved):
+    """Checked arguments of the norm and the rotation of ``x`` [B, N, H, d], as the extension takes them."""
+    d = x.shape[-1]
+    eps = float(eps)
+    if not eps >= 0.0:
+        raise ValueError(f"{what}: eps={eps!r}")
+    if positions is None:
+        if inv_freq is not None or sections is not None:
+            raise ValueError(f"{what}: inv_freq and sections go with positions")
+        return None, None, (), 0, 0, eps, bool(norm), bool(interleaved)
+    if not isinstance(positions, torch.Tensor) or positions.dtype not in _POSITIONS:
+        raise TypeError(f"{what}: positions has to be a tensor of float32, int32 or int64")
+    if not isinstance(inv_freq, torch.Tensor) or inv_freq.dtype != torch.float32 or inv_freq.shape != (d // 2,):
+        raise ValueError(f"{what}: inv_freq has to be a float32 tensor of head_dim / 2 = {d // 2} frequencies")
+    if positions.device != x.device or inv_freq.device != x.device:
+        raise ValueError(f"{what}: positions and inv_freq have to be on {x.device}")
+    if positions.requires_grad or inv_freq.requires_grad:
+        raise ValueError(f"{what}: positions and inv_freq have no gradient")
+    B, N = x.shape[:2]
+    shape = positions.shape
+    if len(shape) not in (2, 3) or shape[-2] != N or (len(shape) == 3 and shape[0] != B):
+        raise ValueError(f"{what}: positions has to be [tokens, axes] or [batch, tokens, axes] for {B} x {N} tokens, not {tuple(shape)}")
+    axes = shape[-1]
+    sections = (d // 2,) if sections is None else tuple(int(v) for v in sections)
+    if not 1 <= axes <= 4 or len(sections) != axes or min(sections) < 0 or sum(sections) != d // 2:
+        raise ValueError(f"{what}: sections={sections} has to split the {d // 2} pairs of a head over the {axes} axes of positions (1 to 4)")
+    return (positions.contiguous(), inv_freq.contiguous(), sections, _POSITIONS[positions.dtype], N * axes if len(shape) == 3 else 0, eps, bool(norm),
+            bool(interleaved))
 
 
 def _check_head_weight(what, name, w, x):
@@ -2097,74 +2063,6 @@ def _check_head_weight(what, name, w, x):
         raise ValueError(f"{what}: {name} has to be a tensor of head_dim = {x.shape[-1]} values")
     if w.dtype not in (torch.float32, x.dtype) or w.device != x.device:
         raise TypeError(f"{what}: {name} has to be float32 or {x.dtype} on {x.device}, not {w.dtype} on {w.device}")
-
-
-def _rope_forward(q, k, yq, yk, wq, wk, rot, strides=None):
-    """``qk_norm_rope`` of checked, readable tensors into ``yq`` / ``yk``."""
-    w = wq if wq is not None else wk
-    B, N, Hq, d = q.shape
-    _lib.check(_lib.load().cnx_qk_norm_rope_fwd(
-        q.data_ptr(), k.data_ptr(), yq.data_ptr(), yk.data_ptr(), _code(q), strides or _strides(q, k, yq, yk), _lib.ptr(wq), _lib.ptr(wk),
-        _code(w) if w is not None else 0, *rot.args(), B, N, Hq, k.shape[2], d, rot.eps, rot.norm, rot.interleaved, _raw_stream()),
-        "cnx_qk_norm_rope_fwd")
-
-
-def _rope_backward(dyq, dyk, q, k, dq, dk, wq, wk, rot, want_wq, want_wk, strides=None):
-    """Gradients of ``qk_norm_rope`` into ``dq`` / ``dk``; returns those of the weights (fp32) or None."""
-    lib = _lib.load()
-    w = wq if wq is not None else wk
-    B, N, Hq, d = dyq.shape
-    dwq = torch.empty(d, device=dyq.device, dtype=torch.float32) if want_wq else None
-    dwk = torch.empty(d, device=dyq.device, dtype=torch.float32) if want_wk else None
-    ws = torch.empty(lib.cnx_qk_norm_rope_ws_floats(d), device=dyq.device, dtype=torch.float32) if want_wq or want_wk else None
-    x = (q, k) if rot.norm else (dyq, dyk)                                      # without norm q and k are not read
-    _lib.check(lib.cnx_qk_norm_rope_bwd(
-        dyq.data_ptr(), dyk.data_ptr(), x[0].data_ptr(), x[1].data_ptr(), dq.data_ptr(), dk.data_ptr(), _lib.ptr(dwq), _lib.ptr(dwk),
-        _lib.ptr(ws), _code(dyq), strides or _strides(dyq, dyk, *x, dq, dk), _lib.ptr(wq), _lib.ptr(wk), _code(w) if w is not None else 0, *rot.args(),
-        B, N, Hq, dyk.shape[2], d, rot.eps, rot.norm, rot.interleaved, _raw_stream()), "cnx_qk_norm_rope_bwd")
-    return dwq, dwk
-
-
-def _head_weights(wq, wk):
-    """Weights of one type: where one is float32 and the other is not, both are."""
-    if wq is not None and wk is not None and wq.dtype != wk.dtype:
-        wq, wk = wq.float(), wk.float()
-    return (None if wq is None else wq.contiguous()), (None if wk is None else wk.contiguous())
-
-
-class _QkNormRope(torch.autograd.Function):
-
-    @staticmethod
-    def forward(ctx, q, k, wq, wk, rot):
-        q, k = _head_rows(q), _head_rows(k)
-        yq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        yk = torch.empty(k.shape, device=k.device, dtype=k.dtype)
-        ctx.strides = _strides(yq, yk, q, k, yq, yk)               # dyq, dyk, q, k, dq, dk of the backward; from q on the forward's four
-        ctx.w_dtypes = (None if wq is None else wq.dtype), (None if wk is None else wk.dtype)
-        wq, wk = _head_weights(wq, wk)
-        with _on_device(q):
-            _rope_forward(q, k, yq, yk, wq, wk, rot, (ctypes.c_int64 * 12).from_buffer(ctx.strides, 48))
-        ctx.save_for_backward(*((q, k) if rot.norm else (None, None)), wq, wk)
-        ctx.rot = rot
-        return yq, yk
-
-    @staticmethod
-    def backward(ctx, *grads):
-        return _backward_once(_QkNormRope._gradients, ctx, grads)
-
-    @staticmethod
-    def _gradients(ctx, dyq, dyk):
-        q, k, wq, wk = ctx.saved_tensors
-        dyq, dyk = _head_rows(dyq), _head_rows(dyk)
-        dq, dk = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (dyq, dyk))
-        strides = _put_strides(_put_strides(ctx.strides, 0, dyq), 1, dyk)
-        if not ctx.rot.norm:                                       # q and k are not read: their places are taken by dyq and dyk
-            strides = _put_strides(_put_strides(strides, 2, dyq), 3, dyk)
-        need = ctx.needs_input_grad
-        with _on_device(dyq):
-            dwq, dwk = _rope_backward(dyq, dyk, q, k, dq, dk, wq, wk, ctx.rot, need[2] and not _INPUT_GRAD_ONLY, need[3] and not _INPUT_GRAD_ONLY,
-                                      strides)
-        return dq, dk, None if dwq is None else dwq.to(ctx.w_dtypes[0]), None if dwk is None else dwk.to(ctx.w_dtypes[1]), None
 
 
 def qk_norm_rope(q, k, q_weight=None, k_weight=None, positions=None, inv_freq=None, sections=None, eps=1e-6, norm=True, interleaved=False):
@@ -2188,71 +2086,7 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, positions=None, inv_freq=No
         raise ValueError(f"{what}: q_weight and k_weight go with norm=True")
     _check_head_weight(what, "q_weight", q_weight, q)
     _check_head_weight(what, "k_weight", k_weight, k)
-    rot = _Rotation(what, q, positions, inv_freq, sections, eps, norm, interleaved)
-    if _wants_grad(q, k, q_weight, k_weight):
-        return _QkNormRope.apply(q, k, q_weight, k_weight, rot)
-    q, k = _head_rows(q), _head_rows(k)
-    yq, yk = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k))
-    with _on_device(q):
-        _rope_forward(q, k, yq, yk, *_head_weights(q_weight, k_weight), rot)
-    return yq, yk
-
-
-# ------------------------------------------------------------------------------ attention over any number of tokens
-def _mha_forward(q, k, v, out, scale, causal, q_lens, kv_lens, want_lse, strides=None):
-    """``mha`` of checked, readable tensors into ``out``; returns lse [B, H, Nq] or None."""
-    lib = _lib.load()
-    B, Nq, H, d = q.shape
-    Nk, Hkv = k.shape[1], k.shape[2]
-    lse = torch.empty(B, H, Nq, device=q.device, dtype=torch.float32) if want_lse else None
-    n = lib.cnx_mha_ws_floats(B, Nq, Nk, H, Hkv, d)
-    ws = torch.empty(n, device=q.device, dtype=torch.float32) if n else None
-    _lib.check(lib.cnx_mha_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _lib.ptr(lse), _lib.ptr(q_lens), _lib.ptr(kv_lens),
-                               _lib.ptr(ws), strides or _strides(q, k, v, out), _code(q), B, Nq, Nk, H, Hkv, d, causal, scale, _raw_stream()), "cnx_mha_fwd")
-    return lse
-
-
-def _mha_backward(q, k, v, out, dout, lse, dq, dk, dv, scale, causal, q_lens, kv_lens, strides=None):
-    lib = _lib.load()
-    B, Nq, H, d = q.shape
-    Nk, Hkv = k.shape[1], k.shape[2]
-    dvec = torch.empty(B, H, Nq, device=q.device, dtype=torch.float32)
-    n = lib.cnx_mha_bwd_ws_floats(B, Nq, Nk, H, Hkv, d, causal)
-    ws = torch.empty(n, device=q.device, dtype=torch.float32) if n else None
-    _lib.check(lib.cnx_mha_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), lse.data_ptr(), dq.data_ptr(),
-                               dk.data_ptr(), dv.data_ptr(), dvec.data_ptr(), _lib.ptr(q_lens), _lib.ptr(kv_lens), _lib.ptr(ws),
-                               strides or _strides(q, k, v, out, dout, dq, dk, dv), _code(q), B, Nq, Nk, H, Hkv, d, causal, scale, _raw_stream()), "cnx_mha_bwd")
-
-
-class _Mha(torch.autograd.Function):
-
-    @staticmethod
-    def forward(ctx, q, k, v, scale, causal, q_lens, kv_lens):
-        q, k, v = _head_rows(q), _head_rows(k), _head_rows(v)
-        out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        # q, k, v, out and, contiguous, dout, dq, dk, dv: made here because the backward's thread takes twice as long for the same
-        _, n, h, d = k.shape
-        like_k = n * h * d, h * d, d
-        like_q = out.stride()[:3]
-        ctx.strides = (ctypes.c_int64 * 24)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *like_q, *like_q, *like_q, *like_k, *like_k)
-        with _on_device(q):
-            lse = _mha_forward(q, k, v, out, scale, causal, q_lens, kv_lens, True, ctx.strides)
-        ctx.save_for_backward(q, k, v, out, lse, q_lens, kv_lens)
-        ctx.scale, ctx.causal = scale, causal
-        return out
-
-    @staticmethod
-    def backward(ctx, *grads):
-        return _backward_once(_Mha._gradients, ctx, grads)
-
-    @staticmethod
-    def _gradients(ctx, dout):
-        q, k, v, out, lse, q_lens, kv_lens = ctx.saved_tensors
-        dout = _head_rows(dout)
-        dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
-        with _on_device(q):
-            _mha_backward(q, k, v, out, dout, lse, dq, dk, dv, ctx.scale, ctx.causal, q_lens, kv_lens, _put_strides(ctx.strides, 4, dout))
-        return dq, dk, dv, None, None, None, None
+    return _heads().qk_norm_rope(q, k, q_weight, k_weight, *_rotation(what, q, positions, inv_freq, sections, eps, norm, interleaved))
 
 
 def _check_lens(what, name, lens, q):
@@ -2288,80 +2122,8 @@ def mha(q, k, v, scale=None, causal=False, q_lens=None, kv_lens=None):
         raise ValueError(f"{what}: head_dim {q.shape[3]} is not 64 or 128")
     if k.shape[2] == 0 or q.shape[2] == 0 or q.shape[2] % k.shape[2]:
         raise ValueError(f"{what}: {q.shape[2]} query heads over {k.shape[2]} key heads")
-    scale, causal = _check_scale(what, scale, q.shape[3]), int(bool(causal))
-    q_lens, kv_lens = _check_lens(what, "q_lens", q_lens, q), _check_lens(what, "kv_lens", kv_lens, q)
-    if _wants_grad(q, k, v):
-        return _Mha.apply(q, k, v, scale, causal, q_lens, kv_lens)
-    q, k, v = _head_rows(q), _head_rows(k), _head_rows(v)
-    out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    with _on_device(q):
-        _mha_forward(q, k, v, out, scale, causal, q_lens, kv_lens, False)
-    return out
-
-
-def _attention_rope_forward(qkv, wq, wk, num_heads, scale, rot, want_lse):
-    """(qkv as it is read, q', k' or None, out [B, N, H, d], lse or None) of checked arguments."""
-    B, N, C3 = qkv.shape
-    qkv = qkv.contiguous()
-    if qkv.data_ptr() % 16:
-        qkv = qkv.clone()
-    q, k, v = qkv.view(B, N, 3, num_heads, C3 // 3 // num_heads).unbind(2)
-    turned = rot.norm or rot.positions is not None
-    out, yq, yk = (torch.empty_like(q, memory_format=torch.contiguous_format) if i == 0 or turned else None for i in range(3))
-    with _on_device(qkv):
-        if turned:
-            _rope_forward(q, k, yq, yk, wq, wk, rot)
-            q, k = yq, yk
-        lse = _mha_forward(q, k, v, out, scale, 0, None, None, want_lse)
-    return qkv, yq, yk, out, lse
-
-
-class _AttentionRope(torch.autograd.Function):
-    """``qk_norm_rope`` and ``mha`` on a packed projection: q, k, v and their gradients stay slices of it, no copies between the two."""
-
-    @staticmethod
-    def forward(ctx, qkv, wq, wk, num_heads, scale, rot):
-        ctx.w_dtypes = (None if wq is None else wq.dtype), (None if wk is None else wk.dtype)
-        wq, wk = _head_weights(wq, wk)
-        qkv, yq, yk, out, lse = _attention_rope_forward(qkv, wq, wk, num_heads, scale, rot, True)
-        ctx.save_for_backward(qkv, yq, yk, wq, wk, out, lse)
-        ctx.scale, ctx.rot = scale, rot
-        return out.flatten(2)
-
-    @staticmethod
-    def backward(ctx, *grads):
-        return _backward_once(_AttentionRope._gradients, ctx, grads)
-
-    @staticmethod
-    def _gradients(ctx, dout):
-        qkv, yq, yk, wq, wk, out, lse = ctx.saved_tensors
-        B, N, H, d = out.shape
-        q, k, v = qkv.view(B, N, 3, H, d).unbind(2)
-        turned = yq is not None
-        dout = _head_rows(dout.reshape(B, N, H, d))
-        dqkv = torch.empty_like(qkv)
-        dq, dk, dv = dqkv.view(B, N, 3, H, d).unbind(2)
-        dwq = dwk = None
-        with _on_device(qkv):
-            want = [ctx.needs_input_grad[i] and not _INPUT_GRAD_ONLY for i in (1, 2)]
-            n = _lib.load().cnx_attention_rope_bwd_ws_floats(B, N, H, d, ctx.rot.batch_stride != 0) if turned else 0
-            if n:
-                ws = torch.empty(n, device=qkv.device, dtype=torch.float32)
-                dwq, dwk = (torch.empty(d, device=qkv.device, dtype=torch.float32) if w else None for w in want)
-                fq, fk = (None if w is None else w.float() for w in (wq, wk))
-                _lib.check(_lib.load().cnx_attention_rope_bwd(
-                    qkv.data_ptr(), yq.data_ptr(), yk.data_ptr(), out.data_ptr(), dout.data_ptr(), lse.data_ptr(), dqkv.data_ptr(), _lib.ptr(dwq),
-                    _lib.ptr(dwk), ws.data_ptr(), _strides(dout), _code(qkv), _lib.ptr(fq), _lib.ptr(fk), *ctx.rot.args(), B, N, H, d, ctx.rot.eps,
-                    ctx.rot.norm, ctx.rot.interleaved, ctx.scale, _raw_stream()), "cnx_attention_rope_bwd")
-                dwq, dwk = (None if g is None else g.to(dt) for g, dt in zip((dwq, dwk), ctx.w_dtypes))
-            elif turned:
-                dyq, dyk = torch.empty_like(yq), torch.empty_like(yk)
-                _mha_backward(yq, yk, v, out, dout, lse, dyq, dyk, dv, ctx.scale, 0, None, None)
-                dwq, dwk = _rope_backward(dyq, dyk, q, k, dq, dk, wq, wk, ctx.rot, *want)
-                dwq, dwk = (None if g is None else g.to(dt) for g, dt in zip((dwq, dwk), ctx.w_dtypes))
-            else:
-                _mha_backward(q, k, v, out, dout, lse, dq, dk, dv, ctx.scale, 0, None, None)
-        return dqkv, dwq, dwk, None, None, None
+    return _heads().mha(q, k, v, _check_scale(what, scale, q.shape[3]), bool(causal), _check_lens(what, "q_lens", q_lens, q),
+                        _check_lens(what, "kv_lens", kv_lens, q))
 
 
 def attention_rope(qkv, num_heads, scale=None, q_weight=None, k_weight=None, positions=None, inv_freq=None, sections=None, eps=1e-6,
@@ -2386,11 +2148,8 @@ def attention_rope(qkv, num_heads, scale=None, q_weight=None, k_weight=None, pos
     x = qkv.detach().unsqueeze(2)[..., :d]                                     # [B, N, 1, d]: what the checks go by
     _check_head_weight(what, "q_weight", q_weight, x)
     _check_head_weight(what, "k_weight", k_weight, x)
-    rot = _Rotation(what, x, positions, inv_freq, sections, eps, norm, interleaved)
-    scale = _check_scale(what, scale, d)
-    if _wants_grad(qkv, q_weight, k_weight):
-        return _AttentionRope.apply(qkv, q_weight, k_weight, num_heads, scale, rot)
-    return _attention_rope_forward(qkv, *_head_weights(q_weight, k_weight), num_heads, scale, rot, False)[3].flatten(2)
+    return _heads().attention_rope(qkv, num_heads, _check_scale(what, scale, d), q_weight, k_weight,
+                                   *_rotation(what, x, positions, inv_freq, sections, eps, norm, interleaved))
 
 
 # ------------------------------------------------------------------------------ kernel sets (run-time A/B)
