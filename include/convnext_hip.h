@@ -420,11 +420,19 @@ int cnx_qk_norm_rope_bwd(const void* dyq, const void* dyk, const void* q, const 
                          int64_t B, int64_t N, int32_t Hq, int32_t Hk, int32_t d, float eps, int32_t norm, int32_t interleaved,
                          void* stream);
 
-/* Backward pass of the two chained on a packed projection in one: mha's of q', k' and v, whose dq' and dk' go through the rotation and the
- * norm where they are summed, in fp32, without a pass of their own.  qkv, dqkv [B, N, 3, H, d], yq, yk (q', k' as cnx_qk_norm_rope_fwd left
- * them), out [B, N, H, d]: contiguous; dout: `dout_strides` (sample, token, head).  No lengths, not causal; wq, wk fp32 [d] or NULL; dwq, dwk
- * fp32 [d] or NULL; the rest as above.  ws: cnx_attention_rope_bwd_ws_floats(...) floats (own_positions: the samples have their own);
- * 0 = not in this form (few rows, which are split over workgroups: cnx_mha_bwd and cnx_qk_norm_rope_bwd). */
+/* The two chained on a packed projection qkv [B, N, 3, H, d] (contiguous, bf16 or fp16): out [B, N, H, d], lse [B, H, N] (nullable).  yq, yk
+ * [B, N, H, d]: room for q' and k', which the backward reads again (not used, and may be NULL, without norm and positions).  Where a bf16
+ * projection is normalised they are in fp16: their size is the weights' (2^-14 .. 5000 is within fp16's range; beyond it they end at its
+ * largest number), and fp16 keeps three bits more of them, which the scores and the gradients see.  No lengths, not causal.
+ * ws: cnx_mha_ws_floats(B, N, N, H, H, head_dim) floats; the rest as above. */
+int cnx_attention_rope_fwd(const void* qkv, void* yq, void* yk, void* out, float* lse, float* ws, int dtype, const void* wq, const void* wk,
+                           int w_dtype, const void* positions, int pos_dtype, int64_t pos_batch_stride, int32_t axes, const int32_t* sections,
+                           const float* inv_freq, int64_t B, int32_t N, int32_t H, int32_t head_dim, float eps, int32_t norm,
+                           int32_t interleaved, float scale, void* stream);
+/* Their backward pass in one (with a norm or positions; without either it is cnx_mha_bwd's): mha's of q', k' and v, whose dq' and dk' go
+ * through the rotation and the norm where they are summed, in fp32, without a pass of their own.  dqkv like qkv; dout: `dout_strides`
+ * (sample, token, head); wq, wk fp32 [d] or NULL; dwq, dwk fp32 [d] or NULL.  ws: cnx_attention_rope_bwd_ws_floats(...) floats
+ * (own_positions: the samples have their own). */
 int64_t cnx_attention_rope_bwd_ws_floats(int64_t B, int32_t N, int32_t H, int32_t head_dim, int32_t own_positions);
 int cnx_attention_rope_bwd(const void* qkv, const void* yq, const void* yk, const void* out, const void* dout, const float* lse, void* dqkv,
                            float* dwq, float* dwk, float* ws, const int64_t* dout_strides, int dtype, const float* wq, const float* wk,

@@ -101,6 +101,8 @@ PROTOTYPES = {
     "cnx_mha_bwd_ws_floats": (C.c_int64, [_i64, _i32, _i32, _i32, _i32, _i32, _i32]),
     "cnx_mha_fwd": (C.c_int, [_p, _p, _p, _p, _p, _p, _p, _p, _p, C.c_int, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _f, _p]),
     "cnx_mha_bwd": (C.c_int, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, C.c_int, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _f, _p]),
+    "cnx_attention_rope_fwd": (C.c_int, [_p, _p, _p, _p, _p, _p, C.c_int, _p, _p, C.c_int, _p, C.c_int, _i64, _i32, _p, _p, _i64, _i32, _i32, _i32, _f,
+                                         _i32, _i32, _f, _p]),
     "cnx_attention_rope_bwd_ws_floats": (C.c_int64, [_i64, _i32, _i32, _i32, _i32]),
     "cnx_attention_rope_bwd": (C.c_int, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, C.c_int, _p, _p, _p, C.c_int, _i64, _i32, _p, _p, _i64, _i32,
                                          _i32, _i32, _f, _i32, _i32, _f, _p]),

@@ -31,6 +31,7 @@ struct Library {
   decltype(&cnx_qk_norm_rope_ws_floats) rope_ws_floats;
   decltype(&cnx_qk_norm_rope_fwd) rope_fwd;
   decltype(&cnx_qk_norm_rope_bwd) rope_bwd;
+  decltype(&cnx_attention_rope_fwd) layer_fwd;
   decltype(&cnx_attention_rope_bwd_ws_floats) layer_bwd_ws_floats;
   decltype(&cnx_attention_rope_bwd) layer_bwd;
 } lib = {};
@@ -50,6 +51,7 @@ void bind(uintptr_t handle, uintptr_t flag) {
   find(lib.rope_ws_floats, "cnx_qk_norm_rope_ws_floats");
   find(lib.rope_fwd, "cnx_qk_norm_rope_fwd");
   find(lib.rope_bwd, "cnx_qk_norm_rope_bwd");
+  find(lib.layer_fwd, "cnx_attention_rope_fwd");
   find(lib.layer_bwd_ws_floats, "cnx_attention_rope_bwd_ws_floats");
   find(lib.layer_bwd, "cnx_attention_rope_bwd");
   input_grad_only = reinterpret_cast<const volatile int32_t*>(flag);
@@ -290,9 +292,9 @@ struct AttentionRopeBackward : Node {
     const Tensor out = saved[6].unpack(shared_from_this()).view({B, N, heads, d}), dout = head_rows(in[0].reshape({B, N, heads, d})), dqkv = fresh(qkv);
     const bool want_q = wants(1) && !*input_grad_only, want_k = wants(2) && !*input_grad_only;
     Tensor dwq, dwk;
-    const int64_t n = rot.turns() ? lib.layer_bwd_ws_floats(B, N, heads, d, rot.batch_stride != 0) : 0;
-    if (n) {
-      const Tensor ws = floats(n, qkv), fq = wq.defined() ? wq.to(at::kFloat) : wq, fk = wk.defined() ? wk.to(at::kFloat) : wk;
+    if (rot.turns()) {
+      const Tensor ws = floats(lib.layer_bwd_ws_floats(B, N, heads, d, rot.batch_stride != 0), qkv);
+      const Tensor fq = wq.defined() ? wq.to(at::kFloat) : wq, fk = wk.defined() ? wk.to(at::kFloat) : wk;
       if (want_q) dwq = floats(d, qkv);
       if (want_k) dwk = floats(d, qkv);
       check(lib.layer_bwd(qkv.data_ptr(), yq.data_ptr(), yk.data_ptr(), out.data_ptr(), dout.data_ptr(), ptr<float>(lse), dqkv.data_ptr(), ptr<float>(dwq),
@@ -302,13 +304,7 @@ struct AttentionRopeBackward : Node {
             "cnx_attention_rope_bwd");
     } else {
       const auto x = parts(qkv, heads), g = parts(dqkv, heads);
-      if (rot.turns()) {
-        const Tensor dyq = fresh(yq), dyk = fresh(yk);
-        mha_backward(yq, yk, x[2], out, dout, lse, dyq, dyk, g[2], scale, false, Tensor(), Tensor());
-        rope_backward(dyq, dyk, x[0], x[1], g[0], g[1], wq, wk, rot, want_q, want_k, dwq, dwk);
-      } else {
-        mha_backward(x[0], x[1], x[2], out, dout, lse, g[0], g[1], g[2], scale, false, Tensor(), Tensor());
-      }
+      mha_backward(x[0], x[1], x[2], out, dout, lse, g[0], g[1], g[2], scale, false, Tensor(), Tensor());
     }
     return {dqkv, dwq.defined() ? dwq.to(wq_type) : dwq, dwk.defined() ? dwk.to(wk_type) : dwk};
   }
@@ -326,15 +322,19 @@ Tensor attention_rope(const Tensor& qkv0, int64_t heads, double scale, const May
     qkv = qkv0.contiguous();
     if (reinterpret_cast<uintptr_t>(qkv.data_ptr()) % 16) qkv = qkv.clone();
     std::tie(wq, wk) = head_weights(w0, w1);
-    const int64_t B = qkv.size(0), N = qkv.size(1), C = qkv.size(2) / 3;
-    const auto x = parts(qkv, heads);
+    const int64_t B = qkv.size(0), N = qkv.size(1), C = qkv.size(2) / 3, d = C / heads;
     out = at::empty({B, N, C}, qkv.options());
-    const Tensor out4 = out.view({B, N, heads, C / heads});
-    if (rot.turns()) {
-      yq = fresh(x[0]); yk = fresh(x[1]);
-      rope_forward(x[0], x[1], yq, yk, wq, wk, rot);
+    if (rot.turns()) {                           // (16 bits, of either type)
+      yq = fresh(out);
+      yk = fresh(out);
     }
-    lse = mha_forward(rot.turns() ? yq : x[0], rot.turns() ? yk : x[1], x[2], out4, scale, false, Tensor(), Tensor(), grad);
+    if (grad) lse = at::empty({B, heads, N}, qkv.options().dtype(at::kFloat));
+    const Tensor ws = floats(lib.mha_ws_floats(B, N, N, heads, heads, d), qkv);
+    check(lib.layer_fwd(qkv.data_ptr(), ptr<void>(yq), ptr<void>(yk), out.data_ptr(), ptr<float>(lse), ptr<float>(ws), code_of(qkv), ptr<void>(wq),
+                        ptr<void>(wk), weight_code(wq, wk), ptr<void>(rot.positions), rot.pos_dtype, rot.batch_stride,
+                        static_cast<int32_t>(rot.sections.size()), rot.sections.data(), ptr<float>(rot.inv_freq), B, N, heads, d, rot.eps, rot.norm,
+                        rot.interleaved, static_cast<float>(scale), current()),
+          "cnx_attention_rope_fwd");
   }
   if (grad) {
     auto n = node_of<AttentionRopeBackward>(qkv0, w0, w1);

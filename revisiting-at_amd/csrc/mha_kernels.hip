@@ -50,7 +50,10 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kKT = 64;                          // keys (rows) of a staged tile
 constexpr float kSlack = 8.f;                    // see mha_fwd_kernel
 
+// Operand types.  Io: of the tensors; mfma, pack: products with v or dout (P, dP); mfma_s, pack_s: products with q or k (S, dS).
 struct Bf16 {
+  using Io = Bf16;
+  static constexpr bool kScaled = false;
   static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
@@ -58,10 +61,14 @@ struct Bf16 {
     const f32x2 v = {lo, hi};
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
   }
+  static __device__ __forceinline__ f32x16 mfma_s(u32x4 a, u32x4 b, f32x16 c) { return mfma(a, b, c); }
+  static __device__ __forceinline__ uint32_t pack_s(float lo, float hi) { return pack(lo, hi); }
   static __device__ __forceinline__ float lo(uint32_t w) { return __uint_as_float(w << 16); }
   static __device__ __forceinline__ float hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 };
 struct Fp16 {
+  using Io = Fp16;
+  static constexpr bool kScaled = false;
   static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
@@ -69,8 +76,17 @@ struct Fp16 {
     const f32x2 v = {lo, hi};
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
   }
+  static __device__ __forceinline__ f32x16 mfma_s(u32x4 a, u32x4 b, f32x16 c) { return mfma(a, b, c); }
+  static __device__ __forceinline__ uint32_t pack_s(float lo, float hi) { return pack(lo, hi); }
   static __device__ __forceinline__ float lo(uint32_t w) { return static_cast<float>(__builtin_bit_cast(f16x2, w)[0]); }
   static __device__ __forceinline__ float hi(uint32_t w) { return static_cast<float>(__builtin_bit_cast(f16x2, w)[1]); }
+};
+
+// attention_rope on bf16 tensors: q' and k', normalised and so of known size, are in fp16, and with them dS
+struct Mixed : Bf16 {
+  static constexpr bool kScaled = true;
+  static __device__ __forceinline__ f32x16 mfma_s(u32x4 a, u32x4 b, f32x16 c) { return Fp16::mfma(a, b, c); }
+  static __device__ __forceinline__ uint32_t pack_s(float lo, float hi) { return Fp16::pack(lo, hi); }
 };
 
 struct View {                                    // 16-bit [B, N, heads, d], unit stride in d
@@ -103,6 +119,8 @@ struct MhaArgs {
   int64_t cs_b;                                  // pairs between the samples' (0: shared)
   float eps;
   int32_t norm, il;
+  const float2* range;                           // kScaled: [B][H][pieces] largest |v| and |dout| of a row
+  int32_t pieces;
 };
 
 // what a sample allows
@@ -244,6 +262,31 @@ __device__ __forceinline__ f32x16 first_terms(u32x2 terms, u32x2 ones) {
   return __builtin_amdgcn_mfma_f32_32x32x8bf16_1k(__builtin_bit_cast(s16x4, terms), __builtin_bit_cast(s16x4, ones), zeros16(), 0, 0, 0);
 }
 
+// dS in fp16 (kScaled): |dS| <= 2 |dout| |v|, and a power of two, carried by dout or v (in bf16, exactly) and D, brings that bound to 2^13 .. 2^14:
+// no dS overflows, and one 2^-27 of it still has all its bits.  (The exponents end at 2^+-100, so the powers and their inverses are normal.)
+__device__ __forceinline__ int scale_exponent(float bound) {
+  const int e = static_cast<int>((__float_as_uint(bound) >> 23) & 255u) - 127;
+  return min(max(13 - e, -100), 100);
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
+// largest |v| and |dout| of a head
+__device__ __forceinline__ float2 range_of(const float2* range, int64_t bh, int pieces) {
+  float2 r = range[bh * pieces];
+  for (int p = 1; p < pieces; ++p) {
+    const float2 x = range[bh * pieces + p];
+    r.x = fmaxf(r.x, x.x);
+    r.y = fmaxf(r.y, x.y);
+  }
+  return r;
+}
+template <int N>
+__device__ __forceinline__ void scale_bf16(u32x4 (&f)[N], float s) {
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[i][j] = Bf16::pack(Bf16::lo(f[i][j]) * s, Bf16::hi(f[i][j]) * s);
+}
+
 template <typename T> __device__ __forceinline__ uint2 pack4(float a, float b, float c, float d) { return make_uint2(T::pack(a, b), T::pack(c, d)); }
 
 // A workgroup of the forward or of dq: 128 rows of one key head against the keys [k_begin, k_end), tile by tile.
@@ -344,7 +387,7 @@ __global__ __launch_bounds__(256, 2) void mha_fwd_kernel(const MhaArgs a) {
     for (int blk = 0; blk < NB; ++blk) {
       s[blk] = zeros16();
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) s[blk] = T::mfma(L.row(kimg, blk, ks), qf[ks], s[blk]);
+      for (int ks = 0; ks < KS; ++ks) s[blk] = T::mfma_s(L.row(kimg, blk, ks), qf[ks], s[blk]);
     }
     if (__any(w.end < k0 + kKT)) {
 #pragma unroll
@@ -575,6 +618,36 @@ __device__ __forceinline__ void turn_back(const MhaArgs& a, const Turn& t, f32x1
     for (int r = 0; r < 16; ++r) g[db][r] = rn * fmaf(-x[db][r], dot, g[db][r]);
 }
 
+// Largest |v| and |dout| of the rows of a head, `pieces` workgroups each.  16 bytes per lane, D / 8 lanes a row.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void mha_range_kernel(const MhaArgs a, float2* __restrict__ range) {
+  constexpr int LANES = D / 8, ROWS = 256 / LANES;
+  const int64_t bh = blockIdx.x / a.pieces, b = bh / a.H, h = bh - b * a.H;
+  const int piece = static_cast<int>(blockIdx.x - bh * a.pieces), c = threadIdx.x % LANES;
+  float top[2] = {0.f, 0.f};
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    const View& view = which ? a.vdo : a.vv;
+    const uint16_t* p = (which ? a.dout : a.v) + b * view.b + h * view.h + c * 8;
+    for (int i = piece * ROWS + threadIdx.x / LANES; i < a.Nk; i += a.pieces * ROWS) {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(p + i * view.n);
+      float s = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s = fmaf(T::lo(x[j]), T::lo(x[j]), fmaf(T::hi(x[j]), T::hi(x[j]), s));
+      for (int m = 1; m < LANES; m <<= 1) s += __shfl_xor(s, m, 64);   // (a row's lanes are here together)
+      top[which] = s > top[which] || s != s ? s : top[which];
+    }
+    for (int m = LANES; m < 64; m <<= 1) top[which] = fmaxf(top[which], __shfl_xor(top[which], m, 64));
+  }
+  __shared__ float2 red[4];
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = make_float2(top[0], top[1]);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int k = 1; k < 4; ++k) { top[0] = fmaxf(top[0], red[k].x); top[1] = fmaxf(top[1], red[k].y); }
+    range[blockIdx.x] = make_float2(sqrtf(top[0]), sqrtf(top[1]));
+  }
+}
+
 // dq: workgroup = 4 wavefronts x 32 rows, over the keys [split * span, + span).  Also leaves D in dvec.
 template <typename T, int D, bool TURN>
 __global__ __launch_bounds__(256, 2) void mha_dq_kernel(const MhaArgs a) {
@@ -584,14 +657,14 @@ __global__ __launch_bounds__(256, 2) void mha_dq_kernel(const MhaArgs a) {
   const int half = (threadIdx.x >> 5) & 1, h = w.hk * a.G + w.hd;
   const int64_t at = (w.b * a.H + h) * a.Nq + w.tok;
   u32x4 qf[KS], gf[KS];
-  float lse2, dd;
+  float lse2, dd, mul = a.scale;
   {
     const bool live = w.end > 0;                 // a row without keys has no gradient
     const int64_t i = live ? w.tok : 0;
     const uint16_t* pq = a.q + w.b * a.vq.b + h * a.vq.h + i * a.vq.n + half * 8;
     const uint16_t* pg = a.dout + w.b * a.vdo.b + h * a.vdo.h + i * a.vdo.n + half * 8;
     const uint16_t* po = a.out + w.b * a.vo.b + h * a.vo.h + i * a.vo.n + half * 8;
-    float part = 0.f;
+    float part = 0.f, size = 0.f;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       qf[ks] = gf[ks] = u32x4{0, 0, 0, 0};
@@ -601,11 +674,21 @@ __global__ __launch_bounds__(256, 2) void mha_dq_kernel(const MhaArgs a) {
         const u32x4 of = *reinterpret_cast<const u32x4*>(po + ks * 16);
 #pragma unroll
         for (int j = 0; j < 4; ++j) part = fmaf(T::lo(gf[ks][j]), T::lo(of[j]), fmaf(T::hi(gf[ks][j]), T::hi(of[j]), part));
+        if constexpr (T::kScaled) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) size = fmaf(T::lo(gf[ks][j]), T::lo(gf[ks][j]), fmaf(T::hi(gf[ks][j]), T::hi(gf[ks][j]), size));
+        }
       }
     }
     dd = both_halves_sum(part);
     lse2 = live ? a.lse[at] * kLog2e : INFINITY;                       // exp2(s - inf) = 0
     if (w.split == 0 && half == 0 && w.tok < a.Nq) a.dvec[at] = dd;
+    if constexpr (T::kScaled) {                  // a row's own scale
+      const int e = scale_exponent(2.f * sqrtf(both_halves_sum(size)) * range_of(a.range, w.b * a.H + h, a.pieces).x);
+      scale_bf16(gf, power_of_two(e));
+      dd *= power_of_two(e);
+      mul *= power_of_two(-e);
+    }
   }
   const float c2 = a.scale * kLog2e;
   f32x16 dq[DB];
@@ -620,7 +703,7 @@ __global__ __launch_bounds__(256, 2) void mha_dq_kernel(const MhaArgs a) {
       f32x16 s = zeros16(), dp = zeros16();
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        s = T::mfma(L.row(kimg, blk, ks), qf[ks], s);
+        s = T::mfma_s(L.row(kimg, blk, ks), qf[ks], s);
         dp = T::mfma(L.row(vimg, blk, ks), gf[ks], dp);
       }
 #pragma unroll
@@ -636,14 +719,13 @@ __global__ __launch_bounds__(256, 2) void mha_dq_kernel(const MhaArgs a) {
       for (int t = 0; t < 2; ++t) {
         u32x4 p;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) p[j] = T::pack(s[t * 8 + 2 * j], s[t * 8 + 2 * j + 1]);
+        for (int j = 0; j < 4; ++j) p[j] = T::pack_s(s[t * 8 + 2 * j], s[t * 8 + 2 * j + 1]);
 #pragma unroll
-        for (int db = 0; db < DB; ++db) dq[db] = T::mfma(L.col(kimg, blk, t, db), p, dq[db]);
+        for (int db = 0; db < DB; ++db) dq[db] = T::mfma_s(L.col(kimg, blk, t, db), p, dq[db]);
       }
     }
   };
   w.walk(a, compute);
-  float mul = a.scale;
   if constexpr (TURN) {
 #pragma unroll
     for (int db = 0; db < DB; ++db)
@@ -770,11 +852,19 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void mha_dkv_kernel(const Mha
   }
 #pragma unroll
   for (int db = 0; db < DB; ++db) { dk[db] = zeros16(); dv[db] = zeros16(); }
+  float dk_mul = a.scale, d_mul = -1.f;
+  if constexpr (T::kScaled) {                    // one scale for the head: a key's dk sums over rows
+    const float2 r = range_of(a.range, b * a.H + hk, a.pieces);
+    const int e = scale_exponent(2.f * r.x * r.y);
+    scale_bf16(vf, power_of_two(e));
+    d_mul = -power_of_two(e);
+    dk_mul *= power_of_two(-e);
+  }
   const float c2 = a.scale * kLog2e;
   const Lane<D> L(base);
   const u32x2 ones = {0x3f803f80u, 0x00003f80u};                       // bf16 (1, 1, 1, 0)
   const u32x2 ones_s = half ? u32x2{0, 0} : ones, ones_d = half ? ones : u32x2{0, 0};
-  const float st_mul = half ? -1.f : -1.f / a.scale;
+  const float st_mul = half ? d_mul : -1.f / a.scale;
   const int last_tok[2] = {31 / gt, 63 / gt};                          // token in the tile of a block's last row
   const int wave_key = key0 + wave * 32, wave_last = min(wave_key + 32, lim.kv_len) - 1;       // the wavefront's keys
   auto step = [&](int buf) {
@@ -810,7 +900,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void mha_dkv_kernel(const Mha
       f32x16 s = first_terms(init[blk], ones_s), dp = first_terms(init[blk], ones_d);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        s = T::mfma(qr[ks], kf[ks], s);
+        s = T::mfma_s(qr[ks], kf[ks], s);
         dp = T::mfma(gr[ks], vf[ks], dp);
       }
       u32x4 gc[2][DB], qc[2][DB];
@@ -844,12 +934,12 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void mha_dkv_kernel(const Mha
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           pf[j] = T::pack(s[t * 8 + 2 * j], s[t * 8 + 2 * j + 1]);
-          df[j] = T::pack(dp[t * 8 + 2 * j], dp[t * 8 + 2 * j + 1]);
+          df[j] = T::pack_s(dp[t * 8 + 2 * j], dp[t * 8 + 2 * j + 1]);
         }
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
           dv[db] = T::mfma(gc[t][db], pf, dv[db]);
-          dk[db] = T::mfma(qc[t][db], df, dk[db]);
+          dk[db] = T::mfma_s(qc[t][db], df, dk[db]);
         }
       }
     }
@@ -871,7 +961,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void mha_dkv_kernel(const Mha
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) dk[db][r] *= a.scale;
+      for (int r = 0; r < 16; ++r) dk[db][r] *= dk_mul;
     turn_back<T, D>(a, a.tk, dk, b, key, hk, live);
     if (!live) return;
     uint16_t* pk = a.dk + b * a.vdk.b + key * a.vdk.n + hk * a.vdk.h;
@@ -940,6 +1030,8 @@ __global__ __launch_bounds__(256) void mha_dkv_join_kernel(const MhaArgs a) {
 }
 
 // ===================================================================================================================== host
+constexpr int kPieces = 8;                       // workgroups that look for a head's largest rows, at most
+
 // Splits of the keys for `groups` workgroups over Nk keys: enough to give the chip two workgroups per CU, at least 256 keys each.
 int splits_for(int64_t groups, int32_t Nk) {
   if (groups <= 0 || groups >= 256) return 1;
@@ -984,44 +1076,43 @@ int check_args(const MhaArgs& a, int dtype, int32_t head_dim) {
   if (a.B > 0 && tiles > 0 && a.B > (1LL << 23) / tiles / a.H) return APGD_ERR_SIZE;
   return APGD_OK;
 }
-void cut(MhaArgs& a, int64_t tiles) {
+void cut(MhaArgs& a, int64_t tiles, bool split) {
   a.tiles = static_cast<int32_t>(tiles);
-  a.splits = splits_for(a.B * a.Hkv * tiles, a.Nk);
+  a.splits = split ? splits_for(a.B * a.Hkv * tiles, a.Nk) : 1;
   const int64_t per = ((a.Nk + a.splits - 1) / a.splits + kKT - 1) / kKT * kKT;
   a.span = static_cast<int32_t>(per < kKT ? kKT : per);
 }
 
 template <typename T, int D>
 int launch_fwd(MhaArgs& a, hipStream_t s) {
-  cut(a, row_tiles(a.Nq, a.G));
+  cut(a, row_tiles(a.Nq, a.G), true);
   hipLaunchKernelGGL((mha_fwd_kernel<T, D>), dim3(static_cast<unsigned>(a.B * a.Hkv * a.tiles * a.splits)), dim3(256), 0, s, a);
   if (a.splits > 1)
-    hipLaunchKernelGGL((mha_join_kernel<T, D>), dim3(static_cast<unsigned>((a.B * a.H * a.Nq * (D / 4) + 255) / 256)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((mha_join_kernel<typename T::Io, D>), dim3(static_cast<unsigned>((a.B * a.H * a.Nq * (D / 4) + 255) / 256)), dim3(256), 0, s, a);
   return launch_status();
 }
 template <typename T, int D, bool TURN>
 int launch_bwd(MhaArgs& a, hipStream_t s) {
   if (a.Nq > 0) {
-    cut(a, row_tiles(a.Nq, a.G));
+    cut(a, row_tiles(a.Nq, a.G), !TURN);
     hipLaunchKernelGGL((mha_dq_kernel<T, D, TURN>), dim3(static_cast<unsigned>(a.B * a.Hkv * a.tiles * a.splits)), dim3(256), 0, s, a);
-    if (a.splits > 1)
-      hipLaunchKernelGGL((mha_dq_join_kernel<T, D>), dim3(static_cast<unsigned>((a.B * a.H * a.Nq * (D / 4) + 255) / 256)), dim3(256), 0, s, a);
+    if (!TURN && a.splits > 1)
+      hipLaunchKernelGGL((mha_dq_join_kernel<typename T::Io, D>), dim3(static_cast<unsigned>((a.B * a.H * a.Nq * (D / 4) + 255) / 256)), dim3(256), 0, s, a);
   }
   if (a.Nk > 0) {
     a.tiles = (a.Nk + 127) / 128;
-    a.splits = dkv_splits(a.B, a.Nq, a.Nk, a.Hkv, a.G, D, a.causal != 0);
+    a.splits = TURN ? 1 : dkv_splits(a.B, a.Nq, a.Nk, a.Hkv, a.G, D, a.causal != 0);
     hipLaunchKernelGGL((mha_dkv_kernel<T, D, TURN>), dim3(static_cast<unsigned>(a.B * a.Hkv * a.tiles * a.splits)), dim3(256), 0, s, a);
-    if (a.splits > 1)
-      hipLaunchKernelGGL((mha_dkv_join_kernel<T, D>), dim3(static_cast<unsigned>((a.B * a.Hkv * a.Nk * (D / 4) + 255) / 256), 2), dim3(256), 0, s, a);
+    if (!TURN && a.splits > 1)
+      hipLaunchKernelGGL((mha_dkv_join_kernel<typename T::Io, D>), dim3(static_cast<unsigned>((a.B * a.Hkv * a.Nk * (D / 4) + 255) / 256), 2), dim3(256), 0, s, a);
   }
   return launch_status();
 }
 
-template <bool TURN>
-int launch_bwd(MhaArgs& a, int dtype, int32_t head_dim, hipStream_t s) {
-  if (dtype == APGD_BF16) return head_dim == 64 ? launch_bwd<Bf16, 64, TURN>(a, s) : launch_bwd<Bf16, 128, TURN>(a, s);
-  return head_dim == 64 ? launch_bwd<Fp16, 64, TURN>(a, s) : launch_bwd<Fp16, 128, TURN>(a, s);
-}
+template <typename T>
+int launch_fwd(MhaArgs& a, int32_t head_dim, hipStream_t s) { return head_dim == 64 ? launch_fwd<T, 64>(a, s) : launch_fwd<T, 128>(a, s); }
+template <typename T, bool TURN>
+int launch_bwd(MhaArgs& a, int32_t head_dim, hipStream_t s) { return head_dim == 64 ? launch_bwd<T, 64, TURN>(a, s) : launch_bwd<T, 128, TURN>(a, s); }
 
 View view_of(const int64_t* s) { return View{s[0], s[1], s[2]}; }
 // a staged tile's rows lie within 31 bits of bytes of its first: 64 tokens and the heads that share a key head
@@ -1066,8 +1157,7 @@ int cnx_mha_fwd(const void* q, const void* k, const void* v, void* out, float* l
   a.vq = view_of(strides); a.vk = view_of(strides + 3); a.vv = view_of(strides + 6); a.vo = view_of(strides + 9);
   if (!near_enough(a.vk, 1) || !near_enough(a.vv, 1)) return APGD_ERR_ARG;
   hipStream_t s = as_stream(stream);
-  if (dtype == APGD_BF16) return head_dim == 64 ? launch_fwd<Bf16, 64>(a, s) : launch_fwd<Bf16, 128>(a, s);
-  return head_dim == 64 ? launch_fwd<Fp16, 64>(a, s) : launch_fwd<Fp16, 128>(a, s);
+  return dtype == APGD_BF16 ? launch_fwd<Bf16>(a, head_dim, s) : launch_fwd<Fp16>(a, head_dim, s);
 }
 
 int cnx_mha_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse, void* dq, void* dk, void* dv,
@@ -1088,13 +1178,43 @@ int cnx_mha_bwd(const void* q, const void* k, const void* v, const void* out, co
   a.vdq = view_of(strides + 15); a.vdk = view_of(strides + 18); a.vdv = view_of(strides + 21);
   if (!near_enough(a.vq, a.G) || !near_enough(a.vk, 1) || !near_enough(a.vv, 1) || !near_enough(a.vdo, a.G)) return APGD_ERR_ARG;
   hipStream_t s = as_stream(stream);
-  return launch_bwd<false>(a, dtype, head_dim, s);
+  return dtype == APGD_BF16 ? launch_bwd<Bf16, false>(a, head_dim, s) : launch_bwd<Fp16, false>(a, head_dim, s);
+}
+
+int cnx_attention_rope_fwd(const void* qkv, void* yq, void* yk, void* out, float* lse, float* ws, int dtype, const void* wq, const void* wk,
+                           int w_dtype, const void* positions, int pos_dtype, int64_t pos_batch_stride, int32_t axes, const int32_t* sections,
+                           const float* inv_freq, int64_t B, int32_t N, int32_t H, int32_t head_dim, float eps, int32_t norm,
+                           int32_t interleaved, float scale, void* stream) {
+  MhaArgs a = {};
+  const bool turns = norm || positions, half = dtype == APGD_BF16 && norm;
+  const int64_t D = head_dim, C = H * D;
+  const uint16_t* x = static_cast<const uint16_t*>(qkv);
+  a.B = B; a.Nq = a.Nk = N; a.H = a.Hkv = H; a.G = 1; a.scale = scale;
+  if (const int rc = check_args(a, dtype, head_dim)) return rc;
+  if (B == 0 || N == 0) return APGD_OK;
+  if (!qkv || !out || (turns && (!yq || !yk))) return APGD_ERR_NULL;
+  if (cnx_mha_ws_floats(B, N, N, H, H, head_dim) > 0 && !ws) return APGD_ERR_NULL;
+  const View packed = {N * 3 * C, 3 * C, D}, dense = {N * C, C, D};
+  if (!near_enough(packed, 1)) return APGD_ERR_ARG;
+  hipStream_t s = as_stream(stream);
+  if (turns) {
+    const int64_t strides[12] = {packed.b, packed.n, D, packed.b, packed.n, D, dense.b, dense.n, D, dense.b, dense.n, D};
+    if (const int rc = rope_forward(x, x + C, yq, yk, dtype, half, strides, wq, wk, w_dtype, positions, pos_dtype, pos_batch_stride, axes, sections,
+                                    inv_freq, B, N, H, H, head_dim, eps, norm, interleaved, s))
+      return rc;
+  }
+  a.q = turns ? static_cast<const uint16_t*>(yq) : x; a.k = turns ? static_cast<const uint16_t*>(yk) : x + C; a.v = x + 2 * C;
+  a.vq = a.vk = turns ? dense : packed;
+  a.vv = packed; a.vo = dense;
+  a.o = static_cast<uint16_t*>(out); a.lse = lse; a.part = ws;
+  if (half) return launch_fwd<Mixed>(a, head_dim, s);
+  return dtype == APGD_BF16 ? launch_fwd<Bf16>(a, head_dim, s) : launch_fwd<Fp16>(a, head_dim, s);
 }
 
 int64_t cnx_attention_rope_bwd_ws_floats(int64_t B, int32_t N, int32_t H, int32_t head_dim, int32_t own_positions) {
-  if (B <= 0 || N <= 0 || H < 1 || !cnx_mha_supported(head_dim) || cnx_mha_bwd_ws_floats(B, N, N, H, H, head_dim, 0) > 0) return 0;
-  const int64_t tiles = (N + 127) / 128;         // D; cosines and sines; weight gradients of the workgroups
-  return (B * H * N + 3) / 4 * 4 + (own_positions ? B : 1) * N * head_dim + 2 * B * H * tiles * head_dim;
+  if (B <= 0 || N <= 0 || H < 1 || !cnx_mha_supported(head_dim)) return 0;
+  const int64_t tiles = (N + 127) / 128;         // D; cosines and sines; weight gradients of the workgroups; sizes of v and dout
+  return (B * H * N + 3) / 4 * 4 + (own_positions ? B : 1) * N * head_dim + 2 * B * H * tiles * head_dim + 2 * B * H * kPieces;
 }
 
 int cnx_attention_rope_bwd(const void* qkv, const void* yq, const void* yk, const void* out, const void* dout, const float* lse, void* dqkv,
@@ -1104,38 +1224,48 @@ int cnx_attention_rope_bwd(const void* qkv, const void* yq, const void* yk, cons
                            int32_t interleaved, float scale, void* stream) {
   MhaArgs a = {};
   const int64_t D = head_dim, C = H * D;
-  a.q = static_cast<const uint16_t*>(yq); a.k = static_cast<const uint16_t*>(yk);
-  a.out = static_cast<const uint16_t*>(out); a.dout = static_cast<const uint16_t*>(dout); a.lse = const_cast<float*>(lse);
+  const bool want_w = dwq || dwk, turns = norm || positions, half = dtype == APGD_BF16 && norm;
+  const uint16_t* x = static_cast<const uint16_t*>(qkv);
   a.B = B; a.Nq = a.Nk = N; a.H = a.Hkv = H; a.G = 1; a.scale = scale;
   a.eps = eps; a.norm = norm != 0; a.il = interleaved != 0;
   if (const int rc = check_args(a, dtype, head_dim)) return rc;
-  if ((dwq || dwk) && !norm) return APGD_ERR_ARG;
-  if (B == 0 || N == 0) return APGD_ERR_SIZE;
-  const int64_t need = cnx_attention_rope_bwd_ws_floats(B, N, H, head_dim, pos_batch_stride != 0);
-  if (need == 0) return APGD_ERR_SIZE;           // few rows: the two operators' own backward passes
+  if (!turns || (want_w && !norm)) return APGD_ERR_ARG;
+  hipStream_t s = as_stream(stream);
+  if (B == 0 || N == 0) return want_w ? rope_dw(nullptr, 0, head_dim, dwq, dwk, s) : APGD_OK;          // no row: zeros
   if (!qkv || !yq || !yk || !out || !dout || !lse || !dqkv || !ws || !dout_strides) return APGD_ERR_NULL;
   const View packed = {N * 3 * C, 3 * C, D}, dense = {N * C, C, D};
-  a.v = static_cast<const uint16_t*>(qkv) + 2 * C;
+  a.q = static_cast<const uint16_t*>(yq); a.k = static_cast<const uint16_t*>(yk); a.v = x + 2 * C;
+  a.out = static_cast<const uint16_t*>(out); a.dout = static_cast<const uint16_t*>(dout); a.lse = const_cast<float*>(lse);
   a.dq = static_cast<uint16_t*>(dqkv); a.dk = a.dq + C; a.dv = a.dk + C;
   a.vq = a.vk = a.vo = dense;
   a.vv = a.vdq = a.vdk = a.vdv = packed;
   a.vdo = view_of(dout_strides);
-  if (!near_enough(a.vk, 1) || !near_enough(a.vv, 1) || !near_enough(a.vdo, 1)) return APGD_ERR_ARG;
-  hipStream_t s = as_stream(stream);
+  if (!near_enough(packed, 1) || !near_enough(a.vdo, 1)) return APGD_ERR_ARG;
+  const int64_t groups = B * H * ((N + 127) / 128);
   a.dvec = ws;
   float* table = ws + (B * H * N + 3) / 4 * 4;
   float* part = table + (pos_batch_stride ? B : 1) * N * D;
-  const int64_t groups = B * H * ((N + 127) / 128);
-  a.tq = Turn{static_cast<const uint16_t*>(qkv), packed, wq, dwq || dwk ? part : nullptr};
-  a.tk = Turn{static_cast<const uint16_t*>(qkv) + C, packed, wk, dwq || dwk ? part + groups * D : nullptr};
+  float2* range = reinterpret_cast<float2*>(part + 2 * groups * D);
+  a.tq = Turn{x, packed, wq, want_w ? part : nullptr};
+  a.tk = Turn{x + C, packed, wk, want_w ? part + groups * D : nullptr};
   if (positions) {
     a.cs = reinterpret_cast<const float2*>(table);
     a.cs_b = pos_batch_stride ? N * D / 2 : 0;
     if (const int rc = rope_table(positions, pos_dtype, pos_batch_stride, axes, sections, inv_freq, B, N, head_dim, reinterpret_cast<float2*>(table), s))
       return rc;
   }
-  if (const int rc = launch_bwd<true>(a, dtype, head_dim, s)) return rc;
-  return dwq || dwk ? rope_dw(part, static_cast<int>(groups), head_dim, dwq, dwk, s) : APGD_OK;
+  int rc;
+  if (half) {
+    a.range = range;
+    a.pieces = static_cast<int32_t>(B * H >= 512 ? 1 : std::min<int64_t>(kPieces, (N + 127) / 128));
+    const dim3 grid(static_cast<unsigned>(B * H * a.pieces));
+    if (head_dim == 64) hipLaunchKernelGGL((mha_range_kernel<Bf16, 64>), grid, dim3(256), 0, s, a, range);
+    else hipLaunchKernelGGL((mha_range_kernel<Bf16, 128>), grid, dim3(256), 0, s, a, range);
+    rc = launch_bwd<Mixed, true>(a, head_dim, s);
+  } else {
+    rc = dtype == APGD_BF16 ? launch_bwd<Bf16, true>(a, head_dim, s) : launch_bwd<Fp16, true>(a, head_dim, s);
+  }
+  return rc || !want_w ? rc : rope_dw(part, static_cast<int>(groups), head_dim, dwq, dwk, s);
 }
 
 }  // extern "C"

@@ -17,6 +17,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "apgd_hip.h"
 #include "convnext_hip.h"
 #include "rope_internal.h"
@@ -185,7 +187,8 @@ __global__ __launch_bounds__(256) void rope_table_kernel(const RopeArgs a, float
 }
 
 // blockIdx.y: 0 = queries, 1 = keys (so that a thread holds one side's sums)
-template <typename T, bool BWD, bool IL>
+// TO: type of the results (T, or fp16 for the attention's own copy of normalised bf16 heads)
+template <typename T, typename TO, bool BWD, bool IL>
 __global__ __launch_bounds__(256, BWD ? 3 : 4) void qk_norm_rope_kernel(const RopeArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char lds_raw[];
   float* wl = reinterpret_cast<float*>(lds_raw);                      // [2][d / 2] weights of the pairs' first and second members
@@ -214,7 +217,7 @@ __global__ __launch_bounds__(256, BWD ? 3 : 4) void qk_norm_rope_kernel(const Ro
     const int nt = static_cast<int>(a.N - n0 < a.tile ? a.N - n0 : a.tile), ns = static_cast<int>(a.B - b0 < a.samples ? a.B - b0 : a.samples);
     const T* px = static_cast<const T*>(z.x) + b0 * z.vx.b + n0 * z.vx.n;
     const T* pg = static_cast<const T*>(z.dy) + b0 * z.vdy.b + n0 * z.vdy.n;
-    T* po = static_cast<T*>(z.o) + b0 * z.vo.b + n0 * z.vo.n;
+    TO* po = static_cast<TO*>(z.o) + b0 * z.vo.b + n0 * z.vo.n;
     // item = (sample, token, head): places past the tile's last token are passed over
     const int items = (ns << a.log_tile) * z.heads;
     struct Item { int s, t, h; bool live; };
@@ -297,6 +300,13 @@ __global__ __launch_bounds__(256, BWD ? 3 : 4) void qk_norm_rope_kernel(const Ro
         for (int i = 0; i < 8; ++i) {
           ga[i] = fmaf(xa[i], c[i], -xb[i] * s[i]);
           gb[i] = fmaf(xb[i], c[i], xa[i] * s[i]);
+        }
+      }
+      if constexpr (!std::is_same_v<T, TO>) {                         // (a NaN stays one)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          ga[i] = ga[i] > 65504.f ? 65504.f : ga[i] < -65504.f ? -65504.f : ga[i];
+          gb[i] = gb[i] > 65504.f ? 65504.f : gb[i] < -65504.f ? -65504.f : gb[i];
         }
       }
       if (live) store_pairs<IL>(po + now.s * z.vo.b + now.t * z.vo.n + now.h * z.vo.h, j, d, ga, gb);
@@ -393,17 +403,23 @@ void cut(RopeArgs& a) {
 }
 
 template <bool BWD, bool IL>
-void launch(const RopeArgs& a, int dtype, unsigned grid, hipStream_t s) {
+void launch(const RopeArgs& a, int dtype, bool half, unsigned grid, hipStream_t s) {
   const size_t lds = static_cast<size_t>(BWD && a.tile < 3 ? 4 : a.tile + 1) * a.d * 4;     // d weights and tile x d / 2 (cos, sin); BWD: 4 x d sums
   const dim3 blocks(grid, 2);
-  if (dtype == APGD_F32) hipLaunchKernelGGL((qk_norm_rope_kernel<float, BWD, IL>), blocks, dim3(256), lds, s, a);
-  else if (dtype == APGD_BF16) hipLaunchKernelGGL((qk_norm_rope_kernel<bf16_t, BWD, IL>), blocks, dim3(256), lds, s, a);
-  else hipLaunchKernelGGL((qk_norm_rope_kernel<__half, BWD, IL>), blocks, dim3(256), lds, s, a);
+  if constexpr (!BWD) {
+    if (half) {
+      hipLaunchKernelGGL((qk_norm_rope_kernel<bf16_t, __half, false, IL>), blocks, dim3(256), lds, s, a);
+      return;
+    }
+  }
+  if (dtype == APGD_F32) hipLaunchKernelGGL((qk_norm_rope_kernel<float, float, BWD, IL>), blocks, dim3(256), lds, s, a);
+  else if (dtype == APGD_BF16) hipLaunchKernelGGL((qk_norm_rope_kernel<bf16_t, bf16_t, BWD, IL>), blocks, dim3(256), lds, s, a);
+  else hipLaunchKernelGGL((qk_norm_rope_kernel<__half, __half, BWD, IL>), blocks, dim3(256), lds, s, a);
 }
 template <bool BWD>
-void launch(const RopeArgs& a, int dtype, bool interleaved, unsigned grid, hipStream_t s) {
-  if (interleaved) launch<BWD, true>(a, dtype, grid, s);
-  else launch<BWD, false>(a, dtype, grid, s);
+void launch(const RopeArgs& a, int dtype, bool half, bool interleaved, unsigned grid, hipStream_t s) {
+  if (interleaved) launch<BWD, true>(a, dtype, half, grid, s);
+  else launch<BWD, false>(a, dtype, half, grid, s);
 }
 
 View view_of(const int64_t* s) { return View{s[0], s[1], s[2]}; }
@@ -417,6 +433,23 @@ int rope_table(const void* positions, int pos_dtype, int64_t pos_b, int32_t axes
   if (const int rc = check_args(a, APGD_F32, sections, B, N, 0, 0, d)) return rc;
   const int64_t rows = pos_b ? B * N : N, blocks = (rows * (d / 2) + 255) / 256;
   hipLaunchKernelGGL(rope_table_kernel, dim3(static_cast<unsigned>(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s, a, cs, rows);
+  return launch_status();
+}
+int rope_forward(const void* q, const void* k, void* yq, void* yk, int dtype, bool half, const int64_t* strides, const void* wq, const void* wk,
+                 int w_dtype, const void* positions, int pos_dtype, int64_t pos_batch_stride, int32_t axes, const int32_t* sections,
+                 const float* inv_freq, int64_t B, int64_t N, int32_t Hq, int32_t Hk, int32_t d, float eps, int32_t norm, int32_t interleaved,
+                 hipStream_t s) {
+  RopeArgs a = {};
+  a.q.x = q; a.k.x = k; a.q.o = yq; a.k.o = yk;
+  a.q.w = wq; a.k.w = wk; a.w_dtype = w_dtype;
+  a.pos = positions; a.pos_dtype = pos_dtype; a.pos_b = pos_batch_stride; a.axes = axes; a.inv_freq = inv_freq;
+  a.norm = norm != 0; a.eps = eps;
+  if (const int rc = check_args(a, dtype, sections, B, N, Hq, Hk, d)) return rc;
+  if (B == 0 || N == 0 || Hq + Hk == 0) return APGD_OK;
+  if (!strides || (Hq && (!q || !yq)) || (Hk && (!k || !yk))) return APGD_ERR_NULL;
+  a.q.vx = view_of(strides); a.k.vx = view_of(strides + 3); a.q.vo = view_of(strides + 6); a.k.vo = view_of(strides + 9);
+  cut(a);
+  launch<false>(a, dtype, half, interleaved != 0, static_cast<unsigned>(a.tiles < kFwdGrid ? a.tiles : kFwdGrid), s);
   return launch_status();
 }
 int rope_dw(const float* part, int rows, int32_t d, float* dwq, float* dwk, hipStream_t s) {
@@ -434,18 +467,8 @@ int cnx_qk_norm_rope_fwd(const void* q, const void* k, void* yq, void* yk, int d
                          int w_dtype, const void* positions, int pos_dtype, int64_t pos_batch_stride, int32_t axes, const int32_t* sections,
                          const float* inv_freq, int64_t B, int64_t N, int32_t Hq, int32_t Hk, int32_t d, float eps, int32_t norm,
                          int32_t interleaved, void* stream) {
-  RopeArgs a = {};
-  a.q.x = q; a.k.x = k; a.q.o = yq; a.k.o = yk;
-  a.q.w = wq; a.k.w = wk; a.w_dtype = w_dtype;
-  a.pos = positions; a.pos_dtype = pos_dtype; a.pos_b = pos_batch_stride; a.axes = axes; a.inv_freq = inv_freq;
-  a.norm = norm != 0; a.eps = eps;
-  if (const int rc = check_args(a, dtype, sections, B, N, Hq, Hk, d)) return rc;
-  if (B == 0 || N == 0 || Hq + Hk == 0) return APGD_OK;
-  if (!strides || (Hq && (!q || !yq)) || (Hk && (!k || !yk))) return APGD_ERR_NULL;
-  a.q.vx = view_of(strides); a.k.vx = view_of(strides + 3); a.q.vo = view_of(strides + 6); a.k.vo = view_of(strides + 9);
-  cut(a);
-  launch<false>(a, dtype, interleaved != 0, static_cast<unsigned>(a.tiles < kFwdGrid ? a.tiles : kFwdGrid), as_stream(stream));
-  return launch_status();
+  return rope_forward(q, k, yq, yk, dtype, false, strides, wq, wk, w_dtype, positions, pos_dtype, pos_batch_stride, axes, sections, inv_freq, B, N, Hq,
+                      Hk, d, eps, norm, interleaved, as_stream(stream));
 }
 
 int cnx_qk_norm_rope_bwd(const void* dyq, const void* dyk, const void* q, const void* k, void* dq, void* dk, float* dwq, float* dwk, float* ws,
@@ -470,7 +493,7 @@ int cnx_qk_norm_rope_bwd(const void* dyq, const void* dyk, const void* q, const 
     a.part = want_w ? ws : nullptr;
     cut(a);
     grid = static_cast<unsigned>(a.tiles < kBwdGrid ? a.tiles : kBwdGrid);
-    launch<true>(a, dtype, interleaved != 0, grid, as_stream(stream));
+    launch<true>(a, dtype, false, interleaved != 0, grid, as_stream(stream));
   }
   return want_w ? rope_dw(ws, static_cast<int>(grid), d, dwq, dwk, as_stream(stream)) : launch_status();
 }

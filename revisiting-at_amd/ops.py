@@ -2130,7 +2130,8 @@ def attention_rope(qkv, num_heads, scale=None, q_weight=None, k_weight=None, pos
                    norm=True, interleaved=False):
     """``attention`` with normalised heads and rotary positions: ``qk_norm_rope`` of q and k, then ``mha``, from a packed ``[B, N, 3C]``
     bfloat16 or float16 projection -> ``[B, N, C]``, for any N; head_dim 64 or 128.  The arguments behind ``scale`` are those of
-    ``qk_norm_rope``; with ``norm=False`` and no positions it is ``attention`` without a limit on N.  Differentiable in qkv and the weights."""
+    ``qk_norm_rope``; with ``norm=False`` and no positions it is ``attention`` without a limit on N.  Normalised q and k of a bfloat16
+    projection are kept in float16 (three bits more; weights between 2^-14 and 5000 in size).  Differentiable in qkv and the weights (once)."""
     what = "attention_rope"
     if not isinstance(qkv, torch.Tensor) or qkv.dim() != 3:
         raise ValueError(f"{what}: qkv has to be a tensor [batch, tokens, 3 * width]")

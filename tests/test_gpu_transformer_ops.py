@@ -186,10 +186,11 @@ def test_qk_norm_rope_strides_and_shared_inputs(R):
 
 
 # ------------------------------------------------------------------------------------------------------------------ mha
-def mha_ref(q, k, v, scale, causal, q_lens, kv_lens, dout, u, rounded=True):
+def mha_ref(q, k, v, scale, causal, q_lens, kv_lens, dout, u, rounded=True, scaled=False):
     """The definition in 64 bits, a sample and head at a time, and how far the kernel's roundings may lead from it:
     out: P is rounded to 16 bits (u) and the result once more; exp's argument and the sums in 32 bits (t).
-    dv: the same with P^T and dout.   D is formed from the rounded out.   dS is rounded once, the products' results once."""
+    dv: the same with P^T and dout.   D is formed from the rounded out.   dS is rounded once, the products' results once.
+    scaled: dS is rounded to fp16 after a power of two has brought 2 max|dout| max|v| to 2^13 or more: 2^-11 of it, or half of fp16's smallest step."""
     B, Nq, H, d = q.shape
     Nk, Hkv = k.shape[1], k.shape[2]
     q, k, v, dout = (x.detach().double().cpu() for x in (q, k, v, dout))
@@ -223,7 +224,10 @@ def mha_ref(q, k, v, scale, causal, q_lens, kv_lens, dout, u, rounded=True):
             DS = P * (DP - Dv)
             size = G.abs() @ V.abs().T
             eD = (G.abs() * (eo + u * (O.abs() + eo))).sum(1, keepdim=True) + d * E * (G.abs() * O.abs()).sum(1, keepdim=True)
-            eS = (u + 2 * t) * DS.abs() + (1 + u) * P * (d * E * size + eD)
+            us = 2.0 ** -11 if scaled else u
+            eS = (us + 2 * t) * DS.abs() + (1 + us) * P * (d * E * size + eD)
+            if scaled:
+                eS = eS + 2.0 ** -25 * 2.0 ** -13 * 2 * G.norm(dim=1).max() * V.norm(dim=1).max()
             # the 16-bit type's smallest steps (fp16: 2^-25 half a step below 2^-14)
             tiny = 2.0 ** -25 if u == 2.0 ** -11 else 0.0
             eP = torch.where(ok, (u + 2 * t) * P + tiny, 0.0)
@@ -416,20 +420,23 @@ def test_refusals_name_what_is_wrong(R):
 
 
 # ------------------------------------------------------------------------------------------------------------------ attention_rope
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
 @pytest.mark.parametrize("norm,rotate", [(True, True), (True, False), (False, True), (False, False)])
 @pytest.mark.parametrize("B,side,H,d", [(2, 14, 3, 64), (1, 24, 2, 64), (2, 6, 2, 128), (1, 0, 1, 64)])
-def test_attention_rope_is_its_two_operators(R, B, side, H, d, norm, rotate):
-    """Bit for bit ``qk_norm_rope`` then ``mha`` on slices of the projection, forward and dv; all gradients where the rows are split over workgroups or
-    nothing is turned (elsewhere dq' and dk' are not rounded in between)."""
+def test_attention_rope_is_its_two_operators(R, B, side, H, d, norm, rotate, dtype):
+    """Bit for bit ``qk_norm_rope`` then ``mha`` on slices of the projection, where q' and k' are of the projection's type: forward, and dv where no row
+    is split over workgroups; all gradients where nothing is turned.  (Elsewhere dq' and dk' are not rounded in between.)"""
+    if norm and dtype == torch.bfloat16:
+        pytest.skip("q' and k' in fp16: against the definition below")
     N = side * side + 1
     g = torch.Generator().manual_seed(N)
-    qkv = torch.randn(B, N, 3 * H * d, generator=g).to(torch.bfloat16).cuda().requires_grad_()
+    qkv = torch.randn(B, N, 3 * H * d, generator=g).to(dtype).cuda().requires_grad_()
     wq, wk = ((1 + 0.1 * torch.randn(d, generator=g)).cuda().requires_grad_() for _ in range(2)) if norm else (None, None)
     n = torch.arange(side * side)
     pos = torch.cat([torch.zeros(1, 2, dtype=torch.int64), torch.stack([n // max(side, 1), n % max(side, 1)], -1) + 1]).cuda() if rotate else None
     sec = [d // 4, d // 4] if rotate else None
     inv = torch.cat([100.0 ** (-torch.arange(s).float() / s) for s in sec]).cuda() if rotate else None
-    dout = torch.randn(B, N, H * d, generator=g).to(torch.bfloat16).cuda()
+    dout = torch.randn(B, N, H * d, generator=g).to(dtype).cuda()
     out = R.ops.attention_rope(qkv, H, None, wq, wk, pos, inv, sec, norm=norm)
     leaves = (qkv,) + ((wq, wk) if norm else ())
     got = (out,) + torch.autograd.grad(out, leaves, dout)
@@ -439,11 +446,11 @@ def test_attention_rope_is_its_two_operators(R, B, side, H, d, norm, rotate):
         q, k = R.ops.qk_norm_rope(q, k, wq, wk, pos, inv, sec, norm=norm)
     o2 = R.ops.mha(q, k, v).reshape(B, N, H * d)
     want = (o2,) + torch.autograd.grad(o2, (x,) + ((wq, wk) if norm else ()), dout)
-    assert torch.equal(got[0], want[0]) and torch.equal(got[1][..., 2 * H * d:], want[1][..., 2 * H * d:])
-    fused = R._lib.load().cnx_attention_rope_bwd_ws_floats(B, N, H, d, 0) > 0 and (norm or rotate)
-    assert fused == (N != 577 and (norm or rotate))
-    if not fused:
-        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.equal(got[0], want[0])
+    if R._lib.load().cnx_mha_bwd_ws_floats(B, N, N, H, H, d, 0) == 0:
+        assert torch.equal(got[1][..., 2 * H * d:], want[1][..., 2 * H * d:])
+    if not norm and not rotate:
+        assert torch.equal(got[1], want[1])
     with torch.no_grad():
         assert torch.equal(R.ops.attention_rope(qkv, H, None, wq, wk, pos, inv, sec, norm=norm), out)
 
@@ -456,17 +463,18 @@ ATTN = [  # B, N, H, d, norm, rotate, interleaved, per-batch positions, weights'
     (2, 129, 1, 128, True, True, True, False, torch.float32, "whole"),
     (1, 64, 3, 64, True, False, False, False, "x", "expanded"),
     (1, 65, 2, 64, False, True, False, True, None, "whole"),
-    (43, 257, 2, 64, True, True, False, False, torch.float32, "whole"),          # more than 256 keys: enough samples that no row is split
+    (43, 257, 2, 64, True, True, False, False, torch.float32, "whole"),          # more than one tile of rows and keys
+    (3, 577, 2, 64, True, True, False, True, torch.float32, "whole"),
     (29, 260, 3, 128, False, True, True, False, None, "part"),
 ]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
 @pytest.mark.parametrize("case", ATTN, ids=lambda c: "-".join(str(v).split(".")[-1] for v in c))
-def test_attention_rope_gradients_against_their_definition(R, case, dtype):
-    """The backward pass in one: dq' and dk' of q' and k' as they were rounded, through the rotation and the norm, rounded once at the end."""
+def test_attention_rope_against_its_definition(R, case, dtype):
+    """The result of q' and k' as they are rounded - to fp16 where they are normalised, whatever the projection's type - and the backward pass in one:
+    dq' and dk' of the same, through the rotation and the norm, rounded once at the end."""
     B, N, H, d, norm, rotate, il, per_batch, wt, part = case
-    assert R._lib.load().cnx_attention_rope_bwd_ws_floats(B, N, H, d, per_batch) > 0
     g = torch.Generator().manual_seed(N + d)
     u = half_step(dtype)
     qkv = torch.randn(B, N, 3 * H * d, generator=g).to(dtype).cuda().requires_grad_()
@@ -481,11 +489,14 @@ def test_attention_rope_gradients_against_their_definition(R, case, dtype):
     leaves = (qkv,) + (() if wt is None else (wq, wk))
     got = torch.autograd.grad(out, leaves, dout)
     q, k, v = qkv.detach().view(B, N, 3, H, d).unbind(2)
-    with torch.no_grad():
-        yq, yk = R.ops.qk_norm_rope(q, k, wq, wk, pos, inv, sec, norm=norm, interleaved=il)
-    (_, dq, dk, dv), (_, bq, bk, bv) = mha_ref(yq, yk, v, d ** -0.5, False, None, None, dout.reshape(B, N, H, d), u, rounded=False)
+    with torch.no_grad():                                                           # the same arithmetic in 32 bits on the same numbers
+        yq, yk = R.ops.qk_norm_rope(q.float(), k.float(), *(None if w is None else w.float() for w in (wq, wk)), pos, inv, sec, norm=norm, interleaved=il)
+    yq, yk = (y.to(torch.float16 if norm else dtype) for y in (yq, yk))
+    scaled = norm and dtype == torch.bfloat16
+    (o, dq, dk, dv), (bo, bq, bk, bv) = mha_ref(yq, yk, v, d ** -0.5, False, None, None, dout.reshape(B, N, H, d), u, rounded=False, scaled=scaled)
     angle = rope_angles(pos, inv, sec) if rotate else None
     mine = got[0].view(B, N, 3, H, d).unbind(2)
+    inside(out.view(B, N, H, d), o, bo, "out")
     inside(mine[2], dv, bv, "dv")
     tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
     for i, (name, x, w, dy, b) in enumerate((("dq", q, wq, dq, bq), ("dk", k, wk, dk, bk))):
@@ -505,6 +516,8 @@ def test_attention_rope_gradients_against_their_definition(R, case, dtype):
         if w is not None:
             last = u if w.dtype == dtype else 0.0
             inside(got[1 + i], dw, 1.01 * dwb + last * (dw.abs() + 1.01 * dwb) + (2.0 ** -25 if w.dtype == torch.float16 else 0.0), "d" + name[1] + " weight")
+    with torch.no_grad():
+        assert torch.equal(R.ops.attention_rope(qkv, H, None, wq, wk, pos, inv, sec, norm=norm, interleaved=il), out)
     x2 = qkv.detach().requires_grad_()                                              # without weight gradients: the same bits
     (again,) = torch.autograd.grad(R.ops.attention_rope(x2, H, None, None if wq is None else wq.detach(), None if wk is None else wk.detach(), pos, inv, sec,
                                                         norm=norm, interleaved=il), (x2,), dout)
@@ -555,3 +568,32 @@ def test_attention_rope_backward_in_a_graph(R):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
         assert all(torch.equal(a, b) for a, b in zip(both(), want))
+
+
+def test_attention_rope_with_gradients_and_values_of_any_size(R):
+    """dS travels in fp16 behind a power of two: gradients and values far from 1 give the same bits, scaled; rows of very different sizes stay within
+    what the scale allows; an infinite gradient does not come out finite."""
+    B, N, H, d = 2, 150, 2, 64
+    g = torch.Generator().manual_seed(9)
+    qkv = torch.randn(B, N, 3 * H * d, generator=g).to(torch.bfloat16).cuda()
+    dout = torch.randn(B, N, H * d, generator=g).to(torch.bfloat16).cuda()
+
+    def run(qkv, dout):
+        x = qkv.clone().requires_grad_()
+        out = R.ops.attention_rope(x, H)
+        return out.detach(), torch.autograd.grad(out, x, dout)[0]
+    out, grad = run(qkv, dout)
+    for up in (2.0 ** 40, 2.0 ** -40):
+        assert torch.equal(run(qkv, dout * up)[1], grad * up)
+        big = qkv.clone()
+        big[..., 2 * H * d:] *= up
+        o, gr = run(big, dout)
+        assert torch.equal(o, out * up) and torch.equal(gr[..., :2 * H * d], grad[..., :2 * H * d] * up) and torch.equal(gr[..., 2 * H * d:], grad[..., 2 * H * d:])
+    # a row with 2^-20 of the others' gradient: its dq has a scale of its own
+    small = dout.clone()
+    small[:, 7] *= 2.0 ** -20
+    dq = run(qkv, small)[1][:, 7, :H * d]
+    assert torch.equal(dq, grad[:, 7, :H * d] * 2.0 ** -20)
+    bad = dout.clone()
+    bad[0, 3, 5] = float("inf")
+    assert not bool(torch.isfinite(run(qkv, bad)[1][0, 3, :d]).any())

@@ -60,17 +60,26 @@ def attn_bwd(lib, qkv=P, out=P, dqkv=P, ws=P, strides=S24, dtype=1, pos=P, pos_d
 
 @pytest.mark.parametrize("kw,code", [
     (dict(qkv=None), NULL), (dict(out=None), NULL), (dict(dqkv=None), NULL), (dict(ws=None), NULL), (dict(strides=None), NULL), (dict(dtype=0), DTYPE),
-    (dict(d=32), ARG), (dict(H=0), SIZE), (dict(B=0), SIZE), (dict(N=0), SIZE), (dict(N=-1), SIZE), (dict(B=1, N=1000), SIZE), (dict(scale=0.0), ARG),
+    (dict(d=32), ARG), (dict(H=0), SIZE), (dict(B=0), 0), (dict(N=0), 0), (dict(N=-1), SIZE), (dict(scale=0.0), ARG), (dict(norm=0, pos=None), ARG),
     (dict(dw=P, norm=0), ARG), (dict(inv=None), NULL), (dict(sections=None), NULL), (dict(pos_dtype=3), DTYPE), (dict(axes=5), ARG),
     (dict(sections=(16, 17)), ARG), (dict(B=2 ** 40), SIZE)])
 def test_attention_rope_backward_refuses(R, kw, code):
     assert attn_bwd(R._lib.load(), **kw) == code
 
 
-def test_attention_rope_backward_workspace(R):
-    size = R._lib.load().cnx_attention_rope_bwd_ws_floats
-    assert size(2, 17, 2, 64, 0) == 68 + 17 * 64 + 2 * 4 * 64 and size(2, 17, 2, 64, 1) == 68 + 2 * 17 * 64 + 2 * 4 * 64
-    assert size(1, 1000, 2, 64, 0) == 0 and size(1, 17, 2, 96, 0) == 0 and size(0, 17, 2, 64, 0) == 0     # rows split, no such head, empty
+def test_attention_rope_workspaces_and_forward_refusals(R):
+    lib = R._lib.load()
+    size = lib.cnx_attention_rope_bwd_ws_floats
+    assert size(2, 17, 2, 64, 1) - size(2, 17, 2, 64, 0) == 17 * 64 and size(2, 17, 2, 64, 0) >= 68 + 17 * 64 + 2 * 4 * 64
+    assert size(1, 17, 2, 96, 0) == 0 and size(0, 17, 2, 64, 0) == 0
+
+    def fwd(qkv=P, y=P, out=P, ws=P, dtype=1, w=None, w_dtype=0, pos=P, axes=2, sections=(16, 16), B=1, N=4, H=2, d=64, norm=1, scale=0.125):
+        sec = (ctypes.c_int32 * len(sections))(*sections)
+        return lib.cnx_attention_rope_fwd(qkv, y, y, out, None, ws, dtype, w, w, w_dtype, pos, 2, 0, axes, sec, P, B, N, H, d, 1e-6, norm, 0, scale, None)
+    for kw, code in ((dict(qkv=None), NULL), (dict(y=None), NULL), (dict(out=None), NULL), (dict(ws=None, N=1000), NULL), (dict(dtype=0), DTYPE),
+                     (dict(w=P, w_dtype=2), DTYPE), (dict(d=32), ARG), (dict(axes=0), ARG), (dict(sections=(1, 2)), ARG), (dict(H=0), SIZE),
+                     (dict(N=-1), SIZE), (dict(scale=-1.0), ARG), (dict(B=0, qkv=None), 0), (dict(N=0), 0)):
+        assert fwd(**kw) == code, kw
 
 
 def rope(lib, fwd=True, q=P, out=P, strides=S24, dtype=1, w=None, w_dtype=0, pos=P, pos_dtype=2, axes=2, sections=(16, 16), inv=P, B=1, N=4, Hq=2,
