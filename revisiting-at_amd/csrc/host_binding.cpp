@@ -1,8 +1,9 @@
-// heads_binding.cpp — the host side of ops.mha, ops.qk_norm_rope and ops.attention_rope: their autograd nodes and launches, as a Python module.
+// host_binding.cpp — the host side of ops.mha, ops.qk_norm_rope and ops.attention_rope (autograd nodes and launches) and of optim.FusedAdamW
+// (its look at the parameters and gradients), as a Python module.
 //
 // A small attention is a few 10 us kernels; in Python the same node costs the host more than that - twice over in the backward, which the
-// autograd engine runs in a thread of its own.  Arguments have been checked by ops.py.  The kernels are reached through the C ABI of the
-// library that ops.py has loaded (bind()); nothing is kept from one call for the next.
+// autograd engine runs in a thread of its own.  (Forward and backward of 4 x 197 tokens: 133 us in Python, 65 here, 58 of them the engine's.)
+// Arguments have been checked by ops.py.  The kernels are reached through the C ABI of the library that ops.py has loaded (bind()).
 #include <dlfcn.h>
 
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
@@ -349,6 +350,50 @@ Tensor attention_rope(const Tensor& qkv0, int64_t heads, double scale, const May
   return out;
 }
 
+// ------------------------------------------------------------------------------------------------------------------ optimizer
+// Parameters as the optimizer's tables describe them.  (The address alone does not tell: memory that was given back comes again for other
+// sizes and types.)
+class Layout {
+ public:
+  explicit Layout(const std::vector<Tensor>& params) {
+    for (const Tensor& p : params) all_.push_back({p.data_ptr(), p.scalar_type(), p.sizes().vec(), p.strides().vec()});
+  }
+  bool matches(const std::vector<Tensor>& params) const {
+    if (params.size() != all_.size()) return false;
+    for (size_t i = 0; i < all_.size(); ++i) {
+      const Tensor& p = params[i];
+      const One& o = all_[i];
+      if (p.data_ptr() != o.at || p.scalar_type() != o.type || p.sizes() != at::IntArrayRef(o.sizes) || p.strides() != at::IntArrayRef(o.strides)) return false;
+    }
+    return true;
+  }
+  // Addresses of the gradients (0: none) into `to`; those of another type or order of elements are copied, and the copies returned.
+  std::vector<Tensor> gradients(const std::vector<Tensor>& params, uintptr_t to) const {
+    const at::NoGradGuard no_grad;
+    std::vector<Tensor> kept;
+    void** out = reinterpret_cast<void**>(to);
+    for (size_t i = 0; i < all_.size(); ++i) {
+      Tensor g = params[i].grad();
+      if (!g.defined()) { out[i] = nullptr; continue; }
+      TORCH_CHECK(g.layout() == at::kStrided, "FusedAdamW does not take sparse gradients");
+      if (g.scalar_type() != all_[i].type || g.strides() != at::IntArrayRef(all_[i].strides)) {
+        g = at::empty_like(params[i]).copy_(g);
+        kept.push_back(g);
+      }
+      out[i] = g.data_ptr();
+    }
+    return kept;
+  }
+
+ private:
+  struct One {
+    void* at;
+    at::ScalarType type;
+    std::vector<int64_t> sizes, strides;
+  };
+  std::vector<One> all_;
+};
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -356,4 +401,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("mha", &mha);
   m.def("qk_norm_rope", &qk_norm_rope);
   m.def("attention_rope", &attention_rope);
+  py::class_<Layout>(m, "Layout")
+      .def(py::init<const std::vector<Tensor>&>())
+      .def("matches", &Layout::matches)
+      .def("gradients", &Layout::gradients);
 }

@@ -1978,22 +1978,22 @@ def attention(qkv, num_heads, scale):
 
 
 # ------------------------------------------------------------------------------ heads: norm and rotation, attention of any length
-# Autograd nodes and launches of the three operators are C++ (csrc/heads_binding.cpp); what a call may be is checked here.
-_HEADS = None
+# Autograd nodes and launches of the three operators are C++ (csrc/host_binding.cpp); what a call may be is checked here.
+_HOST = None
 
 
-def _heads():
+def _host():
     """The extension, bound to the library that ``_lib`` has loaded and to the flag of ``input_grad_only``."""
-    global _HEADS
-    if _HEADS is None:
+    global _HOST
+    if _HOST is None:
         try:
-            from . import _heads as module
+            from . import _host as module
         except ImportError as e:
-            raise _lib.ApgdHipError(f"revisiting-at_amd/_heads.so cannot be loaded ({e}): build it with `python -c 'import __graft_entry__ as g; "
+            raise _lib.ApgdHipError(f"revisiting-at_amd/_host.so cannot be loaded ({e}): build it with `python -c 'import __graft_entry__ as g; "
                                     "g.build()'` or `make -C revisiting-at_amd/csrc`") from e
         module.bind(_lib.load()._handle, ctypes.addressof(_INPUT_GRAD_ONLY_NATIVE))
-        _HEADS = module
-    return _HEADS
+        _HOST = module
+    return _HOST
 
 
 def _on_device(t):
@@ -2086,7 +2086,7 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, positions=None, inv_freq=No
         raise ValueError(f"{what}: q_weight and k_weight go with norm=True")
     _check_head_weight(what, "q_weight", q_weight, q)
     _check_head_weight(what, "k_weight", k_weight, k)
-    return _heads().qk_norm_rope(q, k, q_weight, k_weight, *_rotation(what, q, positions, inv_freq, sections, eps, norm, interleaved))
+    return _host().qk_norm_rope(q, k, q_weight, k_weight, *_rotation(what, q, positions, inv_freq, sections, eps, norm, interleaved))
 
 
 def _check_lens(what, name, lens, q):
@@ -2122,7 +2122,7 @@ def mha(q, k, v, scale=None, causal=False, q_lens=None, kv_lens=None):
         raise ValueError(f"{what}: head_dim {q.shape[3]} is not 64 or 128")
     if k.shape[2] == 0 or q.shape[2] == 0 or q.shape[2] % k.shape[2]:
         raise ValueError(f"{what}: {q.shape[2]} query heads over {k.shape[2]} key heads")
-    return _heads().mha(q, k, v, _check_scale(what, scale, q.shape[3]), bool(causal), _check_lens(what, "q_lens", q_lens, q),
+    return _host().mha(q, k, v, _check_scale(what, scale, q.shape[3]), bool(causal), _check_lens(what, "q_lens", q_lens, q),
                         _check_lens(what, "kv_lens", kv_lens, q))
 
 
@@ -2149,7 +2149,7 @@ def attention_rope(qkv, num_heads, scale=None, q_weight=None, k_weight=None, pos
     x = qkv.detach().unsqueeze(2)[..., :d]                                     # [B, N, 1, d]: what the checks go by
     _check_head_weight(what, "q_weight", q_weight, x)
     _check_head_weight(what, "k_weight", k_weight, x)
-    return _heads().attention_rope(qkv, num_heads, _check_scale(what, scale, d), q_weight, k_weight,
+    return _host().attention_rope(qkv, num_heads, _check_scale(what, scale, d), q_weight, k_weight,
                                    *_rotation(what, x, positions, inv_freq, sections, eps, norm, interleaved))
 
 

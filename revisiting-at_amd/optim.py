@@ -50,7 +50,8 @@ class _Plan:
 
     def __init__(self, params, groups, bits):
         dev = params[0].device
-        self.layout = [(p.data_ptr(), p.dtype, p.shape, p.stride()) for p in params]
+        self.layout = ops._host().Layout(params)
+        self.grads = (ctypes.c_void_p * len(params))()
         self.bits = bits
         self.at, size = [], {32: 0, 8: 0}
         for p, b in zip(params, self.bits):
@@ -152,8 +153,7 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def _ready(self, params):
         plan = self._plan
-        # (the address alone does not tell: memory that was given back comes again for other sizes and types)
-        if plan is None or self._stale or [(p.data_ptr(), p.dtype, p.shape, p.stride()) for p in params] != plan.layout:
+        if plan is None or self._stale or not plan.layout.matches(params):
             plan = self._build()
         return plan
 
@@ -165,18 +165,7 @@ class FusedAdamW(torch.optim.Optimizer):
                 loss = closure()
         params = self._params()
         plan = self._ready(params)
-        grads, keep = [], []
-        for p, (_, dtype, _, stride) in zip(params, plan.layout):
-            g = p.grad
-            if g is None:
-                grads.append(None)
-                continue
-            if g.is_sparse:
-                raise RuntimeError("FusedAdamW does not take sparse gradients")
-            if g.dtype != dtype or g.stride() != stride:
-                g = torch.empty_like(p).copy_(g)                   # the parameter's type and order of elements
-                keep.append(g)
-            grads.append(g.data_ptr())
+        kept = plan.layout.gradients(params, ctypes.addressof(plan.grads))                     # copies that live until the launch
         n = len(self.param_groups)
         hyper, lr_dev = (ctypes.c_double * (5 * n))(), (ctypes.c_void_p * n)()
         for i, g in enumerate(self.param_groups):
@@ -193,10 +182,10 @@ class FusedAdamW(torch.optim.Optimizer):
         lib = _lib.load()
         with ops._on_device(params[0]):
             for first, count, table, chunks in plan.runs:
-                _lib.check(lib.cnx_adamw_step(table.data_ptr(), chunks.data_ptr(), chunks.shape[0], (ctypes.c_void_p * count)(*grads[first:first + count]),
-                                              count, hyper, lr_dev, n, plan.steps.data_ptr(), plan.coef.data_ptr() + 32 * first, _lib.ptr(plan.m),
+                _lib.check(lib.cnx_adamw_step(table.data_ptr(), chunks.data_ptr(), chunks.shape[0], ctypes.byref(plan.grads, 8 * first), count, hyper, lr_dev, n, plan.steps.data_ptr(), plan.coef.data_ptr() + 32 * first, _lib.ptr(plan.m),
                                               _lib.ptr(plan.v), _lib.ptr(plan.mc), _lib.ptr(plan.ms), _lib.ptr(plan.vc), _lib.ptr(plan.vs),
                                               ops._stream()), "cnx_adamw_step")
+        del kept
         return loss
 
     @torch.no_grad()
