@@ -259,7 +259,9 @@ __device__ __forceinline__ float both_halves_max(float v) { return fmaxf(v, __sh
 __device__ __forceinline__ float both_halves_sum(float v) { return v + __shfl_xor(v, 32, 64); }
 
 // Workgroups go round robin over the 8 XCDs, each with an L2 of its own: a contiguous run of the work per XCD keeps the tiles that read
-// one key head's k and v (or q and dout) on one L2.
+// one key head's k and v (or q and dout) on one L2.  In that order the samples of a head follow each other, so that every XCD gets some of all
+// lengths of a padded batch (16 samples of up to 777 tokens, 12 heads:
+// 35 + 43 + 58 us; in the samples' order 48 + 62 + 82).
 __device__ __forceinline__ int64_t xcd_order(int64_t bid, int64_t total) {
   const int64_t per = total >> 3, rest = total & 7, x = bid & 7, i = bid >> 3;
   return x * per + (x < rest ? x : rest) + i;
@@ -314,12 +316,12 @@ struct Tile {
   uint32_t base;
 
   __device__ __forceinline__ Tile(const MhaArgs& a, uint32_t lds) : Tile(a, lds, xcd_order(blockIdx.x, gridDim.x)) {}
-  __device__ __forceinline__ Tile(const MhaArgs& a, uint32_t lds, int64_t w) : lim(a, w / (static_cast<int64_t>(a.Hkv) * a.tiles * a.splits)) {
+  __device__ __forceinline__ Tile(const MhaArgs& a, uint32_t lds, int64_t w) : lim(a, w / (a.tiles * a.splits) % a.B) {
     const int per_h = a.tiles * a.splits;
-    b = w / (static_cast<int64_t>(a.Hkv) * per_h);
-    int rest = static_cast<int>(w - b * a.Hkv * per_h);
-    hk = rest / per_h;
-    rest -= hk * per_h;
+    const int64_t head = w / per_h;
+    hk = static_cast<int>(head / a.B);
+    b = head - hk * a.B;
+    const int rest = static_cast<int>(w - head * per_h);
     const int tile = a.tiles - 1 - rest / a.splits;                    // causal: the long tiles first
     split = rest % a.splits;
     base = lds;
@@ -800,12 +802,12 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void mha_dkv_kernel(const Mha
   __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * 2 * IMG];              // [buffer][q, dout]
   __shared__ __attribute__((aligned(16))) int row_tok[RT];                               // token of a tile's row, from the tile's first
   const int wave = threadIdx.x >> 6, l32 = threadIdx.x & 31, half = (threadIdx.x >> 5) & 1;
-  const int64_t per_h = static_cast<int64_t>(a.tiles) * a.splits, per_b = a.Hkv * per_h;
+  const int64_t per_h = static_cast<int64_t>(a.tiles) * a.splits;
   int64_t w = xcd_order(blockIdx.x, gridDim.x);
-  const int64_t b = w / per_b;
-  w -= b * per_b;
-  const int hk = static_cast<int>(w / per_h);
-  w -= hk * per_h;
+  const int64_t head = w / per_h;
+  const int hk = static_cast<int>(head / a.B);
+  const int64_t b = head - hk * a.B;
+  w -= head * per_h;
   const int tile = static_cast<int>(w / a.splits), split = static_cast<int>(w - static_cast<int64_t>(tile) * a.splits);    // causal: long ones first
   const Limits lim(a, b);
   const uint16_t* qb = a.q + b * a.vq.b + static_cast<int64_t>(hk) * a.G * a.vq.h;
