@@ -2004,10 +2004,18 @@ def _on_device(t):
 def _check_heads(what, *named):
     """``named``: (name, tensor or None) - device tensors [B, N, H, d] of one type on one device."""
     first = named[0][1]
-    if all(isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 4 for _, t in named):
+    try:                                                           # the usual call in few steps
         B, _, _, d = first.shape
-        if all(t.dtype is first.dtype and t.device == first.device and t.shape[0] == B and t.shape[3] == d for _, t in named[1:]):
-            return
+        dtype, dev = first.dtype, first.get_device()
+        if dev >= 0:
+            for _, t in named[1:]:
+                b, _, _, e = t.shape
+                if b != B or e != d or t.dtype is not dtype or t.get_device() != dev:
+                    break
+            else:
+                return
+    except (AttributeError, ValueError):
+        pass
     for name, t in named:
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{what}: {name} has to be a tensor, not {type(t).__name__}")
@@ -2026,9 +2034,8 @@ def _check_heads(what, *named):
 _POSITIONS = {torch.float32: 0, torch.int32: 1, torch.int64: 2}                # CNX_POS_*
 
 
-def _rotation(what, x, positions, inv_freq, sections, eps, norm, interleaved):
-    """Checked arguments of the norm and the rotation of ``x`` [B, N, H, d], as the extension takes them."""
-    d = x.shape[-1]
+def _rotation(what, B, N, d, device, positions, inv_freq, sections, eps, norm, interleaved):
+    """Checked arguments of the norm and the rotation of [B, N, H, d] heads, as the extension takes them."""
     eps = float(eps)
     if not eps >= 0.0:
         raise ValueError(f"{what}: eps={eps!r}")
@@ -2036,33 +2043,33 @@ def _rotation(what, x, positions, inv_freq, sections, eps, norm, interleaved):
         if inv_freq is not None or sections is not None:
             raise ValueError(f"{what}: inv_freq and sections go with positions")
         return None, None, (), 0, 0, eps, bool(norm), bool(interleaved)
-    if not isinstance(positions, torch.Tensor) or positions.dtype not in _POSITIONS:
+    code = _POSITIONS.get(positions.dtype) if isinstance(positions, torch.Tensor) else None
+    if code is None:
         raise TypeError(f"{what}: positions has to be a tensor of float32, int32 or int64")
-    if not isinstance(inv_freq, torch.Tensor) or inv_freq.dtype != torch.float32 or inv_freq.shape != (d // 2,):
-        raise ValueError(f"{what}: inv_freq has to be a float32 tensor of head_dim / 2 = {d // 2} frequencies")
-    if positions.device != x.device or inv_freq.device != x.device:
-        raise ValueError(f"{what}: positions and inv_freq have to be on {x.device}")
+    pairs = d // 2
+    if not isinstance(inv_freq, torch.Tensor) or inv_freq.dtype is not torch.float32 or inv_freq.shape != (pairs,):
+        raise ValueError(f"{what}: inv_freq has to be a float32 tensor of head_dim / 2 = {pairs} frequencies")
+    if positions.get_device() != device or inv_freq.get_device() != device:
+        raise ValueError(f"{what}: positions and inv_freq have to be on device {device}, as the heads are")
     if positions.requires_grad or inv_freq.requires_grad:
         raise ValueError(f"{what}: positions and inv_freq have no gradient")
-    B, N = x.shape[:2]
     shape = positions.shape
     if len(shape) not in (2, 3) or shape[-2] != N or (len(shape) == 3 and shape[0] != B):
         raise ValueError(f"{what}: positions has to be [tokens, axes] or [batch, tokens, axes] for {B} x {N} tokens, not {tuple(shape)}")
     axes = shape[-1]
-    sections = (d // 2,) if sections is None else tuple(int(v) for v in sections)
-    if not 1 <= axes <= 4 or len(sections) != axes or min(sections) < 0 or sum(sections) != d // 2:
-        raise ValueError(f"{what}: sections={sections} has to split the {d // 2} pairs of a head over the {axes} axes of positions (1 to 4)")
-    return (positions.contiguous(), inv_freq.contiguous(), sections, _POSITIONS[positions.dtype], N * axes if len(shape) == 3 else 0, eps, bool(norm),
-            bool(interleaved))
+    sections = (pairs,) if sections is None else tuple(map(int, sections))
+    if not 1 <= axes <= 4 or len(sections) != axes or min(sections) < 0 or sum(sections) != pairs:
+        raise ValueError(f"{what}: sections={sections} has to split the {pairs} pairs of a head over the {axes} axes of positions (1 to 4)")
+    return positions.contiguous(), inv_freq.contiguous(), sections, code, N * axes if len(shape) == 3 else 0, eps, bool(norm), bool(interleaved)
 
 
-def _check_head_weight(what, name, w, x):
+def _check_head_weight(what, name, w, d, dtype, device):
     if w is None:
         return
-    if not isinstance(w, torch.Tensor) or tuple(w.shape) != (x.shape[-1],):
-        raise ValueError(f"{what}: {name} has to be a tensor of head_dim = {x.shape[-1]} values")
-    if w.dtype not in (torch.float32, x.dtype) or w.device != x.device:
-        raise TypeError(f"{what}: {name} has to be float32 or {x.dtype} on {x.device}, not {w.dtype} on {w.device}")
+    if not isinstance(w, torch.Tensor) or w.shape != (d,):
+        raise ValueError(f"{what}: {name} has to be a tensor of head_dim = {d} values")
+    if w.dtype is not torch.float32 and w.dtype is not dtype or w.get_device() != device:
+        raise TypeError(f"{what}: {name} has to be float32 or {dtype} on device {device}, not {w.dtype} on {w.device}")
 
 
 def qk_norm_rope(q, k, q_weight=None, k_weight=None, positions=None, inv_freq=None, sections=None, eps=1e-6, norm=True, interleaved=False):
@@ -2084,9 +2091,10 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, positions=None, inv_freq=No
         raise ValueError(f"{what}: head_dim {q.shape[3]} is no multiple of 16 up to 256")
     if not norm and (q_weight is not None or k_weight is not None):
         raise ValueError(f"{what}: q_weight and k_weight go with norm=True")
-    _check_head_weight(what, "q_weight", q_weight, q)
-    _check_head_weight(what, "k_weight", k_weight, k)
-    return _host().qk_norm_rope(q, k, q_weight, k_weight, *_rotation(what, q, positions, inv_freq, sections, eps, norm, interleaved))
+    (B, N, _, d), dtype, device = q.shape, q.dtype, q.get_device()
+    _check_head_weight(what, "q_weight", q_weight, d, dtype, device)
+    _check_head_weight(what, "k_weight", k_weight, d, dtype, device)
+    return _host().qk_norm_rope(q, k, q_weight, k_weight, *_rotation(what, B, N, d, device, positions, inv_freq, sections, eps, norm, interleaved))
 
 
 def _check_lens(what, name, lens, q):
@@ -2146,11 +2154,11 @@ def attention_rope(qkv, num_heads, scale=None, q_weight=None, k_weight=None, pos
         raise ValueError(f"{what}: head_dim {d} is not 64 or 128")
     if not norm and (q_weight is not None or k_weight is not None):
         raise ValueError(f"{what}: q_weight and k_weight go with norm=True")
-    x = qkv.detach().unsqueeze(2)[..., :d]                                     # [B, N, 1, d]: what the checks go by
-    _check_head_weight(what, "q_weight", q_weight, x)
-    _check_head_weight(what, "k_weight", k_weight, x)
+    dtype, device = qkv.dtype, qkv.get_device()
+    _check_head_weight(what, "q_weight", q_weight, d, dtype, device)
+    _check_head_weight(what, "k_weight", k_weight, d, dtype, device)
     return _host().attention_rope(qkv, num_heads, _check_scale(what, scale, d), q_weight, k_weight,
-                                   *_rotation(what, x, positions, inv_freq, sections, eps, norm, interleaved))
+                                   *_rotation(what, *qkv.shape[:2], d, device, positions, inv_freq, sections, eps, norm, interleaved))
 
 
 # ------------------------------------------------------------------------------ kernel sets (run-time A/B)
