@@ -159,10 +159,17 @@ struct Node : torch::autograd::Node {
     released = true;
   }
   bool wants(size_t i) const { return task_should_compute_output(i); }
-  // gradients have no derivative of their own: where a graph of them is recorded, using it raises
+  // Gradients have no derivative of their own: where a graph of them is recorded, going back through them - to the incoming gradients or to
+  // this node's inputs - raises.
   variable_list once(variable_list&& grads, const variable_list& in) {
-    if (!at::GradMode::is_enabled() || !torch::autograd::any_variable_requires_grad(in)) return std::move(grads);
-    return std::make_shared<torch::autograd::DelayedError>(name() + " is differentiable once", static_cast<int64_t>(grads.size()))->operator()(std::move(grads));
+    if (!at::GradMode::is_enabled()) return std::move(grads);
+    torch::autograd::edge_list edges = collect_next_edges(in);
+    for (const auto& e : next_edges()) edges.push_back(e);
+    const std::shared_ptr<torch::autograd::Node> error(new torch::autograd::Error(name() + " is differentiable once", std::move(edges)),
+                                                       torch::autograd::deleteNode);
+    for (const Tensor& g : grads)
+      if (g.defined()) torch::autograd::set_history(g, error);
+    return std::move(grads);
   }
   variable_list apply(variable_list&& in) final {
     std::lock_guard<std::mutex> lock(mutex_);

@@ -597,3 +597,46 @@ def test_attention_rope_with_gradients_and_values_of_any_size(R):
     bad = dout.clone()
     bad[0, 3, 5] = float("inf")
     assert not bool(torch.isfinite(run(qkv, bad)[1][0, 3, :d]).any())
+
+
+def test_uses_of_autograd(R):
+    """Some of the outputs or inputs only, a graph used twice, checkpointing, inputs changed under a graph, a second derivative."""
+    g = torch.Generator().manual_seed(11)
+    q, k, v = (torch.randn(2, 40, 2, 64, generator=g).to(torch.bfloat16).cuda().requires_grad_() for _ in range(3))
+    qkv = torch.randn(2, 40, 384, generator=g).to(torch.bfloat16).cuda().requires_grad_()
+    w = (1 + 0.1 * torch.randn(64, generator=g)).cuda().requires_grad_()
+    pos, inv = torch.arange(40, device="cuda").view(-1, 1), 100.0 ** (-torch.arange(32, device="cuda") / 32)
+    do = torch.randn(2, 40, 2, 64, generator=g).to(torch.bfloat16).cuda()
+    calls = {"mha": (lambda: R.ops.mha(q, k, v), (q, k, v), do), "rope": (lambda: R.ops.qk_norm_rope(q, k, w, w, pos, inv)[0], (q, w), do),
+             "layer": (lambda: R.ops.attention_rope(qkv, 2, None, w, w, pos, inv), (qkv, w), do.flatten(2))}
+    for name, (f, leaves, cot) in calls.items():
+        want = torch.autograd.grad(f(), leaves, cot)
+        out = f()
+        for _ in range(2):
+            assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, leaves, cot, retain_graph=True), want)), name
+        for leaf, x in zip(leaves, want):                                           # one at a time
+            assert torch.equal(torch.autograd.grad(out, leaf, cot, retain_graph=True)[0], x), name
+        torch.autograd.grad(out, leaves, cot)
+        with pytest.raises(RuntimeError, match="second time"):
+            torch.autograd.grad(out, leaves, cot)
+        out = torch.utils.checkpoint.checkpoint(f, use_reentrant=False)
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, leaves, cot), want)), name
+        (gx,) = torch.autograd.grad(f().float().square().sum(), leaves[0], create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(gx.float().sum(), leaves[0])
+        out = f()
+        with torch.no_grad():
+            leaves[0].mul_(1)
+        with pytest.raises(RuntimeError, match="inplace"):
+            torch.autograd.grad(out, leaves, cot)
+        assert f().requires_grad and not f().detach().requires_grad
+        with torch.no_grad():
+            assert not f().requires_grad
+    yq, yk = R.ops.qk_norm_rope(q, k, w, w, pos, inv)                               # one output only: the other's gradient is zeros
+    a = torch.autograd.grad(yq, (q, k), do, retain_graph=True)
+    b = torch.autograd.grad((yq, yk), (q, k), (do, torch.zeros_like(do)))
+    assert all(torch.equal(x, y) for x, y in zip(a, b)) and not bool(a[1].any())
+    x = qkv.detach().requires_grad_()
+    with R.ops.input_grad_only():                                                   # the attack's backward: the input's gradient, no weights'
+        gx, gw = torch.autograd.grad(R.ops.attention_rope(x, 2, None, w, w, pos, inv), (x, w), do.flatten(2), allow_unused=True)
+    assert gw is None and torch.equal(gx, torch.autograd.grad(R.ops.attention_rope(qkv, 2, None, w, w, pos, inv), qkv, do.flatten(2))[0])
