@@ -13,8 +13,9 @@
 // 32 (a position of 10^6 at frequency 1 would be off by 0.03 rad in 32 bits).  x r is computed again in the backward instead of kept: it is in
 // registers anyway and would cost as much memory as x.
 // Sums (mean of squares, weight gradients) in 32 bits; one rounding to the output's type at the end.
-// Measured: 32 x 1025 tokens, 12 + 12 heads of 64, bf16: forward 38 us (201 MB, 5.3 TB/s), backward 69 us (302 MB, 4.4 TB/s) + 4 us for the
-// weights' sums; a copy of 2 GiB reaches 4.9 TB/s.
+// Measured: 32 x 1025 tokens, 12 + 12 heads of 64, bf16: forward 38 us (201 MB, 5.3 TB/s), backward 70 us (302 MB, 4.3 TB/s) + 4 us for the
+// weights' sums; 2 x 1571 tokens, 16 + 4 heads of 128, fp32, interleaved: forward 13 us (64 MB, 4.9 TB/s; 19 us before the threads of a head took
+// its 16-byte pieces in turn).  A copy of 2 GiB reaches 4.9 TB/s.
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -67,13 +68,8 @@ struct bf16_t { uint16_t u; };
 template <typename T> struct Io;
 template <> struct Io<float> {
   struct Raw { float4 a, b; };
-  static __device__ __forceinline__ Raw raw8(const float* p) { return Raw{*reinterpret_cast<const float4*>(p), *reinterpret_cast<const float4*>(p + 4)}; }
   static __device__ __forceinline__ void widen(const Raw& r, float* x) {
     x[0] = r.a.x; x[1] = r.a.y; x[2] = r.a.z; x[3] = r.a.w; x[4] = r.b.x; x[5] = r.b.y; x[6] = r.b.z; x[7] = r.b.w;
-  }
-  static __device__ __forceinline__ void store8(float* p, const float* x) {
-    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
-    *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
   }
 };
 template <> struct Io<bf16_t> {
@@ -111,11 +107,19 @@ template <> struct Io<__half> {
   }
 };
 
-// the 16 values of a thread: a = first members of its 8 pairs, b = second members
+// The 16 values of a thread: a = first members of its 8 pairs, b = second members, in 16-byte pieces that the threads of a head take in turn, so
+// that each load or store covers a head's bytes without gaps.  A piece holds kPer pairs (interleaved) or their first or second members.
+template <bool IL, typename T> constexpr int kPer = (IL ? 8 : 16) / static_cast<int>(sizeof(T));
+template <bool IL, typename T> __device__ __forceinline__ int pair_of(int i, int j, int tph) { return kPer<IL, T> * (j + i / kPer<IL, T> * tph) + i % kPer<IL, T>; }
 template <typename T> struct Pairs { typename Io<T>::Raw lo, hi; };
 template <bool IL, typename T>
-__device__ __forceinline__ Pairs<T> raw_pairs(const T* head, int j, int d) {
-  return IL ? Pairs<T>{Io<T>::raw8(head + 16 * j), Io<T>::raw8(head + 16 * j + 8)} : Pairs<T>{Io<T>::raw8(head + 8 * j), Io<T>::raw8(head + d / 2 + 8 * j)};
+__device__ __forceinline__ Pairs<T> raw_pairs(const T* head, int j, int tph) {
+  if constexpr (sizeof(T) == 4) {
+    const float4* p = reinterpret_cast<const float4*>(head) + j;
+    return Pairs<T>{{p[0], p[tph]}, {p[2 * tph], p[3 * tph]}};         // (the second members begin at d / 2 = 2 tph pieces)
+  } else {
+    return Pairs<T>{Io<T>::raw8(head + 8 * j), Io<T>::raw8(head + 8 * tph + 8 * j)};
+  }
 }
 template <bool IL, typename T>
 __device__ __forceinline__ void widen(const Pairs<T>& r, float* a, float* b) {
@@ -131,16 +135,20 @@ __device__ __forceinline__ void widen(const Pairs<T>& r, float* a, float* b) {
   }
 }
 template <bool IL, typename T>
-__device__ __forceinline__ void store_pairs(T* head, int j, int d, const float* a, const float* b) {
-  if constexpr (IL) {
-    float t[16];
+__device__ __forceinline__ void store_pairs(T* head, int j, int tph, const float* a, const float* b) {
+  float t[16];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) { t[2 * i] = a[i]; t[2 * i + 1] = b[i]; }
-    Io<T>::store8(head + 16 * j, t);
-    Io<T>::store8(head + 16 * j + 8, t + 8);
+  for (int i = 0; i < 8; ++i) {
+    t[IL ? 2 * i : i] = a[i];
+    t[IL ? 2 * i + 1 : 8 + i] = b[i];
+  }
+  if constexpr (sizeof(T) == 4) {
+    float4* p = reinterpret_cast<float4*>(head) + j;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) p[c * tph] = make_float4(t[4 * c], t[4 * c + 1], t[4 * c + 2], t[4 * c + 3]);
   } else {
-    Io<T>::store8(head + 8 * j, a);
-    Io<T>::store8(head + d / 2 + 8 * j, b);
+    Io<T>::store8(head + 8 * j, t);
+    Io<T>::store8(head + 8 * tph + 8 * j, t + 8);
   }
 }
 
@@ -233,8 +241,8 @@ __global__ __launch_bounds__(256, BWD ? 3 : 4) void qk_norm_rope_kernel(const Ro
     Item cur = item(g0);
     Pairs<T> rx, rg;
     auto load = [&](const Item& i) {
-      if (!BWD || a.norm) rx = raw_pairs<IL>(px + i.s * z.vx.b + i.t * z.vx.n + i.h * z.vx.h, jj, d);
-      if constexpr (BWD) rg = raw_pairs<IL>(pg + i.s * z.vdy.b + i.t * z.vdy.n + i.h * z.vdy.h, jj, d);
+      if (!BWD || a.norm) rx = raw_pairs<IL>(px + i.s * z.vx.b + i.t * z.vx.n + i.h * z.vx.h, jj, tph);
+      if constexpr (BWD) rg = raw_pairs<IL>(pg + i.s * z.vdy.b + i.t * z.vdy.n + i.h * z.vdy.h, jj, tph);
     };
     if (items > 0) load(cur);
     if (a.pos) {
@@ -255,7 +263,7 @@ __global__ __launch_bounds__(256, BWD ? 3 : 4) void qk_norm_rope_kernel(const Ro
       const bool live = here && now.live;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float2 v = a.pos ? cs[now.t * pairs + 8 * jj + i] : make_float2(1.f, 0.f);
+        const float2 v = a.pos ? cs[now.t * pairs + pair_of<IL, T>(i, jj, tph)] : make_float2(1.f, 0.f);
         c[i] = v.x; s[i] = v.y;
       }
       if (a.norm) {                                                   // x -> x r
@@ -272,7 +280,8 @@ __global__ __launch_bounds__(256, BWD ? 3 : 4) void qk_norm_rope_kernel(const Ro
           for (int i = 0; i < 8; ++i) {                               // the rotation's transpose, then the norm's
             const float u = fmaf(ga[i], c[i], gb[i] * s[i]), v = fmaf(gb[i], c[i], -ga[i] * s[i]);
             const float ta = u * xa[i], tb = v * xb[i];
-            const float wa = wl[8 * jj + i], wb = wl[pairs + 8 * jj + i];
+            const int at = pair_of<IL, T>(i, jj, tph);
+            const float wa = wl[at], wb = wl[pairs + at];
             sa[i] += live ? ta : 0.f;
             sb[i] += live ? tb : 0.f;
             dot = fmaf(ta, wa, fmaf(tb, wb, dot));
@@ -287,7 +296,11 @@ __global__ __launch_bounds__(256, BWD ? 3 : 4) void qk_norm_rope_kernel(const Ro
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) { xa[i] *= wl[8 * jj + i]; xb[i] *= wl[pairs + 8 * jj + i]; }
+          for (int i = 0; i < 8; ++i) {
+            const int at = pair_of<IL, T>(i, jj, tph);
+            xa[i] *= wl[at];
+            xb[i] *= wl[pairs + at];
+          }
         }
       } else if constexpr (BWD) {
 #pragma unroll
@@ -311,7 +324,7 @@ __global__ __launch_bounds__(256, BWD ? 3 : 4) void qk_norm_rope_kernel(const Ro
           gb[i] = gb[i] > 65504.f ? 65504.f : gb[i] < -65504.f ? -65504.f : gb[i];
         }
       }
-      if (live) store_pairs<IL>(po + now.s * z.vo.b + now.t * z.vo.n + now.h * z.vo.h, j, d, ga, gb);
+      if (live) store_pairs<IL>(po + now.s * z.vo.b + now.t * z.vo.n + now.h * z.vo.h, j, tph, ga, gb);
     }
   }
   if constexpr (BWD) {
@@ -326,7 +339,7 @@ __global__ __launch_bounds__(256, BWD ? 3 : 4) void qk_norm_rope_kernel(const Ro
           sb[i] += __shfl_xor(sb[i], m, 64);
         }
         if (lane < group && here) {
-          const int ia = IL ? 16 * j + 2 * i : 8 * j + i, ib = IL ? ia + 1 : ia + pairs;
+          const int at = pair_of<IL, T>(i, j, tph), ia = IL ? 2 * at : at, ib = IL ? ia + 1 : ia + pairs;
           red[wave * d + ia] = sa[i];
           red[wave * d + ib] = sb[i];
         }
