@@ -124,7 +124,7 @@ struct MhaArgs {
   int32_t span;                                  // keys of one split, a multiple of the key tile
   int64_t B;
   float scale;
-  Turn tq, tk;                                   // TURN: G = 1, no key splits, no lengths
+  Turn tq, tk;                                   // TURN: G = 1, no lengths
   const float2* cs;                              // cosines and sines [(B,) N][D / 2] or NULL
   int64_t cs_b;                                  // pairs between the samples' (0: shared)
   float eps;
@@ -747,10 +747,10 @@ __global__ __launch_bounds__(256, 2) void mha_dq_kernel(const MhaArgs a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) dq[db][r] *= mul;
     mul = 1.f;
-    turn_back<T, D>(a, a.tq, dq, w.b, w.tok, h, w.tok < a.Nq);
+    if (a.splits == 1) turn_back<T, D>(a, a.tq, dq, w.b, w.tok, h, w.tok < a.Nq);
   }
   if (w.tok >= a.Nq) return;
-  if (!TURN && a.splits > 1) {
+  if (a.splits > 1) {
     float* po = a.part + (w.split * a.B * a.H * a.Nq + at) * D;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
@@ -964,6 +964,12 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void mha_dkv_kernel(const Mha
     if (t0 < t_end) step(1);
   }
   if constexpr (TURN) {
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dk[db][r] *= dk_mul;
+  }
+  if (TURN && a.splits == 1) {
     const bool live = key < a.Nk;
     if (live) {
       uint16_t* pv = a.dv + b * a.vdv.b + key * a.vdv.n + hk * a.vdv.h;
@@ -973,10 +979,6 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void mha_dkv_kernel(const Mha
         for (int g = 0; g < 4; ++g)
           *reinterpret_cast<uint2*>(pv + db * 32 + 8 * g + 4 * half) = pack4<T>(dv[db][4 * g], dv[db][4 * g + 1], dv[db][4 * g + 2], dv[db][4 * g + 3]);
     }
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) dk[db][r] *= dk_mul;
     turn_back<T, D>(a, a.tk, dk, b, key, hk, live);
     if (!live) return;
     uint16_t* pk = a.dk + b * a.vdk.b + key * a.vdk.n + hk * a.vdk.h;
@@ -1044,6 +1046,90 @@ __global__ __launch_bounds__(256) void mha_dkv_join_kernel(const MhaArgs a) {
   *reinterpret_cast<uint2*>(po + d4 * 4) = pack4<T>(x[0] * mul, x[1] * mul, x[2] * mul, x[3] * mul);
 }
 
+// The splits' sums of rows of dq' (blockIdx.y = 0 of one), or of dk' and dv (of two), and of the former the way back to dq (dk): as turn_back, with
+// D / 4 threads to a row, 4 consecutive values each.  (Layer forward + backward, host included: 2 x 626 tokens, 3 heads 125 -> 93 us, 3 x 530, 8 heads
+// 127 -> 85 against workgroups that meet all keys or rows.)
+template <typename T, int D>
+__global__ __launch_bounds__(256) void mha_turn_join_kernel(const MhaArgs a) {
+  constexpr int TPR = D / 4, ROWS = 256 / TPR;
+  __shared__ float red[ROWS * D];
+  const bool keys = gridDim.y == 2, is_v = blockIdx.y == 1;
+  const int64_t rows = a.B * a.H * a.Nk, at = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / TPR, row = at < rows ? at : rows - 1;
+  const int d4 = threadIdx.x % TPR;
+  const float* part = a.part + ((is_v ? rows : 0) + row) * D + d4 * 4;
+  const int64_t step = (keys ? 2 : 1) * rows * D;
+  float g[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < a.splits; s0 += 4) {
+    float4 v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const float4*>(part + min(s0 + u, a.splits - 1) * step);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (s0 + u < a.splits) { g[0] += v[u].x; g[1] += v[u].y; g[2] += v[u].z; g[3] += v[u].w; }
+  }
+  const int64_t bh = row / a.Nk, b = bh / a.H;
+  const int tok = static_cast<int>(row - bh * a.Nk), h = static_cast<int>(bh - b * a.H);
+  const Turn& t = keys ? a.tk : a.tq;
+  if (!is_v) {                                   // (uniform)
+    if (a.cs) {
+      const float2* cs = a.cs + b * a.cs_b + static_cast<int64_t>(tok) * (D / 2);
+      if (a.il) {
+        const float4 p = *reinterpret_cast<const float4*>(cs + 2 * d4);
+        const float g0 = g[0], g2 = g[2];
+        g[0] = fmaf(g0, p.x, g[1] * p.y);
+        g[1] = fmaf(g[1], p.x, -g0 * p.y);
+        g[2] = fmaf(g2, p.z, g[3] * p.w);
+        g[3] = fmaf(g[3], p.z, -g2 * p.w);
+      } else {
+        const bool second = d4 >= TPR / 2;
+        const float4* p = reinterpret_cast<const float4*>(cs + 4 * (d4 & (TPR / 2 - 1)));
+        const float4 p0 = p[0], p1 = p[1];
+        const float c[4] = {p0.x, p0.z, p1.x, p1.z}, s[4] = {p0.y, p0.w, p1.y, p1.w};
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const float o = __shfl_xor(g[u], TPR / 2, 64);
+          g[u] = fmaf(g[u], c[u], second ? -o * s[u] : o * s[u]);
+        }
+      }
+    }
+    if (a.norm) {
+      const uint2 xp = *reinterpret_cast<const uint2*>(t.x + b * t.vx.b + tok * t.vx.n + h * t.vx.h + d4 * 4);
+      float x[4] = {T::lo(xp.x), T::hi(xp.x), T::lo(xp.y), T::hi(xp.y)}, ss = 0.f, dot = 0.f;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) ss = fmaf(x[u], x[u], ss);
+      for (int m = 1; m < TPR; m <<= 1) ss += __shfl_xor(ss, m, 64);
+      const float rn = 1.f / sqrtf(ss * (1.f / D) + a.eps);
+      f32x4u w = {1.f, 1.f, 1.f, 1.f};
+      if (t.w) w = *reinterpret_cast<const f32x4u*>(t.w + d4 * 4);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        x[u] *= rn;
+        if (t.part) red[threadIdx.x * 4 + u] = at < rows ? g[u] * x[u] : 0.f;
+        g[u] *= w[u];
+        dot = fmaf(g[u], x[u], dot);
+      }
+      for (int m = 1; m < TPR; m <<= 1) dot += __shfl_xor(dot, m, 64);
+      dot *= 1.f / D;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) g[u] = rn * fmaf(-x[u], dot, g[u]);
+      if (t.part) {                              // the weights' gradients of the workgroup's rows
+        __syncthreads();
+        if (threadIdx.x < D) {
+          float s = 0.f;
+#pragma unroll
+          for (int r = 0; r < ROWS; ++r) s += red[r * D + threadIdx.x];
+          t.part[static_cast<int64_t>(blockIdx.x) * D + threadIdx.x] = s;
+        }
+      }
+    }
+  }
+  if (at >= rows) return;
+  uint16_t* po = !keys ? a.dq + b * a.vdq.b + tok * a.vdq.n + h * a.vdq.h
+                       : is_v ? a.dv + b * a.vdv.b + tok * a.vdv.n + h * a.vdv.h : a.dk + b * a.vdk.b + tok * a.vdk.n + h * a.vdk.h;
+  *reinterpret_cast<uint2*>(po + d4 * 4) = pack4<T>(g[0], g[1], g[2], g[3]);
+}
+template <int D> int64_t join_groups(const MhaArgs& a) { return (a.B * a.H * a.Nk * (D / 4) + 255) / 256; }
+
 // ===================================================================================================================== host
 constexpr int kPieces = 8;                       // workgroups that look for a head's largest rows, at most
 
@@ -1091,16 +1177,16 @@ int check_args(const MhaArgs& a, int dtype, int32_t head_dim) {
   if (a.B > 0 && tiles > 0 && a.B > (1LL << 23) / tiles / a.H) return APGD_ERR_SIZE;
   return APGD_OK;
 }
-void cut(MhaArgs& a, int64_t tiles, bool split) {
+void cut(MhaArgs& a, int64_t tiles) {
   a.tiles = static_cast<int32_t>(tiles);
-  a.splits = split ? splits_for(a.B * a.Hkv * tiles, a.Nk) : 1;
+  a.splits = splits_for(a.B * a.Hkv * tiles, a.Nk);
   const int64_t per = ((a.Nk + a.splits - 1) / a.splits + kKT - 1) / kKT * kKT;
   a.span = static_cast<int32_t>(per < kKT ? kKT : per);
 }
 
 template <typename T, int D>
 int launch_fwd(MhaArgs& a, hipStream_t s) {
-  cut(a, row_tiles(a.Nq, a.G), true);
+  cut(a, row_tiles(a.Nq, a.G));
   hipLaunchKernelGGL((mha_fwd_kernel<T, D>), dim3(static_cast<unsigned>(a.B * a.Hkv * a.tiles * a.splits)), dim3(256), 0, s, a);
   if (a.splits > 1)
     hipLaunchKernelGGL((mha_join_kernel<typename T::Io, D>), dim3(static_cast<unsigned>((a.B * a.H * a.Nq * (D / 4) + 255) / 256)), dim3(256), 0, s, a);
@@ -1109,17 +1195,21 @@ int launch_fwd(MhaArgs& a, hipStream_t s) {
 template <typename T, int D, bool TURN>
 int launch_bwd(MhaArgs& a, hipStream_t s) {
   if (a.Nq > 0) {
-    cut(a, row_tiles(a.Nq, a.G), !TURN);
+    cut(a, row_tiles(a.Nq, a.G));
     hipLaunchKernelGGL((mha_dq_kernel<T, D, TURN>), dim3(static_cast<unsigned>(a.B * a.Hkv * a.tiles * a.splits)), dim3(256), 0, s, a);
-    if (!TURN && a.splits > 1)
-      hipLaunchKernelGGL((mha_dq_join_kernel<typename T::Io, D>), dim3(static_cast<unsigned>((a.B * a.H * a.Nq * (D / 4) + 255) / 256)), dim3(256), 0, s, a);
+    if (a.splits > 1) {
+      if constexpr (TURN) hipLaunchKernelGGL((mha_turn_join_kernel<typename T::Io, D>), dim3(static_cast<unsigned>(join_groups<D>(a)), 1), dim3(256), 0, s, a);
+      else hipLaunchKernelGGL((mha_dq_join_kernel<T, D>), dim3(static_cast<unsigned>((a.B * a.H * a.Nq * (D / 4) + 255) / 256)), dim3(256), 0, s, a);
+    }
   }
   if (a.Nk > 0) {
     a.tiles = (a.Nk + 127) / 128;
-    a.splits = TURN ? 1 : dkv_splits(a.B, a.Nq, a.Nk, a.Hkv, a.G, D, a.causal != 0);
+    a.splits = dkv_splits(a.B, a.Nq, a.Nk, a.Hkv, a.G, D, a.causal != 0);
     hipLaunchKernelGGL((mha_dkv_kernel<T, D, TURN>), dim3(static_cast<unsigned>(a.B * a.Hkv * a.tiles * a.splits)), dim3(256), 0, s, a);
-    if (!TURN && a.splits > 1)
-      hipLaunchKernelGGL((mha_dkv_join_kernel<typename T::Io, D>), dim3(static_cast<unsigned>((a.B * a.Hkv * a.Nk * (D / 4) + 255) / 256), 2), dim3(256), 0, s, a);
+    if (a.splits > 1) {
+      if constexpr (TURN) hipLaunchKernelGGL((mha_turn_join_kernel<typename T::Io, D>), dim3(static_cast<unsigned>(join_groups<D>(a)), 2), dim3(256), 0, s, a);
+      else hipLaunchKernelGGL((mha_dkv_join_kernel<T, D>), dim3(static_cast<unsigned>((a.B * a.Hkv * a.Nk * (D / 4) + 255) / 256), 2), dim3(256), 0, s, a);
+    }
   }
   return launch_status();
 }
@@ -1226,10 +1316,15 @@ int cnx_attention_rope_fwd(const void* qkv, void* yq, void* yk, void* out, float
   return dtype == APGD_BF16 ? launch_fwd<Bf16>(a, head_dim, s) : launch_fwd<Fp16>(a, head_dim, s);
 }
 
+// rows of partial weight gradients of a side: the workgroups of dq (of dk/dv), or of the join behind its splits
+static int64_t turn_rows(int64_t B, int64_t N, int64_t H, int64_t D, bool joined) { return joined ? (B * H * N * (D / 4) + 255) / 256 : B * H * ((N + 127) / 128); }
+
 int64_t cnx_attention_rope_bwd_ws_floats(int64_t B, int32_t N, int32_t H, int32_t head_dim, int32_t own_positions) {
   if (B <= 0 || N <= 0 || H < 1 || !cnx_mha_supported(head_dim)) return 0;
-  const int64_t tiles = (N + 127) / 128;         // D; cosines and sines; weight gradients of the workgroups; sizes of v and dout
-  return (B * H * N + 3) / 4 * 4 + (own_positions ? B : 1) * N * head_dim + 2 * B * H * tiles * head_dim + 2 * B * H * kPieces;
+  const int64_t D = head_dim;                    // D of the rows; cosines and sines; sizes of v and dout; weight gradients; the splits' sums
+  const int64_t most = std::max(turn_rows(B, N, H, D, false), turn_rows(B, N, H, D, true));
+  return (B * H * N + 3) / 4 * 4 + (own_positions ? B : 1) * N * D + (2 * B * H * kPieces + 3) / 4 * 4 + 2 * most * D +
+         cnx_mha_bwd_ws_floats(B, N, N, H, H, head_dim, 0);
 }
 
 int cnx_attention_rope_bwd(const void* qkv, const void* yq, const void* yk, const void* out, const void* dout, const float* lse, void* dqkv,
@@ -1246,7 +1341,7 @@ int cnx_attention_rope_bwd(const void* qkv, const void* yq, const void* yk, cons
   if (const int rc = check_args(a, dtype, head_dim)) return rc;
   if (!turns || (want_w && !norm)) return APGD_ERR_ARG;
   hipStream_t s = as_stream(stream);
-  if (B == 0 || N == 0) return want_w ? rope_dw(nullptr, 0, head_dim, dwq, dwk, s) : APGD_OK;          // no row: zeros
+  if (B == 0 || N == 0) return want_w ? rope_dw(nullptr, 0, nullptr, 0, head_dim, dwq, dwk, s) : APGD_OK;          // no row: zeros
   if (!qkv || !yq || !yk || !out || !dout || !lse || !dqkv || !ws || !dout_strides) return APGD_ERR_NULL;
   const View packed = {N * 3 * C, 3 * C, D}, dense = {N * C, C, D};
   a.q = static_cast<const uint16_t*>(yq); a.k = static_cast<const uint16_t*>(yk); a.v = x + 2 * C;
@@ -1256,13 +1351,15 @@ int cnx_attention_rope_bwd(const void* qkv, const void* yq, const void* yk, cons
   a.vv = a.vdq = a.vdk = a.vdv = packed;
   a.vdo = view_of(dout_strides);
   if (!near_enough(packed, 1) || !near_enough(a.vdo, 1)) return APGD_ERR_ARG;
-  const int64_t groups = B * H * ((N + 127) / 128);
+  const int64_t nq = turn_rows(B, N, H, D, splits_for(B * H * row_tiles(N, 1), N) > 1), nk = turn_rows(B, N, H, D, dkv_splits(B, N, N, H, 1, head_dim, false) > 1);
   a.dvec = ws;
   float* table = ws + (B * H * N + 3) / 4 * 4;
-  float* part = table + (pos_batch_stride ? B : 1) * N * D;
-  float2* range = reinterpret_cast<float2*>(part + 2 * groups * D);
-  a.tq = Turn{x, packed, wq, want_w ? part : nullptr};
-  a.tk = Turn{x + C, packed, wk, want_w ? part + groups * D : nullptr};
+  float2* range = reinterpret_cast<float2*>(table + (pos_batch_stride ? B : 1) * N * D);
+  float* pq = reinterpret_cast<float*>(range) + (2 * B * H * kPieces + 3) / 4 * 4;
+  float* pk = pq + nq * D;
+  a.part = pk + nk * D;
+  a.tq = Turn{x, packed, wq, want_w ? pq : nullptr};
+  a.tk = Turn{x + C, packed, wk, want_w ? pk : nullptr};
   if (positions) {
     a.cs = reinterpret_cast<const float2*>(table);
     a.cs_b = pos_batch_stride ? N * D / 2 : 0;
@@ -1280,7 +1377,7 @@ int cnx_attention_rope_bwd(const void* qkv, const void* yq, const void* yk, cons
   } else {
     rc = dtype == APGD_BF16 ? launch_bwd<Bf16, true>(a, head_dim, s) : launch_bwd<Fp16, true>(a, head_dim, s);
   }
-  return rc || !want_w ? rc : rope_dw(part, static_cast<int>(groups), head_dim, dwq, dwk, s);
+  return rc || !want_w ? rc : rope_dw(pq, static_cast<int>(nq), pk, static_cast<int>(nk), head_dim, dwq, dwk, s);
 }
 
 }  // extern "C"

@@ -11,5 +11,5 @@ int rope_forward(const void* q, const void* k, void* yq, void* yk, int dtype, bo
                  int w_dtype, const void* positions, int pos_dtype, int64_t pos_batch_stride, int32_t axes, const int32_t* sections,
                  const float* inv_freq, int64_t B, int64_t N, int32_t Hq, int32_t Hk, int32_t d, float eps, int32_t norm, int32_t interleaved,
                  hipStream_t s);
-// dwq, dwk [d] (either may be NULL) = sums over the rows of part [2][rows][d], in a fixed order
-int rope_dw(const float* part, int rows, int32_t d, float* dwq, float* dwk, hipStream_t s);
+// dwq, dwk [d] (either may be NULL) = sums over the rows of pq [nq][d], pk [nk][d], in a fixed order
+int rope_dw(const float* pq, int nq, const float* pk, int nk, int32_t d, float* dwq, float* dwk, hipStream_t s);

@@ -352,10 +352,12 @@ __global__ __launch_bounds__(256, BWD ? 3 : 4) void qk_norm_rope_kernel(const Ro
 }
 
 // dw[e] = sum over the workgroups' rows, in a fixed order: 16 columns x 64 row lanes, every lane its rows one after the other
-__global__ __launch_bounds__(1024) void rope_dw_kernel(const float* __restrict__ part, int rows, int d, float* __restrict__ dwq,
-                                                       float* __restrict__ dwk) {
+__global__ __launch_bounds__(1024) void rope_dw_kernel(const float* __restrict__ pq, int nq, const float* __restrict__ pk, int nk, int d,
+                                                       float* __restrict__ dwq, float* __restrict__ dwk) {
   __shared__ float red[64][17];
   float* dw = blockIdx.y ? dwk : dwq;
+  const float* part = blockIdx.y ? pk : pq;
+  const int rows = blockIdx.y ? nk : nq;
   const int col = threadIdx.x & 15, row = threadIdx.x >> 4, e = blockIdx.x * 16 + col;        // d is a multiple of 16
   float s = 0.f;
   for (int r0 = 0; r0 < rows; r0 += 512) {                            // eight loads at a time
@@ -363,7 +365,7 @@ __global__ __launch_bounds__(1024) void rope_dw_kernel(const float* __restrict__
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
       const int r = r0 + u * 64 + row;
-      v[u] = r < rows ? part[(static_cast<int64_t>(blockIdx.y) * rows + r) * d + e] : 0.f;
+      v[u] = r < rows ? part[static_cast<int64_t>(r) * d + e] : 0.f;
     }
 #pragma unroll
     for (int u = 0; u < 8; ++u) s += v[u];
@@ -467,8 +469,8 @@ int rope_forward(const void* q, const void* k, void* yq, void* yk, int dtype, bo
   launch<false>(a, dtype, half, interleaved != 0, static_cast<unsigned>(a.tiles < kFwdGrid ? a.tiles : kFwdGrid), s);
   return launch_status();
 }
-int rope_dw(const float* part, int rows, int32_t d, float* dwq, float* dwk, hipStream_t s) {
-  hipLaunchKernelGGL(rope_dw_kernel, dim3(static_cast<unsigned>(d / 16), 2), dim3(1024), 0, s, part, rows, d, dwq, dwk);
+int rope_dw(const float* pq, int nq, const float* pk, int nk, int32_t d, float* dwq, float* dwk, hipStream_t s) {
+  hipLaunchKernelGGL(rope_dw_kernel, dim3(static_cast<unsigned>(d / 16), 2), dim3(1024), 0, s, pq, nq, pk, nk, d, dwq, dwk);
   return launch_status();
 }
 
@@ -510,7 +512,7 @@ int cnx_qk_norm_rope_bwd(const void* dyq, const void* dyk, const void* q, const 
     grid = static_cast<unsigned>(a.tiles < kBwdGrid ? a.tiles : kBwdGrid);
     launch<true>(a, dtype, false, interleaved != 0, grid, as_stream(stream));
   }
-  return want_w ? rope_dw(ws, static_cast<int>(grid), d, dwq, dwk, as_stream(stream)) : launch_status();
+  return want_w ? rope_dw(ws, static_cast<int>(grid), ws + static_cast<int64_t>(grid) * d, static_cast<int>(grid), d, dwq, dwk, as_stream(stream)) : launch_status();
 }
 
 }  // extern "C"

@@ -464,7 +464,10 @@ ATTN = [  # B, N, H, d, norm, rotate, interleaved, per-batch positions, weights'
     (1, 64, 3, 64, True, False, False, False, "x", "expanded"),
     (1, 65, 2, 64, False, True, False, True, None, "whole"),
     (43, 257, 2, 64, True, True, False, False, torch.float32, "whole"),          # more than one tile of rows and keys
-    (3, 577, 2, 64, True, True, False, True, torch.float32, "whole"),
+    (3, 577, 2, 64, True, True, False, True, torch.float32, "whole"),           # few tiles: keys and rows split, joined with the way back
+    (1, 600, 2, 128, True, True, True, True, torch.float32, "part"),
+    (2, 520, 1, 64, False, True, False, False, None, "whole"),
+    (1, 1030, 1, 64, True, False, False, False, "x", "expanded"),
     (29, 260, 3, 128, False, True, True, False, None, "part"),
 ]
 

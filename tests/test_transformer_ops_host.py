@@ -71,6 +71,7 @@ def test_attention_rope_workspaces_and_forward_refusals(R):
     lib = R._lib.load()
     size = lib.cnx_attention_rope_bwd_ws_floats
     assert size(2, 17, 2, 64, 1) - size(2, 17, 2, 64, 0) == 17 * 64 and size(2, 17, 2, 64, 0) >= 68 + 17 * 64 + 2 * 4 * 64
+    assert size(1, 1000, 1, 64, 0) > size(1, 1000, 1, 64, 0) - lib.cnx_mha_bwd_ws_floats(1, 1000, 1000, 1, 1, 64, 0) > 0        # rows split
     assert size(1, 17, 2, 96, 0) == 0 and size(0, 17, 2, 64, 0) == 0
 
     def fwd(qkv=P, y=P, out=P, ws=P, dtype=1, w=None, w_dtype=0, pos=P, axes=2, sections=(16, 16), B=1, N=4, H=2, d=64, norm=1, scale=0.125):
