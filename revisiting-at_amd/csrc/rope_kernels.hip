@@ -13,7 +13,7 @@
 // 32 (a position of 10^6 at frequency 1 would be off by 0.03 rad in 32 bits).  x r is computed again in the backward instead of kept: it is in
 // registers anyway and would cost as much memory as x.
 // Sums (mean of squares, weight gradients) in 32 bits; one rounding to the output's type at the end.
-// Measured: 32 x 1025 tokens, 12 + 12 heads of 64, bf16: forward 38 us (201 MB, 5.3 TB/s), backward 70 us (302 MB, 4.3 TB/s) + 4 us for the
+// Measured: 32 x 1025 tokens, 12 + 12 heads of 64, bf16: forward 38 us (201 MB, 5.3 TB/s), backward 73 us (302 MB, 4.1 TB/s) + 4 us for the
 // weights' sums; 2 x 1571 tokens, 16 + 4 heads of 128, fp32, interleaved: forward 13 us (64 MB, 4.9 TB/s; 19 us before the threads of a head took
 // its 16-byte pieces in turn).  A copy of 2 GiB reaches 4.9 TB/s.
 #include <hip/hip_fp16.h>
@@ -118,7 +118,7 @@ __device__ __forceinline__ Pairs<T> raw_pairs(const T* head, int j, int tph) {
     const float4* p = reinterpret_cast<const float4*>(head) + j;
     return Pairs<T>{{p[0], p[tph]}, {p[2 * tph], p[3 * tph]}};         // (the second members begin at d / 2 = 2 tph pieces)
   } else {
-    return Pairs<T>{Io<T>::raw8(head + 8 * j), Io<T>::raw8(head + 8 * tph + 8 * j)};
+    return Pairs<T>{Io<T>::raw8(head + 8 * j), Io<T>::raw8(head + 8 * (j + tph))};
   }
 }
 template <bool IL, typename T>
@@ -137,18 +137,21 @@ __device__ __forceinline__ void widen(const Pairs<T>& r, float* a, float* b) {
 template <bool IL, typename T>
 __device__ __forceinline__ void store_pairs(T* head, int j, int tph, const float* a, const float* b) {
   float t[16];
+  if constexpr (IL) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    t[IL ? 2 * i : i] = a[i];
-    t[IL ? 2 * i + 1 : 8 + i] = b[i];
+    for (int i = 0; i < 8; ++i) { t[2 * i] = a[i]; t[2 * i + 1] = b[i]; }
+    a = t;
+    b = t + 8;
   }
   if constexpr (sizeof(T) == 4) {
     float4* p = reinterpret_cast<float4*>(head) + j;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) p[c * tph] = make_float4(t[4 * c], t[4 * c + 1], t[4 * c + 2], t[4 * c + 3]);
+    p[0] = make_float4(a[0], a[1], a[2], a[3]);
+    p[tph] = make_float4(a[4], a[5], a[6], a[7]);
+    p[2 * tph] = make_float4(b[0], b[1], b[2], b[3]);
+    p[3 * tph] = make_float4(b[4], b[5], b[6], b[7]);
   } else {
-    Io<T>::store8(head + 8 * j, t);
-    Io<T>::store8(head + 8 * tph + 8 * j, t + 8);
+    Io<T>::store8(head + 8 * j, a);
+    Io<T>::store8(head + 8 * (j + tph), b);
   }
 }
 
