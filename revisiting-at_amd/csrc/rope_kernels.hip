@@ -13,7 +13,7 @@
 // 32 (a position of 10^6 at frequency 1 would be off by 0.03 rad in 32 bits).  x r is computed again in the backward instead of kept: it is in
 // registers anyway and would cost as much memory as x.
 // Sums (mean of squares, weight gradients) in 32 bits; one rounding to the output's type at the end.
-// Measured: 32 x 1025 tokens, 12 + 12 heads of 64, bf16: forward 38 us (201 MB, 5.3 TB/s), backward 73 us (302 MB, 4.1 TB/s) + 4 us for the
+// Measured: 32 x 1025 tokens, 12 + 12 heads of 64, bf16: forward 38 us (201 MB, 5.3 TB/s), backward 69 us (302 MB, 4.4 TB/s) + 4 us for the
 // weights' sums; 2 x 1571 tokens, 16 + 4 heads of 128, fp32, interleaved: forward 13 us (64 MB, 4.9 TB/s; 19 us before the threads of a head took
 // its 16-byte pieces in turn).  A copy of 2 GiB reaches 4.9 TB/s.
 #include <hip/hip_fp16.h>
@@ -113,12 +113,12 @@ template <bool IL, typename T> constexpr int kPer = (IL ? 8 : 16) / static_cast<
 template <bool IL, typename T> __device__ __forceinline__ int pair_of(int i, int j, int tph) { return kPer<IL, T> * (j + i / kPer<IL, T> * tph) + i % kPer<IL, T>; }
 template <typename T> struct Pairs { typename Io<T>::Raw lo, hi; };
 template <bool IL, typename T>
-__device__ __forceinline__ Pairs<T> raw_pairs(const T* head, int j, int tph) {
+__device__ __forceinline__ Pairs<T> raw_pairs(const T* head, int j, int tph, int d2) {
   if constexpr (sizeof(T) == 4) {
     const float4* p = reinterpret_cast<const float4*>(head) + j;
     return Pairs<T>{{p[0], p[tph]}, {p[2 * tph], p[3 * tph]}};         // (the second members begin at d / 2 = 2 tph pieces)
   } else {
-    return Pairs<T>{Io<T>::raw8(head + 8 * j), Io<T>::raw8(head + 8 * (j + tph))};
+    return Pairs<T>{Io<T>::raw8(head + 8 * j), Io<T>::raw8(head + (IL ? 8 * (j + tph) : 8 * j + d2))};
   }
 }
 template <bool IL, typename T>
@@ -135,7 +135,7 @@ __device__ __forceinline__ void widen(const Pairs<T>& r, float* a, float* b) {
   }
 }
 template <bool IL, typename T>
-__device__ __forceinline__ void store_pairs(T* head, int j, int tph, const float* a, const float* b) {
+__device__ __forceinline__ void store_pairs(T* head, int j, int tph, int d2, const float* a, const float* b) {
   float t[16];
   if constexpr (IL) {
 #pragma unroll
@@ -151,7 +151,7 @@ __device__ __forceinline__ void store_pairs(T* head, int j, int tph, const float
     p[3 * tph] = make_float4(b[4], b[5], b[6], b[7]);
   } else {
     Io<T>::store8(head + 8 * j, a);
-    Io<T>::store8(head + 8 * (j + tph), b);
+    Io<T>::store8(head + (IL ? 8 * (j + tph) : 8 * j + d2), b);
   }
 }
 
@@ -244,8 +244,8 @@ __global__ __launch_bounds__(256, BWD ? 3 : 4) void qk_norm_rope_kernel(const Ro
     Item cur = item(g0);
     Pairs<T> rx, rg;
     auto load = [&](const Item& i) {
-      if (!BWD || a.norm) rx = raw_pairs<IL>(px + i.s * z.vx.b + i.t * z.vx.n + i.h * z.vx.h, jj, tph);
-      if constexpr (BWD) rg = raw_pairs<IL>(pg + i.s * z.vdy.b + i.t * z.vdy.n + i.h * z.vdy.h, jj, tph);
+      if (!BWD || a.norm) rx = raw_pairs<IL>(px + i.s * z.vx.b + i.t * z.vx.n + i.h * z.vx.h, jj, tph, d / 2);
+      if constexpr (BWD) rg = raw_pairs<IL>(pg + i.s * z.vdy.b + i.t * z.vdy.n + i.h * z.vdy.h, jj, tph, d / 2);
     };
     if (items > 0) load(cur);
     if (a.pos) {
@@ -327,7 +327,7 @@ __global__ __launch_bounds__(256, BWD ? 3 : 4) void qk_norm_rope_kernel(const Ro
           gb[i] = gb[i] > 65504.f ? 65504.f : gb[i] < -65504.f ? -65504.f : gb[i];
         }
       }
-      if (live) store_pairs<IL>(po + now.s * z.vo.b + now.t * z.vo.n + now.h * z.vo.h, j, tph, ga, gb);
+      if (live) store_pairs<IL>(po + now.s * z.vo.b + now.t * z.vo.n + now.h * z.vo.h, j, tph, d / 2, ga, gb);
     }
   }
   if constexpr (BWD) {
