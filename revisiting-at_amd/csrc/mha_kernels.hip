@@ -129,7 +129,7 @@ struct MhaArgs {
   int64_t cs_b;                                  // pairs between the samples' (0: shared)
   float eps;
   int32_t norm, il;
-  const float2* range;                           // kScaled: [B][H][pieces] largest |v| and |dout| of a row
+  const float2* range;                           // kScaled: [B][H][pieces] largest sizes (row_size) of v's and dout's rows
   int32_t pieces;
 };
 
@@ -275,13 +275,23 @@ __device__ __forceinline__ f32x16 first_terms(u32x2 terms, u32x2 ones) {
 }
 
 // dS in fp16 (kScaled): |dS| <= 2 |dout| |v|, and a power of two, carried by dout or v (in bf16, exactly) and D, brings that bound to 2^13 .. 2^14:
-// no dS overflows, and one 2^-27 of it still has all its bits.  (The exponents end at 2^+-100, so the powers and their inverses are normal.)
-__device__ __forceinline__ int scale_exponent(float bound) {
-  const int e = static_cast<int>((__float_as_uint(bound) >> 23) & 255u) - 127;
-  return min(max(13 - e, -100), 100);
+// no dS overflows, and one 2^-27 of it still has all its bits.
+// The size |x| of a row is the root of its sum of squares, which 32 bits hold for values of 2^-32 .. 2^32 only; beyond, the squares are formed behind
+// a power of two that the row's largest value chooses.  Sizes are kept behind 2^-4: 2^128 sqrt(128) is a number then, and bf16's smallest one still is.
+__device__ __forceinline__ float square_scale(float top) { return top >= 0x1p32f ? 0x1p-72f : top < 0x1p-32f ? 0x1p72f : 1.f; }
+__device__ __forceinline__ float row_size(float top, float squares) {
+  return sqrtf(squares) * (top >= 0x1p32f ? 0x1p68f : top < 0x1p-32f ? 0x1p-76f : 0x1p-4f);
+}
+// The exponent, from the exponents of the sizes (2 |x| |y| itself may be no number), for the power that x carries: it and its inverse are normal and
+// x times it is finite.  Where that leaves the bound below 2^13, dS times it is still above 2^-13, or the gradient below bf16's numbers.  A size of zero,
+// or one that is not finite, may give any power: dS is zero or not finite behind all of them.
+__device__ __forceinline__ int scale_exponent(float x, float y) {
+  const int ex = __builtin_amdgcn_frexp_expf(x), ey = __builtin_amdgcn_frexp_expf(y);
+  const bool carry = __builtin_amdgcn_frexp_mantf(x) * __builtin_amdgcn_frexp_mantf(y) >= 0.5f;
+  return max(min(13 - (ex + ey + (carry ? 8 : 7)), min(126, 123 - ex)), -126);
 }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
-// largest |v| and |dout| of a head
+// largest sizes of v's and dout's rows of a head
 __device__ __forceinline__ float2 range_of(const float2* range, int64_t bh, int pieces) {
   float2 r = range[bh * pieces];
   for (int p = 1; p < pieces; ++p) {
@@ -632,8 +642,8 @@ __device__ __forceinline__ void turn_back(const MhaArgs& a, const Turn& t, f32x1
     for (int r = 0; r < 16; ++r) g[db][r] = rn * fmaf(-x[db][r], dot, g[db][r]);
 }
 
-// Largest |v| and |dout| of the rows of a head, `pieces` workgroups each.  16 bytes per lane, D / 8 lanes a row; bound by memory (32 x 577 tokens,
-// 12 heads: 57 MB in 10 us).
+// Largest sizes (row_size) of v's and dout's rows of a head, `pieces` workgroups each.  16 bytes per lane, D / 8 lanes a row; bound by memory (32 x 577 tokens,
+// 12 heads: 57 MB in 11 us).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void mha_range_kernel(const MhaArgs a, float2* __restrict__ range) {
   constexpr int LANES = D / 8, ROWS = 256 / LANES;
@@ -646,10 +656,26 @@ __global__ __launch_bounds__(256) void mha_range_kernel(const MhaArgs a, float2*
     const uint16_t* p = (which ? a.dout : a.v) + b * view.b + h * view.h + c * 8;
     for (int i = piece * ROWS + threadIdx.x / LANES; i < a.Nk; i += a.pieces * ROWS) {
       const u32x4 x = *reinterpret_cast<const u32x4*>(p + i * view.n);
-      float s = 0.f;
+      float largest = 1.f;
+      auto squares = [&](float up) {                                   // (a row's lanes are here together)
+        float s = 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s = fmaf(T::lo(x[j]), T::lo(x[j]), fmaf(T::hi(x[j]), T::hi(x[j]), s));
-      for (int m = 1; m < LANES; m <<= 1) s += __shfl_xor(s, m, 64);   // (a row's lanes are here together)
+        for (int j = 0; j < 4; ++j) {
+          const float lo = T::lo(x[j]) * up, hi = T::hi(x[j]) * up;
+          s = fmaf(lo, lo, fmaf(hi, hi, s));
+        }
+        for (int m = 1; m < LANES; m <<= 1) s += __shfl_xor(s, m, 64);
+        return s;
+      };
+      float s = squares(1.f);
+      if (__any(!(s >= 0x1p-60f && s <= 0x1p60f))) {                   // (rows of zeros, too)
+        largest = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) largest = fmaxf(largest, fmaxf(fabsf(T::lo(x[j])), fabsf(T::hi(x[j]))));
+        for (int m = 1; m < LANES; m <<= 1) largest = fmaxf(largest, __shfl_xor(largest, m, 64));
+        s = squares(square_scale(largest));
+      }
+      s = row_size(largest, s);
       top[which] = s > top[which] || s != s ? s : top[which];
     }
     for (int m = LANES; m < 64; m <<= 1) top[which] = fmaxf(top[which], __shfl_xor(top[which], m, 64));
@@ -659,7 +685,7 @@ __global__ __launch_bounds__(256) void mha_range_kernel(const MhaArgs a, float2*
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int k = 1; k < 4; ++k) { top[0] = fmaxf(top[0], red[k].x); top[1] = fmaxf(top[1], red[k].y); }
-    range[blockIdx.x] = make_float2(sqrtf(top[0]), sqrtf(top[1]));
+    range[blockIdx.x] = make_float2(top[0], top[1]);
   }
 }
 
@@ -679,7 +705,7 @@ __global__ __launch_bounds__(256, 2) void mha_dq_kernel(const MhaArgs a) {
     const uint16_t* pq = a.q + w.b * a.vq.b + h * a.vq.h + i * a.vq.n + half * 8;
     const uint16_t* pg = a.dout + w.b * a.vdo.b + h * a.vdo.h + i * a.vdo.n + half * 8;
     const uint16_t* po = a.out + w.b * a.vo.b + h * a.vo.h + i * a.vo.n + half * 8;
-    float part = 0.f, size = 0.f;
+    float part = 0.f;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       qf[ks] = gf[ks] = u32x4{0, 0, 0, 0};
@@ -689,17 +715,27 @@ __global__ __launch_bounds__(256, 2) void mha_dq_kernel(const MhaArgs a) {
         const u32x4 of = *reinterpret_cast<const u32x4*>(po + ks * 16);
 #pragma unroll
         for (int j = 0; j < 4; ++j) part = fmaf(T::lo(gf[ks][j]), T::lo(of[j]), fmaf(T::hi(gf[ks][j]), T::hi(of[j]), part));
-        if constexpr (T::kScaled) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) size = fmaf(T::lo(gf[ks][j]), T::lo(gf[ks][j]), fmaf(T::hi(gf[ks][j]), T::hi(gf[ks][j]), size));
-        }
       }
     }
     dd = both_halves_sum(part);
     lse2 = live ? a.lse[at] * kLog2e : INFINITY;                       // exp2(s - inf) = 0
     if (w.split == 0 && half == 0 && w.tok < a.Nq) a.dvec[at] = dd;
     if constexpr (T::kScaled) {                  // a row's own scale
-      const int e = scale_exponent(2.f * sqrtf(both_halves_sum(size)) * range_of(a.range, w.b * a.H + h, a.pieces).x);
+      float largest = 0.f, squares = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) largest = fmaxf(largest, fmaxf(fabsf(T::lo(gf[ks][j])), fabsf(T::hi(gf[ks][j]))));
+      largest = both_halves_max(largest);
+      const float up = square_scale(largest);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float lo = T::lo(gf[ks][j]) * up, hi = T::hi(gf[ks][j]) * up;
+          squares = fmaf(lo, lo, fmaf(hi, hi, squares));
+        }
+      const int e = scale_exponent(row_size(largest, both_halves_sum(squares)), range_of(a.range, w.b * a.H + h, a.pieces).x);
       scale_bf16(gf, power_of_two(e));
       dd *= power_of_two(e);
       mul *= power_of_two(-e);
@@ -870,7 +906,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void mha_dkv_kernel(const Mha
   float dk_mul = a.scale, d_mul = -1.f;
   if constexpr (T::kScaled) {                    // one scale for the head: a key's dk sums over rows
     const float2 r = range_of(a.range, b * a.H + hk, a.pieces);
-    const int e = scale_exponent(2.f * r.x * r.y);
+    const int e = scale_exponent(r.x, r.y);
     scale_bf16(vf, power_of_two(e));
     d_mul = -power_of_two(e);
     dk_mul *= power_of_two(-e);

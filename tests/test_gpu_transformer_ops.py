@@ -643,3 +643,46 @@ def test_uses_of_autograd(R):
     with R.ops.input_grad_only():                                                   # the attack's backward: the input's gradient, no weights'
         gx, gw = torch.autograd.grad(R.ops.attention_rope(x, 2, None, w, w, pos, inv), (x, w), do.flatten(2), allow_unused=True)
     assert gw is None and torch.equal(gx, torch.autograd.grad(R.ops.attention_rope(qkv, 2, None, w, w, pos, inv), qkv, do.flatten(2))[0])
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_rope_with_gradients_whose_squares_no_fp32_holds(R, d):
+    """The power of two that dS is formed behind: gradients and values whose sums of squares would vanish or overflow in 32 bits give the same bits,
+    scaled; so do the weights' gradients."""
+    B, N, H = 2, 150, 2
+    g = torch.Generator().manual_seed(19)
+    qkv = torch.randn(B, N, 3 * H * d, generator=g).to(torch.bfloat16).cuda()
+    dout = torch.randn(B, N, H * d, generator=g).to(torch.bfloat16).cuda()
+    w = (1 + 0.1 * torch.randn(d, generator=g)).cuda()
+
+    def run(qkv, dout):
+        x, wq, wk = qkv.clone().requires_grad_(), w.clone().requires_grad_(), w.clone().requires_grad_()
+        return torch.autograd.grad(R.ops.attention_rope(x, H, None, wq, wk), (x, wq, wk), dout)
+    want = run(qkv, dout)
+    C = H * d
+    for k in (-75, -77, -79, -80, -82, -86, -90, 64, 80):
+        up = 2.0 ** k
+        for a, b in zip(run(qkv, dout * up), want):
+            assert torch.equal(a, b * up), k
+        big = qkv.clone()
+        big[..., 2 * C:] *= up                                                      # dq, dk and the weights' follow v, dv does not
+        gx, gq, gk = run(big, dout)
+        assert torch.equal(gx[..., :2 * C], want[0][..., :2 * C] * up) and torch.equal(gx[..., 2 * C:], want[0][..., 2 * C:]), k
+        assert torch.equal(gq, want[1] * up) and torch.equal(gk, want[2] * up), k
+        gx, gq, gk = run(big, dout * (1 / up))                                      # and both: their product is what it was
+        assert torch.equal(gx[..., :2 * C], want[0][..., :2 * C]) and torch.equal(gx[..., 2 * C:], want[0][..., 2 * C:] * (1 / up)), k
+        assert torch.equal(gq, want[1]) and torch.equal(gk, want[2]), k
+    # one sample's gradient tiny or zero, or one row's: the others keep their bits (dq), nothing becomes infinite
+    for up in (2.0 ** -80, 0.0):
+        one = dout.clone()
+        one[1] *= up
+        gx = run(qkv, one)[0]
+        assert torch.equal(gx[0], want[0][0]) and torch.equal(gx[1], want[0][1] * up)
+        one = dout.clone()
+        one[:, 7] *= up
+        gx, gq, gk = run(qkv, one)
+        assert all(bool(torch.isfinite(t).all()) for t in (gx, gq, gk))
+        rest = [i for i in range(N) if i != 7]
+        assert torch.equal(gx[:, 7, :C], want[0][:, 7, :C] * up) and torch.equal(gx[:, rest, :C], want[0][:, rest, :C])
+    for a, b in zip(run(qkv, dout * 2.0 ** -110), want):                            # down to bf16's smallest normal number
+        assert bool(((a.double() - b.double() * 2.0 ** -110).abs() <= 2.0 ** -8 * b.double().abs() * 2.0 ** -110 + 2.0 ** -126).all())
