@@ -90,7 +90,9 @@ class FusedAdamW(torch.optim.Optimizer):
     scale for every 256 elements; the second moment as its root), the others in 32 bits.
 
     Step counters live on the device and ``lr`` may be a device tensor, so a step can be captured into a hipGraph after one eager step (or
-    ``load_state_dict``) has built the tables.  Parameters without a gradient are left alone.  ``state_dict`` has torch's layout: ``step`` and
+    ``load_state_dict``) has built the tables.  ``load_state_dict`` writes into the buffers, counters and device learning rates that are there, so
+    a captured step goes on from what was loaded; a parameter that moves, changes its type or joins needs new tables, and with them a new capture.
+    Parameters without a gradient are left alone.  ``state_dict`` has torch's layout: ``step`` and
     ``exp_avg`` / ``exp_avg_sq`` (torch's AdamW loads and is loaded), or ``exp_avg_codes``, ``exp_avg_scales``, ``exp_avg_sq_codes``,
     ``exp_avg_sq_scales`` where the moments have 8 bits.  ``moments()`` gives all moments as numbers.  The optimizer steps on the stream that
     is current; its buffers belong to one stream at a time, as the parameters do."""
@@ -102,7 +104,7 @@ class FusedAdamW(torch.optim.Optimizer):
             raise ValueError(f"FusedAdamW: lr={lr!r}")
         if not 0.0 <= betas[0] < 1.0 or not 0.0 <= betas[1] < 1.0 or not eps >= 0.0 or not weight_decay >= 0.0:
             raise ValueError(f"FusedAdamW: betas={betas!r}, eps={eps!r}, weight_decay={weight_decay!r}")
-        self.state_bits, self._plan = state_bits, None
+        self.state_bits, self._plan, self._captured = state_bits, None, []
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
 
     def add_param_group(self, group):
@@ -142,14 +144,14 @@ class FusedAdamW(torch.optim.Optimizer):
         old = {p: dict(self.state[p]) for p in params if self.state.get(p)}
         with ops._on_device(params[0]), torch.no_grad():
             plan = _Plan(params, [i for i, g in enumerate(self.param_groups) for _ in g["params"]], [self._bits(p) for p in params])
-            pairs = []
-            for i, (p, step) in enumerate(zip(params, plan.steps.unbind())):
-                self.state[p] = {"step": step, **plan.moments(i, p)}
-                if p in old:
-                    pairs += [(t, old[p][k]) for k, t in self.state[p].items()]
-            _copy(pairs)
-        self._plan, self._stale = plan, False
+            self._adopt(plan, params)
+            _copy([(t, old[p][k]) for p in params if p in old for k, t in self.state[p].items()])
         return plan
+
+    def _adopt(self, plan, params):
+        for i, (p, step) in enumerate(zip(params, plan.steps.unbind())):
+            self.state[p] = {"step": step, **plan.moments(i, p)}
+        self._plan, self._stale = plan, False
 
     def _ready(self, params):
         plan = self._plan
@@ -165,6 +167,8 @@ class FusedAdamW(torch.optim.Optimizer):
                 loss = closure()
         params = self._params()
         plan = self._ready(params)
+        if torch.cuda.is_current_stream_capturing() and plan not in self._captured:
+            self._captured.append(plan)                            # replays write into its buffers, also after tables have been built anew
         kept = plan.layout.gradients(params, ctypes.addressof(plan.grads))                     # copies that live until the launch
         n = len(self.param_groups)
         hyper, lr_dev = (ctypes.c_double * (5 * n))(), (ctypes.c_void_p * n)()
@@ -182,7 +186,8 @@ class FusedAdamW(torch.optim.Optimizer):
         lib = _lib.load()
         with ops._on_device(params[0]):
             for first, count, table, chunks in plan.runs:
-                _lib.check(lib.cnx_adamw_step(table.data_ptr(), chunks.data_ptr(), chunks.shape[0], ctypes.byref(plan.grads, 8 * first), count, hyper, lr_dev, n, plan.steps.data_ptr(), plan.coef.data_ptr() + 32 * first, _lib.ptr(plan.m),
+                _lib.check(lib.cnx_adamw_step(table.data_ptr(), chunks.data_ptr(), chunks.shape[0], ctypes.byref(plan.grads, 8 * first), count,
+                                              hyper, lr_dev, n, plan.steps.data_ptr(), plan.coef.data_ptr() + 32 * first, _lib.ptr(plan.m),
                                               _lib.ptr(plan.v), _lib.ptr(plan.mc), _lib.ptr(plan.ms), _lib.ptr(plan.vc), _lib.ptr(plan.vs),
                                               ops._stream()), "cnx_adamw_step")
         del kept
@@ -231,10 +236,32 @@ class FusedAdamW(torch.optim.Optimizer):
             for k, shape in shapes.items():
                 if tuple(given[k].shape) != shape:
                     raise ValueError(f"FusedAdamW: {k} of parameter {i} is {tuple(given[k].shape)}, not {shape}")
+        plan = None if self._plan is None or self._stale or not self._plan.layout.matches(params) else self._plan
+        if plan is not None and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("FusedAdamW: load_state_dict has to run outside a graph capture")
+        rates = [g["lr"] for g in self.param_groups]
         super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})     # checks and takes the groups
-        self._build()
+        for g, lr in zip(self.param_groups, rates):
+            if isinstance(lr, torch.Tensor) and lr.is_cuda:                                    # (a captured step reads this one)
+                g["lr"] = lr.copy_(torch.as_tensor(g["lr"]).reshape(lr.shape))
+        if plan is None:
+            self._build()
+        else:
+            self._adopt(plan, params)
+        mine = {t.untyped_storage().data_ptr() for s in self.state.values() for t in s.values()}
+        pairs, never = [], []
+        for p, at in zip(params, ids):
+            given = state_dict["state"].get(at) or {}
+            for k, t in self.state[p].items():
+                if k in given:
+                    x = torch.as_tensor(given[k])
+                    pairs.append((t, x.clone() if x.untyped_storage().data_ptr() in mine else x))
+                else:
+                    never.append(t)
         with ops._on_device(params[0]):
-            _copy([(self.state[p][k], x) for p, at in zip(params, ids) for k, x in (state_dict["state"].get(at) or {}).items() if k in self.state[p]])
+            _copy(pairs)
+            if never:
+                torch._foreach_zero_(never)
 
     def __getstate__(self):
         return {**super().__getstate__(), "state_bits": self.state_bits}
@@ -242,3 +269,4 @@ class FusedAdamW(torch.optim.Optimizer):
     def __setstate__(self, state):
         super().__setstate__(state)
         self._plan, self._stale = None, True
+        self.__dict__.setdefault("_captured", [])

@@ -470,3 +470,47 @@ def test_vit_options_leave_the_plain_model_alone(R):
     assert extra == {f"blocks.{i}.attn.{n}_norm.weight" for i in range(12) for n in "qk"} and not set(a.state_dict()) - set(b.state_dict())
     with pytest.raises(ValueError):
         A.get_new_model("convnext_tiny", pretrained=False, rope=True)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_loading_a_state_keeps_the_buffers_of_a_captured_step(R, bits):
+    """load_state_dict writes into the moments, counters and learning rates that are there, so that a captured step goes on from the loaded state."""
+    def build():
+        ps, g = make([(4096 + 5,), (64, 100), (7,)], torch.float32, 5)
+        set_grads(ps, g)
+        opt = R.FusedAdamW(ps, lr=torch.tensor(LR, device="cuda"), betas=BETAS, state_bits=bits)
+        opt.step()
+        return ps, opt
+    (ps, opt), (qs, eager) = build(), build()
+    saved, start = copy.deepcopy(opt.state_dict()), [p.detach().clone() for p in ps]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    places = lambda: [t.data_ptr() for p in ps for k, t in opt.state[p].items() if t.is_cuda] + [opt.param_groups[0]["lr"].data_ptr()]      # noqa: E731
+    before, table = places(), opt._plan
+    own = opt.state_dict()
+    for _ in range(2):
+        graph.replay()
+        eager.step()
+    saved["param_groups"][0]["lr"] = 0.5 * LR
+    for which, o, params in ((0, opt, ps), (1, eager, qs)):
+        o.load_state_dict(saved)
+        with torch.no_grad():
+            for p, x in zip(params, start):
+                p.copy_(x)
+    # (a graph is only replayed where all it reads and writes is where it was)
+    assert places() == before and opt._plan is table and float(opt.param_groups[0]["lr"]) == float(torch.tensor(0.5 * LR))
+    for k in range(3):
+        graph.replay()
+        eager.step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(ps, qs))
+        assert float(opt.state[ps[0]]["step"]) == float(eager.state[qs[0]]["step"]) == k + 2
+    now = [{k: t.clone() for k, t in opt.state[p].items()} for p in ps]
+    opt.load_state_dict(own)                                                        # its own buffers: nothing changes
+    assert all(torch.equal(opt.state[p][k], t) for p, s in zip(ps, now) for k, t in s.items())
+    partial = copy.deepcopy(saved)
+    del partial["state"][1]                                                         # a parameter that was never stepped
+    opt.load_state_dict(partial)
+    assert not any(bool(t.any()) for k, t in opt.state[ps[1]].items() if not k.endswith("order")) and float(opt.state[ps[0]]["step"]) == 1
+    assert places() == before
