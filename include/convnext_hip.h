@@ -341,8 +341,8 @@ int cnx_attention_bwd(const void* qkv, const void* out, const void* dout, const 
  * scratch, 8 * n_tensors floats.  m, v: 32-bit moments; m_codes / v_codes (a byte per element), m_scales / v_scales (fp32 per block): 8-bit
  * ones - a set that no tensor of the table uses may be NULL.  At most CNX_ADAMW_TENSORS tensors and CNX_ADAMW_GROUPS groups a call.
  * 8-bit moments: code * scale of the block; m: sign bit and 7 bits, v: its root in 8 bits; code c > 0 is the fp32 number whose pattern is
- * (c + 889) << 20 (m) or (c + 1777) << 19 (root of v), 1.0 the largest, 0 is zero; rounded to nearest even; a root above zero is never
- * rounded to zero. */
+ * (c + 889) << 20 (m) or (c + 1777) << 19 (root of v), 1.0 the largest, 0 is zero; rounded to nearest even, below code 1 to zero from half a
+ * step of its binade beneath it on; a root above zero is never rounded to zero. */
 #define CNX_ADAMW_BLOCK 256
 #define CNX_ADAMW_CHUNK 4096
 #define CNX_ADAMW_TENSORS 440

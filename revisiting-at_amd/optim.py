@@ -6,6 +6,7 @@ keep 2 bytes instead of 8 in memory."""
 from __future__ import annotations
 
 import ctypes
+import warnings
 
 import numpy as np
 import torch
@@ -31,6 +32,64 @@ def _dense(p):
             return False
         need *= size
     return True
+
+
+def _order(p):
+    """Dimensions of more than one element, from the slowest to the fastest; empty where that is their own order."""
+    dims = sorted((d for d, n in enumerate(p.shape) if n > 1), key=lambda d: -p.stride(d))
+    return () if dims == sorted(dims) else tuple(dims)
+
+
+# 8-bit moments outside the kernel (csrc/optim_kernels.hip): mantissa bits, code of 1.0, sign bit
+_CODES = {"exp_avg": (3, 127, 128), "exp_avg_sq": (4, 255, 0)}
+
+
+def _decode(codes, scales, kind):
+    """The numbers that 8-bit moments stand for (of the second moment: its root)."""
+    mant, top, sign = _CODES[kind]
+    c = codes.to(torch.int32)
+    x = ((c & top) + ((0x3f800000 >> (23 - mant)) - top) << (23 - mant)).view(torch.float32)
+    x = torch.where(c & top > 0, x, 0.0)
+    return (torch.where(c & sign > 0, -x, x).view(-1, BLOCK) * scales.unsqueeze(1)).view(-1)
+
+
+def _encode(x, kind):
+    """(codes, scales) of whole blocks of numbers, rounded as the kernel does."""
+    mant, top, sign = _CODES[kind]
+    shift = 23 - mant
+    scales = x.view(torch.int32).bitwise_and(0x7fffffff).view(-1, BLOCK).amax(1).view(torch.float32)       # (patterns: a NaN is the largest)
+    scales = torch.where(scales < torch.finfo(torch.float32).tiny, 0.0, scales)
+    inv = torch.where(scales > 0, 1 / scales, 0.0).unsqueeze(1)
+    b = (x.abs().view(-1, BLOCK) * inv).view(-1).view(torch.int32) & 0x7fffffff
+    c = ((b + ((1 << (shift - 1)) - 1) + ((b >> shift) & 1) >> shift) - ((0x3f800000 >> shift) - top)).clamp_(0, top)
+    if sign:
+        c |= torch.where(x < 0, sign, 0).to(torch.int32)
+    else:
+        some = (x.view(-1, BLOCK) > 0) & (scales > 0).unsqueeze(1)
+        c = torch.where(some.view(-1) & (c == 0), 1, c)
+    return c.to(torch.uint8), scales
+
+
+def _reorder(state, p):
+    """The four 8-bit tensors of a state for the memory order of ``p``: where it was another one, blocks get other members, and the numbers are
+    rounded again to the new blocks' scales."""
+    old = state.get("exp_avg_order")
+    old = _order(p) if old is None else tuple(torch.as_tensor(old).tolist())
+    if old == _order(p):
+        return state
+    dims = old or tuple(d for d, n in enumerate(p.shape) if n > 1)
+    strides, step = [0] * p.dim(), 1
+    for d in reversed(dims):
+        strides[d] = step
+        step *= p.shape[d]
+    n, out = p.numel(), dict(state)
+    for kind in _CODES:
+        codes, scales = (torch.as_tensor(state[f"{kind}_{k}"]) for k in ("codes", "scales"))
+        was = _decode(codes, scales, kind)
+        now = torch.zeros_like(was)
+        now.as_strided(p.shape, p.stride()).copy_(was[:n].as_strided(p.shape, strides))
+        out[f"{kind}_codes"], out[f"{kind}_scales"] = _encode(now, kind)
+    return out
 
 
 def _copy(pairs):
@@ -81,7 +140,8 @@ class _Plan:
         a, e = self.at[i], self.at[i] + -(-p.numel() // BLOCK) * BLOCK
         if self.bits[i] == 32:
             return {k: t.as_strided(p.shape, p.stride(), a) for k, t in zip(_KEYS[32], (self.m, self.v))}
-        return dict(zip(_KEYS[8], (self.mc[a:e], self.ms[a // BLOCK:e // BLOCK], self.vc[a:e], self.vs[a // BLOCK:e // BLOCK])))
+        return {**dict(zip(_KEYS[8], (self.mc[a:e], self.ms[a // BLOCK:e // BLOCK], self.vc[a:e], self.vs[a // BLOCK:e // BLOCK]))),
+                "exp_avg_order": torch.tensor(_order(p), dtype=torch.int64)}
 
 
 class FusedAdamW(torch.optim.Optimizer):
@@ -94,7 +154,8 @@ class FusedAdamW(torch.optim.Optimizer):
     a captured step goes on from what was loaded; a parameter that moves, changes its type or joins needs new tables, and with them a new capture.
     Parameters without a gradient are left alone.  ``state_dict`` has torch's layout: ``step`` and
     ``exp_avg`` / ``exp_avg_sq`` (torch's AdamW loads and is loaded), or ``exp_avg_codes``, ``exp_avg_scales``, ``exp_avg_sq_codes``,
-    ``exp_avg_sq_scales`` where the moments have 8 bits.  ``moments()`` gives all moments as numbers.  The optimizer steps on the stream that
+    ``exp_avg_sq_scales`` where the moments have 8 bits; those lie in the memory order of their parameter, which ``exp_avg_order`` tells (a state
+    without it is taken to be in the present one), and are brought into another order's blocks when that changes.  ``moments()`` gives all moments as numbers.  The optimizer steps on the stream that
     is current; its buffers belong to one stream at a time, as the parameters do."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32):
@@ -145,7 +206,8 @@ class FusedAdamW(torch.optim.Optimizer):
         with ops._on_device(params[0]), torch.no_grad():
             plan = _Plan(params, [i for i, g in enumerate(self.param_groups) for _ in g["params"]], [self._bits(p) for p in params])
             self._adopt(plan, params)
-            _copy([(t, old[p][k]) for p in params if p in old for k, t in self.state[p].items()])
+            old = {p: _reorder(s, p) if "exp_avg_codes" in s else s for p, s in old.items()}
+            _copy([(t, old[p][k]) for p in params if p in old for k, t in self.state[p].items() if k != "exp_avg_order"])
         return plan
 
     def _adopt(self, plan, params):
@@ -236,6 +298,13 @@ class FusedAdamW(torch.optim.Optimizer):
             for k, shape in shapes.items():
                 if tuple(given[k].shape) != shape:
                     raise ValueError(f"FusedAdamW: {k} of parameter {i} is {tuple(given[k].shape)}, not {shape}")
+            if bits == 8 and "exp_avg_order" not in given:
+                if sum(n > 1 for n in p.shape) > 2:                                            # (memory formats)
+                    warnings.warn(f"FusedAdamW: the 8-bit state of parameter {i} does not tell its memory order; it is taken to be the parameter's")
+            elif bits == 8:
+                order = torch.as_tensor(given["exp_avg_order"]).tolist()
+                if order and sorted(order) != [d for d, n in enumerate(p.shape) if n > 1]:
+                    raise ValueError(f"FusedAdamW: exp_avg_order of parameter {i} is {order} for {tuple(p.shape)}")
         plan = None if self._plan is None or self._stale or not self._plan.layout.matches(params) else self._plan
         if plan is not None and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("FusedAdamW: load_state_dict has to run outside a graph capture")
@@ -252,7 +321,11 @@ class FusedAdamW(torch.optim.Optimizer):
         pairs, never = [], []
         for p, at in zip(params, ids):
             given = state_dict["state"].get(at) or {}
+            if "exp_avg_codes" in given:
+                given = _reorder(given, p)
             for k, t in self.state[p].items():
+                if k == "exp_avg_order":
+                    continue
                 if k in given:
                     x = torch.as_tensor(given[k])
                     pairs.append((t, x.clone() if x.untyped_storage().data_ptr() in mine else x))

@@ -514,3 +514,72 @@ def test_loading_a_state_keeps_the_buffers_of_a_captured_step(R, bits):
     opt.load_state_dict(partial)
     assert not any(bool(t.any()) for k, t in opt.state[ps[1]].items() if not k.endswith("order")) and float(opt.state[ps[0]]["step"]) == 1
     assert places() == before
+
+
+def logical(opt, p):
+    """exp_avg, root of exp_avg_sq of one parameter as numbers, in its logical order."""
+    st = opt.state[p]
+    if "exp_avg" in st:
+        return st["exp_avg"].double().cpu(), st["exp_avg_sq"].double().cpu().sqrt()
+    n = p.numel()
+    mc, vc = (st[k].cpu().numpy().astype(np.int64) for k in ("exp_avg_codes", "exp_avg_sq_codes"))
+    m = VALUES["m"][mc & 127] * np.where(mc > 127, -1, 1) * st["exp_avg_scales"].cpu().numpy().repeat(256)
+    r = VALUES["v"][vc] * st["exp_avg_sq_scales"].cpu().numpy().repeat(256)
+    return tuple(torch.from_numpy(x[:n]).as_strided(p.shape, p.stride()).contiguous() for x in (m, r))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_moments_follow_the_memory_order_of_their_parameter(R, bits):
+    """Contiguous <-> channels_last, in place and through a state dict: the moments stay with their elements."""
+    for first, then in ((torch.contiguous_format, torch.channels_last), (torch.channels_last, torch.contiguous_format)):
+        g = torch.Generator().manual_seed(31)
+        make_one = lambda fmt: torch.nn.Parameter(torch.randn(24, 20, 3, 3, generator=torch.Generator().manual_seed(1)).cuda().to(memory_format=fmt))  # noqa: E731
+        grad = (torch.randn(24, 20, 3, 3, generator=g) * 10.0 ** (torch.rand(24, 20, 3, 3, generator=g) * 3 - 3)).cuda()
+        p = make_one(first)
+        opt = R.FusedAdamW([p], lr=LR, betas=BETAS, state_bits=bits)
+        p.grad = grad.to(memory_format=first)
+        opt.step()
+        m, r = logical(opt, p)
+        sd = copy.deepcopy(opt.state_dict())
+        q = make_one(then)                                                          # through a state dict
+        other = R.FusedAdamW([q], lr=LR, betas=BETAS, state_bits=bits)
+        other.load_state_dict(sd)
+        p.grad = None
+        p.data = p.data.to(memory_format=then)                                      # in place
+        opt.state_dict()
+        for a, b in ((opt, p), (other, q)):
+            m2, r2 = logical(a, b)
+            if bits == 32:
+                assert torch.equal(m2, m) and torch.equal(r2, r)
+            else:
+                # a block has other members and with them another scale: half a step of a code, a 16th (32nd) of the value at most; of m below the smallest
+                # code, 1.25 2^-16 of the scale, zero from half a step beneath it on (1.1875 2^-16); a root above zero at least its smallest, 1.125 2^-16
+                sm, sr = (a.state[b][k].max().item() for k in ("exp_avg_scales", "exp_avg_sq_scales"))
+                assert bool(((m2 - m).abs() <= m.abs() * 2.0 ** -4 * 1.01 + sm * 1.1875 * 1.01 * 2.0 ** -16).all())
+                assert bool(((r2 - r).abs() <= r * 2.0 ** -5 * 1.01 + sr * 1.125 * 1.01 * 2.0 ** -16).all())
+                assert bool(((r2 > 0) == (r > 0)).all())
+        assert all(torch.equal(x, y) for x, y in zip(logical(opt, p), logical(other, q)))
+        q.data.copy_(p.data)
+        for x in (p, q):
+            x.grad = grad.to(memory_format=then)
+        opt.step(), other.step()
+        assert torch.equal(p, q)
+        back = R.FusedAdamW([make_one(then)], state_bits=bits)                      # the same order: the same bits
+        back.load_state_dict(opt.state_dict())
+        s, t = opt.state[p], back.state[back.param_groups[0]["params"][0]]
+        assert all(torch.equal(s[k], t[k]) for k in s)
+
+
+def test_memory_orders_of_loaded_states(R):
+    p = torch.nn.Parameter(torch.ones(32, 16, 3, 3, device="cuda"))
+    p.grad = torch.ones_like(p)
+    opt = R.FusedAdamW([p], state_bits=8, betas=BETAS)
+    opt.step()
+    sd = copy.deepcopy(opt.state_dict())
+    sd["state"][0]["exp_avg_order"] = torch.tensor([0, 2, 1])
+    with pytest.raises(ValueError, match="exp_avg_order"):
+        opt.load_state_dict(sd)
+    del sd["state"][0]["exp_avg_order"]                                             # taken to be in the parameter's
+    with pytest.warns(UserWarning, match="memory order"):
+        opt.load_state_dict(sd)
+    assert float(opt.state[p]["step"]) == 1 and bool((opt.state[p]["exp_avg_codes"] == 127).all())
