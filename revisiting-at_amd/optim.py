@@ -110,6 +110,7 @@ class _Plan:
     def __init__(self, params, groups, bits):
         dev = params[0].device
         self.layout = ops._host().Layout(params)
+        self.groups = groups                                       # of each parameter
         self.grads = (ctypes.c_void_p * len(params))()
         self.bits = bits
         self.at, size = [], {32: 0, 8: 0}
@@ -178,8 +179,16 @@ class FusedAdamW(torch.optim.Optimizer):
     def _bits(self, p):
         return 8 if self.state_bits == 8 and p.numel() >= SMALL else 32
 
+    def _shapes(self, p):
+        """Names and shapes of a parameter's moments."""
+        bits, blocks = self._bits(p), -(-p.numel() // BLOCK)
+        return dict(zip(_KEYS[bits], [tuple(p.shape)] * 2 if bits == 32 else [(blocks * BLOCK,), (blocks,)] * 2))
+
     def _params(self):
         return [p for g in self.param_groups for p in g["params"]]
+
+    def _groups(self):
+        return [i for i, g in enumerate(self.param_groups) for _ in g["params"]]
 
     def _build(self):
         """Tables and buffers for the parameters as they are now; moments that exist are kept."""
@@ -204,7 +213,7 @@ class FusedAdamW(torch.optim.Optimizer):
             raise RuntimeError("FusedAdamW: the first step (and one after parameters were moved or added) has to run outside a graph capture")
         old = {p: dict(self.state[p]) for p in params if self.state.get(p)}
         with ops._on_device(params[0]), torch.no_grad():
-            plan = _Plan(params, [i for i, g in enumerate(self.param_groups) for _ in g["params"]], [self._bits(p) for p in params])
+            plan = _Plan(params, self._groups(), [self._bits(p) for p in params])
             self._adopt(plan, params)
             old = {p: _reorder(s, p) if "exp_avg_codes" in s else s for p, s in old.items()}
             _copy([(t, old[p][k]) for p in params if p in old for k, t in self.state[p].items() if k != "exp_avg_order"])
@@ -217,7 +226,7 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def _ready(self, params):
         plan = self._plan
-        if plan is None or self._stale or not plan.layout.matches(params):
+        if plan is None or self._stale or plan.groups != self._groups() or not plan.layout.matches(params):
             plan = self._build()
         return plan
 
@@ -290,8 +299,7 @@ class FusedAdamW(torch.optim.Optimizer):
             given = state_dict["state"].get(at)
             if given is None:                                                                  # never stepped
                 continue
-            bits, blocks = self._bits(p), -(-p.numel() // BLOCK)
-            shapes = dict(zip(_KEYS[bits], [tuple(p.shape)] * 2 if bits == 32 else [(blocks * BLOCK,), (blocks,)] * 2))
+            bits, shapes = self._bits(p), self._shapes(p)
             if {"step", *shapes} - set(given):
                 raise ValueError(f"FusedAdamW: the state of parameter {i} lacks {sorted({'step', *shapes} - set(given))} (state_bits="
                                  f"{self.state_bits} keeps its moments in {bits} bits)")
@@ -305,7 +313,7 @@ class FusedAdamW(torch.optim.Optimizer):
                 order = torch.as_tensor(given["exp_avg_order"]).tolist()
                 if order and sorted(order) != [d for d, n in enumerate(p.shape) if n > 1]:
                     raise ValueError(f"FusedAdamW: exp_avg_order of parameter {i} is {order} for {tuple(p.shape)}")
-        plan = None if self._plan is None or self._stale or not self._plan.layout.matches(params) else self._plan
+        plan = None if self._plan is None or self._stale or self._plan.groups != self._groups() or not self._plan.layout.matches(params) else self._plan
         if plan is not None and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("FusedAdamW: load_state_dict has to run outside a graph capture")
         rates = [g["lr"] for g in self.param_groups]

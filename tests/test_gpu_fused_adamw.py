@@ -583,3 +583,23 @@ def test_memory_orders_of_loaded_states(R):
     with pytest.warns(UserWarning, match="memory order"):
         opt.load_state_dict(sd)
     assert float(opt.state[p]["step"]) == 1 and bool((opt.state[p]["exp_avg_codes"] == 127).all())
+
+
+def two_groups(R):
+    ps = [torch.nn.Parameter(torch.ones(5000, device="cuda")) for _ in range(2)]
+    opt = R.FusedAdamW([{"params": [ps[0]], "lr": 0.0, "weight_decay": 0.0}, {"params": [ps[1]], "lr": 1e-2, "weight_decay": 0.0}], betas=BETAS, state_bits=8)
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    opt.step()
+    return ps, opt
+
+
+def test_a_parameter_moved_between_groups(R):
+    """takes its new group's numbers."""
+    ps, opt = two_groups(R)
+    assert bool((ps[0] == 1).all()) and bool((ps[1] < 1).all())
+    a, b = opt.param_groups
+    b["params"].insert(0, a["params"].pop())
+    held = ps[1].detach().clone()
+    opt.step()
+    assert bool((ps[0] < 1).all()) and bool((ps[1] < held).all())
