@@ -212,6 +212,10 @@ class FusedAdamW(torch.optim.Optimizer):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("FusedAdamW: the first step (and one after parameters were moved or added) has to run outside a graph capture")
         old = {p: dict(self.state[p]) for p in params if self.state.get(p)}
+        for i, p in enumerate(params):                             # (before anything is changed)
+            for k, shape in self._shapes(p).items() if p in old else ():
+                if k not in old[p] or tuple(old[p][k].shape) != shape:
+                    raise RuntimeError(f"FusedAdamW: the moments of parameter {i} do not go with its shape {tuple(p.shape)}")
         with ops._on_device(params[0]), torch.no_grad():
             plan = _Plan(params, self._groups(), [self._bits(p) for p in params])
             self._adopt(plan, params)

@@ -603,3 +603,19 @@ def test_a_parameter_moved_between_groups(R):
     held = ps[1].detach().clone()
     opt.step()
     assert bool((ps[0] < 1).all()) and bool((ps[1] < held).all())
+
+
+def test_a_state_that_cannot_follow_its_parameter(R):
+    """is refused, and kept."""
+    ps, opt = two_groups(R)
+    now = {k: t.clone() for k, t in opt.state[ps[1]].items()}
+    whole = ps[1].data
+    ps[1].grad, ps[1].data = None, whole[:4500]
+    ps[1].grad = torch.ones_like(ps[1])
+    with pytest.raises(RuntimeError, match="moments"):
+        opt.step()
+    ps[1].grad, ps[1].data = None, whole
+    ps[1].grad = torch.ones_like(ps[1])
+    assert all(torch.equal(opt.state[ps[1]][k], t) for k, t in now.items())
+    opt.step()
+    assert float(opt.state[ps[1]]["step"]) == 2
