@@ -230,7 +230,7 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def _ready(self, params):
         plan = self._plan
-        if plan is None or self._stale or plan.groups != self._groups() or not plan.layout.matches(params):
+        if plan is None or self._stale or plan.groups != self._groups() or not plan.layout.matches(params) or params[0] not in self.state:
             plan = self._build()
         return plan
 

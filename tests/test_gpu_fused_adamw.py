@@ -619,3 +619,15 @@ def test_a_state_that_cannot_follow_its_parameter(R):
     assert all(torch.equal(opt.state[ps[1]][k], t) for k, t in now.items())
     opt.step()
     assert float(opt.state[ps[1]]["step"]) == 2
+
+
+def test_a_cleared_state_starts_again(R):
+    ps, opt = two_groups(R)
+    opt.state.clear()
+    opt.step()
+    assert float(opt.state[ps[1]]["step"]) == float(opt.state[ps[0]]["step"]) == 1
+    fresh = torch.nn.Parameter(torch.ones(5000, device="cuda"))
+    fresh.grad = torch.ones_like(fresh)
+    other = R.FusedAdamW([fresh], lr=1e-2, weight_decay=0.0, betas=BETAS, state_bits=8)
+    other.step()
+    assert all(torch.equal(opt.state[ps[1]][k], t) for k, t in other.state[fresh].items())
