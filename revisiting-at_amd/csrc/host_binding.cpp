@@ -94,6 +94,9 @@ struct Rotation {
   int32_t norm, interleaved;
   bool turns() const { return norm || positions.defined(); }
 };
+// what a node saves of a rotation's tensors, so that a change in place raises as any other input's does (one made in inference mode has no version
+// to tell a change by, and is copied)
+Tensor kept(const Tensor& t) { return t.defined() && t.is_inference() ? t.clone() : t; }
 // weights of one type: where one is float32 and the other is not, both are
 std::pair<Tensor, Tensor> head_weights(Tensor wq, Tensor wk) {
   if (wq.defined() && wk.defined() && wq.scalar_type() != wk.scalar_type()) {
@@ -238,10 +241,12 @@ struct QkNormRopeBackward : Node {
     if (!in[0].defined() && !in[1].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
     const c10::DeviceGuard guard(options.device());
     const Tensor q = at(0), k = at(1), wq = at(2), wk = at(3);
+    Rotation turn = rot;
+    turn.positions = at(4); turn.inv_freq = at(5);
     const Tensor dyq = head_rows(in[0].defined() ? in[0] : at::zeros(q_size, options)), dyk = head_rows(in[1].defined() ? in[1] : at::zeros(k_size, options));
     const Tensor dq = fresh(dyq), dk = fresh(dyk);
     Tensor dwq, dwk;
-    rope_backward(dyq, dyk, q, k, dq, dk, wq, wk, rot, wants(2) && !*input_grad_only, wants(3) && !*input_grad_only, dwq, dwk);
+    rope_backward(dyq, dyk, q, k, dq, dk, wq, wk, turn, wants(2) && !*input_grad_only, wants(3) && !*input_grad_only, dwq, dwk);
     return {dq, dk, dwq.defined() ? dwq.to(wq_type) : dwq, dwk.defined() ? dwk.to(wk_type) : dwk};
   }
 };
@@ -272,7 +277,8 @@ std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q0, const Tensor& k0, cons
     if (w1.defined()) n->wk_type = w1.scalar_type();
     n->q_size = q.sizes().vec(); n->k_size = k.sizes().vec(); n->options = q.options();
     torch::autograd::set_history({yq, yk}, n);
-    n->save({norm ? q : Tensor(), norm ? k : Tensor(), wq, wk});
+    n->save({norm ? q : Tensor(), norm ? k : Tensor(), wq, wk, kept(rot.positions), kept(rot.inv_freq)});
+    rot.positions = rot.inv_freq = Tensor();
     n->rot = std::move(rot);
   }
   return {yq, yk};
@@ -295,20 +301,22 @@ struct AttentionRopeBackward : Node {
   variable_list gradients(const variable_list& in) override {
     if (!in[0].defined()) return {Tensor(), Tensor(), Tensor()};
     const Tensor qkv = at(0), yq = at(1), yk = at(2), wq = at(3), wk = at(4), lse = at(5);
+    Rotation turn = rot;
+    turn.positions = at(6); turn.inv_freq = at(7);
     const c10::DeviceGuard guard(qkv.device());
     const int64_t B = qkv.size(0), N = qkv.size(1), C = qkv.size(2) / 3, d = C / heads;
-    const Tensor out = saved[6].unpack(shared_from_this()).view({B, N, heads, d}), dout = head_rows(in[0].reshape({B, N, heads, d})), dqkv = fresh(qkv);
+    const Tensor out = saved[8].unpack(shared_from_this()).view({B, N, heads, d}), dout = head_rows(in[0].reshape({B, N, heads, d})), dqkv = fresh(qkv);
     const bool want_q = wants(1) && !*input_grad_only, want_k = wants(2) && !*input_grad_only;
     Tensor dwq, dwk;
-    if (rot.turns()) {
-      const Tensor ws = floats(lib.layer_bwd_ws_floats(B, N, heads, d, rot.batch_stride != 0), qkv);
+    if (turn.turns()) {
+      const Tensor ws = floats(lib.layer_bwd_ws_floats(B, N, heads, d, turn.batch_stride != 0), qkv);
       const Tensor fq = wq.defined() ? wq.to(at::kFloat) : wq, fk = wk.defined() ? wk.to(at::kFloat) : wk;
       if (want_q) dwq = floats(d, qkv);
       if (want_k) dwk = floats(d, qkv);
       check(lib.layer_bwd(qkv.data_ptr(), yq.data_ptr(), yk.data_ptr(), out.data_ptr(), dout.data_ptr(), ptr<float>(lse), dqkv.data_ptr(), ptr<float>(dwq),
-                          ptr<float>(dwk), ptr<float>(ws), strides(dout).data(), code_of(qkv), ptr<float>(fq), ptr<float>(fk), ptr<void>(rot.positions),
-                          rot.pos_dtype, rot.batch_stride, static_cast<int32_t>(rot.sections.size()), rot.sections.data(), ptr<float>(rot.inv_freq), B, N,
-                          heads, d, rot.eps, rot.norm, rot.interleaved, static_cast<float>(scale), current()),
+                          ptr<float>(dwk), ptr<float>(ws), strides(dout).data(), code_of(qkv), ptr<float>(fq), ptr<float>(fk), ptr<void>(turn.positions),
+                          turn.pos_dtype, turn.batch_stride, static_cast<int32_t>(turn.sections.size()), turn.sections.data(), ptr<float>(turn.inv_freq), B, N,
+                          heads, d, turn.eps, turn.norm, turn.interleaved, static_cast<float>(scale), current()),
             "cnx_attention_rope_bwd");
     } else {
       const auto x = parts(qkv, heads), g = parts(dqkv, heads);
@@ -350,8 +358,9 @@ Tensor attention_rope(const Tensor& qkv0, int64_t heads, double scale, const May
     if (w1.defined()) n->wk_type = w1.scalar_type();
     n->heads = heads; n->scale = scale;
     torch::autograd::set_history(out, n);
-    n->save({qkv, yq, yk, wq, wk, lse});
+    n->save({qkv, yq, yk, wq, wk, lse, kept(rot.positions), kept(rot.inv_freq)});
     n->saved.emplace_back(out, true);
+    rot.positions = rot.inv_freq = Tensor();
     n->rot = std::move(rot);
   }
   return out;

@@ -686,3 +686,27 @@ def test_attention_rope_with_gradients_whose_squares_no_fp32_holds(R, d):
         assert torch.equal(gx[:, 7, :C], want[0][:, 7, :C] * up) and torch.equal(gx[:, rest, :C], want[0][:, rest, :C])
     for a, b in zip(run(qkv, dout * 2.0 ** -110), want):                            # down to bf16's smallest normal number
         assert bool(((a.double() - b.double() * 2.0 ** -110).abs() <= 2.0 ** -8 * b.double().abs() * 2.0 ** -110 + 2.0 ** -126).all())
+
+
+def test_positions_changed_under_a_graph_raise(R):
+    """Positions and frequencies are inputs like the others: changed in place between forward and backward, the backward raises."""
+    q, k = (torch.randn(2, 40, 2, 64, device="cuda").to(torch.bfloat16).requires_grad_() for _ in range(2))
+    qkv = torch.randn(2, 40, 384, device="cuda").to(torch.bfloat16).requires_grad_()
+    pos, inv = torch.arange(40, device="cuda").view(-1, 1), 100.0 ** (-torch.arange(32, device="cuda") / 32)
+    calls = ((lambda: R.ops.qk_norm_rope(q, k, None, None, pos, inv)[0], q), (lambda: R.ops.attention_rope(qkv, 2, None, None, None, pos, inv), qkv))
+    for f, leaf in calls:
+        for change in (lambda: pos.add_(1), lambda: inv.mul_(0.5)):
+            out = f()
+            change()
+            with pytest.raises(RuntimeError, match="inplace"):
+                torch.autograd.grad(out, leaf, torch.ones_like(out))
+        out = f()                                                                   # unchanged ones, twice, from the same graph
+        a, b = (torch.autograd.grad(out, leaf, torch.ones_like(out), retain_graph=True)[0] for _ in range(2))
+        assert torch.equal(a, b)
+        with torch.no_grad():
+            out = f()
+            pos.add_(1)                                                             # no graph: nobody minds
+    with torch.inference_mode():
+        frozen = torch.arange(40, device="cuda").view(-1, 1)
+    out = R.ops.qk_norm_rope(q, k, None, None, frozen, inv)[0]                      # a tensor that has no version
+    torch.autograd.grad(out, q, torch.ones_like(out))
