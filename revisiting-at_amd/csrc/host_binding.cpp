@@ -195,6 +195,11 @@ std::shared_ptr<N> node_of(const Ts&... inputs) {
 }
 template <typename... Ts>
 bool wants_grad(const Ts&... ts) { return at::GradMode::is_enabled() && ((ts.defined() && ts.requires_grad()) || ...); }
+// Dual tensors are refused: their tangents would be lost without a word, which reads as a derivative of zero.
+template <typename... Ts>
+void no_tangents(const char* what, const Ts&... ts) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!((ts.defined() && ts._fw_grad(0).defined()) || ...), what, " has no forward-mode derivative");
+}
 
 struct MhaBackward : Node {
   double scale;
@@ -211,6 +216,7 @@ struct MhaBackward : Node {
 };
 
 Tensor mha(const Tensor& q0, const Tensor& k0, const Tensor& v0, double scale, bool causal, const Maybe& q_lens, const Maybe& kv_lens) {
+  no_tangents("mha", q0, k0, v0);
   const c10::DeviceGuard guard(q0.device());
   const bool grad = wants_grad(q0, k0, v0);
   Tensor q, k, v, out, lse;
@@ -262,6 +268,7 @@ std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q0, const Tensor& k0, cons
   const c10::DeviceGuard guard(q0.device());
   Rotation rot = rotation(positions, inv_freq, std::move(sections), pos_dtype, batch_stride, eps, norm, interleaved);
   const Tensor w0 = of(wq0), w1 = of(wk0);
+  no_tangents("qk_norm_rope", q0, k0, w0, w1, rot.positions, rot.inv_freq);
   const bool grad = wants_grad(q0, k0, w0, w1);
   Tensor q, k, wq, wk, yq, yk;
   {
@@ -331,6 +338,7 @@ Tensor attention_rope(const Tensor& qkv0, int64_t heads, double scale, const May
   const c10::DeviceGuard guard(qkv0.device());
   Rotation rot = rotation(positions, inv_freq, std::move(sections), pos_dtype, batch_stride, eps, norm, interleaved);
   const Tensor w0 = of(wq0), w1 = of(wk0);
+  no_tangents("attention_rope", qkv0, w0, w1, rot.positions, rot.inv_freq);
   const bool grad = wants_grad(qkv0, w0, w1);
   Tensor qkv, wq, wk, yq, yk, out, lse;
   {

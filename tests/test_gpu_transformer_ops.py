@@ -710,3 +710,21 @@ def test_positions_changed_under_a_graph_raise(R):
         frozen = torch.arange(40, device="cuda").view(-1, 1)
     out = R.ops.qk_norm_rope(q, k, None, None, frozen, inv)[0]                      # a tensor that has no version
     torch.autograd.grad(out, q, torch.ones_like(out))
+
+
+def test_forward_mode_derivatives_are_refused(R):
+    """A dual tensor raises, where it would come back without a tangent (a derivative of zero)."""
+    import torch.autograd.forward_ad as fwd
+    q = torch.randn(2, 40, 2, 64, device="cuda").to(torch.bfloat16)
+    qkv = torch.randn(2, 40, 384, device="cuda").to(torch.bfloat16)
+    w, pos, inv = torch.ones(64, device="cuda"), torch.arange(40.0, device="cuda").view(-1, 1), torch.ones(32, device="cuda")
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))                       # noqa: E731
+        for f in (lambda: R.ops.mha(dual(q), q, q), lambda: R.ops.mha(q, q, dual(q)), lambda: R.ops.qk_norm_rope(q, dual(q)),
+                  lambda: R.ops.qk_norm_rope(q, q, dual(w)), lambda: R.ops.attention_rope(dual(qkv), 2), lambda: R.ops.attention_rope(qkv, 2, None, w, dual(w)),
+                  lambda: R.ops.qk_norm_rope(q, q, None, None, dual(pos), inv), lambda: R.ops.attention_rope(qkv, 2, None, None, None, pos, dual(inv))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                f()
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                f()
+        assert bool(torch.isfinite(R.ops.mha(q, q, q)).all())
