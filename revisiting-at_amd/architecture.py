@@ -392,6 +392,13 @@ class Attention(nn.Module):
             self.register_buffer("inv_freq", rope[1], persistent=False)
             self.sections = rope[2]
 
+    def _apply(self, fn, *args, **kwargs):
+        inv_freq = self.inv_freq if self.rope else None
+        super()._apply(fn, *args, **kwargs)
+        if inv_freq is not None and self.inv_freq.dtype != inv_freq.dtype:          # a cast model's angles: frequencies stay in 32 bits
+            self.inv_freq = inv_freq.to(self.inv_freq.device)
+        return self
+
     def _head_args(self):
         return ((self.q_norm.weight, self.k_norm.weight) if self.qk_norm else (None, None)) + \
             ((self.positions, self.inv_freq, self.sections) if self.rope else (None, None, None))

@@ -631,3 +631,38 @@ def test_a_cleared_state_starts_again(R):
     other = R.FusedAdamW([fresh], lr=1e-2, weight_decay=0.0, betas=BETAS, state_bits=8)
     other.step()
     assert all(torch.equal(opt.state[ps[1]][k], t) for k, t in other.state[fresh].items())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+def test_a_cast_vit_keeps_its_rotary_frequencies(R, dtype):
+    """model.to(bfloat16) runs forward and backward with the frequencies in 32 bits; there and back they are what they were."""
+    model = stem_vit(R).cuda()
+    attn = model.blocks[0].attn
+    inv, pos = attn.inv_freq.clone(), attn.positions.clone()
+    model.to(dtype)
+    assert attn.q_norm.weight.dtype == attn.qkv.weight.dtype == dtype
+    assert attn.inv_freq.dtype == torch.float32 and torch.equal(attn.inv_freq, inv) and torch.equal(attn.positions, pos)
+    x = torch.randn(2, 197, 384, device="cuda").to(dtype).requires_grad_()
+    out = model.blocks[0].attn(x)
+    grads = torch.autograd.grad(out, [x, attn.q_norm.weight, attn.qkv.weight], torch.randn_like(out))
+    assert out.dtype == dtype and all(g.dtype == dtype and bool(torch.isfinite(g).all()) for g in grads)
+    model.float()
+    assert attn.inv_freq.dtype == torch.float32 and torch.equal(attn.inv_freq, inv) and torch.equal(attn.positions, pos)
+    model.double()
+    assert torch.equal(attn.inv_freq, inv)
+    ref = R.architecture.Attention(384, 6, True, R.architecture.rope_grid((14, 14), 64)).cuda()
+    assert ref.inv_freq.is_cuda and ref.positions.is_cuda and torch.equal(ref.cpu().inv_freq, inv.cpu()) and not ref.positions.is_cuda
+
+
+def test_a_cast_vit_runs_under_autocast(R):
+    model = stem_vit(R).cuda()
+    x = torch.rand(2, 3, 224, 224, generator=torch.Generator().manual_seed(3)).cuda()
+    with torch.no_grad():
+        ref = model(x)
+    model.to(torch.bfloat16)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        out = model(x.to(torch.bfloat16))
+    out.float().square().sum().backward()
+    # the roundings of test_stem_vit_with_rope_gradients_follow_its_definition, and the weights' and the image's own
+    assert float((out.detach().float() - ref).norm() / ref.norm()) < 0.06
+    assert all(p.grad is not None and bool(torch.isfinite(p.grad).all()) for p in model.parameters())
