@@ -234,10 +234,13 @@ struct Stage {
   }
   static __device__ __forceinline__ u32x4 buffer(const uint16_t* base) {                       // raw buffer of 2 GiB
     const uint64_t p64 = reinterpret_cast<uint64_t>(base);
-    return u32x4{static_cast<uint32_t>(p64), static_cast<uint32_t>(p64 >> 32) & 0xffffu, 0x80000000u, 0x00020000u};
+    u32x4 rs = {static_cast<uint32_t>(p64), static_cast<uint32_t>(p64 >> 32) & 0xffffu, 0x80000000u, 0x00020000u};
+    asm volatile("s_nop 4" : "+s"(rs));          // a scalar register written by a vector instruction is read by a load 5 wait states later; the compiler
+    return rs;                                   // sees to that for its own loads only
   }
   // 64 lanes x 16 bytes to LDS addresses dst + 16 lane.  Inline, because the compiler waits for the builtin's load before any LDS read that it
-  // cannot tell apart - the other buffer's; tile_barrier() waits instead.  (No destination registers.)
+  // cannot tell apart - the other buffer's; tile_barrier() waits instead.  (No destination registers; m0 is a reserved register, which the compiler
+  // writes in front of each use of its own and does not take in a clobber list.)
   static __device__ __forceinline__ void piece(u32x4 rs, uint32_t dst, uint32_t off) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(dst), "v"(off), "s"(rs) : "memory");
   }
