@@ -374,7 +374,8 @@ int cnx_adamw_values(const uint8_t* m_codes, const float* m_scales, const uint8_
  * tensor in the order given at the function.  q_lens / kv_lens [B] (nullable, clamped to [0, Nq] / [0, Nk]): queries and keys at or beyond
  * them are padding: never used, padded queries give zeros (lse -inf), padded rows of every gradient are zeros.  causal: query i sees keys
  * j <= i + kv_len - q_len (the last query sees the last key).  A query that sees no key gives zeros and no gradient.  A masked key's own
- * values have no influence, except that causal order needs finite v: the tile that holds a row's last key may hold later ones.
+ * values have no influence, except that causal order needs finite ones: the tile that holds a row's last key may hold later keys (a key's tile
+ * earlier rows), and zero times what is not finite in their v or, in the backward, k (q, dout) reaches that row (key).
  * lse [B, H, Nq] (nullable in the forward) = log sum exp of the scaled scores.  ws: cnx_mha_ws_floats(...) floats for the forward,
  * cnx_mha_bwd_ws_floats(...) for the backward (0 = none: NULL is fine), for calls with few rows or key tiles, which are split over
  * workgroups and joined in a fixed order; dvec: B * H * Nq floats.  scale > 0.  Deterministic. */

@@ -462,6 +462,12 @@ __global__ __launch_bounds__(256, 2) void mha_fwd_kernel(const MhaArgs a) {
   // lane = row: results of the row in registers, d = db * 32 + (r & 3) + 8 (r >> 2) + 4 half
   const float sum = both_halves_sum(l);
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  if (__any(sum == 0.f)) {                       // rows that see no key, beside others whose keys are not finite: 0 x inf is in their registers
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[db][r] = sum == 0.f ? 0.f : o[db][r];
+  }
   if (w.tok >= a.Nq) return;
   const int h = w.hk * a.G + w.hd;
   const int64_t at = (w.b * a.H + h) * a.Nq + w.tok;
@@ -780,6 +786,12 @@ __global__ __launch_bounds__(256, 2) void mha_dq_kernel(const MhaArgs a) {
     }
   };
   w.walk(a, compute);
+  if (__any(w.end <= w.k_begin)) {               // (as in the forward)
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dq[db][r] = w.end <= w.k_begin ? 0.f : dq[db][r];
+  }
   if constexpr (TURN) {
 #pragma unroll
     for (int db = 0; db < DB; ++db)

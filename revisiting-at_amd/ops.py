@@ -2118,7 +2118,8 @@ def mha(q, k, v, scale=None, causal=False, q_lens=None, kv_lens=None):
     ``q`` [B, Nq, H, d], ``k`` / ``v`` [B, Nk, Hkv, d] in bfloat16 or float16, d 64 or 128; H a multiple of Hkv (query head h reads key head
     h // (H / Hkv)).  Views of a packed projection or of a [B, H, N, d] cache are read in place.  ``scale`` defaults to d^-1/2.
     ``causal``: query i sees the keys up to i + kv_len - q_len (the last query sees the last key).  ``q_lens`` / ``kv_lens`` [B] int32: queries
-    and keys of a padded batch at or beyond these are never used; a padded query, or one that sees no key, gives zeros and no gradient.
+    and keys of a padded batch at or beyond these are never used; a padded query, or one that sees no key, gives zeros and no gradient.  What a
+    length masks may hold anything; what only causal order masks has to be finite (zero times an infinity or NaN in the same tile is NaN).
     Differentiable in q, k and v (once); nothing of size Nq x Nk is kept.  ``attention`` is the packed form for up to 416 tokens."""
     what = "mha"
     _check_heads(what, ("q", q), ("k", k), ("v", v))

@@ -728,3 +728,21 @@ def test_forward_mode_derivatives_are_refused(R):
             with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
                 f()
         assert bool(torch.isfinite(R.ops.mha(q, q, q)).all())
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_padded_queries_give_zeros_beside_keys_that_are_not_finite(R, d):
+    """A query that sees no key has zeros and no gradient also where its tile holds queries that see infinities and NaN."""
+    g = torch.Generator().manual_seed(4)
+    for N, H, Hkv in ((130, 2, 2), (70, 4, 1), (1000, 2, 1)):                       # (1000 keys under 2 heads: split)
+        q, k, v, dout = (torch.randn(2, N, h, d, generator=g).to(torch.bfloat16).cuda() for h in (H, Hkv, Hkv, H))
+        k[:, 3], v[:, 5], v[:, 6] = float("inf"), float("inf"), float("nan")
+        ql, kl = torch.tensor([20, 0], dtype=torch.int32, device="cuda"), torch.tensor([N, N], dtype=torch.int32, device="cuda")
+        x = [t.clone().requires_grad_() for t in (q, k, v)]
+        for causal in (False, True):
+            out = R.ops.mha(*x, causal=causal, q_lens=ql, kv_lens=kl)
+            dq, dk, dv = torch.autograd.grad(out, x, dout)
+            for t in (out, dq):
+                assert not bool(torch.isfinite(t[0, :20]).all())
+                assert not bool(t[0, 20:].any()) and not bool(t[1].any())
+            assert not bool(dk[1].any()) and not bool(dv[1].any())
