@@ -67,12 +67,12 @@ Tensor floats(int64_t n, const Tensor& like) { return n ? at::empty({n}, like.op
 Tensor of(const Maybe& t) { return t ? *t : Tensor(); }
 
 // t [B, N, H, d] itself where the kernels can read it in place (contiguous heads that begin at 16 bytes, any other strides up to 2^22 elements
-// between tokens and 2^28 over a token's heads, zero included), else a contiguous copy
-Tensor head_rows(const Tensor& t) {
+// between tokens and 2^28 over the heads that share a key head, zero included), else a contiguous copy
+Tensor head_rows(const Tensor& t, int64_t share = 1) {
   const int64_t piece = 16 / t.element_size();
   const auto s = t.strides();
   if (s[3] == 1 && s[0] % piece == 0 && s[1] % piece == 0 && s[2] % piece == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 &&
-      s[1] < 1 << 22 && s[2] * t.size(2) < 1 << 28)
+      s[1] < 1 << 22 && s[2] * share < 1 << 28)
     return t;
   return fresh(t).copy_(t);
 }
@@ -209,7 +209,7 @@ struct MhaBackward : Node {
     if (!in[0].defined()) return {Tensor(), Tensor(), Tensor()};
     const Tensor q = at(0), k = at(1), v = at(2), lse = at(3);
     const c10::DeviceGuard guard(q.device());
-    const Tensor dout = head_rows(in[0]), dq = fresh(q), dk = fresh(k), dv = fresh(v);
+    const Tensor dout = head_rows(in[0], q.size(2) / k.size(2)), dq = fresh(q), dk = fresh(k), dv = fresh(v);
     mha_backward(q, k, v, saved[4].unpack(shared_from_this()), dout, lse, dq, dk, dv, scale, causal, at(5), at(6));
     return {dq, dk, dv};
   }
@@ -222,7 +222,7 @@ Tensor mha(const Tensor& q0, const Tensor& k0, const Tensor& v0, double scale, b
   Tensor q, k, v, out, lse;
   {
     at::AutoDispatchBelowADInplaceOrView below;
-    q = head_rows(q0); k = head_rows(k0); v = head_rows(v0);
+    q = head_rows(q0, q0.size(2) / k0.size(2)); k = head_rows(k0); v = head_rows(v0);
     out = fresh(q);
     lse = mha_forward(q, k, v, out, scale, causal, of(q_lens), of(kv_lens), grad);
   }

@@ -746,3 +746,23 @@ def test_padded_queries_give_zeros_beside_keys_that_are_not_finite(R, d):
                 assert not bool(torch.isfinite(t[0, :20]).all())
                 assert not bool(t[0, 20:].any()) and not bool(t[1].any())
             assert not bool(dk[1].any()) and not bool(dv[1].any())
+
+
+def test_long_caches_are_read_in_place(R):
+    """A [B, H, N, d] cache whose heads lie 2^25 and more elements apart, offsets beyond 32 bits: one query over a view of it, and no copy."""
+    H, N, d, n = 9, 2 ** 18 + 77, 128, 2 ** 18 - 5
+    k, v = (torch.empty(1, H, N, d, device="cuda", dtype=torch.bfloat16).normal_(generator=torch.Generator("cuda").manual_seed(s)) for s in (1, 2))
+    q = torch.randn(1, 1, H, d, device="cuda").to(torch.bfloat16)
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    with torch.no_grad():
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        out = R.ops.mha(q, k.transpose(1, 2), v.transpose(1, 2), kv_lens=lens)
+        assert torch.cuda.max_memory_allocated() - before < k.numel()               # (a copy of one of them: twice that)
+    s = torch.stack([k[0, h, :n].float() @ q[0, 0, h].float() for h in range(H)]).double() * d ** -0.5
+    p = torch.softmax(s, 1)
+    ref = torch.stack([p[h].float() @ v[0, h, :n].float() for h in range(H)])
+    # P is rounded to 16 bits (u) and the result once; sums of |v| weighted by P are below the largest |v|, 6 here: 2 u 6, and 2^-20 n^(1/2) of 32-bit sums
+    assert float((out[0, 0].float() - ref).abs().max()) <= 2 * 2.0 ** -8 * 6
+    assert float((out[0, 0].float() - ref).norm() / ref.norm()) < 2.0 ** -7
