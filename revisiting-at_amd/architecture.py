@@ -399,8 +399,8 @@ class Attention(nn.Module):
             self.inv_freq = inv_freq.to(self.inv_freq.device)
         return self
 
-    def _head_args(self):
-        return ((self.q_norm.weight, self.k_norm.weight) if self.qk_norm else (None, None)) + \
+    def _head_args(self, dtype=None):
+        return (tuple(w if dtype is None else w.to(dtype) for w in (self.q_norm.weight, self.k_norm.weight)) if self.qk_norm else (None, None)) + \
             ((self.positions, self.inv_freq, self.sections) if self.rope else (None, None, None))
 
     def forward(self, x):
@@ -408,12 +408,14 @@ class Attention(nn.Module):
         qkv = ops.linear_lib(x, self.qkv.weight, self.qkv.bias)
         if not self.qk_norm and not self.rope:
             o = ops.attention(qkv, self.num_heads, self.scale)      # [B, N, C]
-        elif qkv.dtype in (torch.bfloat16, torch.float16):
+        elif qkv.dtype in (torch.bfloat16, torch.float16) and C // self.num_heads in (64, 128):
             o = ops.attention_rope(qkv, self.num_heads, self.scale, *self._head_args(), norm=self.qk_norm)
-        else:                                                       # fp32 (evaluation without autocast): library products, as ops.attention
-            q, k, v = qkv.view(B, N, 3, self.num_heads, C // self.num_heads).unbind(2)
-            q, k = ops.qk_norm_rope(q, k, *self._head_args(), norm=self.qk_norm)
-            o = ops.attention(torch.stack((q, k, v), 2).view(B, N, 3 * C), self.num_heads, self.scale)
+        else:                             # fp32 (evaluation without autocast) and head dims without a kernel: library products in fp32, as ops.attention
+            wide = torch.float32 if qkv.dtype in (torch.bfloat16, torch.float16) else qkv.dtype
+            q, k, v = qkv.to(wide).view(B, N, 3, self.num_heads, C // self.num_heads).unbind(2)
+            q, k = ops.qk_norm_rope(q, k, *self._head_args(wide), norm=self.qk_norm)
+            with torch.autocast(x.device.type, enabled=False):
+                o = ops.attention(torch.stack((q, k, v), 2).view(B, N, 3 * C), self.num_heads, self.scale).to(qkv.dtype)
         return ops.linear_lib(o, self.proj.weight, self.proj.bias)
 
 

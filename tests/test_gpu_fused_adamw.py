@@ -666,3 +666,23 @@ def test_a_cast_vit_runs_under_autocast(R):
     # the roundings of test_stem_vit_with_rope_gradients_follow_its_definition, and the weights' and the image's own
     assert float((out.detach().float() - ref).norm() / ref.norm()) < 0.06
     assert all(p.grad is not None and bool(torch.isfinite(p.grad).all()) for p in model.parameters())
+
+
+@pytest.mark.parametrize("qk_norm,rope", [(True, True), (True, False), (False, True)])
+def test_vit_options_with_other_head_dims(R, qk_norm, rope):
+    """Head dims that ops.attention_rope has no kernel for: the same layer under autocast as in fp32."""
+    torch.manual_seed(0)
+    layer = R.architecture.Attention(128, 4, qk_norm, R.architecture.rope_grid((4, 4), 32) if rope else None).cuda()
+    x = torch.randn(3, 17, 128, device="cuda", requires_grad=True)
+    ref = layer(x)
+    cot = torch.randn_like(ref)
+    names = [n for n, _ in layer.named_parameters()]
+    gr = torch.autograd.grad(ref, [x, *layer.parameters()], cot)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        out = layer(x)
+    assert out.dtype == torch.bfloat16
+    gd = torch.autograd.grad(out, [x, *layer.parameters()], cot.to(out.dtype))
+    # about 10 roundings to bf16 each way, u = 2^-8, adding up like independent ones: sqrt(10) u = 1.3 %; twice that, both ways for a gradient
+    assert float((out.float() - ref).norm() / ref.norm()) < 0.026
+    for name, a, b in zip(["x"] + names, gd, gr):
+        assert float((a.float() - b).norm()) <= 0.052 * float(b.norm()) + 1e-3 * float(gr[0].norm()), name
