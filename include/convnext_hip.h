@@ -342,7 +342,8 @@ int cnx_attention_bwd(const void* qkv, const void* out, const void* dout, const 
  * ones - a set that no tensor of the table uses may be NULL.  At most CNX_ADAMW_TENSORS tensors and CNX_ADAMW_GROUPS groups a call.
  * 8-bit moments: code * scale of the block; m: sign bit and 7 bits, v: its root in 8 bits; code c > 0 is the fp32 number whose pattern is
  * (c + 889) << 20 (m) or (c + 1777) << 19 (root of v), 1.0 the largest, 0 is zero; rounded to nearest even, below code 1 to zero from half a
- * step of its binade beneath it on; a root above zero is never rounded to zero. */
+ * step of its binade beneath it on; where beta is above 31/32, and a step would be rounded away again, up or down by a hash of element and step
+ * with the value's mean; a root above zero is never rounded to zero. */
 #define CNX_ADAMW_BLOCK 256
 #define CNX_ADAMW_CHUNK 4096
 #define CNX_ADAMW_TENSORS 440

@@ -148,7 +148,9 @@ class _Plan:
 class FusedAdamW(torch.optim.Optimizer):
     """``torch.optim.AdamW`` (decoupled weight decay, bias correction) for fp32 or bf16 parameters on one device: one prepared launch updates
     them all (at most 8 parameter groups).  ``state_bits=8`` keeps the moments of tensors with 4096 or more elements in a byte each (a
-    scale for every 256 elements; the second moment as its root), the others in 32 bits.
+    scale for every 256 elements; the second moment as its root), the others in 32 bits.  Codes are rounded to nearest up to betas of 31/32 (a
+    moment then follows its gradients because they vary, to about 8 % of a root at 0.95) and, above, up or down by a hash of element and step
+    (about 20 % at 0.999): a step of a moment is less than half a step of its code there.
 
     Step counters live on the device and ``lr`` may be a device tensor, so a step can be captured into a hipGraph after one eager step (or
     ``load_state_dict``) has built the tables.  ``load_state_dict`` writes into the buffers, counters and device learning rates that are there, so

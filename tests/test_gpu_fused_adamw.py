@@ -686,3 +686,67 @@ def test_vit_options_with_other_head_dims(R, qk_norm, rope):
     assert float((out.float() - ref).norm() / ref.norm()) < 0.026
     for name, a, b in zip(["x"] + names, gd, gr):
         assert float((a.float() - b).norm()) <= 0.052 * float(b.norm()) + 1e-3 * float(gr[0].norm()), name
+
+
+@pytest.mark.parametrize("up", [0.1, 10.0])
+def test_8_bit_roots_follow_gradients_at_slow_betas(R, up):
+    """Where a step changes a moment by less than half a step of its code (beta2 = 0.999), the stored root still follows gradients whose size changes
+    for three quarters of a block."""
+    n, b2, first, then = 8192, 0.999, 2000, 8000                                    # 0.999^8000 = 3e-4: what was has left the root to 2 %
+    p = torch.nn.Parameter(torch.zeros(n, device="cuda"))
+    opt = R.FusedAdamW([p], lr=0.0, betas=(0.9, b2), weight_decay=0.0, state_bits=8)
+    g = torch.Generator("cuda").manual_seed(0)
+    some = torch.arange(n, device="cuda") % 4 != 0
+    size, v = torch.ones(n, device="cuda"), torch.zeros(n, device="cuda", dtype=torch.float64)
+    p.grad = torch.empty_like(p)
+    for t in range(first + then):
+        if t == first:
+            size = torch.where(some, up, 1.0)
+        p.grad.normal_(generator=g).mul_(size)
+        v.mul_(b2).addcmul_(p.grad.double(), p.grad.double(), value=1 - b2)
+        opt.step()
+    k = torch.from_numpy(decode(opt.state[p], n)[1]).double().sqrt() / v.sqrt().cpu()
+    # A rounding adds at most delta |drift| to the relative variance, delta = 1/16 a code's step and |drift| (1 - b2) / 2 on average; the root returns at a
+    # rate of 1 - b2: delta / 4 in the long run, 0.125 of standard deviation.  6144 (2048) elements: means to 0.01, six deviations at the ends.
+    for which in (some.cpu(), ~some.cpu()):
+        q = k[which]
+        assert abs(float(q.mean()) - 1) < 0.05 and float((q - 1).std()) < 0.15, (float(q.mean()), float(q.std()))
+        assert 0.25 < float(q.min()) and float(q.max()) < 1.75
+
+
+def test_8_bit_first_moments_follow_gradients_at_slow_betas(R):
+    n, b1 = 8192, 0.99
+    p = torch.nn.Parameter(torch.zeros(n, device="cuda"))
+    opt = R.FusedAdamW([p], lr=0.0, betas=(b1, 0.95), weight_decay=0.0, state_bits=8)
+    g = torch.Generator("cuda").manual_seed(0)
+    some = torch.arange(n, device="cuda") % 4 != 0
+    m = torch.zeros(n, device="cuda", dtype=torch.float64)
+    p.grad = torch.empty_like(p)
+    for t in range(2000):
+        p.grad.normal_(generator=g).mul_(0.1).add_(torch.where(some & (t >= 1000), 0.1, 1.0))
+        m.mul_(b1).add_(p.grad.double(), alpha=1 - b1)
+        opt.step()
+    got, want = torch.from_numpy(decode(opt.state[p], n)[0]).double()[some.cpu()], m.cpu()[some.cpu()]
+    # a rounding adds at most (delta / 2)^2 to the relative variance, delta = 1/8 a code's step, and 1 / (1 - b1^2) = 50 steps add up: 0.44 of m at most
+    assert abs(float((got - want).mean())) < 0.005 and float((got - want).norm() / want.norm()) < 0.44
+
+
+@pytest.mark.parametrize("bits", [8])
+def test_hashed_codes_are_the_same_every_time(R, bits):
+    """Eager and captured steps of two optimizers at beta2 = 0.999 agree bit for bit."""
+    def build():
+        ps, g = make([(4096 + 5,), (64, 100)], torch.float32, 5)
+        set_grads(ps, g)
+        opt = R.FusedAdamW(ps, lr=LR, betas=(0.99, 0.999), state_bits=bits)
+        opt.step()
+        return ps, opt
+    (ps, opt), (qs, eager) = build(), build()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for _ in range(4):
+        graph.replay()
+        eager.step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(ps, qs))
+        assert all(torch.equal(t, eager.state[q][k]) for p, q in zip(ps, qs) for k, t in opt.state[p].items())
