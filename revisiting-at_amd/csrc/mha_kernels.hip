@@ -21,8 +21,10 @@
 // Masks.  Each row has an end: keys at or beyond it are not seen (key lengths, causal order, padded queries: end 0).  A row that sees no
 // key gives zeros and lse = -inf, and no gradient.  Rows at or beyond their sample's length are staged as zeros whatever memory holds.
 //
-// Roundings.  Scores, maxima, sums, lse, D and all accumulators are 32 bits.  P and dS are rounded to 16 bits because they are matrix
-// operands; the results once, at the end.  attention_rope's q' and k' have to lie in memory between two kernels and are rounded there - to
+// Roundings.  Scores, maxima, sums, lse and all accumulators are 32 bits.  P and dS are rounded to 16 bits because they are matrix
+// operands; the results once, at the end.  D is a 32-bit sum, of dout and the rounded out (u |dout| |out| off), or - for rows that see no key
+// behind the first tile - of P dP as the tile gives them (errors against 64 bits, 2 keys: 2.4 -> 1.5 times those of one rounding at the end; dq's
+// kernel 1 % slower at 512 px).  attention_rope's q' and k' have to lie in memory between two kernels and are rounded there - to
 // fp16 where the norm bounds them, since every score and gradient sees that rounding.
 //
 // Measured (us; TFLOP/s of the products a kernel forms; a library product of 8192^3: 1263 bf16, 1214 fp16):
@@ -326,6 +328,7 @@ struct Tile {
   int tok, hd, end;                              // this lane's row: token (Nq where there is none), head of the key head, first key it does not see
   int wave_end;                                  // the same of the wavefront's rows together
   int k_begin, k_end;
+  bool few;                                      // (uniform) some rows see no key behind the first tile
   uint32_t base;
 
   __device__ __forceinline__ Tile(const MhaArgs& a, uint32_t lds) : Tile(a, lds, xcd_order(blockIdx.x, gridDim.x)) {}
@@ -353,6 +356,7 @@ struct Tile {
     tok = r < R ? over(r, a.G) : a.Nq;
     hd = r < R ? r - tok * a.G : 0;
     end = lim.end(tok, a.causal);
+    few = k_begin == 0 && k_end > 0 && lim.end(over(row0, a.G), a.causal) <= kKT;
     sk.rows_apart(a.vk.n);
     sv.rows_apart(a.vv.n);
     if (k_begin < k_end) fetch(a, k_begin, 0);
@@ -707,7 +711,7 @@ __global__ __launch_bounds__(256, 2) void mha_dq_kernel(const MhaArgs a) {
   const int half = (threadIdx.x >> 5) & 1, h = w.hk * a.G + w.hd;
   const int64_t at = (w.b * a.H + h) * a.Nq + w.tok;
   u32x4 qf[KS], gf[KS];
-  float lse2, dd, mul = a.scale;
+  float lse2, dd, mul = a.scale, dd_mul = 1.f;
   {
     const bool live = w.end > 0;                 // a row without keys has no gradient
     const int64_t i = live ? w.tok : 0;
@@ -728,7 +732,6 @@ __global__ __launch_bounds__(256, 2) void mha_dq_kernel(const MhaArgs a) {
     }
     dd = both_halves_sum(part);
     lse2 = live ? a.lse[at] * kLog2e : INFINITY;                       // exp2(s - inf) = 0
-    if (w.split == 0 && half == 0 && w.tok < a.Nq) a.dvec[at] = dd;
     if constexpr (T::kScaled) {                  // a row's own scale
       float largest = 0.f, squares = 0.f;
 #pragma unroll
@@ -747,14 +750,37 @@ __global__ __launch_bounds__(256, 2) void mha_dq_kernel(const MhaArgs a) {
       const int e = scale_exponent(row_size(largest, both_halves_sum(squares)), range_of(a.range, w.b * a.H + h, a.pieces).x);
       scale_bf16(gf, power_of_two(e));
       dd *= power_of_two(e);
-      mul *= power_of_two(-e);
+      dd_mul = power_of_two(-e);
+      mul *= dd_mul;
     }
   }
   const float c2 = a.scale * kLog2e;
+  const Lane<D> L(w.base);
+  // D of rows with few keys from the tile itself, sum P dP: out is rounded, and of two or three keys' dP little is left when D is taken away
+  if (w.few) {
+    tile_barrier();
+    float sum = 0.f;
+#pragma unroll
+    for (int blk = 0; blk < kKT / 32; ++blk) {
+      f32x16 s = zeros16(), dp = zeros16();
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        s = T::mfma_s(L.row(0, blk, ks), qf[ks], s);
+        dp = T::mfma(L.row(IMG, blk, ks), gf[ks], dp);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int key = blk * 32 + (r & 3) + 8 * (r >> 2) + 4 * half;
+        sum += key < w.end ? __builtin_amdgcn_exp2f(fmaf(s[r], c2, -lse2)) * dp[r] : 0.f;
+      }
+    }
+    sum = both_halves_sum(sum);
+    if (w.end <= kKT) dd = sum;
+  }
+  if (w.split == 0 && half == 0 && w.tok < a.Nq) a.dvec[at] = dd * dd_mul;
   f32x16 dq[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) dq[db] = zeros16();
-  const Lane<D> L(w.base);
   auto compute = [&](int k0, uint32_t kimg) {
     const uint32_t vimg = kimg + IMG;
     const bool masked = __any(w.end < k0 + kKT);

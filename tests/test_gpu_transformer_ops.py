@@ -766,3 +766,37 @@ def test_long_caches_are_read_in_place(R):
     # P is rounded to 16 bits (u) and the result once; sums of |v| weighted by P are below the largest |v|, 6 here: 2 u 6, and 2^-20 n^(1/2) of 32-bit sums
     assert float((out[0, 0].float() - ref).abs().max()) <= 2 * 2.0 ** -8 * 6
     assert float((out[0, 0].float() - ref).norm() / ref.norm()) < 2.0 ** -7
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("Nq,Nk,causal,lens", [(300, 1, False, None), (300, 2, False, None), (40, 3, True, None), (70, 64, False, None), (200, 200, True, None),
+                                               (130, 600, False, [5, 64, 600])])
+def test_mha_gradients_of_queries_with_few_keys(R, Nq, Nk, causal, lens, dtype):
+    """Of two or three keys' dP little is left when D is taken away: for queries that see 64 keys or fewer, all in the first tile, D does not come from
+    the rounded output."""
+    B, H, Hkv, d = 3, 4, 2, 64
+    g = torch.Generator().manual_seed(Nq + Nk)
+    q, k, v, dout = (torch.randn(B, n, h, d, generator=g).to(dtype).cuda() for n, h in ((Nq, H), (Nk, Hkv), (Nk, Hkv), (Nq, H)))
+    x = [t.requires_grad_() for t in (q, k, v)]
+    kl = None if lens is None else torch.tensor(lens, dtype=torch.int32, device="cuda")
+    dq = torch.autograd.grad(R.ops.mha(*x, causal=causal, kv_lens=kl), x, dout)[0].double().cpu()
+    u, scale = half_step(dtype), d ** -0.5
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    for b in range(B):
+        n = Nk if lens is None else lens[b]
+        ok = torch.arange(Nk).view(1, -1) < n
+        if causal:
+            ok = ok & (torch.arange(Nk).view(1, -1) <= torch.arange(Nq).view(-1, 1) + n - Nq)
+        ok = ok.expand(Nq, Nk)
+        few = (ok.sum(1) <= 64) & (ok.sum(1) > 0)
+        for h in range(H):
+            Q, G, K, V = (t.detach()[b, :, i].double().cpu() for t, i in ((q, h), (dout, h), (k, h // 2), (v, h // 2)))
+            P = torch.softmax(((Q @ K.T) * scale).masked_fill(~ok, -1e300), 1) * ok
+            DP = G @ V.T
+            DS = P * (DP - (P * DP).sum(1, keepdim=True))
+            # dS is rounded once (u); its 32-bit part: the score's d + 2 operations of sum |q k|, exp and log (2^-20) twice over, dP and D d deep
+            t = 2 * (d + 4) * E * scale * float((Q.abs() @ K.abs().T).max()) + 2.0 ** -20
+            size = G.abs() @ V.abs().T
+            eS = u * DS.abs() + 2 * t * P * (DP.abs() + (P * DP.abs()).sum(1, keepdim=True)) + 2 * (d + 64) * E * P * (size + (P * size).sum(1, keepdim=True)) + tiny * ok
+            want, bound = (DS @ K) * scale, (eS @ K.abs()) * scale
+            inside(dq[b, few, h], want[few], (bound * (1 + u) + u * want.abs() + tiny)[few], (b, h))
