@@ -750,3 +750,26 @@ def test_hashed_codes_are_the_same_every_time(R, bits):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(ps, qs))
         assert all(torch.equal(t, eager.state[q][k]) for p, q in zip(ps, qs) for k, t in opt.state[p].items())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_trainer_loads_its_optimizer_between_replays(R, bits):
+    """The replayed training pass goes on from the loaded moments, counters and learning rate, in the buffers that it was captured with."""
+    step = R.ATTrainStep(stem_vit(R), "vit_s", R.AdvConfig(attack="apgd", n_iter=2, graph=1), "cuda:0", lr=1e-3, state_bits=bits)
+    g = torch.Generator().manual_seed(1)
+    x, y = torch.rand(2, 3, 224, 224, generator=g).cuda(), torch.randint(0, 1000, (2,), generator=g).cuda()
+    for _ in range(6):
+        step.step(x, y)
+    opt, ps = step.optimizer, [p for gr in step.optimizer.param_groups for p in gr["params"]]
+    assert any(prog is not None for prog in step._tg.values())                      # it is replayed
+    saved, table, rate = copy.deepcopy(opt.state_dict()), opt._plan, opt.param_groups[0]["lr"]
+    for _ in range(2):
+        step.step(x, y)
+    assert float(opt.state[ps[0]]["step"]) == 8
+    opt.load_state_dict(saved)
+    assert opt._plan is table and opt.param_groups[0]["lr"] is rate and float(opt.state[ps[0]]["step"]) == 6
+    before = [p.detach().clone() for p in ps]
+    loss = step.step(x, y)
+    torch.cuda.synchronize()
+    assert bool(torch.isfinite(loss)) and float(opt.state[ps[0]]["step"]) == 7
+    assert all(bool(torch.isfinite(p).all()) and not torch.equal(p, b) for p, b in zip(ps, before))
