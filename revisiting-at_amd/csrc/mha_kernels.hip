@@ -29,9 +29,9 @@
 //
 // Measured (us; TFLOP/s of the products a kernel forms; a library product of 8192^3: 1263 bf16, 1214 fp16):
 //                                                       forward      dq           dk, dv
-//   64 x 1025 tokens, 6 heads, d 64, bf16               150   690    196   790    278          740
-//   2 x 4096, causal, 16 heads on 4, d 128, fp16        165   830    240   860    382 + 16     690
-//   32 x 577, 12 heads, d 64, with norm and rotation     60   550     97   510    125          525
+//   64 x 1025 tokens, 6 heads, d 64, bf16               151   685    198   780    282          730
+//   2 x 4096, causal, 16 heads on 4, d 128, fp16        165   830    233   885    373 + 16     705
+//   32 x 577, 12 heads, d 64, with norm and rotation     61   535    101   485    128          510
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 #include <stdint.h>

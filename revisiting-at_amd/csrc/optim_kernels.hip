@@ -3,7 +3,7 @@
 //   p <- p (1 - lr wd);  m <- b1 m + (1 - b1) g;  v <- b2 v + (1 - b2) g^2
 //   p <- p - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 // Element-wise and bound by memory: 28 bytes per fp32 parameter with 32-bit moments (p, m, v in and out, g in), 16.06 with 8-bit ones.
-// Measured: 152 tensors, 21.8 M parameters, 32 bits: 101 us (6.0 TB/s); 152 M parameters, 8 bits: 437 - 517 us (5.6 - 4.7 TB/s; about 60
+// Measured: 152 tensors, 21.8 M parameters, 32 bits: 101 us (6.0 TB/s); 152 M parameters, 8 bits: 427 - 500 us (5.7 - 4.9 TB/s; about 60
 // instructions per element, a quarter of them for the two codes); a copy of 2 GiB reaches 4.9 TB/s.
 //
 // Layout.  The moments of all tensors lie in flat buffers, each tensor from a multiple of 256 elements on.  A workgroup takes a chunk of 4096
